@@ -258,6 +258,63 @@ int rbf_b200_cross_entropy(const void* logits, const int64_t* targets, const flo
  * the kernel returns without touching x. Used by the backward of the cross entropy above. */
 int rbf_b200_scale_unless_one(void* x, const float* factor, int64_t n, int dtype, void* stream);
 
+/* The paged 8-bit cache and RBF attention over it (no counterpart in the reference, whose generation runs the whole prefix again
+ * for every token). A pool holds pages of 256 tokens: `pages` is num_pages x H x rbf_b200_cache_page_bytes(D) bytes, 16-byte
+ * aligned. D is a multiple of 8 up to 128. Per head a page has the 8-bit codes of its 16 blocks of 16 tokens, a key and a value
+ * scale per block (largest magnitude / 127; a block whose largest magnitude is below 1e-30 is held as zeros, one with a
+ * number that is not finite reads back as NaN), and the 16-bit rows of the block that is not complete yet: blocks are
+ * rounded once, when they are full, so what is held does not depend on the portions in which the tokens came.
+ * `page_table` (B x max_pages int32) lists each sequence's pages in order, `lengths` (B int32) its tokens, both in device
+ * memory; nothing is read or written through a page number outside [0, num_pages), whose tokens count as absent, and lengths are
+ * clamped to what the table's row spans. `new_lengths` (B int32, or NULL: T) says how many of a sequence's T new tokens are real.
+ * No two sequences of a call may append to the same page. dtype: 0 = bfloat16, 1 = float16, the same for all calls on a pool. */
+size_t rbf_b200_cache_page_bytes(int D);
+
+/* Writes new tokens behind the `lengths` that are there: k, v (B, H, T, D) with unit stride on D, element strides of dims
+ * (b, h, n) that are multiples of 8, 16-byte aligned. `lengths` is not changed: it is the caller's to advance, once for all
+ * layers of a model. */
+int rbf_b200_cache_append(void* pages, const int* page_table, const int* lengths, const int* new_lengths, const void* k,
+                          const void* v, const int64_t* k_strides, const int64_t* v_strides, int B, int H, int T, int D,
+                          int max_pages, int num_pages, int dtype, void* stream);
+
+/* Tokens first[b] (NULL: 0; below 0: 0) .. + count - 1 of every sequence as k, v (B, H, count, D), dense, zeros from
+ * lengths[b] on. */
+int rbf_b200_cache_read(const void* pages, const int* page_table, const int* lengths, const int* first, void* k, void* v,
+                        int B, int H, int D, int count, int max_pages, int num_pages, int dtype, void* stream);
+
+/* pages[l][dst[i]] = pages[l][src[i]] for all i and all `layers` pools of num_pages x page_bytes bytes behind one another;
+ * page_bytes (all heads) is a multiple of 16. src and dst are host arrays. No page may be a destination twice, nor a source and a destination. */
+int rbf_b200_cache_copy_pages(void* pages, int layers, int num_pages, size_t page_bytes, const int* src, const int* dst,
+                              int count, void* stream);
+
+/* out (B, H * G, T, D), dense: RBF attention (softmax = 0: without the denominator) of T new tokens, which have been appended
+ * already; token i of sequence b sees tokens 0 .. lengths[b] + i. Query head h reads key/value head h / G. q (B, H * G, T, D)
+ * like k above. Rows from new_lengths[b] on are zero, as are rows that see nothing. gamma: usually 1 / sqrt(head dim). The
+ * workspace is 256-byte aligned. */
+size_t rbf_b200_cache_attention_workspace_bytes(int T, int G, int D);
+int rbf_b200_cache_attention(const void* q, const int64_t* q_strides, const void* pages, const int* page_table,
+                             const int* lengths, const int* new_lengths, void* out, void* workspace, size_t workspace_bytes,
+                             int B, int H, int G, int T, int D, int max_pages, int num_pages, int dtype, int softmax,
+                             float gamma, void* stream);
+
+/* log_probs[r] = logits[r, tokens[r]] - logsumexp(logits[r]) in fp32; 0 where the token equals `ignore_index` or lies outside
+ * [0, cols). logits as for rbf_b200_cross_entropy; any alignment runs on 16-byte loads. */
+int rbf_b200_token_log_probs(const void* logits, const int64_t* tokens, float* log_probs, int64_t rows, int cols, int64_t ld,
+                             int64_t ignore_index, int dtype, void* stream);
+
+/* The clipped policy loss with a KL term over the rows whose token counts (see rbf_b200_token_log_probs), lp being the row's
+ * log-probability and r = exp(lp - old_log_probs):
+ *   loss = sum over rows of w * (kl_weight * (exp(ref - lp) - (ref - lp) - 1) - min(r A, clip(r, 1 - clip_low, 1 + clip_high) A))
+ * with w = weights[r], or 1 / number of counting rows where weights is NULL (no such row: NaN); ref_log_probs NULL: no KL term.
+ * Writes lp (as above), the loss, and - unless dlogits is NULL - the gradient with respect to the logits (row pitch ld_out,
+ * in their dtype, zero for rows that do not count). dlogits needs the alignment of logits modulo 16 bytes in every row. Everything is
+ * summed in a fixed order. The workspace is 8-byte aligned. */
+size_t rbf_b200_policy_loss_workspace_bytes(void);
+int rbf_b200_policy_loss(const void* logits, const int64_t* tokens, const float* old_log_probs, const float* advantages,
+                         const float* ref_log_probs, const float* weights, float* loss, float* log_probs, void* dlogits,
+                         void* workspace, size_t workspace_bytes, int64_t rows, int cols, int64_t ld, int64_t ld_out,
+                         int64_t ignore_index, float clip_low, float clip_high, float kl_weight, int dtype, void* stream);
+
 /* Synchronises `stream` and reads the device status word that the last call using `workspace` left:
  * 0 = ok, otherwise (site << 24 | work unit) of the bounded wait that ran out; the work unit is the linear block
  * index of the launch or, for the persistent kernels (head dim 64), the work item the block was on. Returns

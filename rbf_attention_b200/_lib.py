@@ -121,6 +121,33 @@ SIGNATURES = {
     ),
     "rbf_b200_scale_unless_one": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int64, ctypes.c_int,
                                                  ctypes.c_void_p]),
+    "rbf_b200_cache_page_bytes": (ctypes.c_size_t, [ctypes.c_int]),
+    "rbf_b200_cache_append": (
+        ctypes.c_int,
+        [ctypes.c_void_p] * 6 + [_c_i64p] * 2 + [ctypes.c_int] * 7 + [ctypes.c_void_p],
+    ),
+    "rbf_b200_cache_read": (ctypes.c_int, [ctypes.c_void_p] * 6 + [ctypes.c_int] * 7 + [ctypes.c_void_p]),
+    "rbf_b200_cache_copy_pages": (
+        ctypes.c_int,
+        [ctypes.c_void_p, ctypes.c_int, ctypes.c_int, ctypes.c_size_t, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int,
+         ctypes.c_void_p],
+    ),
+    "rbf_b200_cache_attention_workspace_bytes": (ctypes.c_size_t, [ctypes.c_int] * 3),
+    "rbf_b200_cache_attention": (
+        ctypes.c_int,
+        [ctypes.c_void_p, _c_i64p] + [ctypes.c_void_p] * 6 + [ctypes.c_size_t] + [ctypes.c_int] * 9
+        + [ctypes.c_float, ctypes.c_void_p],
+    ),
+    "rbf_b200_token_log_probs": (
+        ctypes.c_int,
+        [ctypes.c_void_p] * 3 + [ctypes.c_int64, ctypes.c_int, ctypes.c_int64, ctypes.c_int64, ctypes.c_int, ctypes.c_void_p],
+    ),
+    "rbf_b200_policy_loss_workspace_bytes": (ctypes.c_size_t, []),
+    "rbf_b200_policy_loss": (
+        ctypes.c_int,
+        [ctypes.c_void_p] * 10 + [ctypes.c_size_t, ctypes.c_int64, ctypes.c_int] + [ctypes.c_int64] * 3
+        + [ctypes.c_float] * 3 + [ctypes.c_int, ctypes.c_void_p],
+    ),
     "rbf_b200_post_device_status": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p]),
     "rbf_b200_qkv_prep": (
         ctypes.c_int,

@@ -20,7 +20,8 @@ HOST_SOURCE = os.path.join(CSRC, "host.cpp")
 HOST_STAMP = os.path.join(HERE, "_host.stamp")      # the torch and interpreter that _host.so was built for
 C_HEADER = os.path.join(os.path.dirname(HERE), "include", "rbf_b200.h")
 SOURCES = ["capi.cu", "rbf_prep.cu", "rbf_fwd.cu", "rbf_fwd_tf32.cu", "rbf_bwd.cu", "rbf_bwd_fused.cu",
-           "rbf_bwd_fused128.cu", "ce_loss.cu", "layer_norm.cu", "col_sums.cu", "gelu.cu", "narrow.cu"]
+           "rbf_bwd_fused128.cu", "ce_loss.cu", "layer_norm.cu", "col_sums.cu", "gelu.cu", "narrow.cu",
+           "cache_write.cu", "cache_attn.cu", "policy_loss.cu"]
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
     "-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC",

@@ -2,6 +2,7 @@
 // maps, and the launch sequence of each call. No device memory is allocated here.
 #include <math.h>
 #include <stdarg.h>
+#include <stdlib.h>
 
 #include <atomic>
 
@@ -9,6 +10,7 @@
 #include <string.h>
 
 #include "../../include/rbf_b200.h"
+#include "cache.cuh"
 #include "common.cuh"
 #include "launch.h"
 #include "tmap.h"
@@ -813,6 +815,222 @@ int rbf_b200_scale_unless_one(void* x, const float* factor, int64_t n, int dtype
   if (sms <= 0) return fail(RBF_B200_ERR_LAUNCH, "cannot read the SM count of the current device");
   const cudaError_t e = rbf::launch_scale_unless_one(x, factor, n, dtype, sms, static_cast<cudaStream_t>(stream_v));
   if (e != cudaSuccess) return fail(RBF_B200_ERR_LAUNCH, "scale launch failed: %s", cudaGetErrorString(e));
+  return RBF_B200_OK;
+}
+
+// ---------------------------------------------------------------------------------------------
+// The paged 8-bit cache and attention over it
+// ---------------------------------------------------------------------------------------------
+size_t rbf_b200_cache_page_bytes(int D) {
+  return D > 0 && D <= 128 ? rbf::cache_page_bytes(rbf::cache_columns(D)) : 0;
+}
+
+static int check_cache(const void* pages, const int* table, const int* lengths, int B, int H, int D, int max_pages,
+                       int num_pages, int dtype) {
+  if (B < 0 || H <= 0 || max_pages < 0 || num_pages < 0)
+    return fail(RBF_B200_ERR_BAD_ARGUMENT, "H must be positive, B, max_pages and num_pages at least 0");
+  if (D <= 0 || D > 128 || D % 8 != 0) return fail(RBF_B200_ERR_BAD_ARGUMENT, "head dim D = %d must be a multiple of 8 up to 128", D);
+  if (dtype != 0 && dtype != 1) return fail(RBF_B200_ERR_BAD_ARGUMENT, "dtype must be 0 (bf16) or 1 (fp16)");
+  if (B == 0) return RBF_B200_OK;
+  if (lengths == nullptr || (max_pages > 0 && table == nullptr) || (num_pages > 0 && pages == nullptr))
+    return fail(RBF_B200_ERR_BAD_ARGUMENT, "pages, page_table or lengths is NULL");
+  if (reinterpret_cast<uintptr_t>(pages) % 16 != 0) return fail(RBF_B200_ERR_BAD_LAYOUT, "pages must be 16-byte aligned");
+  return RBF_B200_OK;
+}
+
+// q, k or v: (B, H, T, D) with 16-byte rows
+static int check_rows(const char* name, const void* ptr, const int64_t* strides, int B, int H, int T) {
+  if (ptr == nullptr || strides == nullptr) return fail(RBF_B200_ERR_BAD_ARGUMENT, "%s is NULL", name);
+  if (reinterpret_cast<uintptr_t>(ptr) % 16 != 0) return fail(RBF_B200_ERR_BAD_LAYOUT, "%s must be 16-byte aligned", name);
+  const int ext[3] = {B, H, T};
+  for (int i = 0; i < 3; ++i)
+    if (ext[i] > 1 && strides[i] % 8 != 0)
+      return fail(RBF_B200_ERR_BAD_LAYOUT, "%s: stride[%d] must be a multiple of 8 elements", name, i);
+  return RBF_B200_OK;
+}
+
+int rbf_b200_cache_append(void* pages, const int* page_table, const int* lengths, const int* new_lengths, const void* k,
+                          const void* v, const int64_t* k_strides, const int64_t* v_strides, int B, int H, int T, int D,
+                          int max_pages, int num_pages, int dtype, void* stream_v) {
+  g_last_error[0] = 0;
+  int rc;
+  if ((rc = check_cache(pages, page_table, lengths, B, H, D, max_pages, num_pages, dtype))) return rc;
+  if (T < 0) return fail(RBF_B200_ERR_BAD_ARGUMENT, "T must be at least 0");
+  if (B == 0 || T == 0 || num_pages == 0) return RBF_B200_OK;
+  if ((rc = check_rows("k", k, k_strides, B, H, T)) || (rc = check_rows("v", v, v_strides, B, H, T))) return rc;
+  rbf::CacheAppendArgs a{};
+  a.k = k; a.v = v; a.pages = static_cast<uint8_t*>(pages); a.table = page_table; a.lengths = lengths; a.fresh = new_lengths;
+  set_strides(a.ks, k_strides); set_strides(a.vs, v_strides);
+  a.B = B; a.H = H; a.T = T; a.D = D; a.max_pages = max_pages; a.num_pages = num_pages;
+  a.blocks = static_cast<int>((static_cast<int64_t>(T) + rbf::kBlockTokens - 2) / rbf::kBlockTokens + 1);
+  if (static_cast<int64_t>(B) * H > 0x7fffffffll / 2 || static_cast<int64_t>(B) * H * 2 * a.blocks / 4 >= 0x7fffffffll)
+    return fail(RBF_B200_ERR_BAD_ARGUMENT, "B * H * T is too large for one call");
+  const cudaError_t e = rbf::launch_cache_append(a, dtype == 0, static_cast<cudaStream_t>(stream_v));
+  if (e != cudaSuccess) return fail(RBF_B200_ERR_LAUNCH, "cache append launch failed: %s", cudaGetErrorString(e));
+  return RBF_B200_OK;
+}
+
+int rbf_b200_cache_read(const void* pages, const int* page_table, const int* lengths, const int* first, void* k, void* v,
+                        int B, int H, int D, int count, int max_pages, int num_pages, int dtype, void* stream_v) {
+  g_last_error[0] = 0;
+  int rc;
+  if ((rc = check_cache(pages, page_table, lengths, B, H, D, max_pages, num_pages, dtype))) return rc;
+  if (count < 0) return fail(RBF_B200_ERR_BAD_ARGUMENT, "count must be at least 0");
+  if (B == 0 || count == 0) return RBF_B200_OK;
+  if (k == nullptr || v == nullptr) return fail(RBF_B200_ERR_BAD_ARGUMENT, "k or v is NULL");
+  if (reinterpret_cast<uintptr_t>(k) % 16 != 0 || reinterpret_cast<uintptr_t>(v) % 16 != 0)
+    return fail(RBF_B200_ERR_BAD_LAYOUT, "k and v must be 16-byte aligned");
+  rbf::CacheReadArgs a{};
+  a.pages = static_cast<const uint8_t*>(pages); a.table = page_table; a.lengths = lengths; a.first = first; a.k = k; a.v = v;
+  a.B = B; a.H = H; a.D = D; a.count = count; a.max_pages = max_pages; a.num_pages = num_pages;
+  a.quads = static_cast<int>((static_cast<int64_t>(count) + 6) / 4);
+  if (static_cast<double>(B) * H * a.quads * (D / 4) / 256 >= 2147483646.0)
+    return fail(RBF_B200_ERR_BAD_ARGUMENT, "B * H * count is too large for one call");
+  const cudaError_t e = rbf::launch_cache_read(a, dtype == 0, static_cast<cudaStream_t>(stream_v));
+  if (e != cudaSuccess) return fail(RBF_B200_ERR_LAUNCH, "cache read launch failed: %s", cudaGetErrorString(e));
+  return RBF_B200_OK;
+}
+
+int rbf_b200_cache_copy_pages(void* pages, int layers, int num_pages, size_t page_bytes, const int* src, const int* dst,
+                              int count, void* stream_v) {
+  g_last_error[0] = 0;
+  if (layers < 0 || num_pages < 0 || count < 0 || page_bytes % 16 != 0)
+    return fail(RBF_B200_ERR_BAD_ARGUMENT, "layers, num_pages and count must be at least 0, page_bytes a multiple of 16");
+  if (count == 0) return RBF_B200_OK;
+  if (src == nullptr || dst == nullptr) return fail(RBF_B200_ERR_BAD_ARGUMENT, "src or dst is NULL");
+  for (int i = 0; i < count; ++i)
+    if (src[i] < 0 || src[i] >= num_pages || dst[i] < 0 || dst[i] >= num_pages)
+      return fail(RBF_B200_ERR_BAD_ARGUMENT, "page %d or %d is not in [0, %d)", src[i], dst[i], num_pages);
+  // 1: source, 2: destination
+  char* use = static_cast<char*>(calloc(num_pages, 1));
+  if (use == nullptr) return fail(RBF_B200_ERR_WORKSPACE, "no host memory for %d page marks", num_pages);
+  int twice = -1, both = -1;
+  for (int i = 0; i < count; ++i) use[src[i]] = 1;
+  for (int i = 0; i < count; ++i) {
+    if (use[dst[i]] == 1) both = dst[i];
+    if (use[dst[i]] == 2) twice = dst[i];
+    use[dst[i]] = 2;
+  }
+  free(use);
+  if (both >= 0) return fail(RBF_B200_ERR_BAD_ARGUMENT, "page %d is a source and a destination", both);
+  if (twice >= 0) return fail(RBF_B200_ERR_BAD_ARGUMENT, "page %d is a destination twice", twice);
+  if (layers == 0 || page_bytes == 0) return RBF_B200_OK;
+  if (pages == nullptr) return fail(RBF_B200_ERR_BAD_ARGUMENT, "pages is NULL");
+  if (reinterpret_cast<uintptr_t>(pages) % 16 != 0) return fail(RBF_B200_ERR_BAD_LAYOUT, "pages must be 16-byte aligned");
+  rbf::CacheCopyArgs a{};
+  a.pages = pages; a.num_pages = num_pages; a.words = static_cast<int64_t>(page_bytes / 16);
+  for (int i = 0; i < count; i += rbf::kMaxPagePairs) {
+    a.count = count - i < rbf::kMaxPagePairs ? count - i : rbf::kMaxPagePairs;
+    for (int j = 0; j < a.count; ++j) a.pair[j] = {src[i + j], dst[i + j]};
+    const cudaError_t e = rbf::launch_cache_copy(a, layers, static_cast<cudaStream_t>(stream_v));
+    if (e != cudaSuccess) return fail(RBF_B200_ERR_LAUNCH, "page copy launch failed: %s", cudaGetErrorString(e));
+  }
+  return RBF_B200_OK;
+}
+
+size_t rbf_b200_cache_attention_workspace_bytes(int T, int G, int D) {
+  const int sms = sm_count();
+  if (sms <= 0 || T < 0 || G <= 0 || D <= 0 || D > 128) return 0;
+  return rbf::cache_attn_workspace_bytes(T, G, D, sms);
+}
+
+int rbf_b200_cache_attention(const void* q, const int64_t* q_strides, const void* pages, const int* page_table,
+                             const int* lengths, const int* new_lengths, void* out, void* workspace, size_t workspace_bytes,
+                             int B, int H, int G, int T, int D, int max_pages, int num_pages, int dtype, int softmax,
+                             float gamma, void* stream_v) {
+  g_last_error[0] = 0;
+  int rc;
+  if ((rc = check_cache(pages, page_table, lengths, B, H, D, max_pages, num_pages, dtype))) return rc;
+  if (T < 0 || G <= 0) return fail(RBF_B200_ERR_BAD_ARGUMENT, "G must be positive, T at least 0");
+  if (!(gamma > 0.f)) return fail(RBF_B200_ERR_BAD_ARGUMENT, "gamma must be positive");
+  if (B == 0 || T == 0) return RBF_B200_OK;
+  if (static_cast<int64_t>(H) * G > 0x7fffffffll || static_cast<int64_t>(T) * G > 0x7fffff00ll)
+    return fail(RBF_B200_ERR_BAD_ARGUMENT, "too many query heads or tokens");
+  if ((rc = check_rows("q", q, q_strides, B, H * G, T))) return rc;
+  if (out == nullptr || reinterpret_cast<uintptr_t>(out) % 16 != 0)
+    return fail(RBF_B200_ERR_BAD_LAYOUT, "out is NULL or not 16-byte aligned");
+  const int sms = sm_count();
+  if (sms <= 0) return fail(RBF_B200_ERR_LAUNCH, "cannot read the SM count of the current device");
+  if (workspace == nullptr || reinterpret_cast<uintptr_t>(workspace) % 256 != 0 ||
+      workspace_bytes < rbf::cache_attn_workspace_bytes(T, G, D, sms))
+    return fail(RBF_B200_ERR_WORKSPACE, "workspace is NULL, not 256-byte aligned or smaller than %zu bytes",
+                rbf::cache_attn_workspace_bytes(T, G, D, sms));
+  rbf::CacheAttnArgs a{};
+  a.q = q; set_strides(a.qs, q_strides);
+  a.pages = static_cast<const uint8_t*>(pages); a.table = page_table; a.lengths = lengths; a.fresh = new_lengths;
+  a.out = out; a.parts = static_cast<float*>(workspace);
+  a.B = B; a.H = H; a.G = G; a.T = T; a.D = D; a.max_pages = max_pages; a.num_pages = num_pages;
+  a.softmax = softmax; a.scale = gamma * rbf::kLog2e;
+  const cudaError_t e = rbf::launch_cache_attn(a, dtype == 0, sms, static_cast<cudaStream_t>(stream_v));
+  if (e != cudaSuccess) return fail(RBF_B200_ERR_LAUNCH, "cache attention launch failed: %s", cudaGetErrorString(e));
+  return RBF_B200_OK;
+}
+
+// ---------------------------------------------------------------------------------------------
+// Log-probabilities of tokens and the policy loss
+// ---------------------------------------------------------------------------------------------
+static int check_logits(const void* logits, const int64_t* tokens, const float* log_probs, int64_t rows, int cols, int64_t ld,
+                        int dtype) {
+  if (rows < 0 || cols <= 0) return fail(RBF_B200_ERR_BAD_ARGUMENT, "rows must be >= 0 and cols > 0");
+  if (dtype < 0 || dtype > 2) return fail(RBF_B200_ERR_BAD_ARGUMENT, "dtype must be 0 (bf16), 1 (fp16) or 2 (fp32)");
+  if (ld < cols) return fail(RBF_B200_ERR_BAD_ARGUMENT, "the row pitch must be at least cols");
+  if (rows > 0 && (!logits || !tokens || !log_probs)) return fail(RBF_B200_ERR_BAD_ARGUMENT, "NULL tensor pointer");
+  if (reinterpret_cast<uintptr_t>(logits) % (dtype == 2 ? 4 : 2) != 0)
+    return fail(RBF_B200_ERR_BAD_LAYOUT, "logits are not aligned to their elements");
+  return RBF_B200_OK;
+}
+
+int rbf_b200_token_log_probs(const void* logits, const int64_t* tokens, float* log_probs, int64_t rows, int cols, int64_t ld,
+                             int64_t ignore_index, int dtype, void* stream_v) {
+  g_last_error[0] = 0;
+  int rc;
+  if ((rc = check_logits(logits, tokens, log_probs, rows, cols, ld, dtype))) return rc;
+  if (rows == 0) return RBF_B200_OK;
+  const int sms = sm_count();
+  if (sms <= 0) return fail(RBF_B200_ERR_LAUNCH, "cannot read the SM count of the current device");
+  rbf::PolicyArgs a{};
+  a.logits = logits; a.ld = ld; a.tokens = tokens; a.ignore_index = ignore_index; a.log_probs = log_probs;
+  a.rows = rows; a.cols = cols;
+  const cudaError_t e = rbf::launch_token_log_probs(a, dtype, sms, static_cast<cudaStream_t>(stream_v));
+  if (e != cudaSuccess) return fail(RBF_B200_ERR_LAUNCH, "log-probability launch failed: %s", cudaGetErrorString(e));
+  return RBF_B200_OK;
+}
+
+size_t rbf_b200_policy_loss_workspace_bytes(void) {
+  const int sms = sm_count();
+  return sms <= 0 ? 0 : static_cast<size_t>(rbf::policy_blocks(sms)) * (sizeof(double) + sizeof(int));
+}
+
+int rbf_b200_policy_loss(const void* logits, const int64_t* tokens, const float* old_log_probs, const float* advantages,
+                         const float* ref_log_probs, const float* weights, float* loss, float* log_probs, void* dlogits,
+                         void* workspace, size_t workspace_bytes, int64_t rows, int cols, int64_t ld, int64_t ld_out,
+                         int64_t ignore_index, float clip_low, float clip_high, float kl_weight, int dtype, void* stream_v) {
+  g_last_error[0] = 0;
+  int rc;
+  if ((rc = check_logits(logits, tokens, log_probs, rows, cols, ld, dtype))) return rc;
+  if (loss == nullptr || (rows > 0 && (!old_log_probs || !advantages)))
+    return fail(RBF_B200_ERR_BAD_ARGUMENT, "NULL tensor pointer");
+  if (!(clip_low >= 0.f) || !(clip_high >= 0.f)) return fail(RBF_B200_ERR_BAD_ARGUMENT, "clip_low and clip_high must be at least 0");
+  const int item = dtype == 2 ? 4 : 2;
+  if (dlogits != nullptr) {
+    if (ld_out < cols) return fail(RBF_B200_ERR_BAD_ARGUMENT, "the row pitches must be at least cols");
+    if ((reinterpret_cast<uintptr_t>(logits) - reinterpret_cast<uintptr_t>(dlogits)) % 16 != 0 ||
+        (rows > 1 && (ld - ld_out) * item % 16 != 0))
+      return fail(RBF_B200_ERR_BAD_LAYOUT, "the rows of dlogits must have the alignment of the logits' modulo 16 bytes");
+  }
+  const int sms = sm_count();
+  if (sms <= 0) return fail(RBF_B200_ERR_LAUNCH, "cannot read the SM count of the current device");
+  if (workspace == nullptr || reinterpret_cast<uintptr_t>(workspace) % 8 != 0 ||
+      workspace_bytes < rbf_b200_policy_loss_workspace_bytes())
+    return fail(RBF_B200_ERR_WORKSPACE, "workspace is NULL, not 8-byte aligned or too small");
+  rbf::PolicyArgs a{};
+  a.logits = logits; a.ld = ld; a.tokens = tokens; a.ignore_index = ignore_index; a.log_probs = log_probs;
+  a.rows = rows; a.cols = cols; a.dlogits = dlogits; a.ld_out = ld_out; a.old_log_probs = old_log_probs;
+  a.ref_log_probs = ref_log_probs; a.advantages = advantages; a.weights = weights; a.clip_low = clip_low;
+  a.clip_high = clip_high; a.kl_weight = kl_weight; a.loss = loss;
+  a.sums = static_cast<double*>(workspace); a.counts = reinterpret_cast<int*>(a.sums + rbf::policy_blocks(sms));
+  const cudaError_t e = rbf::launch_policy_loss(a, dtype, sms, static_cast<cudaStream_t>(stream_v));
+  if (e != cudaSuccess) return fail(RBF_B200_ERR_LAUNCH, "policy loss launch failed: %s", cudaGetErrorString(e));
   return RBF_B200_OK;
 }
 

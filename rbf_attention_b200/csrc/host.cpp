@@ -691,6 +691,261 @@ PyObject* layer_norm_bwd(const Args& a) {
   return tuple(wrap(dx), wrap(dgamma_out), wrap(dbeta_out));
 }
 
+// ------------------------------------------------------------------ the paged 8-bit cache
+// What every call on a cache gets: (pages, H, page bytes) uint8, (B, max_pages) and (B,) int32.
+struct Cache {
+  Tensor pages, table, lengths;
+  int64_t B, H, max_pages, num_pages;
+
+  Cache(const Args& a, Py_ssize_t i)
+      : pages(a.tensor(i, "pages")), table(a.tensor(i + 1, "page_table")), lengths(a.tensor(i + 2, "lengths")) {
+    TORCH_CHECK(pages.is_cuda(), "pages must be a CUDA tensor: rbf_attention_b200 has no CPU path");
+    TORCH_CHECK_VALUE(pages.dim() == 3 && pages.scalar_type() == at::kByte && pages.is_contiguous(),
+                      "pages must be a contiguous uint8 tensor (pages, heads, page bytes), got ", pages.scalar_type(), " ",
+                      pages.sizes());
+    TORCH_CHECK_VALUE(table.dim() == 2 && table.scalar_type() == at::kInt, "page_table must be int32 (B, max_pages), got ",
+                      table.scalar_type(), " ", table.sizes());
+    B = table.size(0);
+    max_pages = table.size(1);
+    num_pages = pages.size(0);
+    H = pages.size(1);
+    TORCH_CHECK_VALUE(H > 0 && num_pages <= 0x7fffffff && max_pages <= 0x7fffffff && B <= 0x7fffffff, "pages ", pages.sizes(),
+                      " with page_table ", table.sizes(), " is not supported");
+    per_sequence("lengths", lengths);
+    TORCH_CHECK_VALUE(table.device() == pages.device(), "page_table must be on the device of pages");
+  }
+  void per_sequence(const char* name, const Tensor& t) const {
+    TORCH_CHECK_VALUE(t.dim() == 1 && t.scalar_type() == at::kInt && t.size(0) == B, name, " must be int32 (", B, ",), got ",
+                      t.scalar_type(), " ", t.sizes());
+    TORCH_CHECK_VALUE(t.device() == pages.device(), name, " must be on the device of pages");
+  }
+  void head_dim(int64_t D) const {
+    TORCH_CHECK_VALUE(D > 0 && D <= 128 && D % 8 == 0, "head dim ", D, " is not supported (a multiple of 8 up to 128)");
+    TORCH_CHECK_VALUE(pages.size(2) == static_cast<int64_t>(rbf_b200_cache_page_bytes(D)), "pages of head dim ", D, " have ",
+                      rbf_b200_cache_page_bytes(D), " bytes per head, got ", pages.sizes());
+  }
+  // (B, heads, T, D), 16 bits
+  void rows(const char* name, const Tensor& t, int64_t heads_multiple) const {
+    TORCH_CHECK_VALUE(t.dim() == 4 && t.size(0) == B && t.size(1) > 0 && t.size(1) % heads_multiple == 0, name,
+                      " must have shape (", B, ", heads, T, D) with heads a multiple of ", heads_multiple, ", got ", t.sizes());
+    TORCH_CHECK_VALUE(is_16bit(t), "unsupported dtype ", t.scalar_type(), " (bfloat16 or float16)");
+    TORCH_CHECK_VALUE(t.device() == pages.device(), name, " must be on the device of pages");
+    TORCH_CHECK_VALUE(t.size(2) <= 0x7fffffff, name, " is too long");
+    head_dim(t.size(3));
+  }
+  void contiguous() {                              // on the device, without the interpreter's lock
+    table = table.contiguous();
+    lengths = lengths.contiguous();
+  }
+  const int* table_ptr() const { return table.const_data_ptr<int>(); }
+  const int* lengths_ptr() const { return lengths.const_data_ptr<int>(); }
+};
+
+const int* int_ptr(const Optional& t) { return t ? t->const_data_ptr<int>() : nullptr; }
+
+// (pages, page_table, lengths, k, v, new_lengths or None)
+PyObject* cache_append(const Args& a) {
+  a.expect(6);
+  Cache c(a, 0);
+  const Tensor k = a.tensor(3, "k"), v = a.tensor(4, "v");
+  Optional fresh = a.optional(5, "new_lengths");
+  c.rows("k", k, c.H);
+  c.rows("v", v, c.H);
+  TORCH_CHECK_VALUE(k.size(1) == c.H && v.sizes() == k.sizes() && v.scalar_type() == k.scalar_type(),
+                    "k and v must be of one type and shape with the ", c.H, " heads of the cache, got ", k.sizes(), " and ",
+                    v.sizes());
+  if (fresh) c.per_sequence("new_lengths", *fresh);
+  Unlocked unlocked;
+  const c10::cuda::CUDAGuard guard(c.pages.device());
+  c.contiguous();
+  if (fresh) fresh = fresh->contiguous();
+  const Tensor kc = tma_ready(k), vc = tma_ready(v);
+  const int rc = rbf_b200_cache_append(c.pages.data_ptr(), c.table_ptr(), c.lengths_ptr(), int_ptr(fresh), kc.const_data_ptr(),
+                                       vc.const_data_ptr(), strides3(kc), strides3(vc), c.B, c.H, k.size(2), k.size(3),
+                                       c.max_pages, c.num_pages, dtype_code(k.scalar_type()), stream_of(c.pages));
+  check(rc, "rbf_b200_cache_append");
+  unlocked.lock();
+  Py_RETURN_NONE;
+}
+
+// (pages, page_table, lengths, head dim, dtype code, count, first or None) -> (k, v)
+PyObject* cache_read(const Args& a) {
+  a.expect(7);
+  Cache c(a, 0);
+  const int64_t D = a.integer(3), code = a.integer(4), count = a.integer(5);
+  Optional first = a.optional(6, "first");
+  c.head_dim(D);
+  TORCH_CHECK_VALUE(code == 0 || code == 1, "unsupported dtype (bfloat16 or float16)");
+  TORCH_CHECK_VALUE(count >= 0 && count <= 0x7ffffff0, "count ", count, " is not supported");
+  if (first) c.per_sequence("first", *first);
+  Unlocked unlocked;
+  const c10::cuda::CUDAGuard guard(c.pages.device());
+  c.contiguous();
+  if (first) first = first->contiguous();
+  const at::ScalarType type = code == 0 ? at::kBFloat16 : at::kHalf;
+  const Tensor k = empty({c.B, c.H, count, D}, type, c.pages.device()), v = empty({c.B, c.H, count, D}, type, c.pages.device());
+  const int rc = rbf_b200_cache_read(c.pages.const_data_ptr(), c.table_ptr(), c.lengths_ptr(), int_ptr(first), k.data_ptr(),
+                                     v.data_ptr(), c.B, c.H, D, count, c.max_pages, c.num_pages, code, stream_of(c.pages));
+  check(rc, "rbf_b200_cache_read");
+  unlocked.lock();
+  return tuple(wrap(k), wrap(v));
+}
+
+std::vector<int> page_numbers(PyObject* sequence, const char* name) {
+  THPObjectPtr list(PySequence_Fast(sequence, "expected a sequence of page numbers"));
+  if (!list) throw python_error();
+  std::vector<int> out(PySequence_Fast_GET_SIZE(list.get()));
+  for (size_t i = 0; i < out.size(); ++i) {
+    const long long x = PyLong_AsLongLong(PySequence_Fast_GET_ITEM(list.get(), static_cast<Py_ssize_t>(i)));
+    if (x == -1 && PyErr_Occurred()) throw python_error();
+    TORCH_CHECK_VALUE(x >= 0 && x <= 0x7fffffff, name, ": page ", x, " is not in the cache");
+    out[i] = static_cast<int>(x);
+  }
+  return out;
+}
+
+// (pages, source pages, destination pages)
+PyObject* cache_copy_pages(const Args& a) {
+  a.expect(3);
+  const Tensor pages = a.tensor(0, "pages");
+  TORCH_CHECK(pages.is_cuda(), "pages must be a CUDA tensor: rbf_attention_b200 has no CPU path");
+  TORCH_CHECK_VALUE((pages.dim() == 3 || pages.dim() == 4) && pages.scalar_type() == at::kByte && pages.is_contiguous(),
+                    "pages must be a contiguous uint8 tensor ([layers,] pages, heads, page bytes), got ", pages.scalar_type(),
+                    " ", pages.sizes());
+  const std::vector<int> src = page_numbers(a.v[1], "src"), dst = page_numbers(a.v[2], "dst");
+  TORCH_CHECK_VALUE(src.size() == dst.size(), "src and dst must be of one length, got ", src.size(), " and ", dst.size());
+  const int64_t layers = pages.dim() == 4 ? pages.size(0) : 1, num_pages = pages.size(-3);
+  TORCH_CHECK_VALUE(layers <= 0x7fffffff && num_pages <= 0x7fffffff && src.size() <= 0x7fffffff, "too many pages");
+  Unlocked unlocked;
+  const c10::cuda::CUDAGuard guard(pages.device());
+  const int rc = rbf_b200_cache_copy_pages(pages.data_ptr(), layers, num_pages, pages.size(-2) * pages.size(-1), src.data(),
+                                           dst.data(), static_cast<int>(src.size()), stream_of(pages));
+  check(rc, "rbf_b200_cache_copy_pages");
+  unlocked.lock();
+  Py_RETURN_NONE;
+}
+
+// (q, pages, page_table, lengths, new_lengths or None, softmax) -> out
+PyObject* cache_attention(const Args& a) {
+  a.expect(6);
+  const Tensor q = a.tensor(0, "q");
+  Cache c(a, 1);
+  Optional fresh = a.optional(4, "new_lengths");
+  const bool softmax = a.flag(5);
+  c.rows("q", q, c.H);
+  if (fresh) c.per_sequence("new_lengths", *fresh);
+  const int64_t Hq = q.size(1), T = q.size(2), D = q.size(3), G = Hq / c.H;
+  Unlocked unlocked;
+  const c10::cuda::CUDAGuard guard(c.pages.device());
+  c.contiguous();
+  if (fresh) fresh = fresh->contiguous();
+  const Tensor qc = tma_ready(q);
+  const Tensor out = empty({c.B, Hq, T, D}, q.scalar_type(), q.device());
+  const Tensor ws = workspace(rbf_b200_cache_attention_workspace_bytes(T, G, D), q.device());
+  const float gamma = static_cast<float>(1.0 / std::sqrt(static_cast<double>(D)));
+  const int rc = rbf_b200_cache_attention(qc.const_data_ptr(), strides3(qc), c.pages.const_data_ptr(), c.table_ptr(),
+                                          c.lengths_ptr(), int_ptr(fresh), out.data_ptr(), ws.data_ptr(), ws.nbytes(), c.B,
+                                          c.H, G, T, D, c.max_pages, c.num_pages, dtype_code(q.scalar_type()), softmax, gamma,
+                                          stream_of(q));
+  check(rc, "rbf_b200_cache_attention");
+  unlocked.lock();
+  return wrap(out);
+}
+
+// ------------------------------------------------------------------ log-probabilities and the policy loss
+// (rows, cols) logits and their tokens; rows with unit stride on the columns
+struct Logits {
+  Tensor x, tokens;
+  int64_t rows, cols;
+  int code;
+
+  Logits(const Args& a, Py_ssize_t i) : x(a.tensor(i, "logits")), tokens(a.tensor(i + 1, "tokens")) {
+    TORCH_CHECK(x.is_cuda(), "logits must be a CUDA tensor: rbf_attention_b200 has no CPU path");
+    TORCH_CHECK_VALUE(x.dim() == 2 && tokens.dim() == 1 && tokens.size(0) == x.size(0),
+                      "logits must be (rows, cols) and tokens (rows,), got ", x.sizes(), " and ", tokens.sizes());
+    TORCH_CHECK_VALUE(dtype_code(x.scalar_type()) >= 0, "unsupported dtype ", x.scalar_type(),
+                      " (bfloat16, float16 or float32)");
+    TORCH_CHECK_VALUE(tokens.scalar_type() == at::kLong, "tokens must be int64, got ", tokens.scalar_type());
+    TORCH_CHECK_VALUE(tokens.device() == x.device(), "logits and tokens must be on one device");
+    TORCH_CHECK_VALUE(x.size(1) > 0 && x.size(1) <= 0x7fffffff, "logits must have columns, got ", x.sizes());
+    rows = x.size(0);
+    cols = x.size(1);
+    code = dtype_code(x.scalar_type());
+  }
+  void contiguous() {
+    tokens = tokens.contiguous();
+    if (x.stride(1) != 1 && cols > 1 || rows > 1 && x.stride(0) < cols) x = x.contiguous();
+  }
+  int64_t pitch() const { return rows > 1 ? x.stride(0) : cols; }
+  // fp32 per row, on the device
+  Optional per_row(const char* name, Optional t) const {
+    if (!t) return t;
+    TORCH_CHECK_VALUE(t->dim() == 1 && t->size(0) == rows && t->scalar_type() == at::kFloat && t->device() == x.device(), name,
+                      " must be float32 (", rows, ",) on the device of logits, got ", t->scalar_type(), " ", t->sizes());
+    return t;
+  }
+};
+
+const float* float_ptr(const Optional& t) { return t ? t->const_data_ptr<float>() : nullptr; }
+
+// (logits, tokens, ignore_index) -> log_probs
+PyObject* token_log_probs(const Args& a) {
+  a.expect(3);
+  Logits in(a, 0);
+  const int64_t ignore = a.integer(2);
+  Unlocked unlocked;
+  const c10::cuda::CUDAGuard guard(in.x.device());
+  in.contiguous();
+  const Tensor out = empty({in.rows}, at::kFloat, in.x.device());
+  const int rc = rbf_b200_token_log_probs(in.x.const_data_ptr(), in.tokens.const_data_ptr<int64_t>(), out.data_ptr<float>(),
+                                          in.rows, in.cols, in.pitch(), ignore, in.code, stream_of(in.x));
+  check(rc, "rbf_b200_token_log_probs");
+  unlocked.lock();
+  return wrap(out);
+}
+
+// (logits, tokens, old_log_probs, advantages, ref_log_probs or None, weights or None, clip_low, clip_high, kl_weight,
+// ignore_index, whether the gradient is wanted) -> (loss, log_probs, dlogits or None): dlogits has the shape of logits and the
+// logits' alignment, its memory may be longer than they are.
+PyObject* policy_loss(const Args& a) {
+  a.expect(11);
+  Logits in(a, 0);
+  Optional old = in.per_row("old_log_probs", a.tensor(2, "old_log_probs"));
+  Optional advantages = in.per_row("advantages", a.tensor(3, "advantages"));
+  Optional ref = in.per_row("ref_log_probs", a.optional(4, "ref_log_probs"));
+  Optional weights = in.per_row("weights", a.optional(5, "weights"));
+  const float low = static_cast<float>(a.number(6)), high = static_cast<float>(a.number(7)),
+              kl = static_cast<float>(a.number(8));
+  const int64_t ignore = a.integer(9);
+  const bool want_grad = a.flag(10);
+  Unlocked unlocked;
+  const at::Device dev = in.x.device();
+  const c10::cuda::CUDAGuard guard(dev);
+  in.contiguous();
+  for (Optional* t : {&old, &advantages, &ref, &weights})
+    if (*t) *t = (*t)->contiguous();
+  const Tensor loss = empty({}, at::kFloat, dev), log_probs = empty({in.rows}, at::kFloat, dev);
+  Optional grad;
+  int64_t pitch = in.cols;
+  if (want_grad) {
+    // the same place within 16 bytes for every row of the two
+    const int64_t per16 = 16 / static_cast<int64_t>(in.x.element_size());
+    pitch = in.cols + (in.pitch() - in.cols) % per16;
+    const int64_t shift = reinterpret_cast<uintptr_t>(in.x.const_data_ptr()) % 16 / in.x.element_size();
+    const Tensor memory = empty({shift + in.rows * pitch}, in.x.scalar_type(), dev);
+    grad = memory.as_strided({in.rows, in.cols}, {pitch, 1}, shift);
+  }
+  const Tensor ws = workspace(rbf_b200_policy_loss_workspace_bytes(), dev);
+  const int rc = rbf_b200_policy_loss(in.x.const_data_ptr(), in.tokens.const_data_ptr<int64_t>(), float_ptr(old),
+                                      float_ptr(advantages), float_ptr(ref), float_ptr(weights), loss.data_ptr<float>(),
+                                      log_probs.data_ptr<float>(), grad ? grad->data_ptr() : nullptr, ws.data_ptr(),
+                                      ws.nbytes(), in.rows, in.cols, in.pitch(), pitch, ignore, low, high, kl, in.code,
+                                      stream_of(in.x));
+  check(rc, "rbf_b200_policy_loss");
+  unlocked.lock();
+  return tuple(wrap(loss), wrap(log_probs), wrap(grad));
+}
+
 // (device index) -> whether the current stream of that device, which is the one that a call on its tensors uses, is being
 // captured into a graph. (The question without a device is answered for the thread's current one.)
 PyObject* capturing(const Args& a) {
@@ -722,6 +977,9 @@ PyMethodDef methods[] = {
     method<gelu_bwd>("gelu_bwd"),             method<layer_norm_fwd>("layer_norm_fwd"),
     method<layer_norm_bwd>("layer_norm_bwd"), method<capturing>("capturing"),
     method<validate_entry>("validate"),       method<tma_ready_entry>("tma_ready"),
+    method<cache_append>("cache_append"),     method<cache_read>("cache_read"),
+    method<cache_copy_pages>("cache_copy_pages"), method<cache_attention>("cache_attention"),
+    method<token_log_probs>("token_log_probs"), method<policy_loss>("policy_loss"),
     {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

@@ -181,6 +181,86 @@ cudaError_t launch_cross_entropy(const CrossEntropyArgs& a, int dtype, int sms, 
 // x *= *factor unless *factor == 1 (decided on the device: nothing synchronises).
 cudaError_t launch_scale_unless_one(void* x, const float* factor, int64_t n, int dtype, int sms, cudaStream_t stream);
 
+// Tokens into the paged 8-bit cache (cache.cuh): k and v (B, H, T, D) through strides (elements, dims b, h, n), D a multiple of
+// 8 up to 128. Sequence b has lengths[b] tokens in the cache, the call adds the first fresh[b] (NULL: T) of its T.
+struct CacheAppendArgs {
+  const void* k;
+  const void* v;
+  int64_t ks[3], vs[3];
+  uint8_t* pages;            // (num_pages, H, page bytes)
+  const int* table;          // (B, max_pages) page numbers
+  const int* lengths;        // (B)
+  const int* fresh;          // (B) or NULL
+  int B, H, T, D, max_pages, num_pages;
+  int blocks;                // blocks of 16 tokens that T tokens can touch
+};
+cudaError_t launch_cache_append(const CacheAppendArgs& a, bool bf16, cudaStream_t stream);
+// Tokens [first[b], first[b] + count) of every sequence as 16-bit k and v (B, H, count, D), zeros from lengths[b] on.
+struct CacheReadArgs {
+  const uint8_t* pages;
+  const int* table;
+  const int* lengths;
+  const int* first;          // (B) or NULL: 0
+  void* k;
+  void* v;
+  int B, H, D, count, max_pages, num_pages;
+  int quads;                 // groups of four tokens that the range can touch
+};
+cudaError_t launch_cache_read(const CacheReadArgs& a, bool bf16, cudaStream_t stream);
+// pages[layer][dst] = pages[layer][src] for a list of pairs, in all layers; the pairs travel as kernel parameters.
+static constexpr int kMaxPagePairs = 480;
+struct CacheCopyArgs {
+  void* pages;               // (layers, num_pages, 16 * words bytes)
+  int64_t num_pages, words;
+  int count, chunks;         // chunks: set by the launcher
+  struct { int src, dst; } pair[kMaxPagePairs];
+};
+cudaError_t launch_cache_copy(CacheCopyArgs a, int layers, cudaStream_t stream);
+// RBF attention over that cache: q (B, H * G, T, D) through strides, out (B, H * G, T, D) dense; query head h reads head h / G.
+struct CacheAttnArgs {
+  const void* q;
+  int64_t qs[3];
+  const uint8_t* pages;
+  const int* table;
+  const int* lengths;        // tokens before the T new ones, which are in the cache too
+  const int* fresh;          // (B) or NULL: T
+  void* out;
+  float* parts;              // cache_attn_workspace_bytes()
+  int B, H, G, T, D, max_pages, num_pages;
+  int softmax;
+  float scale;               // log2(e) / sqrt(head dim)
+  int column_tiles;          // set by the launcher
+};
+int cache_attn_tiles(int T, int G, int P);
+size_t cache_attn_workspace_bytes(int T, int G, int D, int sms);
+cudaError_t launch_cache_attn(CacheAttnArgs a, bool bf16, int sms, cudaStream_t stream);
+
+// Log-probabilities of given tokens, and the clipped policy loss with its gradient (policy_loss.cu).
+struct PolicyArgs {
+  const void* logits;        // (rows, cols), row pitch ld elements
+  int64_t ld;
+  const int64_t* tokens;     // (rows); ignore_index or out of range: the row has no log-probability, no loss, a zero gradient
+  int64_t ignore_index;
+  float* log_probs;          // (rows)
+  int64_t rows;
+  int cols;
+  // the loss only
+  void* dlogits;             // (rows, cols), row pitch ld_out, or NULL
+  int64_t ld_out;
+  const float* old_log_probs;
+  const float* ref_log_probs;  // or NULL: no KL term
+  const float* advantages;
+  const float* weights;      // (rows) or NULL: 1 / number of rows that count
+  float clip_low, clip_high, kl_weight;
+  float* loss;               // one number
+  double* sums;              // policy_blocks() numbers
+  int* counts;               // as many again
+  int count_blocks;          // set by the launcher
+};
+int policy_blocks(int sms);
+cudaError_t launch_token_log_probs(const PolicyArgs& a, int dtype, int sms, cudaStream_t stream);
+cudaError_t launch_policy_loss(const PolicyArgs& a, int dtype, int sms, cudaStream_t stream);
+
 cudaError_t launch_wait_selftest(DeviceStatus* status, long long limit, cudaStream_t stream);
 // One thread stores the status word into mapped page-locked host memory (device-side address of the slot).
 cudaError_t launch_post_status(const DeviceStatus* status, unsigned int* host_slot_device_ptr, cudaStream_t stream);

@@ -1,0 +1,363 @@
+// Log-probabilities of given tokens and the clipped policy loss with a KL term, for fine-tuning the language model on rewards:
+//   lp = z[t] - lse(z),  r = e^(lp - old),  gain = min(r A, clip(r, 1 - low, 1 + high) A),
+//   kl = e^(ref - lp) - (ref - lp) - 1,     loss = sum over rows of w (kl_weight kl - gain)
+//   d loss / d lp = w (kl_weight (1 - e^(ref - lp)) - [r A <= clipped] r A) = c,   d loss / d z = c (onehot(t) - softmax(z))
+// Everything but the row's lse is a handful of scalars per row, so the gradient is known as soon as the row has been read once:
+// one kernel reads the logits and writes the gradient of the loss, as the cross entropy does. Roofline: HBM. A block owns a
+// row, reads it with an online maximum and sum and keeps it in shared memory where two blocks' rows fit an SM; longer rows come
+// a second time out of L2. The rows' bases may have any alignment: a row is a head of single elements up to the first 16-byte
+// boundary, 16-byte words, and a tail. Sums over rows are in 64 bits and in the order of the rows of a block, then of the blocks.
+#include <cstdint>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include "launch.h"
+
+namespace rbf {
+namespace {
+
+constexpr int kThreads = 512;
+constexpr int kRowsPerSm = 2;                       // blocks of the loss kernel
+constexpr int kStageBytes = 113 * 1024;             // a staged row leaves room for a second block on the SM
+constexpr float kLn2 = 0.6931471805599453f;
+
+__device__ __forceinline__ float pl_ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+template <int kDtype> struct Number;                // 0 bfloat16, 1 float16, 2 float32
+template <> struct Number<0> {
+  using type = uint16_t;
+  static __device__ __forceinline__ float widen(uint16_t x) { return __uint_as_float(static_cast<uint32_t>(x) << 16); }
+  static __device__ __forceinline__ uint16_t narrow(float x) { return __bfloat16_as_ushort(__float2bfloat16_rn(x)); }
+};
+template <> struct Number<1> {
+  using type = uint16_t;
+  static __device__ __forceinline__ float widen(uint16_t x) { return __half2float(__ushort_as_half(x)); }
+  static __device__ __forceinline__ uint16_t narrow(float x) { return __half_as_ushort(__float2half_rn(x)); }
+};
+template <> struct Number<2> {
+  using type = float;
+  static __device__ __forceinline__ float widen(float x) { return x; }
+  static __device__ __forceinline__ float narrow(float x) { return x; }
+};
+
+// The numbers of a 16-byte word
+template <int kDtype>
+__device__ __forceinline__ void widen16(const uint4& raw, float (&x)[kDtype == 2 ? 4 : 8]) {
+  const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (kDtype == 2) {
+      x[i] = __uint_as_float(w[i]);
+    } else {
+      const float2 f = unpack2<kDtype == 0>(w[i]);
+      x[2 * i] = f.x;
+      x[2 * i + 1] = f.y;
+    }
+  }
+}
+
+// sum of 2^(y - m) over values y = x * log2(e); m = -inf and s = 0 before any of them is above -inf
+struct Online {
+  float m = -INFINITY, s = 0.f;
+  __device__ __forceinline__ void merge(float m2, float s2) {
+    const float top = fmaxf(m, m2);
+    if (top == -INFINITY) {                         // nothing above -inf yet; a NaN has to stay
+      s += s2;
+      return;
+    }
+    s = s * pl_ex2(m - top) + s2 * pl_ex2(m2 - top);
+    m = top;
+  }
+  template <int kCount>
+  __device__ __forceinline__ void add(const float (&x)[kCount]) {
+    float top = x[0];
+#pragma unroll
+    for (int i = 1; i < kCount; ++i) top = fmaxf(top, x[i]);
+    top *= kLog2e;
+    if (top > m) {
+      s *= pl_ex2(m - top);
+      m = top;
+    }
+    const float neg = m == -INFINITY ? 0.f : -m;    // 2^-inf is zero, 2^NaN is NaN
+    float s0 = 0.f, s1 = 0.f;
+#pragma unroll
+    for (int i = 0; i + 1 < kCount; i += 2) {
+      float y0, y1;
+      ffma2_bcast(y0, y1, x[i], x[i + 1], kLog2e, neg);
+      fadd2(s0, s1, s0, s1, pl_ex2(y0), pl_ex2(y1));
+    }
+    if constexpr (kCount % 2) s0 += pl_ex2(fmaf(x[kCount - 1], kLog2e, neg));
+    s += s0 + s1;
+  }
+};
+
+// Where a row's 16-byte words are: elements [0, head) and [body, cols) are single ones
+template <typename T>
+struct Cut {
+  static constexpr int kPer = 16 / sizeof(T);
+  int head, words, body;
+  __device__ Cut(const T* row, int cols) {
+    const int off = static_cast<int>(reinterpret_cast<uintptr_t>(row) / sizeof(T) % kPer);
+    head = min(cols, off == 0 ? 0 : kPer - off);
+    words = (cols - head) / kPer;
+    body = head + words * kPer;
+  }
+};
+
+// The row's maximum and sum, by all threads of the block; on return thread 0 (and every thread of warp 0) has them.
+template <int kDtype, bool kStage>
+__device__ __forceinline__ Online row_sum(const typename Number<kDtype>::type* x, int cols, uint4* stage) {
+  using T = typename Number<kDtype>::type;
+  __shared__ float s_m[kThreads / 32], s_s[kThreads / 32];
+  const Cut<T> cut(x, cols);
+  const uint4* words = reinterpret_cast<const uint4*>(x + cut.head);
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  Online sum;
+#pragma unroll 4
+  for (int c = tid; c < cut.words; c += kThreads) {
+    const uint4 raw = kStage ? __ldcs(words + c) : words[c];
+    if constexpr (kStage) stage[c] = raw;
+    float v[Cut<T>::kPer];
+    widen16<kDtype>(raw, v);
+    sum.add(v);
+  }
+  const int single = tid < cut.head ? tid : cut.body + tid - cut.head;
+  if (tid < cut.head + cols - cut.body) {
+    const float v[1] = {Number<kDtype>::widen(x[single])};
+    sum.add(v);
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1)
+    sum.merge(__shfl_xor_sync(0xffffffffu, sum.m, o), __shfl_xor_sync(0xffffffffu, sum.s, o));
+  if (lane == 0) {
+    s_m[warp] = sum.m;
+    s_s[warp] = sum.s;
+  }
+  __syncthreads();
+  if (warp == 0) {
+    sum.m = lane < kThreads / 32 ? s_m[lane] : -INFINITY;
+    sum.s = lane < kThreads / 32 ? s_s[lane] : 0.f;
+#pragma unroll
+    for (int o = kThreads / 64; o > 0; o >>= 1)
+      sum.merge(__shfl_xor_sync(0xffffffffu, sum.m, o), __shfl_xor_sync(0xffffffffu, sum.s, o));
+  }
+  return sum;
+}
+
+__device__ __forceinline__ bool counts(const PolicyArgs& a, int64_t token) {
+  return token != a.ignore_index && token >= 0 && token < a.cols;
+}
+
+template <int kDtype>
+__global__ void __launch_bounds__(kThreads) token_log_probs_kernel(const PolicyArgs a) {
+  using N = Number<kDtype>;
+  using T = typename N::type;
+  for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+    const int64_t token = a.tokens[row];
+    if (!counts(a, token)) {
+      if (threadIdx.x == 0) a.log_probs[row] = 0.f;
+      continue;
+    }
+    const T* x = static_cast<const T*>(a.logits) + row * a.ld;
+    const Online sum = row_sum<kDtype, false>(x, a.cols, nullptr);
+    if (threadIdx.x == 0) a.log_probs[row] = (fmaf(N::widen(x[token]), kLog2e, -sum.m) - log2f(sum.s)) * kLn2;
+    __syncthreads();                                // the warps' slots are used again
+  }
+}
+
+// How many rows count: one number per block
+__global__ void __launch_bounds__(kThreads) policy_count_kernel(const PolicyArgs a) {
+  grid_dependents_launch();
+  __shared__ int s_n[kThreads / 32];
+  int n = 0;
+  for (int64_t r = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x; r < a.rows; r += static_cast<int64_t>(gridDim.x) * kThreads)
+    n += counts(a, a.tokens[r]);
+  n = __reduce_add_sync(0xffffffffu, n);
+  if ((threadIdx.x & 31) == 0) s_n[threadIdx.x >> 5] = n;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int w = 1; w < kThreads / 32; ++w) n += s_n[w];
+    a.counts[blockIdx.x] = n;
+  }
+}
+
+template <int kDtype, bool kStage>
+__global__ void __launch_bounds__(kThreads, kRowsPerSm) policy_loss_kernel(const PolicyArgs a) {
+  using N = Number<kDtype>;
+  using T = typename N::type;
+  constexpr int V = Cut<T>::kPer;
+  extern __shared__ uint4 s_row[];                  // kStage: the row's words, each kept by the thread that read it
+  __shared__ float s_shift, s_slope;
+  __shared__ int s_count;
+  const int tid = threadIdx.x;
+  grid_dependency_wait();
+  if (a.weights == nullptr) {
+    if (tid < 32) {
+      int n = 0;
+      for (int i = tid; i < a.count_blocks; i += 32) n += a.counts[i];
+      n = __reduce_add_sync(0xffffffffu, n);
+      if (tid == 0) s_count = n;
+    }
+    __syncthreads();
+  }
+  double loss = 0.0;                                // of this block's rows, thread 0
+  for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+    const T* x = static_cast<const T*>(a.logits) + row * a.ld;
+    T* dx = static_cast<T*>(a.dlogits) + row * a.ld_out;
+    const Cut<T> cut(x, a.cols);
+    const int64_t token = a.tokens[row];
+    const bool counted = counts(a, token);
+    if (counted) {
+      const Online sum = row_sum<kDtype, kStage>(x, a.cols, s_row);
+      if (tid == 0) {
+        const float lse2 = log2f(sum.s), lp = (fmaf(N::widen(x[token]), kLog2e, -sum.m) - lse2) * kLn2;
+        const float A = a.advantages[row], r = expf(lp - a.old_log_probs[row]);
+        const float plain = r * A, clipped = fminf(fmaxf(r, 1.f - a.clip_low), 1.f + a.clip_high) * A;
+        const float w = a.weights != nullptr ? a.weights[row] : 1.f / static_cast<float>(s_count);
+        float value = -fminf(plain, clipped), slope = plain <= clipped ? -plain : 0.f;
+        if (plain != plain) value = slope = plain;  // fminf would pass over it
+        if (a.ref_log_probs != nullptr) {
+          const float gap = a.ref_log_probs[row] - lp, away = expf(gap);
+          value = fmaf(a.kl_weight, away - gap - 1.f, value);
+          slope = fmaf(a.kl_weight, 1.f - away, slope);
+        }
+        a.log_probs[row] = lp;
+        loss += static_cast<double>(w) * static_cast<double>(value);
+        s_slope = w * slope;
+        s_shift = -(sum.m + lse2);
+      }
+    } else if (tid == 0) {
+      a.log_probs[row] = 0.f;
+    }
+    if (a.dlogits == nullptr) {
+      __syncthreads();                              // the warps' slots are used again
+      continue;
+    }
+    uint4* out = reinterpret_cast<uint4*>(dx + cut.head);
+    const int single = tid < cut.head ? tid : cut.body + tid - cut.head;
+    const bool has_single = tid < cut.head + a.cols - cut.body;
+    if (!counted) {
+      for (int c = tid; c < cut.words; c += kThreads) out[c] = make_uint4(0, 0, 0, 0);
+      if (has_single) dx[single] = N::narrow(0.f);
+      continue;
+    }
+    __syncthreads();
+    const float shift = s_shift, slope = s_slope;
+    const int at = static_cast<int>(token) - cut.head, word = at >= 0 ? at / V : -1, in_word = at >= 0 ? at % V : 0;
+    const uint4* words = reinterpret_cast<const uint4*>(x + cut.head);
+#pragma unroll 2
+    for (int c = tid; c < cut.words; c += kThreads) {
+      uint4 raw;
+      if constexpr (kStage) raw = s_row[c];
+      else raw = words[c];
+      float v[V];
+      widen16<kDtype>(raw, v);
+#pragma unroll
+      for (int i = 0; i < V; i += 2) {
+        float y0, y1;
+        ffma2_bcast(y0, y1, v[i], v[i + 1], kLog2e, shift);
+        fmul2(v[i], v[i + 1], pl_ex2(y0), pl_ex2(y1), -slope, -slope);
+      }
+      if (c == word) {
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+          if (i == in_word) v[i] += slope;
+      }
+      uint4 y;
+      if constexpr (kDtype == 2) {
+        y = make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
+      } else {
+        constexpr bool kBf16 = kDtype == 0;
+        y = make_uint4(pack2<kBf16>(v[0], v[1]), pack2<kBf16>(v[2], v[3]), pack2<kBf16>(v[4 % V], v[5 % V]),
+                       pack2<kBf16>(v[6 % V], v[7 % V]));
+      }
+      __stcs(out + c, y);
+    }
+    if (has_single) {
+      float v = -slope * pl_ex2(fmaf(N::widen(x[single]), kLog2e, shift));
+      if (single == token) v += slope;
+      dx[single] = N::narrow(v);
+    }
+    __syncthreads();                                // s_shift, s_slope and the warps' slots are used again
+  }
+  if (tid == 0) a.sums[blockIdx.x] = loss;
+  grid_dependents_launch();
+}
+
+// The blocks' sums in their order
+__global__ void __launch_bounds__(32) policy_finish_kernel(const PolicyArgs a, const int blocks) {
+  grid_dependency_wait();
+  double sum = 0.0;
+  for (int i = threadIdx.x; i < blocks; i += 32) sum += a.sums[i];
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  if (threadIdx.x != 0) return;
+  if (a.weights == nullptr) {                       // no row that counts: the mean of nothing
+    int n = 0;
+    for (int i = 0; i < a.count_blocks; ++i) n += a.counts[i];
+    if (n == 0) sum = __longlong_as_double(0x7ff8000000000000ll);
+  }
+  *a.loss = static_cast<float>(sum);
+}
+
+template <int kDtype>
+cudaError_t log_probs_t(const PolicyArgs& a, int sms, cudaStream_t stream) {
+  const int64_t most = static_cast<int64_t>(sms) * 4;
+  token_log_probs_kernel<kDtype><<<static_cast<unsigned>(a.rows < most ? a.rows : most), kThreads, 0, stream>>>(a);
+  return cudaGetLastError();
+}
+
+template <int kDtype>
+cudaError_t policy_t(PolicyArgs a, int sms, cudaStream_t stream) {
+  using T = typename Number<kDtype>::type;
+  const int64_t most = policy_blocks(sms);
+  const int blocks = a.rows == 0 ? 1 : static_cast<int>(a.rows < most ? a.rows : most);
+  const int64_t wanted = (a.rows + kThreads - 1) / kThreads;
+  a.count_blocks = wanted == 0 ? 1 : static_cast<int>(wanted < sms ? wanted : sms);
+  if (a.weights == nullptr) {
+    policy_count_kernel<<<a.count_blocks, kThreads, 0, stream>>>(a);
+    const cudaError_t e = cudaGetLastError();
+    if (e != cudaSuccess) return e;
+  }
+  const int64_t row_bytes = (static_cast<int64_t>(a.cols) * sizeof(T) + 15) / 16 * 16;
+  cudaError_t e;
+  if (a.dlogits != nullptr && row_bytes <= kStageBytes) {
+    static PerDeviceFlags flags;
+    if ((e = ensure_dynamic_smem(policy_loss_kernel<kDtype, true>, kStageBytes, flags)) != cudaSuccess) return e;
+    e = launch_dependent(policy_loss_kernel<kDtype, true>, dim3(blocks), kThreads, row_bytes, stream, a);
+  } else {
+    e = launch_dependent(policy_loss_kernel<kDtype, false>, dim3(blocks), kThreads, 0, stream, a);
+  }
+  if (e != cudaSuccess) return e;
+  return launch_dependent(policy_finish_kernel, dim3(1), 32, 0, stream, a, blocks);
+}
+
+}  // namespace
+
+int policy_blocks(int sms) { return sms * kRowsPerSm; }
+
+cudaError_t launch_token_log_probs(const PolicyArgs& a, int dtype, int sms, cudaStream_t stream) {
+  if (a.rows == 0) return cudaSuccess;
+  switch (dtype) {
+    case 0: return log_probs_t<0>(a, sms, stream);
+    case 1: return log_probs_t<1>(a, sms, stream);
+    case 2: return log_probs_t<2>(a, sms, stream);
+    default: return cudaErrorInvalidValue;
+  }
+}
+
+cudaError_t launch_policy_loss(const PolicyArgs& a, int dtype, int sms, cudaStream_t stream) {
+  switch (dtype) {
+    case 0: return policy_t<0>(a, sms, stream);
+    case 1: return policy_t<1>(a, sms, stream);
+    case 2: return policy_t<2>(a, sms, stream);
+    default: return cudaErrorInvalidValue;
+  }
+}
+
+}  // namespace rbf

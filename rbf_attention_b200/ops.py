@@ -1072,6 +1072,248 @@ def cross_entropy(logits, targets, ignore_index: int = -100):
 
 
 # ---------------------------------------------------------------------------------------------
+# Log-probabilities of given tokens and the clipped policy loss with a KL term (no counterpart in the reference): fine-tuning
+# of the language model on rewards
+# ---------------------------------------------------------------------------------------------
+def _token_log_probs(logits: torch.Tensor, tokens: torch.Tensor, ignore_index: int) -> torch.Tensor:
+    return _lib.host().token_log_probs(logits, tokens, ignore_index)
+
+
+token_log_probs_fwd = torch.library.custom_op("rbf_attn_b200::token_log_probs", mutates_args=())(_token_log_probs)
+
+
+@token_log_probs_fwd.register_fake
+def _(logits, tokens, ignore_index):
+    return logits.new_empty(logits.shape[0], dtype=torch.float32)
+
+
+def token_log_probs(logits, tokens, ignore_index: int = -100):
+    """``log_softmax(logits)[r, tokens[r]]`` in fp32 for 2-D CUDA logits and int64 tokens, 0 where the token is
+    ``ignore_index`` or no column. Without a backward (``policy_loss`` has one): what a policy loss takes as old and reference
+    values. Logits that require a gradient are refused in grad mode."""
+    if _needs_grad(logits):
+        raise RuntimeError("token_log_probs has no backward: call it under torch.no_grad() or on detached logits")
+    if type(ignore_index) is int and _direct(logits, tokens):
+        return _token_log_probs(logits, tokens, ignore_index)
+    return torch.ops.rbf_attn_b200.token_log_probs(logits, tokens, ignore_index)
+
+
+def _policy_loss_fwd(logits: torch.Tensor, tokens: torch.Tensor, old_log_probs: torch.Tensor, advantages: torch.Tensor,
+                     ref_log_probs: torch.Tensor | None, weights: torch.Tensor | None, clip_low: float, clip_high: float,
+                     kl_weight: float, ignore_index: int,
+                     with_grad: bool) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """(loss, log_probs, d(loss)/d(logits)) from one pass over the logits; without the gradient an empty tensor for it."""
+    loss, log_probs, dlogits = _lib.host().policy_loss(logits, tokens, old_log_probs, advantages, ref_log_probs, weights,
+                                                       clip_low, clip_high, kl_weight, ignore_index, with_grad)
+    return loss, log_probs, logits.new_empty(0) if dlogits is None else dlogits
+
+
+policy_loss_fwd = torch.library.custom_op("rbf_attn_b200::policy_loss_fwd", mutates_args=())(_policy_loss_fwd)
+
+
+@policy_loss_fwd.register_fake
+def _(logits, tokens, old_log_probs, advantages, ref_log_probs, weights, clip_low, clip_high, kl_weight, ignore_index, with_grad):
+    rows, cols = logits.shape
+    if with_grad:
+        pitch = logits.stride(0) if rows > 1 and logits.stride(1) == 1 and logits.stride(0) >= cols else cols
+        pitch = cols + (pitch - cols) % (16 // logits.element_size())       # each row's place within 16 bytes is the logits'
+        dlogits = torch.empty_strided((rows, cols), (pitch, 1), dtype=logits.dtype, device=logits.device)
+    else:
+        dlogits = logits.new_empty(0)
+    return logits.new_empty((), dtype=torch.float32), logits.new_empty(rows, dtype=torch.float32), dlogits
+
+
+def _policy_setup_context(ctx, inputs, output):
+    ctx.save_for_backward(output[2])        # an output, so that under create_graph it is linked to the logits
+    ctx.with_grad = inputs[10]
+    ctx.taken = False
+    ctx.mark_non_differentiable(output[1])
+    ctx.set_materialize_grads(False)        # no zero tensor of the logits' size for the unused third output
+
+
+def _policy_backward(ctx, g_loss, _g_log_probs, _g_dlogits):
+    nothing = (None,) * 11
+    if g_loss is None:
+        return nothing
+    if not ctx.with_grad:
+        raise RuntimeError("policy_loss was called without the gradient")
+    if ctx.taken:           # its memory belongs to the first caller, who may have added to it
+        raise RuntimeError("Trying to backward through policy_loss a second time: the gradient was formed by the forward and "
+                           "has been handed out; call policy_loss again")
+    ctx.taken = True
+    (dlogits,) = ctx.saved_tensors
+    rows, cols = dlogits.shape
+    with torch.no_grad():                   # the memory behind it, the numbers between rows included
+        flat = dlogits.detach().as_strided(((rows - 1) * dlogits.stride(0) + cols if rows else 0,), (1,))
+        if _direct(flat, g_loss):
+            _scale_unless_one(flat, g_loss)
+            torch.autograd.graph.increment_version(dlogits)
+        else:
+            torch.ops.rbf_attn_b200.scale_unless_one_(flat, g_loss)
+    if torch.is_grad_enabled():
+        return (_FirstOrderOnly.apply("policy_loss", dlogits, g_loss), *nothing[1:])
+    return (dlogits.detach(), *nothing[1:])
+
+
+torch.library.register_autograd("rbf_attn_b200::policy_loss_fwd", _policy_backward, setup_context=_policy_setup_context)
+
+
+class _PolicyLoss(torch.autograd.Function):
+    """``rbf_attn_b200::policy_loss_fwd`` and its autograd formula for calls that go around the operator."""
+
+    @staticmethod
+    def forward(ctx, *inputs):
+        output = _policy_loss_fwd(*inputs)
+        _policy_setup_context(ctx, inputs, output)
+        return output
+
+    @staticmethod
+    def backward(ctx, g_loss, g_log_probs, g_dlogits):
+        return _policy_backward(ctx, g_loss, g_log_probs, g_dlogits)
+
+
+def policy_loss(logits, tokens, old_log_probs, advantages, ref_log_probs=None, weights=None, clip_low: float = 0.2,
+                clip_high: float = 0.2, kl_weight: float = 0.0, ignore_index: int = -100):
+    """Clipped policy loss of 2-D CUDA logits: returns (loss, log_probs), the loss an fp32 scalar whose gradient with respect to
+    the logits is formed by the same kernel that reads them, log_probs (rows,) without a gradient. Per row, with
+    ``lp = log_softmax(logits)[tokens]`` and ``r = exp(lp - old_log_probs)``,
+
+        w * (kl_weight * (exp(ref - lp) - (ref - lp) - 1) - min(r * A, clip(r, 1 - clip_low, 1 + clip_high) * A))
+
+    summed over the rows whose token counts (not ``ignore_index``, a column); ``w`` is ``weights`` or, without them, 1 / number of
+    those rows (none: the loss is NaN, the gradient zero). The KL term needs ``ref_log_probs``. old_log_probs, advantages,
+    ref_log_probs and weights are float32 (rows,) constants. The gradient can be taken once."""
+    for name, t in (("old_log_probs", old_log_probs), ("advantages", advantages), ("ref_log_probs", ref_log_probs),
+                    ("weights", weights)):
+        if _needs_grad(t):
+            raise RuntimeError(f"policy_loss has no gradient with respect to {name}: detach it")
+    if kl_weight != 0 and ref_log_probs is None:
+        raise ValueError("kl_weight needs ref_log_probs")
+    if kl_weight == 0:
+        ref_log_probs = None
+    with_grad = _needs_grad(logits)
+    inputs = (logits, tokens, old_log_probs, advantages, ref_log_probs, weights, float(clip_low), float(clip_high),
+              float(kl_weight), ignore_index, with_grad)
+    if type(ignore_index) is int and _direct(*inputs[:6]):
+        return (_PolicyLoss.apply if with_grad else _policy_loss_fwd)(*inputs)[:2]
+    return torch.ops.rbf_attn_b200.policy_loss_fwd(*inputs)[:2]
+
+
+# ---------------------------------------------------------------------------------------------
+# The paged 8-bit cache and RBF attention over it (no counterpart in the reference, whose generation runs the prefix again for
+# every token). See PagedCache in cache.py for the bookkeeping of pages.
+# ---------------------------------------------------------------------------------------------
+def cache_page_bytes(head_dim: int) -> int:
+    """Bytes of a page (256 tokens) per head: what the last dim of ``pages`` has to be."""
+    if not 0 < head_dim <= 128 or head_dim % 8:
+        raise ValueError(f"head dim {head_dim} is not supported (a multiple of 8 up to 128)")
+    return _lib.load().rbf_b200_cache_page_bytes(head_dim)
+
+
+def _written(pages):
+    if not pages.is_inference():
+        torch.autograd.graph.increment_version(pages)       # as the operator layer does for what it mutates
+
+
+def _cache_append(pages: torch.Tensor, page_table: torch.Tensor, lengths: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
+                  new_lengths: torch.Tensor | None) -> None:
+    _lib.host().cache_append(pages, page_table, lengths, k, v, new_lengths)
+
+
+cache_append_ = torch.library.custom_op("rbf_attn_b200::cache_append", mutates_args=("pages",))(_cache_append)
+
+
+@cache_append_.register_fake
+def _(pages, page_table, lengths, k, v, new_lengths):
+    return None
+
+
+def cache_append(pages, page_table, lengths, k, v, new_lengths=None) -> None:
+    """Writes the tokens k, v (B, H, T, D), bfloat16 or float16, behind the ``lengths`` (B,) that the sequences have in the cache:
+    blocks of 16 tokens that get complete are rounded to 8 bits with a scale per block and head, the rest stays in 16 bits.
+    ``pages`` (pages, H, cache_page_bytes(D)) uint8, ``page_table`` (B, max_pages) and ``lengths`` int32, all on the device, where
+    nothing of them is checked: pages outside the pool are not written, tokens beyond the table's row are dropped, and no two
+    sequences may append to one page. ``new_lengths`` (B,) int32: how many of its T tokens a sequence really gets. ``lengths`` is
+    left for the caller to advance, after all layers."""
+    if _needs_grad(k, v):
+        raise RuntimeError("cache_append has no backward: call it under torch.no_grad() or on detached tensors")
+    if _direct(pages, page_table, lengths, k, v, new_lengths):
+        _cache_append(pages, page_table, lengths, k, v, new_lengths)
+        _written(pages)
+    else:
+        torch.ops.rbf_attn_b200.cache_append(pages, page_table, lengths, k, v, new_lengths)
+
+
+def _cache_read(pages: torch.Tensor, page_table: torch.Tensor, lengths: torch.Tensor, head_dim: int, dtype: torch.dtype,
+                count: int, first: torch.Tensor | None) -> tuple[torch.Tensor, torch.Tensor]:
+    return _lib.host().cache_read(pages, page_table, lengths, head_dim, _DTYPE_CODE.get(dtype, -1), count, first)
+
+
+cache_read_ = torch.library.custom_op("rbf_attn_b200::cache_read", mutates_args=())(_cache_read)
+
+
+@cache_read_.register_fake
+def _(pages, page_table, lengths, head_dim, dtype, count, first):
+    shape = (page_table.shape[0], pages.shape[1], count, head_dim)
+    return pages.new_empty(shape, dtype=dtype), pages.new_empty(shape, dtype=dtype)
+
+
+def cache_read(pages, page_table, lengths, head_dim: int, dtype: torch.dtype, count: int, first=None):
+    """What the cache holds: (k, v), each (B, H, count, head_dim) of the 16-bit ``dtype`` that was appended, tokens ``first[b]``
+    (int32, default 0; below 0 counts as 0) onwards, zeros from ``lengths[b]`` on."""
+    if _direct(pages, page_table, lengths, first):
+        return _cache_read(pages, page_table, lengths, head_dim, dtype, count, first)
+    return torch.ops.rbf_attn_b200.cache_read(pages, page_table, lengths, head_dim, dtype, count, first)
+
+
+def _cache_copy_pages(pages: torch.Tensor, src: list[int], dst: list[int]) -> None:
+    _lib.host().cache_copy_pages(pages, src, dst)
+
+
+cache_copy_pages_ = torch.library.custom_op("rbf_attn_b200::cache_copy_pages", mutates_args=("pages",))(_cache_copy_pages)
+
+
+@cache_copy_pages_.register_fake
+def _(pages, src, dst):
+    return None
+
+
+def cache_copy_pages(pages, src, dst) -> None:
+    """``pages[..., dst[i], :, :] = pages[..., src[i], :, :]`` for lists of page numbers, in all layers of a pool ([layers,] pages,
+    H, bytes) with one launch (per 480 pairs). A page may be the source of several copies, but not a destination twice nor both."""
+    if _direct(pages):
+        _cache_copy_pages(pages, src, dst)
+        _written(pages)
+    else:
+        torch.ops.rbf_attn_b200.cache_copy_pages(pages, list(src), list(dst))
+
+
+def _cache_attention(q: torch.Tensor, pages: torch.Tensor, page_table: torch.Tensor, lengths: torch.Tensor,
+                     new_lengths: torch.Tensor | None, softmax: bool) -> torch.Tensor:
+    return _lib.host().cache_attention(q, pages, page_table, lengths, new_lengths, softmax)
+
+
+cache_attention_ = torch.library.custom_op("rbf_attn_b200::cache_attention", mutates_args=())(_cache_attention)
+
+
+@cache_attention_.register_fake
+def _(q, pages, page_table, lengths, new_lengths, softmax):
+    return torch.empty_like(q, memory_format=torch.contiguous_format)
+
+
+def cache_attention(q, pages, page_table, lengths, new_lengths=None, softmax: bool = True):
+    """RBF attention of the T newest tokens of every sequence, q (B, Hq, T, D), over a cache that holds them too (``cache_append``
+    with the same arguments goes first): token i of sequence b sees tokens 0 to ``lengths[b] + i``, its own among them. Query head
+    h reads key/value head ``h // (Hq // H)``. Returns (B, Hq, T, D); rows from ``new_lengths[b]`` on are zero. ``softmax=False``:
+    ``exp(-g |q - k|^2) V``. No backward: a q that requires a gradient is refused in grad mode."""
+    if _needs_grad(q):
+        raise RuntimeError("cache_attention has no backward: call it under torch.no_grad() or on detached tensors")
+    if type(softmax) is bool and _direct(q, pages, page_table, lengths, new_lengths):
+        return _cache_attention(q, pages, page_table, lengths, new_lengths, softmax)
+    return torch.ops.rbf_attn_b200.cache_attention(q, pages, page_table, lengths, new_lengths, softmax)
+
+
+# ---------------------------------------------------------------------------------------------
 # Wrappers with the reference's names (rbf_attention.py:848-853)
 # ---------------------------------------------------------------------------------------------
 class _ScaledAttention(torch.autograd.Function):
