@@ -27,15 +27,30 @@ namespace rbf {
 namespace {
 
 constexpr int kAttnWarps = 8;
+constexpr int kStages = 3;                         // units of a warp that are loaded ahead, the current one among them
 constexpr float kSlack = 8.f;                      // growth of a score, in powers of two, that does not move the maximum
 
 template <int P>
 struct Tile {
   static constexpr int kUnitBlocks = 256 / P;      // blocks of one load: 8 KB of codes
   static constexpr int kUnit = kUnitBlocks * kBlockTokens;
-  static constexpr int kKeyChunks = P / 32;        // 16-byte words of a lane per block and operand
+  static constexpr int kChunks = P / 32;           // 16-byte words of a lane per block and operand
   static constexpr int kDims = P / 16;             // 16-row tiles of the output
+  static constexpr int kScales = 8192;             // a stage: codes or an incomplete block, the scales, whether there is a page
+  static constexpr int kFlag = kScales + 48;
+  static constexpr int kStage = kScales + 64;
 };
+
+__device__ __forceinline__ void copy16(uint32_t to, const void* from) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
+}
+__device__ __forceinline__ void copies_close() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+// The warp's copies up to the `kLeft` last groups have arrived; after it, every lane sees every lane's.
+template <int kLeft>
+__device__ __forceinline__ void copies_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(kLeft) : "memory");
+  __syncwarp();
+}
 
 __device__ __forceinline__ float attn_ex2(float x) {
   float y;
@@ -91,26 +106,42 @@ struct Deal {
   }
 };
 
-// Units of one segment of sequence b
+// A segment's units: groups of complete blocks, then the incomplete block
 template <int P>
-__device__ __forceinline__ int segment_units(const CacheAttnArgs& a, int b) {
-  const CacheSpan s = cache_span(a.lengths, a.fresh, b, a.T, a.max_pages);
-  return s.fresh == 0 ? 0 : (s.held + s.fresh + Tile<P>::kUnit - 1) / Tile<P>::kUnit;
-}
+struct Units {
+  int held, fresh, groups, count;
+  __device__ Units(const CacheAttnArgs& a, int b) {
+    const CacheSpan s = cache_span(a.lengths, a.fresh, b, a.T, a.max_pages);
+    held = s.held;
+    fresh = s.fresh;
+    const int total = held + fresh;
+    groups = fresh == 0 ? 0 : (total / kBlockTokens + Tile<P>::kUnitBlocks - 1) / Tile<P>::kUnitBlocks;
+    count = groups + (fresh != 0 && total % kBlockTokens != 0);
+  }
+};
 
-// Sum over sequences [0, n) of segment_units, by a whole warp
+// Sums over sequences [0, n) and over all of the units of a segment, by a whole warp
 template <int P>
-__device__ __forceinline__ int64_t units_before(const CacheAttnArgs& a, int n) {
-  int64_t sum = 0;
-  for (int b = threadIdx.x & 31; b < n; b += 32) sum += segment_units<P>(a, b);
+__device__ __forceinline__ void sum_units(const CacheAttnArgs& a, int n, int64_t& before, int64_t& all) {
+  before = all = 0;
+  for (int b = threadIdx.x & 31; b < a.B; b += 32) {
+    const int u = Units<P>(a, b).count;
+    all += u;
+    if (b < n) before += u;
+  }
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  return sum;
+  for (int o = 16; o > 0; o >>= 1) {
+    before += __shfl_xor_sync(0xffffffffu, before, o);
+    all += __shfl_xor_sync(0xffffffffu, all, o);
+  }
 }
 
 // Element offset of output column c of a segment (new token c / G of query head h * G + c % G)
 __device__ __forceinline__ int64_t out_offset(const CacheAttnArgs& a, int b, int h, int c) {
   return ((static_cast<int64_t>(b) * a.H * a.G + h * a.G + c % a.G) * a.T + c / a.G) * a.D;
+}
+__device__ __forceinline__ const uint16_t* q_row(const CacheAttnArgs& a, int b, int h, int c) {
+  return static_cast<const uint16_t*>(a.q) + b * a.qs[0] + (h * a.G + c % a.G) * a.qs[1] + c / a.G * a.qs[2];
 }
 
 // One part: per column P outputs, then the maxima and the sums of all columns
@@ -119,55 +150,197 @@ __device__ __forceinline__ float* part_of(const CacheAttnArgs& a, int64_t index)
   return a.parts + index * (8 * NT) * (P + 2);
 }
 
+// A warp's state for one segment
+template <int P, int NT>
+struct Running {
+  float o[Tile<P>::kDims][NT][4];                  // tile j: dims 32 (j / 2) + 4 g + 2 (j % 2), + 1 of columns 2t, 2t + 1
+  float m[NT][2], l[NT][2];                        // of columns 8n + 2t, + 1; l: this lane's share
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int j = 0; j < Tile<P>::kDims; ++j)
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[j][n][e] = 0.f;
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        m[n][e] = -INFINITY;
+        l[n][e] = 0.f;
+      }
+  }
+  // The maximum moves only if a score exceeds it by more than the slack; s becomes the weights, l their sum.
+  template <int kBlocks>
+  __device__ __forceinline__ void weigh(float (&s)[kBlocks][NT][4]) {
+    float top[NT][2];
+    bool over = false;
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        top[n][e] = fmaxf(s[0][n][e], s[0][n][2 + e]);
+#pragma unroll
+        for (int k = 1; k < kBlocks; ++k) top[n][e] = fmaxf(top[n][e], fmaxf(s[k][n][e], s[k][n][2 + e]));
+        over |= top[n][e] > m[n][e] + kSlack;
+      }
+    if (__any_sync(0xffffffffu, over)) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          float x = fmaxf(top[n][e], m[n][e]);
+#pragma unroll
+          for (int w = 4; w < 32; w <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, w));
+          const float f = m[n][e] == x ? 1.f : attn_ex2(m[n][e] - x);
+          m[n][e] = x;
+          l[n][e] *= f;
+#pragma unroll
+          for (int j = 0; j < Tile<P>::kDims; ++j) {
+            o[j][n][e] *= f;
+            o[j][n][2 + e] *= f;
+          }
+        }
+    }
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      float ref[2];
+#pragma unroll
+      for (int e = 0; e < 2; ++e) ref[e] = m[n][e] == -INFINITY ? 0.f : m[n][e];      // no token seen yet
+#pragma unroll
+      for (int k = 0; k < kBlocks; ++k) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[k][n][e] = attn_ex2(s[k][n][e] - ref[e % 2]);
+        l[n][0] += s[k][n][0] + s[k][n][2];
+        l[n][1] += s[k][n][1] + s[k][n][3];
+      }
+    }
+  }
+};
+
 template <bool kBf16, int P, int NT>
 __global__ void __launch_bounds__(kAttnWarps * 32) cache_attn_kernel(const CacheAttnArgs a) {
   using T = Tile<P>;
-  constexpr int UB = T::kUnitBlocks, KC = T::kKeyChunks, J = T::kDims;
+  constexpr int UB = T::kUnitBlocks, KC = T::kChunks, J = T::kDims;
   constexpr int kSlot = cache_slot_bytes(P), kBytes = cache_page_bytes(P);
+  extern __shared__ __align__(128) uint8_t smem[];
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  uint8_t* ring = smem + (threadIdx.x >> 5) * (kStages * T::kStage);       // a warp has its own
   const int64_t workers = static_cast<int64_t>(gridDim.x) * kAttnWarps;
   const int64_t self = static_cast<int64_t>(threadIdx.x >> 5) * gridDim.x + blockIdx.x;    // neighbours on other SMs
   const int segments = a.column_tiles * a.H;       // of a sequence
-  const Deal deal(units_before<P>(a, a.B) * segments, workers);
+  int64_t unused, all;
+  sum_units<P>(a, 0, unused, all);
+  const Deal deal(all * segments, workers);
   int64_t pos = deal.begin(self);
   const int64_t stop = deal.begin(self + 1);
+  if (pos >= stop) return;
 
   // the sequence of the first unit
   int b = 0;
   int64_t seq_begin = 0;
-  if (pos < stop) {
-    for (; b < a.B; b += 32) {
-      const int64_t mine = b + lane < a.B ? static_cast<int64_t>(segment_units<P>(a, b + lane)) * segments : 0;
-      int64_t upto = mine;
+  for (; b < a.B; b += 32) {
+    const int64_t mine = b + lane < a.B ? static_cast<int64_t>(Units<P>(a, b + lane).count) * segments : 0;
+    int64_t upto = mine;
 #pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int64_t x = __shfl_up_sync(0xffffffffu, upto, o);
-        if (lane >= o) upto += x;
-      }
-      const unsigned past = __ballot_sync(0xffffffffu, seq_begin + upto > pos);
-      if (past != 0) {
-        const int l = __ffs(past) - 1;
-        seq_begin += __shfl_sync(0xffffffffu, upto - mine, l);
-        b += l;
-        break;
-      }
-      seq_begin += __shfl_sync(0xffffffffu, upto, 31);
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t x = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += x;
     }
+    const unsigned past = __ballot_sync(0xffffffffu, seq_begin + upto > pos);
+    if (past != 0) {
+      const int l = __ffs(past) - 1;
+      seq_begin += __shfl_sync(0xffffffffu, upto - mine, l);
+      b += l;
+      break;
+    }
+    seq_begin += __shfl_sync(0xffffffffu, upto, 31);
   }
 
-  while (pos < stop && b < a.B) {
-    const CacheSpan span = cache_span(a.lengths, a.fresh, b, a.T, a.max_pages);
-    const int total = span.held + span.fresh;
-    const int units = span.fresh == 0 ? 0 : (total + T::kUnit - 1) / T::kUnit;
-    if (pos >= seq_begin + static_cast<int64_t>(units) * segments) {       // on to the next sequence (some have no units)
-      seq_begin += static_cast<int64_t>(units) * segments;
+  // ---- loads: lane i looks up the i-th of the next 32 units, so that page numbers are waited for once in 32 units
+  struct Lookup {
+    const uint8_t* base;                           // of the head's page, null where there is nothing to load
+    int what;                                      // complete blocks: first in the page | count << 8; incomplete: tokens | 1 << 16
+  };
+  int look_b = b;                                  // this lane's sequence
+  int64_t look_begin = seq_begin;
+  auto look_up = [&](int64_t x) {
+    Lookup r{nullptr, 0};
+    while (x < stop && look_b < a.B) {
+      const Units<P> units(a, look_b);
+      const int64_t span = static_cast<int64_t>(units.count) * segments;
+      if (x >= look_begin + span) {
+        look_begin += span;
+        ++look_b;
+        continue;
+      }
+      const int64_t in = x - look_begin;
+      const int u = static_cast<int>(in % units.count), h = static_cast<int>(in / units.count % a.H);
+      const int total = units.held + units.fresh, blocks = total / kBlockTokens;
+      const int first = u < units.groups ? u * UB : blocks;
+      r.base = cache_page(a.pages, a.table, look_b, a.max_pages, a.num_pages, a.H, h, kBytes, first * kBlockTokens);
+      r.what = u < units.groups ? first % kPageBlocks | min(UB, blocks - first) << 8 : total % kBlockTokens | 1 << 16;
+      break;
+    }
+    return r;
+  };
+  Lookup now = look_up(pos + lane), next = look_up(pos + 32 + lane);
+  int64_t fetched = 0;                             // units asked for
+  const int64_t mine = stop - pos;
+  auto fetch = [&]() {
+    if (fetched < mine) {
+      const int from = static_cast<int>(fetched & 31);
+      if (from == 0 && fetched != 0) {
+        now = next;
+        next = look_up(pos + fetched + 32 + lane);
+      }
+      const uint64_t base64 = __shfl_sync(0xffffffffu, reinterpret_cast<uint64_t>(now.base), from);
+      const int what = __shfl_sync(0xffffffffu, now.what, from);
+      const uint8_t* base = reinterpret_cast<const uint8_t*>(base64);
+      uint8_t* stage = ring + static_cast<int>(fetched % kStages) * T::kStage;
+      const uint32_t to = smem_u32(stage);
+      if (lane == 0) *reinterpret_cast<int*>(stage + T::kFlag) = base != nullptr;
+      if (base != nullptr) {
+        if (what >> 16) {
+          const uint8_t* src = base + kPageHeader + kPageBlocks * kSlot + lane * 16;
+#pragma unroll
+          for (int i = 0; i < 2 * kSlot / 512; ++i)          // keys, then values
+            if ((i % (kSlot / 512) * 512 + lane * 16) / (2 * P) < (what & 0xff)) copy16(to + i * 512 + lane * 16, src + i * 512);
+        } else {
+          const uint8_t* src = base + kPageHeader + (what & 0xff) * kSlot + lane * 16;
+          const int bytes = (what >> 8) * kSlot;
+          if (bytes == UB * kSlot) {
+#pragma unroll
+            for (int i = 0; i < UB * kSlot / 512; ++i) copy16(to + i * 512 + lane * 16, src + i * 512);
+          } else {
+#pragma unroll
+            for (int i = 0; i < UB * kSlot / 512; ++i)
+              if (i * 512 < bytes) copy16(to + i * 512 + lane * 16, src + i * 512);
+          }
+          if (lane < UB / 2) copy16(to + T::kScales + lane * 16, base + (what & 0xff) * 8 + lane * 16);
+        }
+      }
+      ++fetched;
+    }
+    copies_close();
+  };
+#pragma unroll
+  for (int i = 0; i < kStages - 1; ++i) fetch();
+
+  int64_t taken = 0;                               // units worked on
+  int64_t at = pos;
+  while (at < stop && b < a.B) {
+    const Units<P> units(a, b);
+    if (at >= seq_begin + static_cast<int64_t>(units.count) * segments) {  // on to the next sequence (some have no units)
+      seq_begin += static_cast<int64_t>(units.count) * segments;
       ++b;
       continue;
     }
-    const int seg = static_cast<int>((pos - seq_begin) / units);
-    const int u0 = static_cast<int>((pos - seq_begin) % units);
-    const int64_t left = stop - pos;
-    const int u1 = left < units - u0 ? u0 + static_cast<int>(left) : units;
+    const int total = units.held + units.fresh;
+    const int seg = static_cast<int>((at - seq_begin) / units.count);
+    const int u0 = static_cast<int>((at - seq_begin) % units.count);
+    const int64_t left = stop - at;
+    const int u1 = left < units.count - u0 ? u0 + static_cast<int>(left) : units.count;
     const int h = seg % a.H, c0 = seg / a.H * (8 * NT);
 
     // ---- queries: operand columns, their scales, and how far each column sees
@@ -178,7 +351,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32) cache_attn_kernel(const Cache
     auto load_q = [&](int n, uint32_t (&w)[P / 16][2]) {
       const int c = c0 + n * 8 + g;
       const bool real = c < a.T * a.G;
-      const uint16_t* q = static_cast<const uint16_t*>(a.q) + b * a.qs[0] + (real ? (h * a.G + c % a.G) * a.qs[1] + c / a.G * a.qs[2] : 0);
+      const uint16_t* q = q_row(a, b, h, real ? c : 0);
 #pragma unroll
       for (int d = 0; d < P / 64; ++d) {
 #pragma unroll
@@ -230,103 +403,125 @@ __global__ void __launch_bounds__(kAttnWarps * 32) cache_attn_kernel(const Cache
         qmul[n][e] = 2.f * a.scale * __shfl_sync(0xffffffffu, up, from);
         qsq[n][e] = a.scale * __shfl_sync(0xffffffffu, sq, from);
         const int c2 = c0 + n * 8 + 2 * t + e;
-        limit[n][e] = c2 < a.T * a.G ? span.held + c2 / a.G : total - 1;
+        limit[n][e] = c2 < a.T * a.G ? units.held + c2 / a.G : total - 1;
       }
     }
-    const int first_limit = span.held + c0 / a.G;    // every column of the tile sees at least this far
+    const int first_limit = units.held + c0 / a.G;   // every column of the tile sees at least this far,
+    const int last_limit = units.held + (c0 + 8 * NT - 1) / a.G;           // and none further than this
 
-    float o[J][NT][4], m[NT][2], l[NT][2];
-#pragma unroll
-    for (int j = 0; j < J; ++j)
-#pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) o[j][n][e] = 0.f;
-#pragma unroll
-    for (int n = 0; n < NT; ++n)
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        m[n][e] = -INFINITY;
-        l[n][e] = 0.f;
-      }
-
+    Running<P, NT> run;
+    run.clear();
     for (int u = u0; u < u1; ++u) {
-      const int begin = u * T::kUnit;                // first token
-      if (begin > span.held + (c0 + 8 * NT - 1) / a.G) break;              // no column of the tile sees this far
-      const uint8_t* page = cache_page(a.pages, a.table, b, a.max_pages, a.num_pages, a.H, h, kBytes, begin);
-      if (page == nullptr) continue;
-      const uint8_t* slots = page + kPageHeader + begin % kPageTokens / kBlockTokens * kSlot;
-      const float2* scales = reinterpret_cast<const float2*>(page) + begin % kPageTokens / kBlockTokens;
-      const int whole = min(UB, total / kBlockTokens - begin / kBlockTokens);            // complete blocks of the unit
-      const bool hidden = begin + T::kUnit - 1 > first_limit;
-      float s[UB][NT][4];
-      float2 sc[UB];
-      // ---- scores
+      const uint8_t* stage = ring + static_cast<int>(taken % kStages) * T::kStage;
+      copies_wait<kStages - 2>();
+      fetch();
+      ++taken;
+      if (*reinterpret_cast<const int*>(stage + T::kFlag) == 0) continue;  // a page outside the pool: its tokens are absent
+      if (u < units.groups) {
+        // ================================================================ complete blocks
+        const int begin = u * T::kUnit;              // first token
+        if (begin > last_limit) continue;
+        const int whole = min(UB, total / kBlockTokens - begin / kBlockTokens);
+        const bool hidden = begin + T::kUnit - 1 > first_limit;
+        const float2* scales = reinterpret_cast<const float2*>(stage + T::kScales);
+        float s[UB][NT][4];
 #pragma unroll
-      for (int k = 0; k < UB; ++k) {
+        for (int k = 0; k < UB; ++k) {
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
+          for (int n = 0; n < NT; ++n)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) s[k][n][e] = -INFINITY;
-        sc[k] = make_float2(0.f, 0.f);
-        if (k >= whole) continue;
-        sc[k] = scales[k];
-        const uint4* key = reinterpret_cast<const uint4*>(slots + k * kSlot) + lane;
-        uint4 w[KC];
+            for (int e = 0; e < 4; ++e) s[k][n][e] = -INFINITY;
+          if (k >= whole) continue;
+          const float scale = scales[k].x;
+          const uint4* key = reinterpret_cast<const uint4*>(stage + k * kSlot) + lane;
+          int sq0 = 0, sq1 = 0;
+          float acc[NT][4];
 #pragma unroll
-        for (int i = 0; i < KC; ++i) w[i] = key[i * 32];
-        int sq0 = 0, sq1 = 0;
-        float acc[NT][4];
+          for (int n = 0; n < NT; ++n)
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
+            for (int e = 0; e < 4; ++e) acc[n][e] = 0.f;
 #pragma unroll
-          for (int e = 0; e < 4; ++e) acc[n][e] = 0.f;
+          for (int d = 0; d < P / 64; ++d) {
+            const uint4 w0 = key[2 * d * 32], w1 = key[(2 * d + 1) * 32];
+            const uint32_t r0[4] = {w0.x, w0.y, w0.z, w0.w}, r1[4] = {w1.x, w1.y, w1.z, w1.w};
 #pragma unroll
-        for (int d = 0; d < P / 64; ++d) {
-          const uint32_t r0[4] = {w[2 * d].x, w[2 * d].y, w[2 * d].z, w[2 * d].w};
-          const uint32_t r1[4] = {w[2 * d + 1].x, w[2 * d + 1].y, w[2 * d + 1].z, w[2 * d + 1].w};
+            for (int i = 0; i < 4; ++i) {
+              sq0 += dot4(r0[i]);
+              sq1 += dot4(r1[i]);
+              const uint32_t A[4] = {codes_lo(r0[i]), codes_lo(r1[i]), codes_hi(r0[i]), codes_hi(r1[i])};
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            sq0 += dot4(r0[i]);
-            sq1 += dot4(r1[i]);
-            const uint32_t A[4] = {codes_lo(r0[i]), codes_lo(r1[i]), codes_hi(r0[i]), codes_hi(r1[i])};
+              for (int n = 0; n < NT; ++n) mma16816<false>(acc[n], A, qh[n][d * 4 + i][0], qh[n][d * 4 + i][1]);
+            }
+          }
 #pragma unroll
-            for (int n = 0; n < NT; ++n) mma16816<false>(acc[n], A, qh[n][d * 4 + i][0], qh[n][d * 4 + i][1]);
+          for (int x = 1; x < 4; x <<= 1) {
+            sq0 += __shfl_xor_sync(0xffffffffu, sq0, x);
+            sq1 += __shfl_xor_sync(0xffffffffu, sq1, x);
+          }
+          const float bias = a.scale * scale * scale;
+          const float b0 = bias * static_cast<float>(sq0), b1 = bias * static_cast<float>(sq1);
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const float mul = qmul[n][e] * scale;
+              s[k][n][e] = fmaf(acc[n][e], mul, -b0);
+              s[k][n][2 + e] = fmaf(acc[n][2 + e], mul, -b1);
+            }
+          }
+          if (hidden) {
+            const int tok = begin + k * kBlockTokens + 4 * (g >> 1) + (g & 1);
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                if (tok + 2 * (e / 2) > limit[n][e % 2]) s[k][n][e] = -INFINITY;
           }
         }
+        run.weigh(s);
 #pragma unroll
-        for (int x = 1; x < 4; x <<= 1) {
-          sq0 += __shfl_xor_sync(0xffffffffu, sq0, x);
-          sq1 += __shfl_xor_sync(0xffffffffu, sq1, x);
-        }
-        const float bias = a.scale * sc[k].x * sc[k].x;
-        const float b0 = bias * static_cast<float>(sq0), b1 = bias * static_cast<float>(sq1);
-        const int tok = begin + k * kBlockTokens + 4 * (g >> 1) + (g & 1);
+        for (int k = 0; k < UB; ++k) {
+          if (k >= whole) continue;
+          uint32_t p[NT][2];
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
+          for (int n = 0; n < NT; ++n) {
+            p[n][0] = transpose8(pack2<false>(s[k][n][0], s[k][n][1]));
+            p[n][1] = transpose8(pack2<false>(s[k][n][2], s[k][n][3]));
+          }
+          const uint4* value = reinterpret_cast<const uint4*>(stage + k * kSlot + 16 * P) + lane;
+          const float scale = scales[k].y;
+          const bool finite = fabsf(scale) < INFINITY;
+          const int base = begin + k * kBlockTokens;
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const float mul = qmul[n][e] * sc[k].x;
-            s[k][n][e] = fmaf(acc[n][e], mul, -b0);
-            s[k][n][2 + e] = fmaf(acc[n][2 + e], mul, -b1);
-            if (hidden) {
-              if (tok > limit[n][e]) s[k][n][e] = -INFINITY;
-              if (tok + 2 > limit[n][e]) s[k][n][2 + e] = -INFINITY;
+          for (int i = 0; i < KC; ++i) {
+            const uint4 w = value[i * 32];
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+              const uint32_t r0 = half ? w.z : w.x, r1 = half ? w.w : w.y;
+              const uint32_t A[4] = {codes_lo(r0), codes_lo(r1), codes_hi(r0), codes_hi(r1)};
+#pragma unroll
+              for (int n = 0; n < NT; ++n) {
+                float acc[4] = {0.f, 0.f, 0.f, 0.f};
+                mma16816<false>(acc, A, p[n][0], p[n][1]);
+                float(&o)[4] = run.o[2 * i + half][n];
+#pragma unroll
+                for (int e = 0; e < 4; ++e)           // a block that is not finite reaches the columns that see it
+                  if (finite || base <= limit[n][e % 2]) o[e] = fmaf(acc[e], scale, o[e]);
+              }
             }
           }
         }
-      }
-      // the incomplete block, in 16 bits: it is the last one of its unit
-      const int at = whole;                          // its place in the unit, if it is there
-      const bool partial = whole < UB && begin + whole * kBlockTokens < total;
-      const uint16_t* tail = reinterpret_cast<const uint16_t*>(page + kPageHeader + kPageBlocks * kSlot);
-      if (partial) {
-        const int tok = 4 * (g >> 1) + (g & 1), base = begin + at * kBlockTokens;
-        float acc[NT][4];
+      } else {
+        // ================================================================ the incomplete block, in 16 bits
+        const int base = total / kBlockTokens * kBlockTokens, tok = 4 * (g >> 1) + (g & 1);
+        if (base > last_limit) continue;
+        const uint16_t* keys = reinterpret_cast<const uint16_t*>(stage);
+        const uint16_t* values = keys + kSlot / 2;
+        float s[1][NT][4];
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) acc[n][e] = 0.f;
+          for (int e = 0; e < 4; ++e) s[0][n][e] = 0.f;
         float sq[2] = {0.f, 0.f};
         uint32_t qt[NT][P / 16][2];
 #pragma unroll
@@ -336,12 +531,15 @@ __global__ void __launch_bounds__(kAttnWarps * 32) cache_attn_kernel(const Cache
           uint32_t r[2][8];
 #pragma unroll
           for (int half = 0; half < 2; ++half) {
-            const bool there = base + tok + 2 * half < total;
-            const uint4* row = reinterpret_cast<const uint4*>(tail + (tok + 2 * half) * P + d * 64 + t * 16);
+            const bool row_there = base + tok + 2 * half < total;
+            const uint4* row = reinterpret_cast<const uint4*>(keys + (tok + 2 * half) * P + d * 64 + t * 16);
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-              const uint4 x = there ? row[e] : make_uint4(0, 0, 0, 0);
-              r[half][4 * e] = x.x; r[half][4 * e + 1] = x.y; r[half][4 * e + 2] = x.z; r[half][4 * e + 3] = x.w;
+              const uint4 x = row_there ? row[e] : make_uint4(0, 0, 0, 0);
+              r[half][4 * e] = x.x;
+              r[half][4 * e + 1] = x.y;
+              r[half][4 * e + 2] = x.z;
+              r[half][4 * e + 3] = x.w;
             }
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
@@ -353,7 +551,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32) cache_attn_kernel(const Cache
           for (int i = 0; i < 4; ++i) {
             const uint32_t A[4] = {r[0][2 * i], r[1][2 * i], r[0][2 * i + 1], r[1][2 * i + 1]};
 #pragma unroll
-            for (int n = 0; n < NT; ++n) mma16816<kBf16>(acc[n], A, qt[n][d * 4 + i][0], qt[n][d * 4 + i][1]);
+            for (int n = 0; n < NT; ++n) mma16816<kBf16>(s[0][n], A, qt[n][d * 4 + i][0], qt[n][d * 4 + i][1]);
           }
         }
 #pragma unroll
@@ -362,113 +560,38 @@ __global__ void __launch_bounds__(kAttnWarps * 32) cache_attn_kernel(const Cache
           sq[1] += __shfl_xor_sync(0xffffffffu, sq[1], x);
         }
 #pragma unroll
-        for (int k = 0; k < UB; ++k)
-          if (k == at)
-#pragma unroll
-            for (int n = 0; n < NT; ++n)
-#pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                const bool seen = base + tok + 2 * (e / 2) <= limit[n][e % 2] && base + tok + 2 * (e / 2) < total;
-                s[k][n][e] = seen ? fmaf(acc[n][e], 2.f * a.scale, -a.scale * sq[e / 2]) : -INFINITY;
-              }
-      }
-      // ---- the running maximum moves only if a score exceeds it by more than the slack
-      float top[NT][2];
-      bool over = false;
-#pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          top[n][e] = s[0][n][e];
-#pragma unroll
-          for (int k = 0; k < UB; ++k) top[n][e] = fmaxf(top[n][e], fmaxf(s[k][n][e], s[k][n][2 + e]));
-          over |= top[n][e] > m[n][e] + kSlack;
-        }
-      if (__any_sync(0xffffffffu, over)) {
-#pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            float x = fmaxf(top[n][e], m[n][e]);
-#pragma unroll
-            for (int w = 4; w < 32; w <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, w));
-            const float f = m[n][e] == x ? 1.f : attn_ex2(m[n][e] - x);
-            m[n][e] = x;
-            l[n][e] *= f;
-#pragma unroll
-            for (int j = 0; j < J; ++j) {
-              o[j][n][e] *= f;
-              o[j][n][2 + e] *= f;
-            }
+          for (int e = 0; e < 4; ++e) {
+            const int token = base + tok + 2 * (e / 2);
+            s[0][n][e] = token <= limit[n][e % 2] && token < total ? fmaf(s[0][n][e], 2.f * a.scale, -a.scale * sq[e / 2]) : -INFINITY;
           }
-      }
-      // ---- exponentials, the sum, and the products with the values
-      uint32_t p[UB][NT][2], pt[NT][2];              // operand columns; pt: of the incomplete block, in its own type
-#pragma unroll
-      for (int k = 0; k < UB; ++k)
+        run.weigh(s);
+        uint32_t p[NT][2];
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-          float e4[4];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float ref = m[n][e % 2] == -INFINITY ? 0.f : m[n][e % 2];       // no token seen yet
-            e4[e] = attn_ex2(s[k][n][e] - ref);
-          }
-          l[n][0] += e4[0] + e4[2];
-          l[n][1] += e4[1] + e4[3];
-          p[k][n][0] = transpose8(pack2<false>(e4[0], e4[1]));
-          p[k][n][1] = transpose8(pack2<false>(e4[2], e4[3]));
-          if (k == at && partial) {
-            pt[n][0] = transpose8(pack2<kBf16>(e4[0], e4[1]));
-            pt[n][1] = transpose8(pack2<kBf16>(e4[2], e4[3]));
-          }
+          p[n][0] = transpose8(pack2<kBf16>(s[0][n][0], s[0][n][1]));
+          p[n][1] = transpose8(pack2<kBf16>(s[0][n][2], s[0][n][3]));
         }
-#pragma unroll
-      for (int k = 0; k < UB; ++k) {
-        if (k >= whole) continue;
-        const uint4* value = reinterpret_cast<const uint4*>(slots + k * kSlot + 16 * P) + lane;
-        uint4 w[KC];
-#pragma unroll
-        for (int i = 0; i < KC; ++i) w[i] = value[i * 32];
-        const bool finite = fabsf(sc[k].y) < INFINITY;
-        const int base = begin + k * kBlockTokens;
-#pragma unroll
-        for (int j = 0; j < J; ++j) {
-          const uint32_t r0 = j % 2 ? w[j / 2].z : w[j / 2].x, r1 = j % 2 ? w[j / 2].w : w[j / 2].y;
-          const uint32_t A[4] = {codes_lo(r0), codes_lo(r1), codes_hi(r0), codes_hi(r1)};
-#pragma unroll
-          for (int n = 0; n < NT; ++n) {
-            float acc[4] = {0.f, 0.f, 0.f, 0.f};
-            mma16816<false>(acc, A, p[k][n][0], p[k][n][1]);
-#pragma unroll
-            for (int e = 0; e < 4; ++e)               // a block that is not finite reaches the columns that see it
-              if (finite || base <= limit[n][e % 2]) o[j][n][e] = fmaf(acc[e], sc[k].y, o[j][n][e]);
-          }
-        }
-      }
-      if (partial) {
-        const int base = begin + at * kBlockTokens;
-        const uint16_t* values = tail + kSlot / 2;
         uint2 x[KC][4];                              // dims 32 i + 4 g ... + 3 of tokens 4 t + r
-        bool odd = false;                            // a value that is not finite behind what some column sees
+        bool odd = false;                            // a value that is not finite
 #pragma unroll
         for (int i = 0; i < KC; ++i)
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
             x[i][r] = make_uint2(0, 0);
             if (base + 4 * t + r < total) x[i][r] = *reinterpret_cast<const uint2*>(values + (4 * t + r) * P + 32 * i + 4 * g);
-            const uint32_t inf = kBf16 ? 0x7f80u : 0x7c00u;
+            constexpr uint32_t kInf = kBf16 ? 0x7f80u : 0x7c00u;
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
               const uint32_t y = half ? x[i][r].y : x[i][r].x;
-              odd |= (y & inf) == inf || (y >> 16 & inf) == inf;
+              odd |= (y & kInf) == kInf || (y >> 16 & kInf) == kInf;
             }
           }
         // A product 0 * inf of a column that does not see the token must not reach it: such blocks go token by token.
         const bool slow = __any_sync(0xffffffffu, odd) && total - 1 > first_limit;
 #pragma unroll 1
-        for (int only = slow ? 0 : kBlockTokens; only <= kBlockTokens; ++only) {
-          if (slow && only == kBlockTokens) break;
+        for (int only = slow ? 0 : kBlockTokens - 1; only < kBlockTokens; ++only) {
 #pragma unroll
           for (int j = 0; j < J; ++j) {
             uint32_t A[4];
@@ -485,10 +608,10 @@ __global__ void __launch_bounds__(kAttnWarps * 32) cache_attn_kernel(const Cache
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
               float acc[4] = {0.f, 0.f, 0.f, 0.f};
-              mma16816<kBf16>(acc, A, pt[n][0], pt[n][1]);
+              mma16816<kBf16>(acc, A, p[n][0], p[n][1]);
 #pragma unroll
               for (int e = 0; e < 4; ++e)
-                if (!slow || base + only <= limit[n][e % 2]) o[j][n][e] += acc[e];
+                if (!slow || base + only <= limit[n][e % 2]) run.o[j][n][e] += acc[e];
             }
           }
         }
@@ -501,124 +624,161 @@ __global__ void __launch_bounds__(kAttnWarps * 32) cache_attn_kernel(const Cache
 #pragma unroll
       for (int e = 0; e < 2; ++e)
 #pragma unroll
-        for (int w = 4; w < 32; w <<= 1) l[n][e] += __shfl_xor_sync(0xffffffffu, l[n][e], w);
-    if (u0 == 0 && u1 == units) {
+        for (int w = 4; w < 32; w <<= 1) run.l[n][e] += __shfl_xor_sync(0xffffffffu, run.l[n][e], w);
+    const bool complete = u0 == 0 && u1 == units.count;
+    float* part = part_of<P, NT>(a, 2 * self + (u0 == 0));
 #pragma unroll
-      for (int n = 0; n < NT; ++n)
+    for (int n = 0; n < NT; ++n)
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int c = c0 + n * 8 + 2 * t + e;
-          if (c >= a.T * a.G) continue;
-          float f = m[n][e] == -INFINITY ? 0.f : a.softmax ? 1.f / l[n][e] : attn_ex2(m[n][e] - qsq[n][e]);
-          const bool none = c / a.G >= span.fresh || m[n][e] == -INFINITY && l[n][e] == 0.f;
+      for (int e = 0; e < 2; ++e) {
+        const int in = n * 8 + 2 * t + e, c = c0 + in;
+        if (c >= a.T * a.G) continue;
+        const float m = run.m[n][e], l = run.l[n][e];
+        if (complete) {
+          const float f = m == -INFINITY ? 0.f : a.softmax ? 1.f / l : attn_ex2(m - qsq[n][e]);
+          const bool none = c / a.G >= units.fresh || (m == -INFINITY && l == 0.f);
           uint16_t* out = static_cast<uint16_t*>(a.out) + out_offset(a, b, h, c);
 #pragma unroll
           for (int i = 0; i < KC; ++i) {
             const int d = 32 * i + 4 * g;
             if (d >= a.D) continue;
-            uint2 y = make_uint2(pack2<kBf16>(o[2 * i][n][e] * f, o[2 * i][n][2 + e] * f),
-                                 pack2<kBf16>(o[2 * i + 1][n][e] * f, o[2 * i + 1][n][2 + e] * f));
+            uint2 y = make_uint2(pack2<kBf16>(run.o[2 * i][n][e] * f, run.o[2 * i][n][2 + e] * f),
+                                 pack2<kBf16>(run.o[2 * i + 1][n][e] * f, run.o[2 * i + 1][n][2 + e] * f));
             if (none) y = make_uint2(0, 0);
             *reinterpret_cast<uint2*>(out + d) = y;
           }
-        }
-    } else {
-      float* part = part_of<P, NT>(a, 2 * self + (u0 == 0));
-#pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int c = n * 8 + 2 * t + e;
-          if (c0 + c >= a.T * a.G) continue;
+        } else {
 #pragma unroll
           for (int i = 0; i < KC; ++i)
-            *reinterpret_cast<float4*>(part + c * P + 32 * i + 4 * g) =
-                make_float4(o[2 * i][n][e], o[2 * i][n][2 + e], o[2 * i + 1][n][e], o[2 * i + 1][n][2 + e]);
+            *reinterpret_cast<float4*>(part + in * P + 32 * i + 4 * g) =
+                make_float4(run.o[2 * i][n][e], run.o[2 * i][n][2 + e], run.o[2 * i + 1][n][e], run.o[2 * i + 1][n][2 + e]);
           if (g == 0) {
-            part[8 * NT * P + c] = m[n][e];
-            part[8 * NT * (P + 1) + c] = l[n][e];
+            part[8 * NT * P + in] = m;
+            part[8 * NT * (P + 1) + in] = l;
           }
         }
-    }
-    pos += u1 - u0;
+      }
+    at += u1 - u0;
   }
   grid_dependents_launch();
 }
 
-constexpr int kJoinThreads = 128;
+constexpr int kJoinWarps = 8;
 
-// One block per segment joins the parts of segments that several warps worked on, and clears those that no warp did.
+// Joins the parts of the segments that several warps worked on, and clears those that no warp did: `split` warps of a block
+// share the parts of a column, 8 where there are few columns (and many parts of each), else one.
 template <bool kBf16, int P, int NT>
-__global__ void __launch_bounds__(kJoinThreads) cache_join_kernel(const CacheAttnArgs a, const int64_t workers) {
-  grid_dependency_wait();
+__global__ void __launch_bounds__(kJoinWarps * 32) cache_join_kernel(const CacheAttnArgs a, const int64_t workers, const int split) {
+  __shared__ float s_y[kJoinWarps][P], s_m[kJoinWarps], s_l[kJoinWarps];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int segments = a.column_tiles * a.H;
-  const int b = blockIdx.x / segments, seg = blockIdx.x % segments;
-  const int h = seg % a.H, c0 = seg / a.H * (8 * NT);
-  const CacheSpan span = cache_span(a.lengths, a.fresh, b, a.T, a.max_pages);
-  const int units = segment_units<P>(a, b);
-  const int columns = min(8 * NT, a.T * a.G - c0);
-  uint16_t* out = static_cast<uint16_t*>(a.out);
+  const int segments = a.column_tiles * a.H, width = min(8 * NT, a.T * a.G);
+  const int64_t column = static_cast<int64_t>(blockIdx.x) * (kJoinWarps / split) + warp / split;
+  const int64_t segment = column / width;
+  const int in = static_cast<int>(column % width), share = warp % split;
+  const int b = static_cast<int>(segment / segments), seg = static_cast<int>(segment % segments);
+  const int h = seg % a.H, c = seg / a.H * (8 * NT) + in;
+  grid_dependency_wait();
   constexpr int kPer = P / 32;
-  int64_t first = 0, last = 0;
-  if (units > 0) {
-    const Deal deal(units_before<P>(a, a.B) * segments, workers);
-    const int64_t begin = units_before<P>(a, b) * segments + static_cast<int64_t>(seg) * units;
-    first = min(deal.worker(begin), workers - 1);
-    last = min(deal.worker(begin + units - 1), workers - 1);
-    if (first == last) return;
-  }
-  for (int c = warp; c < columns; c += kJoinThreads / 32) {
-    float y[kPer] = {};
-    if (units > 0 && (c0 + c) / a.G < span.fresh) {
-      float top = -INFINITY;
-      for (int64_t w = first + lane; w <= last; w += 32)
-        top = fmaxf(top, part_of<P, NT>(a, 2 * w + (w == first))[8 * NT * P + c]);
+  float y[kPer] = {}, top = -INFINITY, sum = 0.f;
+  bool write = b < a.B && c < a.T * a.G, some = false;
+  if (write) {
+    const Units<P> units(a, b);
+    if (units.count > 0) {
+      int64_t before, all;
+      sum_units<P>(a, b, before, all);
+      const Deal deal(all * segments, workers);
+      const int64_t begin = before * segments + static_cast<int64_t>(seg) * units.count;
+      const int64_t first = min(deal.worker(begin), workers - 1), last = min(deal.worker(begin + units.count - 1), workers - 1);
+      write = first != last;
+      some = write && c / a.G < units.fresh;
+      if (some) {
+        for (int64_t w0 = first + share * 32; w0 <= last; w0 += 32 * split) {
+          const int n = static_cast<int>(min(last - w0 + 1, int64_t{32}));
+          float m = -INFINITY, l = 0.f;
+          if (lane < n) {
+            const float* part = part_of<P, NT>(a, 2 * (w0 + lane) + (w0 + lane == first));
+            m = part[8 * NT * P + in];
+            l = part[8 * NT * (P + 1) + in];
+          }
+          float x = m;
 #pragma unroll
-      for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-      const float ref = top == -INFINITY ? 0.f : top;
-      float sum = 0.f;
-#pragma unroll 4
-      for (int64_t w = first; w <= last; ++w) {
-        const float* part = part_of<P, NT>(a, 2 * w + (w == first));
-        const float f = attn_ex2(part[8 * NT * P + c] - ref);
-        sum = fmaf(part[8 * NT * (P + 1) + c], f, sum);
+          for (int o = 16; o > 0; o >>= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
+          x = fmaxf(x, top);
+          const float ref = x == -INFINITY ? 0.f : x, f = attn_ex2(m - ref), old = attn_ex2(top - ref);
+          top = x;
+          l *= f;
 #pragma unroll
-        for (int i = 0; i < kPer; ++i) y[i] = fmaf(part[c * P + lane * kPer + i], f, y[i]);
-      }
-      float f = 1.f / sum;
-      if (!a.softmax) {
-        const int col = c0 + c;
-        const uint16_t* q = static_cast<const uint16_t*>(a.q) + b * a.qs[0] + (h * a.G + col % a.G) * a.qs[1] + col / a.G * a.qs[2];
-        float sq = 0.f;
-        for (int d = lane * 2; d < a.D; d += 64) {
-          const float2 x = unpack2<kBf16>(*reinterpret_cast<const uint32_t*>(q + d));
-          sq = fmaf(x.x, x.x, fmaf(x.y, x.y, sq));
+          for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+          sum = fmaf(sum, old, l);
+#pragma unroll
+          for (int i = 0; i < kPer; ++i) y[i] *= old;
+#pragma unroll 8
+          for (int j = 0; j < n; ++j) {
+            const float* part = part_of<P, NT>(a, 2 * (w0 + j) + (w0 + j == first)) + in * P + lane * kPer;
+            const float fj = __shfl_sync(0xffffffffu, f, j);
+#pragma unroll
+            for (int i = 0; i < kPer; ++i) y[i] = fmaf(part[i], fj, y[i]);
+          }
         }
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) sq += __shfl_xor_sync(0xffffffffu, sq, o);
-        f = attn_ex2(ref - a.scale * sq);
       }
-      const bool none = top == -INFINITY && sum == 0.f;
-#pragma unroll
-      for (int i = 0; i < kPer; ++i) y[i] = none ? 0.f : y[i] * f;
-    }
-    uint16_t* to = out + out_offset(a, b, h, c0 + c) + lane * kPer;
-    if (lane * kPer < a.D) {
-#pragma unroll
-      for (int i = 0; i < kPer; i += 2) *reinterpret_cast<uint32_t*>(to + i) = pack2<kBf16>(y[i], y[i + 1]);
     }
   }
+  if (split > 1) {                                 // the whole block has one column
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) s_y[warp][lane * kPer + i] = y[i];
+    if (lane == 0) {
+      s_m[warp] = top;
+      s_l[warp] = sum;
+    }
+    __syncthreads();
+    if (warp != 0) return;
+    for (int w = 1; w < kJoinWarps; ++w) {
+      const float x = fmaxf(top, s_m[w]), ref = x == -INFINITY ? 0.f : x;
+      const float f0 = attn_ex2(top - ref), f1 = attn_ex2(s_m[w] - ref);
+      top = x;
+      sum = sum * f0 + s_l[w] * f1;
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) y[i] = y[i] * f0 + s_y[w][lane * kPer + i] * f1;
+    }
+  }
+  if (!write) return;
+  if (some) {
+    float f = 1.f / sum;
+    if (!a.softmax) {
+      const uint16_t* q = q_row(a, b, h, c);
+      float sq = 0.f;
+      for (int d = lane * 2; d < a.D; d += 64) {
+        const float2 x = unpack2<kBf16>(*reinterpret_cast<const uint32_t*>(q + d));
+        sq = fmaf(x.x, x.x, fmaf(x.y, x.y, sq));
+      }
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) sq += __shfl_xor_sync(0xffffffffu, sq, o);
+      f = attn_ex2((top == -INFINITY ? 0.f : top) - a.scale * sq);
+    }
+    if (top == -INFINITY && sum == 0.f) f = 0.f;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) y[i] *= f;
+  }
+  if (lane * kPer >= a.D) return;
+  uint16_t* to = static_cast<uint16_t*>(a.out) + out_offset(a, b, h, c) + lane * kPer;
+#pragma unroll
+  for (int i = 0; i < kPer; i += 2) *reinterpret_cast<uint32_t*>(to + i) = pack2<kBf16>(y[i], y[i + 1]);
 }
 
 template <bool kBf16, int P, int NT>
 cudaError_t attn_t(const CacheAttnArgs& a, int sms, cudaStream_t stream) {
-  cache_attn_kernel<kBf16, P, NT><<<sms, kAttnWarps * 32, 0, stream>>>(a);
-  const cudaError_t e = cudaGetLastError();
+  constexpr int kSmem = kAttnWarps * kStages * Tile<P>::kStage;
+  static PerDeviceFlags flags;
+  cudaError_t e = ensure_dynamic_smem(cache_attn_kernel<kBf16, P, NT>, kSmem, flags);
   if (e != cudaSuccess) return e;
-  const int64_t blocks = static_cast<int64_t>(a.B) * a.column_tiles * a.H;
-  return launch_dependent(cache_join_kernel<kBf16, P, NT>, dim3(static_cast<unsigned>(blocks)), kJoinThreads, 0, stream, a,
-                          static_cast<int64_t>(sms) * kAttnWarps);
+  cache_attn_kernel<kBf16, P, NT><<<sms, kAttnWarps * 32, kSmem, stream>>>(a);
+  if ((e = cudaGetLastError()) != cudaSuccess) return e;
+  const int64_t width = static_cast<int64_t>(a.T) * a.G < 8 * NT ? a.T * a.G : 8 * NT;
+  const int64_t columns = static_cast<int64_t>(a.B) * a.column_tiles * a.H * width;
+  const int split = columns <= sms * 4 ? kJoinWarps : 1;
+  const int64_t blocks = (columns + kJoinWarps / split - 1) / (kJoinWarps / split);
+  return launch_dependent(cache_join_kernel<kBf16, P, NT>, dim3(static_cast<unsigned>(blocks)), kJoinWarps * 32, 0, stream, a,
+                          static_cast<int64_t>(sms) * kAttnWarps, split);
 }
 
 template <bool kBf16, int P>
@@ -639,7 +799,7 @@ size_t cache_attn_workspace_bytes(int T, int G, int D, int sms) {
 cudaError_t launch_cache_attn(CacheAttnArgs a, bool bf16, int sms, cudaStream_t stream) {
   if (a.B == 0 || a.T == 0) return cudaSuccess;
   const int64_t columns = 8 * cache_attn_tiles(a.T, a.G, cache_columns(a.D)), tiles = (static_cast<int64_t>(a.T) * a.G + columns - 1) / columns;
-  if (tiles * a.H * a.B > 0x7fffffffll) return cudaErrorInvalidConfiguration;
+  if (tiles * columns * a.H * a.B > 0x7fffffffll) return cudaErrorInvalidConfiguration;
   a.column_tiles = static_cast<int>(tiles);
   if (cache_columns(a.D) == 64) return bf16 ? attn_p<true, 64>(a, sms, stream) : attn_p<false, 64>(a, sms, stream);
   return bf16 ? attn_p<true, 128>(a, sms, stream) : attn_p<false, 128>(a, sms, stream);
