@@ -30,15 +30,15 @@ constexpr int kAttnWarps = 8;
 constexpr int kStages = 3;                         // units of a warp that are loaded ahead, the current one among them
 constexpr float kSlack = 8.f;                      // growth of a score, in powers of two, that does not move the maximum
 
-template <int P>
+// A warp's unit of work: UB blocks that are complete, or the one that is not
+template <int P, int UB>
 struct Tile {
-  static constexpr int kUnitBlocks = 256 / P;      // blocks of one load: 8 KB of codes
-  static constexpr int kUnit = kUnitBlocks * kBlockTokens;
-  static constexpr int kChunks = P / 32;           // 16-byte words of a lane per block and operand
-  static constexpr int kDims = P / 16;             // 16-row tiles of the output
-  static constexpr int kScales = 8192;             // a stage: codes or an incomplete block, the scales, whether there is a page
+  static constexpr int kUnit = UB * kBlockTokens;
+  static constexpr int kBytes = (UB > 2 ? UB : 2) * cache_slot_bytes(P);
+  static constexpr int kScales = kBytes;           // a stage: the rows, the scales, whether there is a page
   static constexpr int kFlag = kScales + 48;
   static constexpr int kStage = kScales + 64;
+  static_assert(UB == 2 || UB == 4, "scales are loaded 16 bytes at a time into 32");
 };
 
 __device__ __forceinline__ void copy16(uint32_t to, const void* from) {
@@ -107,7 +107,7 @@ struct Deal {
 };
 
 // A segment's units: groups of complete blocks, then the incomplete block
-template <int P>
+template <int UB>
 struct Units {
   int held, fresh, groups, count;
   __device__ Units(const CacheAttnArgs& a, int b) {
@@ -115,17 +115,17 @@ struct Units {
     held = s.held;
     fresh = s.fresh;
     const int total = held + fresh;
-    groups = fresh == 0 ? 0 : (total / kBlockTokens + Tile<P>::kUnitBlocks - 1) / Tile<P>::kUnitBlocks;
+    groups = fresh == 0 ? 0 : (total / kBlockTokens + UB - 1) / UB;
     count = groups + (fresh != 0 && total % kBlockTokens != 0);
   }
 };
 
 // Sums over sequences [0, n) and over all of the units of a segment, by a whole warp
-template <int P>
+template <int UB>
 __device__ __forceinline__ void sum_units(const CacheAttnArgs& a, int n, int64_t& before, int64_t& all) {
   before = all = 0;
   for (int b = threadIdx.x & 31; b < a.B; b += 32) {
-    const int u = Units<P>(a, b).count;
+    const int u = Units<UB>(a, b).count;
     all += u;
     if (b < n) before += u;
   }
@@ -153,11 +153,11 @@ __device__ __forceinline__ float* part_of(const CacheAttnArgs& a, int64_t index)
 // A warp's state for one segment
 template <int P, int NT>
 struct Running {
-  float o[Tile<P>::kDims][NT][4];                  // tile j: dims 32 (j / 2) + 4 g + 2 (j % 2), + 1 of columns 2t, 2t + 1
+  float o[P / 16][NT][4];                  // tile j: dims 32 (j / 2) + 4 g + 2 (j % 2), + 1 of columns 2t, 2t + 1
   float m[NT][2], l[NT][2];                        // of columns 8n + 2t, + 1; l: this lane's share
   __device__ __forceinline__ void clear() {
 #pragma unroll
-    for (int j = 0; j < Tile<P>::kDims; ++j)
+    for (int j = 0; j < P / 16; ++j)
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -169,6 +169,22 @@ struct Running {
         m[n][e] = -INFINITY;
         l[n][e] = 0.f;
       }
+  }
+  // l of the whole warp
+  __device__ __forceinline__ void sum_up() {
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+#pragma unroll
+        for (int w = 4; w < 32; w <<= 1) l[n][e] += __shfl_xor_sync(0xffffffffu, l[n][e], w);
+  }
+  // this lane's outputs of column 8n + 2t + e, in the order of the dims
+  __device__ __forceinline__ void store(float* row, int n, int e) const {
+#pragma unroll
+    for (int i = 0; i < P / 32; ++i)
+      *reinterpret_cast<float4*>(row + 32 * i + (threadIdx.x & 31) / 4 * 4) =
+          make_float4(o[2 * i][n][e], o[2 * i][n][2 + e], o[2 * i + 1][n][e], o[2 * i + 1][n][2 + e]);
   }
   // The maximum moves only if a score exceeds it by more than the slack; s becomes the weights, l their sum.
   template <int kBlocks>
@@ -196,7 +212,7 @@ struct Running {
           m[n][e] = x;
           l[n][e] *= f;
 #pragma unroll
-          for (int j = 0; j < Tile<P>::kDims; ++j) {
+          for (int j = 0; j < P / 16; ++j) {
             o[j][n][e] *= f;
             o[j][n][2 + e] *= f;
           }
@@ -218,11 +234,333 @@ struct Running {
   }
 };
 
+// Operand words of query column c (lane g's of a tile) as they are in memory: k step i has dims 64 (i / 4) + 16 t + 4 (i % 4) ... + 3
+template <int P>
+__device__ __forceinline__ void load_q(const CacheAttnArgs& a, int b, int h, int c, int t, uint32_t (&w)[P / 16][2]) {
+  const bool real = c < a.T * a.G;
+  const uint16_t* q = q_row(a, b, h, real ? c : 0);
+#pragma unroll
+  for (int d = 0; d < P / 64; ++d) {
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int col = d * 64 + t * 16 + e * 8;
+      uint4 raw = make_uint4(0, 0, 0, 0);
+      if (real && col < a.D) raw = *reinterpret_cast<const uint4*>(q + col);
+      w[d * 4 + e * 2][0] = raw.x;
+      w[d * 4 + e * 2][1] = raw.y;
+      w[d * 4 + e * 2 + 1][0] = raw.z;
+      w[d * 4 + e * 2 + 1][1] = raw.w;
+    }
+  }
+}
+
+// The query columns of a segment: operands, their scales, and how far each column sees
+template <bool kBf16, int P, int NT>
+struct Queries {
+  uint32_t w[NT][P / 16][2];                       // fp16, scaled
+  float mul[NT][2], sq[NT][2];                     // of columns 2t, 2t + 1: what the scores are multiplied by, g log2(e) |q|^2
+  int limit[NT][2];                                // last token that the column sees
+  int first_limit, last_limit;                     // every column of the tile sees at least, none sees more
+  int b, h, c0, total;
+
+  __device__ __forceinline__ void load(const CacheAttnArgs& a, int b_, int h_, int c0_, int held, int total_) {
+    b = b_, h = h_, c0 = c0_, total = total_;
+    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      uint32_t raw[P / 16][2];
+      load_q<P>(a, b, h, c0 + n * 8 + g, t, raw);
+      uint32_t top = 0;
+      float square = 0.f;
+#pragma unroll
+      for (int i = 0; i < P / 16; ++i) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const float2 f = unpack2<kBf16>(raw[i][e]);
+          top = max(top, max(__float_as_uint(f.x) & 0x7fffffffu, __float_as_uint(f.y) & 0x7fffffffu));
+          square = fmaf(f.x, f.x, fmaf(f.y, f.y, square));
+        }
+      }
+#pragma unroll
+      for (int o = 1; o < 4; o <<= 1) {
+        top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+        square += __shfl_xor_sync(0xffffffffu, square, o);
+      }
+      uint32_t exponent = top >> 23;                 // of the largest element; zero and infinity keep their meaning
+      exponent = exponent == 0 ? 127u : min(exponent, 253u);
+      const float down = __uint_as_float((254u - exponent) << 23), up = __uint_as_float(exponent << 23);
+#pragma unroll
+      for (int i = 0; i < P / 16; ++i) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const float2 f = unpack2<kBf16>(raw[i][e]);
+          w[n][i][e] = pack2<false>(f.x * down, f.y * down);
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int from = (2 * t + e) * 4;
+        mul[n][e] = 2.f * a.scale * __shfl_sync(0xffffffffu, up, from);
+        sq[n][e] = a.scale * __shfl_sync(0xffffffffu, square, from);
+        const int c = c0 + n * 8 + 2 * t + e;
+        limit[n][e] = c < a.T * a.G ? held + c / a.G : total - 1;
+      }
+    }
+    first_limit = held + c0 / a.G;
+    last_limit = held + (c0 + 8 * NT - 1) / a.G;
+  }
+};
+
+// Asks for a unit's bytes; `what`: first complete block in the page | their count << 8, or tokens of the incomplete block | 1 << 16
+template <int P, int UB>
+__device__ __forceinline__ void fetch_unit(uint8_t* stage, const uint8_t* page, int what) {
+  using T = Tile<P, UB>;
+  constexpr int kSlot = cache_slot_bytes(P);
+  const int lane = threadIdx.x & 31;
+  const uint32_t to = smem_u32(stage);
+  if (lane == 0) *reinterpret_cast<int*>(stage + T::kFlag) = page != nullptr;
+  if (page == nullptr) return;
+  if (what >> 16) {
+    const uint8_t* src = page + kPageHeader + kPageBlocks * kSlot + lane * 16;
+#pragma unroll
+    for (int i = 0; i < 2 * kSlot / 512; ++i)              // keys, then values: the rows that there are
+      if ((i % (kSlot / 512) * 512 + lane * 16) / (2 * P) < (what & 0xff)) copy16(to + i * 512 + lane * 16, src + i * 512);
+    return;
+  }
+  const uint8_t* src = page + kPageHeader + (what & 0xff) * kSlot + lane * 16;
+  const int bytes = (what >> 8) * kSlot;
+  if (bytes == UB * kSlot) {
+#pragma unroll
+    for (int i = 0; i < UB * kSlot / 512; ++i) copy16(to + i * 512 + lane * 16, src + i * 512);
+  } else {
+#pragma unroll
+    for (int i = 0; i < UB * kSlot / 512; ++i)
+      if (i * 512 < bytes) copy16(to + i * 512 + lane * 16, src + i * 512);
+  }
+  if (lane < UB / 2) copy16(to + T::kScales + lane * 16, page + (what & 0xff) * 8 + lane * 16);
+}
+
+// A group of complete blocks, the first of them at token `begin`
+template <bool kBf16, int P, int NT, int UB>
+__device__ __forceinline__ void codes_unit(const CacheAttnArgs& a, const Queries<kBf16, P, NT>& q, Running<P, NT>& run,
+                                           const uint8_t* stage, int begin) {
+  using T = Tile<P, UB>;
+  constexpr int kSlot = cache_slot_bytes(P);
+  const int lane = threadIdx.x & 31, g = lane >> 2;
+  if (begin > q.last_limit) return;
+  const int whole = min(UB, q.total / kBlockTokens - begin / kBlockTokens);
+  const bool hidden = begin + T::kUnit - 1 > q.first_limit;
+  const float2* scales = reinterpret_cast<const float2*>(stage + T::kScales);
+  float s[UB][NT][4];
+#pragma unroll
+  for (int k = 0; k < UB; ++k) {
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s[k][n][e] = -INFINITY;
+    if (k >= whole) continue;
+    const float scale = scales[k].x;
+    const uint4* key = reinterpret_cast<const uint4*>(stage + k * kSlot) + lane;
+    int sq0 = 0, sq1 = 0;
+    float acc[NT][4];
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[n][e] = 0.f;
+#pragma unroll
+    for (int d = 0; d < P / 64; ++d) {
+      const uint4 w0 = key[2 * d * 32], w1 = key[(2 * d + 1) * 32];
+      const uint32_t r0[4] = {w0.x, w0.y, w0.z, w0.w}, r1[4] = {w1.x, w1.y, w1.z, w1.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        sq0 += dot4(r0[i]);
+        sq1 += dot4(r1[i]);
+        const uint32_t A[4] = {codes_lo(r0[i]), codes_lo(r1[i]), codes_hi(r0[i]), codes_hi(r1[i])};
+#pragma unroll
+        for (int n = 0; n < NT; ++n) mma16816<false>(acc[n], A, q.w[n][d * 4 + i][0], q.w[n][d * 4 + i][1]);
+      }
+    }
+#pragma unroll
+    for (int x = 1; x < 4; x <<= 1) {
+      sq0 += __shfl_xor_sync(0xffffffffu, sq0, x);
+      sq1 += __shfl_xor_sync(0xffffffffu, sq1, x);
+    }
+    const float bias = a.scale * scale * scale;
+    const float b0 = bias * static_cast<float>(sq0), b1 = bias * static_cast<float>(sq1);
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const float mul = q.mul[n][e] * scale;
+        s[k][n][e] = fmaf(acc[n][e], mul, -b0);
+        s[k][n][2 + e] = fmaf(acc[n][2 + e], mul, -b1);
+      }
+    }
+    if (hidden) {
+      const int tok = begin + k * kBlockTokens + 4 * (g >> 1) + (g & 1);
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (tok + 2 * (e / 2) > q.limit[n][e % 2]) s[k][n][e] = -INFINITY;
+    }
+  }
+  run.weigh(s);
+#pragma unroll
+  for (int k = 0; k < UB; ++k) {
+    if (k >= whole) continue;
+    uint32_t p[NT][2];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      p[n][0] = transpose8(pack2<false>(s[k][n][0], s[k][n][1]));
+      p[n][1] = transpose8(pack2<false>(s[k][n][2], s[k][n][3]));
+    }
+    const uint4* value = reinterpret_cast<const uint4*>(stage + k * kSlot + 16 * P) + lane;
+    const float scale = scales[k].y;
+    const bool finite = fabsf(scale) < INFINITY;
+    const int base = begin + k * kBlockTokens;
+#pragma unroll
+    for (int i = 0; i < P / 32; ++i) {
+      const uint4 w = value[i * 32];
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const uint32_t r0 = half ? w.z : w.x, r1 = half ? w.w : w.y;
+        const uint32_t A[4] = {codes_lo(r0), codes_lo(r1), codes_hi(r0), codes_hi(r1)};
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          float acc[4] = {0.f, 0.f, 0.f, 0.f};
+          mma16816<false>(acc, A, p[n][0], p[n][1]);
+          float(&o)[4] = run.o[2 * i + half][n];
+#pragma unroll
+          for (int e = 0; e < 4; ++e)               // a block that is not finite reaches the columns that see it
+            if (finite || base <= q.limit[n][e % 2]) o[e] = fmaf(acc[e], scale, o[e]);
+        }
+      }
+    }
+  }
+}
+
+// The block that is not complete, in 16 bits
+template <bool kBf16, int P, int NT>
+__device__ __forceinline__ void rest_unit(const CacheAttnArgs& a, const Queries<kBf16, P, NT>& q, Running<P, NT>& run,
+                                          const uint8_t* stage) {
+  constexpr int J = P / 16, KC = P / 32;
+  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int total = q.total, base = total / kBlockTokens * kBlockTokens, tok = 4 * (g >> 1) + (g & 1);
+  if (base > q.last_limit) return;
+  const uint16_t* keys = reinterpret_cast<const uint16_t*>(stage);
+  const uint16_t* values = keys + cache_slot_bytes(P) / 2;
+  float s[1][NT][4];
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) s[0][n][e] = 0.f;
+  float sq[2] = {0.f, 0.f};
+  uint32_t qt[NT][P / 16][2];
+#pragma unroll
+  for (int n = 0; n < NT; ++n) load_q<P>(a, q.b, q.h, q.c0 + n * 8 + g, t, qt[n]);
+#pragma unroll
+  for (int d = 0; d < P / 64; ++d) {
+    uint32_t r[2][8];
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      const bool there = base + tok + 2 * half < total;
+      const uint4* row = reinterpret_cast<const uint4*>(keys + (tok + 2 * half) * P + d * 64 + t * 16);
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const uint4 x = there ? row[e] : make_uint4(0, 0, 0, 0);
+        r[half][4 * e] = x.x;
+        r[half][4 * e + 1] = x.y;
+        r[half][4 * e + 2] = x.z;
+        r[half][4 * e + 3] = x.w;
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float2 f = unpack2<kBf16>(r[half][i]);
+        sq[half] = fmaf(f.x, f.x, fmaf(f.y, f.y, sq[half]));
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t A[4] = {r[0][2 * i], r[1][2 * i], r[0][2 * i + 1], r[1][2 * i + 1]};
+#pragma unroll
+      for (int n = 0; n < NT; ++n) mma16816<kBf16>(s[0][n], A, qt[n][d * 4 + i][0], qt[n][d * 4 + i][1]);
+    }
+  }
+#pragma unroll
+  for (int x = 1; x < 4; x <<= 1) {
+    sq[0] += __shfl_xor_sync(0xffffffffu, sq[0], x);
+    sq[1] += __shfl_xor_sync(0xffffffffu, sq[1], x);
+  }
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int token = base + tok + 2 * (e / 2);
+      s[0][n][e] = token <= q.limit[n][e % 2] && token < total ? fmaf(s[0][n][e], 2.f * a.scale, -a.scale * sq[e / 2]) : -INFINITY;
+    }
+  run.weigh(s);
+  uint32_t p[NT][2];
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    p[n][0] = transpose8(pack2<kBf16>(s[0][n][0], s[0][n][1]));
+    p[n][1] = transpose8(pack2<kBf16>(s[0][n][2], s[0][n][3]));
+  }
+  uint2 x[KC][4];                                  // dims 32 i + 4 g ... + 3 of tokens 4 t + r
+  bool odd = false;                                // a value that is not finite
+#pragma unroll
+  for (int i = 0; i < KC; ++i)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      x[i][r] = make_uint2(0, 0);
+      if (base + 4 * t + r < total) x[i][r] = *reinterpret_cast<const uint2*>(values + (4 * t + r) * P + 32 * i + 4 * g);
+      constexpr uint32_t kInf = kBf16 ? 0x7f80u : 0x7c00u;
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const uint32_t y = half ? x[i][r].y : x[i][r].x;
+        odd |= (y & kInf) == kInf || (y >> 16 & kInf) == kInf;
+      }
+    }
+  // A product 0 * inf of a column that does not see the token must not reach it: such blocks go token by token.
+  const bool slow = __any_sync(0xffffffffu, odd) && total - 1 > q.first_limit;
+#pragma unroll 1
+  for (int only = slow ? 0 : kBlockTokens - 1; only < kBlockTokens; ++only) {
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+      uint32_t A[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {                // row g: dim 4 g + 2 (j % 2), row g + 8: the next; k 2t.. : tokens 0, 1 then 2, 3
+        uint32_t lo = j % 2 ? x[j / 2][e / 2 * 2].y : x[j / 2][e / 2 * 2].x;
+        uint32_t hi = j % 2 ? x[j / 2][e / 2 * 2 + 1].y : x[j / 2][e / 2 * 2 + 1].x;
+        if (slow) {
+          if (only != 4 * t + e / 2 * 2) lo = 0;
+          if (only != 4 * t + e / 2 * 2 + 1) hi = 0;
+        }
+        A[e] = __byte_perm(lo, hi, e % 2 ? 0x7632 : 0x5410);
+      }
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        float acc[4] = {0.f, 0.f, 0.f, 0.f};
+        mma16816<kBf16>(acc, A, p[n][0], p[n][1]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (!slow || base + only <= q.limit[n][e % 2]) run.o[j][n][e] += acc[e];
+      }
+    }
+  }
+}
+
+// 1 / l, or what the weights of the variant without a denominator lack; 0 where nothing was seen. m, l: of all its tokens.
+__device__ __forceinline__ float last_factor(const CacheAttnArgs& a, float m, float l, float q_sq) {
+  if (m == -INFINITY && l == 0.f) return 0.f;
+  return a.softmax ? 1.f / l : attn_ex2((m == -INFINITY ? 0.f : m) - q_sq);
+}
+
 template <bool kBf16, int P, int NT>
 __global__ void __launch_bounds__(kAttnWarps * 32) cache_attn_kernel(const CacheAttnArgs a) {
-  using T = Tile<P>;
-  constexpr int UB = T::kUnitBlocks, KC = T::kChunks, J = T::kDims;
-  constexpr int kSlot = cache_slot_bytes(P), kBytes = cache_page_bytes(P);
+  constexpr int UB = 256 / P, KC = P / 32;
+  using T = Tile<P, UB>;
+  constexpr int kBytes = cache_page_bytes(P);
   extern __shared__ __align__(128) uint8_t smem[];
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   uint8_t* ring = smem + (threadIdx.x >> 5) * (kStages * T::kStage);       // a warp has its own
@@ -230,24 +568,24 @@ __global__ void __launch_bounds__(kAttnWarps * 32) cache_attn_kernel(const Cache
   const int64_t self = static_cast<int64_t>(threadIdx.x >> 5) * gridDim.x + blockIdx.x;    // neighbours on other SMs
   const int segments = a.column_tiles * a.H;       // of a sequence
   int64_t unused, all;
-  sum_units<P>(a, 0, unused, all);
+  sum_units<UB>(a, 0, unused, all);
   const Deal deal(all * segments, workers);
-  int64_t pos = deal.begin(self);
+  int64_t at = deal.begin(self);
   const int64_t stop = deal.begin(self + 1);
-  if (pos >= stop) return;
+  if (at >= stop) return;
 
   // the sequence of the first unit
   int b = 0;
   int64_t seq_begin = 0;
   for (; b < a.B; b += 32) {
-    const int64_t mine = b + lane < a.B ? static_cast<int64_t>(Units<P>(a, b + lane).count) * segments : 0;
+    const int64_t mine = b + lane < a.B ? static_cast<int64_t>(Units<UB>(a, b + lane).count) * segments : 0;
     int64_t upto = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const int64_t x = __shfl_up_sync(0xffffffffu, upto, o);
       if (lane >= o) upto += x;
     }
-    const unsigned past = __ballot_sync(0xffffffffu, seq_begin + upto > pos);
+    const unsigned past = __ballot_sync(0xffffffffu, seq_begin + upto > at);
     if (past != 0) {
       const int l = __ffs(past) - 1;
       seq_begin += __shfl_sync(0xffffffffu, upto - mine, l);
@@ -259,15 +597,15 @@ __global__ void __launch_bounds__(kAttnWarps * 32) cache_attn_kernel(const Cache
 
   // ---- loads: lane i looks up the i-th of the next 32 units, so that page numbers are waited for once in 32 units
   struct Lookup {
-    const uint8_t* base;                           // of the head's page, null where there is nothing to load
-    int what;                                      // complete blocks: first in the page | count << 8; incomplete: tokens | 1 << 16
+    const uint8_t* page;                           // the head's part, null where there is nothing to load
+    int what;                                      // see fetch_unit
   };
   int look_b = b;                                  // this lane's sequence
   int64_t look_begin = seq_begin;
   auto look_up = [&](int64_t x) {
     Lookup r{nullptr, 0};
     while (x < stop && look_b < a.B) {
-      const Units<P> units(a, look_b);
+      const Units<UB> units(a, look_b);
       const int64_t span = static_cast<int64_t>(units.count) * segments;
       if (x >= look_begin + span) {
         look_begin += span;
@@ -278,48 +616,25 @@ __global__ void __launch_bounds__(kAttnWarps * 32) cache_attn_kernel(const Cache
       const int u = static_cast<int>(in % units.count), h = static_cast<int>(in / units.count % a.H);
       const int total = units.held + units.fresh, blocks = total / kBlockTokens;
       const int first = u < units.groups ? u * UB : blocks;
-      r.base = cache_page(a.pages, a.table, look_b, a.max_pages, a.num_pages, a.H, h, kBytes, first * kBlockTokens);
+      r.page = cache_page(a.pages, a.table, look_b, a.max_pages, a.num_pages, a.H, h, kBytes, first * kBlockTokens);
       r.what = u < units.groups ? first % kPageBlocks | min(UB, blocks - first) << 8 : total % kBlockTokens | 1 << 16;
       break;
     }
     return r;
   };
-  Lookup now = look_up(pos + lane), next = look_up(pos + 32 + lane);
+  const int64_t start = at, mine = stop - at;
+  Lookup now = look_up(start + lane), next = look_up(start + 32 + lane);
   int64_t fetched = 0;                             // units asked for
-  const int64_t mine = stop - pos;
   auto fetch = [&]() {
     if (fetched < mine) {
       const int from = static_cast<int>(fetched & 31);
       if (from == 0 && fetched != 0) {
         now = next;
-        next = look_up(pos + fetched + 32 + lane);
+        next = look_up(start + fetched + 32 + lane);
       }
-      const uint64_t base64 = __shfl_sync(0xffffffffu, reinterpret_cast<uint64_t>(now.base), from);
-      const int what = __shfl_sync(0xffffffffu, now.what, from);
-      const uint8_t* base = reinterpret_cast<const uint8_t*>(base64);
-      uint8_t* stage = ring + static_cast<int>(fetched % kStages) * T::kStage;
-      const uint32_t to = smem_u32(stage);
-      if (lane == 0) *reinterpret_cast<int*>(stage + T::kFlag) = base != nullptr;
-      if (base != nullptr) {
-        if (what >> 16) {
-          const uint8_t* src = base + kPageHeader + kPageBlocks * kSlot + lane * 16;
-#pragma unroll
-          for (int i = 0; i < 2 * kSlot / 512; ++i)          // keys, then values
-            if ((i % (kSlot / 512) * 512 + lane * 16) / (2 * P) < (what & 0xff)) copy16(to + i * 512 + lane * 16, src + i * 512);
-        } else {
-          const uint8_t* src = base + kPageHeader + (what & 0xff) * kSlot + lane * 16;
-          const int bytes = (what >> 8) * kSlot;
-          if (bytes == UB * kSlot) {
-#pragma unroll
-            for (int i = 0; i < UB * kSlot / 512; ++i) copy16(to + i * 512 + lane * 16, src + i * 512);
-          } else {
-#pragma unroll
-            for (int i = 0; i < UB * kSlot / 512; ++i)
-              if (i * 512 < bytes) copy16(to + i * 512 + lane * 16, src + i * 512);
-          }
-          if (lane < UB / 2) copy16(to + T::kScales + lane * 16, base + (what & 0xff) * 8 + lane * 16);
-        }
-      }
+      const uint64_t page = __shfl_sync(0xffffffffu, reinterpret_cast<uint64_t>(now.page), from);
+      fetch_unit<P, UB>(ring + static_cast<int>(fetched % kStages) * T::kStage, reinterpret_cast<const uint8_t*>(page),
+                        __shfl_sync(0xffffffffu, now.what, from));
       ++fetched;
     }
     copies_close();
@@ -328,87 +643,20 @@ __global__ void __launch_bounds__(kAttnWarps * 32) cache_attn_kernel(const Cache
   for (int i = 0; i < kStages - 1; ++i) fetch();
 
   int64_t taken = 0;                               // units worked on
-  int64_t at = pos;
   while (at < stop && b < a.B) {
-    const Units<P> units(a, b);
+    const Units<UB> units(a, b);
     if (at >= seq_begin + static_cast<int64_t>(units.count) * segments) {  // on to the next sequence (some have no units)
       seq_begin += static_cast<int64_t>(units.count) * segments;
       ++b;
       continue;
     }
-    const int total = units.held + units.fresh;
     const int seg = static_cast<int>((at - seq_begin) / units.count);
     const int u0 = static_cast<int>((at - seq_begin) % units.count);
     const int64_t left = stop - at;
     const int u1 = left < units.count - u0 ? u0 + static_cast<int>(left) : units.count;
     const int h = seg % a.H, c0 = seg / a.H * (8 * NT);
-
-    // ---- queries: operand columns, their scales, and how far each column sees
-    uint32_t qh[NT][P / 16][2];                      // fp16, scaled
-    float qmul[NT][2], qsq[NT][2];                   // of columns 2t, 2t + 1
-    int limit[NT][2];                                // last token that the column sees
-    // operand words of column n * 8 + g as they are in memory: k step i has dims 64 (i / 4) + 16 t + 4 (i % 4) ... + 3
-    auto load_q = [&](int n, uint32_t (&w)[P / 16][2]) {
-      const int c = c0 + n * 8 + g;
-      const bool real = c < a.T * a.G;
-      const uint16_t* q = q_row(a, b, h, real ? c : 0);
-#pragma unroll
-      for (int d = 0; d < P / 64; ++d) {
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int col = d * 64 + t * 16 + e * 8;
-          uint4 raw = make_uint4(0, 0, 0, 0);
-          if (real && col < a.D) raw = *reinterpret_cast<const uint4*>(q + col);
-          w[d * 4 + e * 2][0] = raw.x;
-          w[d * 4 + e * 2][1] = raw.y;
-          w[d * 4 + e * 2 + 1][0] = raw.z;
-          w[d * 4 + e * 2 + 1][1] = raw.w;
-        }
-      }
-    };
-#pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      uint32_t raw[P / 16][2];
-      load_q(n, raw);
-      uint32_t top = 0;
-      float sq = 0.f;
-#pragma unroll
-      for (int i = 0; i < P / 16; ++i) {
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const float2 f = unpack2<kBf16>(raw[i][e]);
-          top = max(top, max(__float_as_uint(f.x) & 0x7fffffffu, __float_as_uint(f.y) & 0x7fffffffu));
-          sq = fmaf(f.x, f.x, fmaf(f.y, f.y, sq));
-        }
-      }
-#pragma unroll
-      for (int o = 1; o < 4; o <<= 1) {
-        top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-        sq += __shfl_xor_sync(0xffffffffu, sq, o);
-      }
-      uint32_t exponent = top >> 23;                 // of the largest element; zero and infinity keep their meaning
-      exponent = exponent == 0 ? 127u : min(exponent, 253u);
-      const float down = __uint_as_float((254u - exponent) << 23), up = __uint_as_float(exponent << 23);
-#pragma unroll
-      for (int i = 0; i < P / 16; ++i) {
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const float2 f = unpack2<kBf16>(raw[i][e]);
-          qh[n][i][e] = pack2<false>(f.x * down, f.y * down);
-        }
-      }
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int from = (2 * t + e) * 4;
-        qmul[n][e] = 2.f * a.scale * __shfl_sync(0xffffffffu, up, from);
-        qsq[n][e] = a.scale * __shfl_sync(0xffffffffu, sq, from);
-        const int c2 = c0 + n * 8 + 2 * t + e;
-        limit[n][e] = c2 < a.T * a.G ? units.held + c2 / a.G : total - 1;
-      }
-    }
-    const int first_limit = units.held + c0 / a.G;   // every column of the tile sees at least this far,
-    const int last_limit = units.held + (c0 + 8 * NT - 1) / a.G;           // and none further than this
-
+    Queries<kBf16, P, NT> q;
+    q.load(a, b, h, c0, units.held, units.held + units.fresh);
     Running<P, NT> run;
     run.clear();
     for (int u = u0; u < u1; ++u) {
@@ -417,214 +665,12 @@ __global__ void __launch_bounds__(kAttnWarps * 32) cache_attn_kernel(const Cache
       fetch();
       ++taken;
       if (*reinterpret_cast<const int*>(stage + T::kFlag) == 0) continue;  // a page outside the pool: its tokens are absent
-      if (u < units.groups) {
-        // ================================================================ complete blocks
-        const int begin = u * T::kUnit;              // first token
-        if (begin > last_limit) continue;
-        const int whole = min(UB, total / kBlockTokens - begin / kBlockTokens);
-        const bool hidden = begin + T::kUnit - 1 > first_limit;
-        const float2* scales = reinterpret_cast<const float2*>(stage + T::kScales);
-        float s[UB][NT][4];
-#pragma unroll
-        for (int k = 0; k < UB; ++k) {
-#pragma unroll
-          for (int n = 0; n < NT; ++n)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) s[k][n][e] = -INFINITY;
-          if (k >= whole) continue;
-          const float scale = scales[k].x;
-          const uint4* key = reinterpret_cast<const uint4*>(stage + k * kSlot) + lane;
-          int sq0 = 0, sq1 = 0;
-          float acc[NT][4];
-#pragma unroll
-          for (int n = 0; n < NT; ++n)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) acc[n][e] = 0.f;
-#pragma unroll
-          for (int d = 0; d < P / 64; ++d) {
-            const uint4 w0 = key[2 * d * 32], w1 = key[(2 * d + 1) * 32];
-            const uint32_t r0[4] = {w0.x, w0.y, w0.z, w0.w}, r1[4] = {w1.x, w1.y, w1.z, w1.w};
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              sq0 += dot4(r0[i]);
-              sq1 += dot4(r1[i]);
-              const uint32_t A[4] = {codes_lo(r0[i]), codes_lo(r1[i]), codes_hi(r0[i]), codes_hi(r1[i])};
-#pragma unroll
-              for (int n = 0; n < NT; ++n) mma16816<false>(acc[n], A, qh[n][d * 4 + i][0], qh[n][d * 4 + i][1]);
-            }
-          }
-#pragma unroll
-          for (int x = 1; x < 4; x <<= 1) {
-            sq0 += __shfl_xor_sync(0xffffffffu, sq0, x);
-            sq1 += __shfl_xor_sync(0xffffffffu, sq1, x);
-          }
-          const float bias = a.scale * scale * scale;
-          const float b0 = bias * static_cast<float>(sq0), b1 = bias * static_cast<float>(sq1);
-#pragma unroll
-          for (int n = 0; n < NT; ++n) {
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              const float mul = qmul[n][e] * scale;
-              s[k][n][e] = fmaf(acc[n][e], mul, -b0);
-              s[k][n][2 + e] = fmaf(acc[n][2 + e], mul, -b1);
-            }
-          }
-          if (hidden) {
-            const int tok = begin + k * kBlockTokens + 4 * (g >> 1) + (g & 1);
-#pragma unroll
-            for (int n = 0; n < NT; ++n)
-#pragma unroll
-              for (int e = 0; e < 4; ++e)
-                if (tok + 2 * (e / 2) > limit[n][e % 2]) s[k][n][e] = -INFINITY;
-          }
-        }
-        run.weigh(s);
-#pragma unroll
-        for (int k = 0; k < UB; ++k) {
-          if (k >= whole) continue;
-          uint32_t p[NT][2];
-#pragma unroll
-          for (int n = 0; n < NT; ++n) {
-            p[n][0] = transpose8(pack2<false>(s[k][n][0], s[k][n][1]));
-            p[n][1] = transpose8(pack2<false>(s[k][n][2], s[k][n][3]));
-          }
-          const uint4* value = reinterpret_cast<const uint4*>(stage + k * kSlot + 16 * P) + lane;
-          const float scale = scales[k].y;
-          const bool finite = fabsf(scale) < INFINITY;
-          const int base = begin + k * kBlockTokens;
-#pragma unroll
-          for (int i = 0; i < KC; ++i) {
-            const uint4 w = value[i * 32];
-#pragma unroll
-            for (int half = 0; half < 2; ++half) {
-              const uint32_t r0 = half ? w.z : w.x, r1 = half ? w.w : w.y;
-              const uint32_t A[4] = {codes_lo(r0), codes_lo(r1), codes_hi(r0), codes_hi(r1)};
-#pragma unroll
-              for (int n = 0; n < NT; ++n) {
-                float acc[4] = {0.f, 0.f, 0.f, 0.f};
-                mma16816<false>(acc, A, p[n][0], p[n][1]);
-                float(&o)[4] = run.o[2 * i + half][n];
-#pragma unroll
-                for (int e = 0; e < 4; ++e)           // a block that is not finite reaches the columns that see it
-                  if (finite || base <= limit[n][e % 2]) o[e] = fmaf(acc[e], scale, o[e]);
-              }
-            }
-          }
-        }
-      } else {
-        // ================================================================ the incomplete block, in 16 bits
-        const int base = total / kBlockTokens * kBlockTokens, tok = 4 * (g >> 1) + (g & 1);
-        if (base > last_limit) continue;
-        const uint16_t* keys = reinterpret_cast<const uint16_t*>(stage);
-        const uint16_t* values = keys + kSlot / 2;
-        float s[1][NT][4];
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) s[0][n][e] = 0.f;
-        float sq[2] = {0.f, 0.f};
-        uint32_t qt[NT][P / 16][2];
-#pragma unroll
-        for (int n = 0; n < NT; ++n) load_q(n, qt[n]);
-#pragma unroll
-        for (int d = 0; d < P / 64; ++d) {
-          uint32_t r[2][8];
-#pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            const bool row_there = base + tok + 2 * half < total;
-            const uint4* row = reinterpret_cast<const uint4*>(keys + (tok + 2 * half) * P + d * 64 + t * 16);
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              const uint4 x = row_there ? row[e] : make_uint4(0, 0, 0, 0);
-              r[half][4 * e] = x.x;
-              r[half][4 * e + 1] = x.y;
-              r[half][4 * e + 2] = x.z;
-              r[half][4 * e + 3] = x.w;
-            }
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              const float2 f = unpack2<kBf16>(r[half][i]);
-              sq[half] = fmaf(f.x, f.x, fmaf(f.y, f.y, sq[half]));
-            }
-          }
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const uint32_t A[4] = {r[0][2 * i], r[1][2 * i], r[0][2 * i + 1], r[1][2 * i + 1]};
-#pragma unroll
-            for (int n = 0; n < NT; ++n) mma16816<kBf16>(s[0][n], A, qt[n][d * 4 + i][0], qt[n][d * 4 + i][1]);
-          }
-        }
-#pragma unroll
-        for (int x = 1; x < 4; x <<= 1) {
-          sq[0] += __shfl_xor_sync(0xffffffffu, sq[0], x);
-          sq[1] += __shfl_xor_sync(0xffffffffu, sq[1], x);
-        }
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int token = base + tok + 2 * (e / 2);
-            s[0][n][e] = token <= limit[n][e % 2] && token < total ? fmaf(s[0][n][e], 2.f * a.scale, -a.scale * sq[e / 2]) : -INFINITY;
-          }
-        run.weigh(s);
-        uint32_t p[NT][2];
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          p[n][0] = transpose8(pack2<kBf16>(s[0][n][0], s[0][n][1]));
-          p[n][1] = transpose8(pack2<kBf16>(s[0][n][2], s[0][n][3]));
-        }
-        uint2 x[KC][4];                              // dims 32 i + 4 g ... + 3 of tokens 4 t + r
-        bool odd = false;                            // a value that is not finite
-#pragma unroll
-        for (int i = 0; i < KC; ++i)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            x[i][r] = make_uint2(0, 0);
-            if (base + 4 * t + r < total) x[i][r] = *reinterpret_cast<const uint2*>(values + (4 * t + r) * P + 32 * i + 4 * g);
-            constexpr uint32_t kInf = kBf16 ? 0x7f80u : 0x7c00u;
-#pragma unroll
-            for (int half = 0; half < 2; ++half) {
-              const uint32_t y = half ? x[i][r].y : x[i][r].x;
-              odd |= (y & kInf) == kInf || (y >> 16 & kInf) == kInf;
-            }
-          }
-        // A product 0 * inf of a column that does not see the token must not reach it: such blocks go token by token.
-        const bool slow = __any_sync(0xffffffffu, odd) && total - 1 > first_limit;
-#pragma unroll 1
-        for (int only = slow ? 0 : kBlockTokens - 1; only < kBlockTokens; ++only) {
-#pragma unroll
-          for (int j = 0; j < J; ++j) {
-            uint32_t A[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {            // row g: dim 4 g + 2 (j % 2), row g + 8: the next; k 2t.. : tokens 0, 1 then 2, 3
-              uint32_t lo = j % 2 ? x[j / 2][e / 2 * 2].y : x[j / 2][e / 2 * 2].x;
-              uint32_t hi = j % 2 ? x[j / 2][e / 2 * 2 + 1].y : x[j / 2][e / 2 * 2 + 1].x;
-              if (slow) {
-                if (only != 4 * t + e / 2 * 2) lo = 0;
-                if (only != 4 * t + e / 2 * 2 + 1) hi = 0;
-              }
-              A[e] = __byte_perm(lo, hi, e % 2 ? 0x7632 : 0x5410);
-            }
-#pragma unroll
-            for (int n = 0; n < NT; ++n) {
-              float acc[4] = {0.f, 0.f, 0.f, 0.f};
-              mma16816<kBf16>(acc, A, p[n][0], p[n][1]);
-#pragma unroll
-              for (int e = 0; e < 4; ++e)
-                if (!slow || base + only <= limit[n][e % 2]) run.o[j][n][e] += acc[e];
-            }
-          }
-        }
-      }
+      if (u < units.groups) codes_unit<kBf16, P, NT, UB>(a, q, run, stage, u * T::kUnit);
+      else rest_unit<kBf16, P, NT>(a, q, run, stage);
     }
 
     // ---- the segment's output, or this warp's part of it
-#pragma unroll
-    for (int n = 0; n < NT; ++n)
-#pragma unroll
-      for (int e = 0; e < 2; ++e)
-#pragma unroll
-        for (int w = 4; w < 32; w <<= 1) run.l[n][e] += __shfl_xor_sync(0xffffffffu, run.l[n][e], w);
+    run.sum_up();
     const bool complete = u0 == 0 && u1 == units.count;
     float* part = part_of<P, NT>(a, 2 * self + (u0 == 0));
 #pragma unroll
@@ -635,7 +681,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32) cache_attn_kernel(const Cache
         if (c >= a.T * a.G) continue;
         const float m = run.m[n][e], l = run.l[n][e];
         if (complete) {
-          const float f = m == -INFINITY ? 0.f : a.softmax ? 1.f / l : attn_ex2(m - qsq[n][e]);
+          const float f = last_factor(a, m, l, q.sq[n][e]);
           const bool none = c / a.G >= units.fresh || (m == -INFINITY && l == 0.f);
           uint16_t* out = static_cast<uint16_t*>(a.out) + out_offset(a, b, h, c);
 #pragma unroll
@@ -648,10 +694,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32) cache_attn_kernel(const Cache
             *reinterpret_cast<uint2*>(out + d) = y;
           }
         } else {
-#pragma unroll
-          for (int i = 0; i < KC; ++i)
-            *reinterpret_cast<float4*>(part + in * P + 32 * i + 4 * g) =
-                make_float4(run.o[2 * i][n][e], run.o[2 * i][n][2 + e], run.o[2 * i + 1][n][e], run.o[2 * i + 1][n][2 + e]);
+          run.store(part + in * P, n, e);
           if (g == 0) {
             part[8 * NT * P + in] = m;
             part[8 * NT * (P + 1) + in] = l;
@@ -661,6 +704,152 @@ __global__ void __launch_bounds__(kAttnWarps * 32) cache_attn_kernel(const Cache
     at += u1 - u0;
   }
   grid_dependents_launch();
+}
+
+// A segment per block, or per cluster of blocks, whose warps take its units in turn: for short sequences, whose time is the
+// chain of one load after another. There is no dealing out, no second kernel and no workspace; the warps' parts are joined in
+// shared memory, the blocks' through the cluster's, in a fixed order.
+template <bool kBf16, int P>
+__global__ void __launch_bounds__(kAttnWarps * 32) cache_attn_short_kernel(const CacheAttnArgs a) {
+  constexpr int UB = 2, NT = 1, kRing = 2;
+  using T = Tile<P, UB>;
+  constexpr int kBytes = cache_page_bytes(P);
+  static_assert(kRing * T::kStage >= (8 * P + 16) * 4, "a warp's part takes the place of its ring");
+  extern __shared__ __align__(128) uint8_t smem[];
+  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, warp = threadIdx.x >> 5;
+  uint8_t* ring = smem + warp * (kRing * T::kStage);
+  uint32_t rank, ranks;
+  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
+  asm("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(ranks));
+  const int segment = static_cast<int>(blockIdx.x / ranks), b = segment / a.H, h = segment % a.H;
+  const Units<UB> units(a, b);
+  const int total = units.held + units.fresh, blocks = total / kBlockTokens;
+  const int each = kAttnWarps * static_cast<int>(ranks), first = static_cast<int>(rank) * kAttnWarps + warp;
+  const int mine = units.count > first ? (units.count - first + each - 1) / each : 0;
+
+  const uint8_t* page = nullptr;                   // of this lane's unit among the next 32 of the warp
+  int what = 0;
+  auto look_up = [&](int i) {
+    page = nullptr;
+    const int u = first + (i + lane) * each;
+    if (i + lane >= mine) return;
+    const int block = u < units.groups ? u * UB : blocks;
+    page = cache_page(a.pages, a.table, b, a.max_pages, a.num_pages, a.H, h, kBytes, block * kBlockTokens);
+    what = u < units.groups ? block % kPageBlocks | min(UB, blocks - block) << 8 : total % kBlockTokens | 1 << 16;
+  };
+  int fetched = 0;
+  auto fetch = [&]() {
+    if (fetched < mine) {
+      if (fetched % 32 == 0) look_up(fetched);
+      const uint64_t p = __shfl_sync(0xffffffffu, reinterpret_cast<uint64_t>(page), fetched & 31);
+      fetch_unit<P, UB>(ring + fetched % kRing * T::kStage, reinterpret_cast<const uint8_t*>(p),
+                        __shfl_sync(0xffffffffu, what, fetched & 31));
+      ++fetched;
+    }
+    copies_close();
+  };
+#pragma unroll
+  for (int i = 0; i < kRing; ++i) fetch();
+  Queries<kBf16, P, NT> q;
+  Running<P, NT> run;
+  run.clear();
+  if (units.count > 0) q.load(a, b, h, 0, units.held, total);
+  for (int i = 0; i < mine; ++i) {
+    const uint8_t* stage = ring + i % kRing * T::kStage;
+    copies_wait<kRing - 1>();
+    if (*reinterpret_cast<const int*>(stage + T::kFlag) != 0) {
+      const int u = first + i * each;
+      if (u < units.groups) codes_unit<kBf16, P, NT, UB>(a, q, run, stage, u * T::kUnit);
+      else rest_unit<kBf16, P, NT>(a, q, run, stage);
+    }
+    __syncwarp();                                  // every lane has read the stage
+    fetch();
+  }
+
+  // ---- join: the warps', then the blocks'
+  run.sum_up();
+  const int columns = a.T * a.G;
+  float* part = reinterpret_cast<float*>(ring);    // 8 x P outputs, 8 maxima, 8 sums
+  __syncwarp();
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    run.store(part + (2 * t + e) * P, 0, e);
+    if (g == 0) {
+      part[8 * P + 2 * t + e] = run.m[0][e];
+      part[8 * P + 8 + 2 * t + e] = run.l[0][e];
+    }
+  }
+  __syncthreads();
+  constexpr int kPart = kRing * T::kStage / 4;     // floats from one warp's part to the next
+  float* parts = reinterpret_cast<float*>(smem);
+  constexpr int kPerColumn = P / 4;                // threads of a column, four dims each
+  const int used = columns * kPerColumn;
+  // y, m and l of column i / kPerColumn from `count` parts `pitch` floats apart
+  struct Joined {
+    float m, l;
+    float4 y;
+    __device__ void add(float m2, float l2, float4 y2) {
+      const float x = fmaxf(m, m2), ref = x == -INFINITY ? 0.f : x;
+      const float f0 = attn_ex2(m - ref), f1 = attn_ex2(m2 - ref);
+      m = x;
+      l = l * f0 + l2 * f1;
+      y = make_float4(y.x * f0 + y2.x * f1, y.y * f0 + y2.y * f1, y.z * f0 + y2.z * f1, y.w * f0 + y2.w * f1);
+    }
+  };
+  auto write = [&](int i, const Joined& j) {
+    const int c = i / kPerColumn, d = i % kPerColumn * 4;
+    if (d >= a.D) return;
+    float f = 0.f;
+    if (c / a.G < units.fresh) f = last_factor(a, j.m, j.l, parts[8 * P + 16 + c]);
+    uint2 y = make_uint2(pack2<kBf16>(j.y.x * f, j.y.y * f), pack2<kBf16>(j.y.z * f, j.y.w * f));
+    if (c / a.G >= units.fresh || (j.m == -INFINITY && j.l == 0.f)) y = make_uint2(0, 0);
+    *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.out) + out_offset(a, b, h, c) + d) = y;
+  };
+  if (warp == 0 && g == 0)                         // |q|^2, which every warp has
+    for (int e = 0; e < 2; ++e) parts[8 * P + 16 + 2 * t + e] = units.count > 0 ? q.sq[0][e] : 0.f;
+  __syncthreads();
+  for (int i = threadIdx.x; i < used; i += kAttnWarps * 32) {
+    const int c = i / kPerColumn, at = c * P + i % kPerColumn * 4;
+    Joined j{-INFINITY, 0.f, make_float4(0.f, 0.f, 0.f, 0.f)};
+#pragma unroll
+    for (int w = 0; w < kAttnWarps; ++w) {
+      const float* p = parts + w * kPart;
+      j.add(p[8 * P + c], p[8 * P + 8 + c], *reinterpret_cast<const float4*>(p + at));
+    }
+    if (ranks == 1) {
+      write(i, j);
+    } else {                                       // the block's part, where the second warp's was: read by this thread alone
+      float* p = parts + kPart;
+      *reinterpret_cast<float4*>(p + at) = j.y;
+      if (i % kPerColumn == 0) {
+        p[8 * P + 32 + c] = j.m;
+        p[8 * P + 40 + c] = j.l;
+      }
+    }
+  }
+  if (ranks == 1) return;
+  __syncwarp();
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+  if (rank == 0) {
+    for (int i = threadIdx.x; i < used; i += kAttnWarps * 32) {
+      const int c = i / kPerColumn, at = c * P + i % kPerColumn * 4;
+      Joined j{-INFINITY, 0.f, make_float4(0.f, 0.f, 0.f, 0.f)};
+      for (uint32_t r = 0; r < ranks; ++r) {
+        uint32_t there;
+        asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(smem_u32(parts + kPart)), "r"(r));
+        float m2, l2;
+        float4 y2;
+        asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(m2) : "r"(there + (8 * P + 32 + c) * 4));
+        asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(l2) : "r"(there + (8 * P + 40 + c) * 4));
+        asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                     : "=f"(y2.x), "=f"(y2.y), "=f"(y2.z), "=f"(y2.w) : "r"(there + at * 4));
+        j.add(m2, l2, y2);
+      }
+      write(i, j);
+    }
+  }
+  __syncwarp();
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");   // blocks stay until they have been read
 }
 
 constexpr int kJoinWarps = 8;
@@ -682,10 +871,10 @@ __global__ void __launch_bounds__(kJoinWarps * 32) cache_join_kernel(const Cache
   float y[kPer] = {}, top = -INFINITY, sum = 0.f;
   bool write = b < a.B && c < a.T * a.G, some = false;
   if (write) {
-    const Units<P> units(a, b);
+    const Units<256 / P> units(a, b);
     if (units.count > 0) {
       int64_t before, all;
-      sum_units<P>(a, b, before, all);
+      sum_units<256 / P>(a, b, before, all);
       const Deal deal(all * segments, workers);
       const int64_t begin = before * segments + static_cast<int64_t>(seg) * units.count;
       const int64_t first = min(deal.worker(begin), workers - 1), last = min(deal.worker(begin + units.count - 1), workers - 1);
@@ -743,7 +932,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) cache_join_kernel(const Cache
   }
   if (!write) return;
   if (some) {
-    float f = 1.f / sum;
+    float q_sq = 0.f;
     if (!a.softmax) {
       const uint16_t* q = q_row(a, b, h, c);
       float sq = 0.f;
@@ -753,9 +942,9 @@ __global__ void __launch_bounds__(kJoinWarps * 32) cache_join_kernel(const Cache
       }
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) sq += __shfl_xor_sync(0xffffffffu, sq, o);
-      f = attn_ex2((top == -INFINITY ? 0.f : top) - a.scale * sq);
+      q_sq = a.scale * sq;
     }
-    if (top == -INFINITY && sum == 0.f) f = 0.f;
+    const float f = last_factor(a, top, sum, q_sq);
 #pragma unroll
     for (int i = 0; i < kPer; ++i) y[i] *= f;
   }
@@ -767,7 +956,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) cache_join_kernel(const Cache
 
 template <bool kBf16, int P, int NT>
 cudaError_t attn_t(const CacheAttnArgs& a, int sms, cudaStream_t stream) {
-  constexpr int kSmem = kAttnWarps * kStages * Tile<P>::kStage;
+  constexpr int kSmem = kAttnWarps * kStages * Tile<P, 256 / P>::kStage;
   static PerDeviceFlags flags;
   cudaError_t e = ensure_dynamic_smem(cache_attn_kernel<kBf16, P, NT>, kSmem, flags);
   if (e != cudaSuccess) return e;
@@ -781,8 +970,44 @@ cudaError_t attn_t(const CacheAttnArgs& a, int sms, cudaStream_t stream) {
                           static_cast<int64_t>(sms) * kAttnWarps, split);
 }
 
+// Blocks of a cluster that share a segment in the kernel for short sequences, 0: not that kernel. It is for one tile of columns
+// and page tables of up to kShort tokens - what the lengths are is known on the device alone. A block's warps have the units
+// of 256 tokens (128 at 128 columns) in flight at a time; more blocks where the segments leave SMs free and have units for them.
+constexpr int kShort = 4096;
+int short_ranks(const CacheAttnArgs& a, int P, int sms) {
+  if (static_cast<int64_t>(a.T) * a.G > 8 || a.max_pages > kShort / kPageTokens) return 0;
+  const int64_t segments = static_cast<int64_t>(a.B) * a.H, units = static_cast<int64_t>(a.max_pages) * kPageBlocks / 2;
+  int ranks = 1;
+  while (ranks < 8 && segments * ranks * 2 <= sms && units > kAttnWarps * ranks) ranks *= 2;
+  (void)P;
+  return ranks;
+}
+
+template <bool kBf16, int P>
+cudaError_t short_t(const CacheAttnArgs& a, int ranks, cudaStream_t stream) {
+  constexpr int kSmem = kAttnWarps * 2 * Tile<P, 2>::kStage;
+  static PerDeviceFlags flags;
+  const cudaError_t e = ensure_dynamic_smem(cache_attn_short_kernel<kBf16, P>, kSmem, flags);
+  if (e != cudaSuccess) return e;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = ranks;
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cudaLaunchConfig_t config{};
+  config.gridDim = dim3(static_cast<unsigned>(a.B) * a.H * ranks);
+  config.blockDim = dim3(kAttnWarps * 32);
+  config.dynamicSmemBytes = kSmem;
+  config.stream = stream;
+  config.attrs = &attr;
+  config.numAttrs = 1;
+  const cudaError_t launched = cudaLaunchKernelEx(&config, cache_attn_short_kernel<kBf16, P>, a);
+  if (launched != cudaSuccess) cudaGetLastError();
+  return launched;
+}
+
 template <bool kBf16, int P>
 cudaError_t attn_p(const CacheAttnArgs& a, int sms, cudaStream_t stream) {
+  if (const int ranks = short_ranks(a, P, sms)) return short_t<kBf16, P>(a, ranks, stream);
   return cache_attn_tiles(a.T, a.G, P) == 1 ? attn_t<kBf16, P, 1>(a, sms, stream) : attn_t<kBf16, P, 256 / P>(a, sms, stream);
 }
 

@@ -20,13 +20,15 @@ def _gen(seed):
 class Pool:
     """A pool with scattered pages, its table and lengths, and the tokens that were appended."""
 
-    def __init__(self, B, H, D, tokens, dtype, seed=0, extra=3):
+    def __init__(self, B, H, D, tokens, dtype, seed=0, extra=3, long=False):
         self.B, self.H, self.D, self.dtype = B, H, D, dtype
         self.max_pages = -(-tokens // PAGE)
         n = B * self.max_pages + extra
         self.pages = torch.randint(0, 256, (n, H, ops.cache_page_bytes(D)), dtype=torch.uint8, device=DEV, generator=_gen(seed))
         self.table = torch.randperm(n, device=DEV, generator=_gen(seed + 1))[:B * self.max_pages].to(torch.int32)
         self.table = self.table.view(B, self.max_pages)
+        if long:            # room for 8192 tokens: another kernel than for short sequences, whatever their lengths
+            self.table = torch.cat([self.table, self.table.new_full((B, 32 - self.max_pages), -1)], 1)
         self.lengths = torch.zeros(B, dtype=torch.int32, device=DEV)
         self.k = [torch.zeros(H, 0, D, dtype=dtype, device=DEV) for _ in range(B)]
         self.v = [torch.zeros(H, 0, D, dtype=dtype, device=DEV) for _ in range(B)]
@@ -144,9 +146,10 @@ def test_reading_a_range():
 @pytest.mark.parametrize("dtype", [BF16, FP16])
 @pytest.mark.parametrize("D", [64, 128, 80, 8])
 @pytest.mark.parametrize("lengths", LENGTHS)
-def test_single_tokens(D, lengths, dtype, softmax):
+@pytest.mark.parametrize("long", [False, True])
+def test_single_tokens(long, D, lengths, dtype, softmax):
     std = 1.0 if softmax else 0.5
-    pool = Pool(len(lengths), 2, D, 1024, dtype, seed=D)
+    pool = Pool(len(lengths), 2, D, 1024, dtype, seed=D, long=long)
     T = max(lengths)
     k, v = _randn(pool.B, 2, T, D, dtype=dtype, seed=7, std=std), _randn(pool.B, 2, T, D, dtype=dtype, seed=8)
     new = [min(n, 1) for n in lengths]
@@ -163,11 +166,12 @@ def test_single_tokens(D, lengths, dtype, softmax):
 @pytest.mark.parametrize("softmax", [True, False])
 @pytest.mark.parametrize("G,T", [(2, 1), (4, 3), (1, 9), (8, 1), (16, 2), (3, 37), (1, 100)])
 @pytest.mark.parametrize("D,dtype", [(64, BF16), (128, FP16), (80, BF16)])
-def test_several_columns(D, dtype, G, T, softmax):
+@pytest.mark.parametrize("long", [False, True])
+def test_several_columns(long, D, dtype, G, T, softmax):
     """Heads that share keys and chunks of tokens, padded to one length, histories that end anywhere."""
     std = 1.0 if softmax else 0.5
     before, new = [0, 3, 250, 600], [T, max(T - 1, 1), T, T // 2]
-    pool = Pool(4, 2, D, 768, dtype, seed=T)
+    pool = Pool(4, 2, D, 768, dtype, seed=T, long=long)
     pool.append(_randn(4, 2, 600, D, dtype=dtype, seed=10, std=std), _randn(4, 2, 600, D, dtype=dtype, seed=11), before)
     start = pool.lengths.clone()
     pool.append(_randn(4, 2, T, D, dtype=dtype, seed=12, std=std), _randn(4, 2, T, D, dtype=dtype, seed=13), new)
@@ -178,16 +182,18 @@ def test_several_columns(D, dtype, G, T, softmax):
         assert not got[b, :, new[b]:].any()
 
 
-@pytest.mark.parametrize("B,H,N", [(1, 1, 20000), (1, 8, 5000), (40, 3, 330), (300, 1, 40)])
-def test_shares_of_the_work(B, H, N):
+@pytest.mark.parametrize("B,H,N", [(1, 1, 20000), (1, 1, 4096), (3, 5, 2500), (1, 8, 5000), (40, 3, 330), (300, 1, 40)])
+@pytest.mark.parametrize("long", [False, True])
+@pytest.mark.parametrize("D", [64, 128])
+def test_shares_of_the_work(D, long, B, H, N):
     """Few long sequences that many warps share, many short ones of which a warp has several, all at once."""
     g = torch.Generator().manual_seed(N)
     new = [N] + [int(torch.randint(0, N + 1, (1,), generator=g)) for _ in range(B - 1)]
-    pool = Pool(B, H, 64, N, BF16)
-    pool.append(_randn(B, H, N, 64, seed=15), _randn(B, H, N, 64, seed=16), new)
+    pool = Pool(B, H, D, N, BF16, long=long and N <= 4096)
+    pool.append(_randn(B, H, N, D, seed=15), _randn(B, H, N, D, seed=16), new)
     one = [min(n, 1) for n in new]
     before = [n - x for n, x in zip(new, one)]
-    q = _randn(B, H, 1, 64, seed=17)
+    q = _randn(B, H, 1, D, seed=17)
     got = ops.cache_attention(q, pool.pages, pool.table, _ints(before), _ints(one))
     _check(got, _reference(pool, q, before, one, True), BF16)
 
@@ -214,9 +220,10 @@ def test_layouts_of_the_tensors():
 
 @pytest.mark.parametrize("T", [1, 12])
 @pytest.mark.parametrize("D", [64, 128])
-def test_pages_outside_the_pool_and_lengths_beyond_the_table(D, T):
+@pytest.mark.parametrize("long", [False, True])
+def test_pages_outside_the_pool_and_lengths_beyond_the_table(long, D, T):
     """They count as absent tokens; what is in the pool behind other pages stays as it was."""
-    pool = Pool(3, 2, D, 512, BF16, extra=2)
+    pool = Pool(3, 2, D, 512, BF16, extra=2, long=long)
     k, v = _randn(3, 2, 300, D, seed=20), _randn(3, 2, 300, D, seed=21)
     pool.append(k, v)
     start = pool.lengths - T
@@ -236,7 +243,7 @@ def test_pages_outside_the_pool_and_lengths_beyond_the_table(D, T):
     assert not ops.cache_attention(q, pool.pages, table, start).any()
     before = pool.pages.clone()
     ops.cache_append(pool.pages, table, pool.lengths, k, v)
-    ops.cache_append(pool.pages, pool.table, _ints([512, 2**31 - 1, 600]), k, v)
+    ops.cache_append(pool.pages, pool.table, _ints([8192, 2**31 - 1, 9000] if long else [512, 2**31 - 1, 600]), k, v)
     assert torch.equal(before, pool.pages)
     kk, vv = ops.cache_read(pool.pages, table, pool.lengths, D, BF16, 300)
     assert not kk.any() and not vv.any()
