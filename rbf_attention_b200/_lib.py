@@ -132,7 +132,7 @@ SIGNATURES = {
         [ctypes.c_void_p, ctypes.c_int, ctypes.c_int, ctypes.c_size_t, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int,
          ctypes.c_void_p],
     ),
-    "rbf_b200_cache_attention_workspace_bytes": (ctypes.c_size_t, [ctypes.c_int] * 3),
+    "rbf_b200_cache_attention_workspace_bytes": (ctypes.c_size_t, [ctypes.c_int] * 6),
     "rbf_b200_cache_attention": (
         ctypes.c_int,
         [ctypes.c_void_p, _c_i64p] + [ctypes.c_void_p] * 6 + [ctypes.c_size_t] + [ctypes.c_int] * 9

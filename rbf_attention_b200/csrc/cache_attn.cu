@@ -709,8 +709,8 @@ __global__ void __launch_bounds__(kAttnWarps * 32) cache_attn_kernel(const Cache
 // A segment per block, or per cluster of blocks, whose warps take its units in turn: for short sequences, whose time is the
 // chain of one load after another. There is no dealing out, no second kernel and no workspace; the warps' parts are joined in
 // shared memory, the blocks' through the cluster's, in a fixed order.
-template <bool kBf16, int P>
-__global__ void __launch_bounds__(kAttnWarps * 32) cache_attn_short_kernel(const CacheAttnArgs a) {
+template <bool kBf16, int P, int kWarps>
+__global__ void __launch_bounds__(kWarps * 32, 16 / kWarps) cache_attn_short_kernel(const CacheAttnArgs a) {
   constexpr int UB = 2, NT = 1, kRing = 2;
   using T = Tile<P, UB>;
   constexpr int kBytes = cache_page_bytes(P);
@@ -722,19 +722,21 @@ __global__ void __launch_bounds__(kAttnWarps * 32) cache_attn_short_kernel(const
   asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
   asm("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(ranks));
   const int segment = static_cast<int>(blockIdx.x / ranks), b = segment / a.H, h = segment % a.H;
+  // the row of the page table (at most 32 pages), asked for beside the lengths
+  const int id_of_lane = lane < a.max_pages ? a.table[static_cast<int64_t>(b) * a.max_pages + lane] : -1;
   const Units<UB> units(a, b);
   const int total = units.held + units.fresh, blocks = total / kBlockTokens;
-  const int each = kAttnWarps * static_cast<int>(ranks), first = static_cast<int>(rank) * kAttnWarps + warp;
+  const int each = kWarps * static_cast<int>(ranks), first = static_cast<int>(rank) * kWarps + warp;
   const int mine = units.count > first ? (units.count - first + each - 1) / each : 0;
 
   const uint8_t* page = nullptr;                   // of this lane's unit among the next 32 of the warp
   int what = 0;
   auto look_up = [&](int i) {
     page = nullptr;
-    const int u = first + (i + lane) * each;
-    if (i + lane >= mine) return;
-    const int block = u < units.groups ? u * UB : blocks;
-    page = cache_page(a.pages, a.table, b, a.max_pages, a.num_pages, a.H, h, kBytes, block * kBlockTokens);
+    const int u = first + (i + lane) * each, block = u < units.groups ? u * UB : blocks;
+    const int id = __shfl_sync(0xffffffffu, id_of_lane, block / kPageBlocks & 31);
+    if (i + lane >= mine || id < 0 || id >= a.num_pages) return;
+    page = a.pages + (static_cast<int64_t>(id) * a.H + h) * kBytes;
     what = u < units.groups ? block % kPageBlocks | min(UB, blocks - block) << 8 : total % kBlockTokens | 1 << 16;
   };
   int fetched = 0;
@@ -808,11 +810,11 @@ __global__ void __launch_bounds__(kAttnWarps * 32) cache_attn_short_kernel(const
   if (warp == 0 && g == 0)                         // |q|^2, which every warp has
     for (int e = 0; e < 2; ++e) parts[8 * P + 16 + 2 * t + e] = units.count > 0 ? q.sq[0][e] : 0.f;
   __syncthreads();
-  for (int i = threadIdx.x; i < used; i += kAttnWarps * 32) {
+  for (int i = threadIdx.x; i < used; i += kWarps * 32) {
     const int c = i / kPerColumn, at = c * P + i % kPerColumn * 4;
     Joined j{-INFINITY, 0.f, make_float4(0.f, 0.f, 0.f, 0.f)};
 #pragma unroll
-    for (int w = 0; w < kAttnWarps; ++w) {
+    for (int w = 0; w < kWarps; ++w) {
       const float* p = parts + w * kPart;
       j.add(p[8 * P + c], p[8 * P + 8 + c], *reinterpret_cast<const float4*>(p + at));
     }
@@ -831,7 +833,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32) cache_attn_short_kernel(const
   __syncwarp();
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
   if (rank == 0) {
-    for (int i = threadIdx.x; i < used; i += kAttnWarps * 32) {
+    for (int i = threadIdx.x; i < used; i += kWarps * 32) {
       const int c = i / kPerColumn, at = c * P + i % kPerColumn * 4;
       Joined j{-INFINITY, 0.f, make_float4(0.f, 0.f, 0.f, 0.f)};
       for (uint32_t r = 0; r < ranks; ++r) {
@@ -974,20 +976,20 @@ cudaError_t attn_t(const CacheAttnArgs& a, int sms, cudaStream_t stream) {
 // and page tables of up to kShort tokens - what the lengths are is known on the device alone. A block's warps have the units
 // of 256 tokens (128 at 128 columns) in flight at a time; more blocks where the segments leave SMs free and have units for them.
 constexpr int kShort = 4096;
-int short_ranks(const CacheAttnArgs& a, int P, int sms) {
-  if (static_cast<int64_t>(a.T) * a.G > 8 || a.max_pages > kShort / kPageTokens) return 0;
-  const int64_t segments = static_cast<int64_t>(a.B) * a.H, units = static_cast<int64_t>(a.max_pages) * kPageBlocks / 2;
+int short_ranks(int64_t segments, int64_t columns, int max_pages, int sms) {
+  static_assert(kShort / kPageTokens <= 32, "a lane holds a page number");
+  if (columns > 8 || max_pages > kShort / kPageTokens) return 0;
+  const int64_t units = static_cast<int64_t>(max_pages) * kPageBlocks / 2;
   int ranks = 1;
   while (ranks < 8 && segments * ranks * 2 <= sms && units > kAttnWarps * ranks) ranks *= 2;
-  (void)P;
   return ranks;
 }
 
-template <bool kBf16, int P>
+template <bool kBf16, int P, int kWarps>
 cudaError_t short_t(const CacheAttnArgs& a, int ranks, cudaStream_t stream) {
-  constexpr int kSmem = kAttnWarps * 2 * Tile<P, 2>::kStage;
+  constexpr int kSmem = kWarps * 2 * Tile<P, 2>::kStage;
   static PerDeviceFlags flags;
-  const cudaError_t e = ensure_dynamic_smem(cache_attn_short_kernel<kBf16, P>, kSmem, flags);
+  const cudaError_t e = ensure_dynamic_smem(cache_attn_short_kernel<kBf16, P, kWarps>, kSmem, flags);
   if (e != cudaSuccess) return e;
   cudaLaunchAttribute attr{};
   attr.id = cudaLaunchAttributeClusterDimension;
@@ -995,19 +997,21 @@ cudaError_t short_t(const CacheAttnArgs& a, int ranks, cudaStream_t stream) {
   attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
   cudaLaunchConfig_t config{};
   config.gridDim = dim3(static_cast<unsigned>(a.B) * a.H * ranks);
-  config.blockDim = dim3(kAttnWarps * 32);
+  config.blockDim = dim3(kWarps * 32);
   config.dynamicSmemBytes = kSmem;
   config.stream = stream;
   config.attrs = &attr;
   config.numAttrs = 1;
-  const cudaError_t launched = cudaLaunchKernelEx(&config, cache_attn_short_kernel<kBf16, P>, a);
+  const cudaError_t launched = cudaLaunchKernelEx(&config, cache_attn_short_kernel<kBf16, P, kWarps>, a);
   if (launched != cudaSuccess) cudaGetLastError();
   return launched;
 }
 
 template <bool kBf16, int P>
 cudaError_t attn_p(const CacheAttnArgs& a, int sms, cudaStream_t stream) {
-  if (const int ranks = short_ranks(a, P, sms)) return short_t<kBf16, P>(a, ranks, stream);
+  const int64_t segments = static_cast<int64_t>(a.B) * a.H;
+  if (const int ranks = short_ranks(segments, static_cast<int64_t>(a.T) * a.G, a.max_pages, sms))
+    return segments > 2 * sms ? short_t<kBf16, P, 4>(a, ranks, stream) : short_t<kBf16, P, 8>(a, ranks, stream);
   return cache_attn_tiles(a.T, a.G, P) == 1 ? attn_t<kBf16, P, 1>(a, sms, stream) : attn_t<kBf16, P, 256 / P>(a, sms, stream);
 }
 
@@ -1016,8 +1020,9 @@ cudaError_t attn_p(const CacheAttnArgs& a, int sms, cudaStream_t stream) {
 // Operand tiles of 8 columns that a warp works on at a time: as many as its registers hold where there is more than one.
 int cache_attn_tiles(int T, int G, int P) { return static_cast<int64_t>(T) * G <= 8 ? 1 : 256 / P; }
 
-size_t cache_attn_workspace_bytes(int T, int G, int D, int sms) {
+size_t cache_attn_workspace_bytes(int B, int H, int G, int T, int D, int max_pages, int sms) {
   const int P = cache_columns(D);
+  if (short_ranks(static_cast<int64_t>(B) * H, static_cast<int64_t>(T) * G, max_pages, sms)) return 0;
   return static_cast<size_t>(sms) * kAttnWarps * 2 * 8 * cache_attn_tiles(T, G, P) * (P + 2) * sizeof(float);
 }
 

@@ -928,10 +928,10 @@ int rbf_b200_cache_copy_pages(void* pages, int layers, int num_pages, size_t pag
   return RBF_B200_OK;
 }
 
-size_t rbf_b200_cache_attention_workspace_bytes(int T, int G, int D) {
+size_t rbf_b200_cache_attention_workspace_bytes(int B, int H, int G, int T, int D, int max_pages) {
   const int sms = sm_count();
-  if (sms <= 0 || T < 0 || G <= 0 || D <= 0 || D > 128) return 0;
-  return rbf::cache_attn_workspace_bytes(T, G, D, sms);
+  if (sms <= 0 || B <= 0 || H <= 0 || G <= 0 || T <= 0 || D <= 0 || D > 128 || max_pages < 0) return 0;
+  return rbf::cache_attn_workspace_bytes(B, H, G, T, D, max_pages, sms);
 }
 
 int rbf_b200_cache_attention(const void* q, const int64_t* q_strides, const void* pages, const int* page_table,
@@ -951,10 +951,9 @@ int rbf_b200_cache_attention(const void* q, const int64_t* q_strides, const void
     return fail(RBF_B200_ERR_BAD_LAYOUT, "out is NULL or not 16-byte aligned");
   const int sms = sm_count();
   if (sms <= 0) return fail(RBF_B200_ERR_LAUNCH, "cannot read the SM count of the current device");
-  if (workspace == nullptr || reinterpret_cast<uintptr_t>(workspace) % 256 != 0 ||
-      workspace_bytes < rbf::cache_attn_workspace_bytes(T, G, D, sms))
-    return fail(RBF_B200_ERR_WORKSPACE, "workspace is NULL, not 256-byte aligned or smaller than %zu bytes",
-                rbf::cache_attn_workspace_bytes(T, G, D, sms));
+  const size_t need = rbf::cache_attn_workspace_bytes(B, H, G, T, D, max_pages, sms);
+  if (need > 0 && (workspace == nullptr || reinterpret_cast<uintptr_t>(workspace) % 256 != 0 || workspace_bytes < need))
+    return fail(RBF_B200_ERR_WORKSPACE, "workspace is NULL, not 256-byte aligned or smaller than %zu bytes", need);
   rbf::CacheAttnArgs a{};
   a.q = q; set_strides(a.qs, q_strides);
   a.pages = static_cast<const uint8_t*>(pages); a.table = page_table; a.lengths = lengths; a.fresh = new_lengths;

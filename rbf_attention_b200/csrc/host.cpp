@@ -841,11 +841,13 @@ PyObject* cache_attention(const Args& a) {
   if (fresh) fresh = fresh->contiguous();
   const Tensor qc = tma_ready(q);
   const Tensor out = empty({c.B, Hq, T, D}, q.scalar_type(), q.device());
-  const Tensor ws = workspace(rbf_b200_cache_attention_workspace_bytes(T, G, D), q.device());
+  const size_t bytes = rbf_b200_cache_attention_workspace_bytes(c.B, c.H, G, T, D, c.max_pages);
+  Tensor ws;
+  if (bytes > 0) ws = workspace(bytes, q.device());
   const float gamma = static_cast<float>(1.0 / std::sqrt(static_cast<double>(D)));
   const int rc = rbf_b200_cache_attention(qc.const_data_ptr(), strides3(qc), c.pages.const_data_ptr(), c.table_ptr(),
-                                          c.lengths_ptr(), int_ptr(fresh), out.data_ptr(), ws.data_ptr(), ws.nbytes(), c.B,
-                                          c.H, G, T, D, c.max_pages, c.num_pages, dtype_code(q.scalar_type()), softmax, gamma,
+                                          c.lengths_ptr(), int_ptr(fresh), out.data_ptr(),
+                                          bytes > 0 ? ws.data_ptr() : nullptr, bytes, c.B, c.H, G, T, D, c.max_pages, c.num_pages, dtype_code(q.scalar_type()), softmax, gamma,
                                           stream_of(q));
   check(rc, "rbf_b200_cache_attention");
   unlocked.lock();

@@ -232,7 +232,7 @@ struct CacheAttnArgs {
   int column_tiles;          // set by the launcher
 };
 int cache_attn_tiles(int T, int G, int P);
-size_t cache_attn_workspace_bytes(int T, int G, int D, int sms);
+size_t cache_attn_workspace_bytes(int B, int H, int G, int T, int D, int max_pages, int sms);
 cudaError_t launch_cache_attn(CacheAttnArgs a, bool bf16, int sms, cudaStream_t stream);
 
 // Log-probabilities of given tokens, and the clipped policy loss with its gradient (policy_loss.cu).
