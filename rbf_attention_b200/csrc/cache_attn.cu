@@ -26,8 +26,17 @@
 namespace rbf {
 namespace {
 
-constexpr int kAttnWarps = 8;
-constexpr int kStages = 3;                         // units of a warp that are loaded ahead, the current one among them
+// Warps of a block (one per SM), blocks of a unit, and units of a warp that are loaded ahead, the current one among them: what
+// registers (65536) and shared memory (227 KB) hold. One tile of columns: 8 KB units, 12 warps with two each; 16 x 32768 tokens
+// of 128 columns took 115 us with 8 warps and three units, 104 so; 8 x 16384 of 64 columns 36 and 33.5 us, with 16 warps and
+// three units of 4 KB 35.5. Several tiles: 216 to 255 registers, 8 warps; units of two blocks, whose code is half as long.
+template <int P, int NT>
+struct Shape {
+  static constexpr int kUnitBlocks = NT == 1 ? 256 / P : 2;
+  static constexpr int kWarps = NT == 1 ? 12 : 8;
+  static constexpr int kStages = NT == 1 ? 2 : 3;
+};
+constexpr int kShortWarps = 8;                     // of the kernel for short sequences, 4 where there are many
 constexpr float kSlack = 8.f;                      // growth of a score, in powers of two, that does not move the maximum
 
 // A warp's unit of work: UB blocks that are complete, or the one that is not
@@ -68,6 +77,19 @@ __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], 
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  }
+}
+// The product alone: with the zeros as an operand nothing has to be cleared, which took four moves a product.
+template <bool kBf16>
+__device__ __forceinline__ void mma16816_first(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if constexpr (kBf16) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+                 : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
+  } else {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+                 : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
   }
 }
 
@@ -364,10 +386,6 @@ __device__ __forceinline__ void codes_unit(const CacheAttnArgs& a, const Queries
     int sq0 = 0, sq1 = 0;
     float acc[NT][4];
 #pragma unroll
-    for (int n = 0; n < NT; ++n)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) acc[n][e] = 0.f;
-#pragma unroll
     for (int d = 0; d < P / 64; ++d) {
       const uint4 w0 = key[2 * d * 32], w1 = key[(2 * d + 1) * 32];
       const uint32_t r0[4] = {w0.x, w0.y, w0.z, w0.w}, r1[4] = {w1.x, w1.y, w1.z, w1.w};
@@ -377,7 +395,10 @@ __device__ __forceinline__ void codes_unit(const CacheAttnArgs& a, const Queries
         sq1 += dot4(r1[i]);
         const uint32_t A[4] = {codes_lo(r0[i]), codes_lo(r1[i]), codes_hi(r0[i]), codes_hi(r1[i])};
 #pragma unroll
-        for (int n = 0; n < NT; ++n) mma16816<false>(acc[n], A, q.w[n][d * 4 + i][0], q.w[n][d * 4 + i][1]);
+        for (int n = 0; n < NT; ++n) {
+          if (d == 0 && i == 0) mma16816_first<false>(acc[n], A, q.w[n][0][0], q.w[n][0][1]);
+          else mma16816<false>(acc[n], A, q.w[n][d * 4 + i][0], q.w[n][d * 4 + i][1]);
+        }
       }
     }
 #pragma unroll
@@ -428,12 +449,17 @@ __device__ __forceinline__ void codes_unit(const CacheAttnArgs& a, const Queries
         const uint32_t A[4] = {codes_lo(r0), codes_lo(r1), codes_hi(r0), codes_hi(r1)};
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-          float acc[4] = {0.f, 0.f, 0.f, 0.f};
-          mma16816<false>(acc, A, p[n][0], p[n][1]);
+          float acc[4];
+          mma16816_first<false>(acc, A, p[n][0], p[n][1]);
           float(&o)[4] = run.o[2 * i + half][n];
+          if (finite) {
+            ffma2v(o[0], o[1], acc[0], acc[1], scale, scale, o[0], o[1]);
+            ffma2v(o[2], o[3], acc[2], acc[3], scale, scale, o[2], o[3]);
+          } else {                                  // a block that is not finite reaches the columns that see it
 #pragma unroll
-          for (int e = 0; e < 4; ++e)               // a block that is not finite reaches the columns that see it
-            if (finite || base <= q.limit[n][e % 2]) o[e] = fmaf(acc[e], scale, o[e]);
+            for (int e = 0; e < 4; ++e)
+              if (base <= q.limit[n][e % 2]) o[e] = fmaf(acc[e], scale, o[e]);
+          }
         }
       }
     }
@@ -540,8 +566,8 @@ __device__ __forceinline__ void rest_unit(const CacheAttnArgs& a, const Queries<
       }
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
-        float acc[4] = {0.f, 0.f, 0.f, 0.f};
-        mma16816<kBf16>(acc, A, p[n][0], p[n][1]);
+        float acc[4];
+        mma16816_first<kBf16>(acc, A, p[n][0], p[n][1]);
 #pragma unroll
         for (int e = 0; e < 4; ++e)
           if (!slow || base + only <= q.limit[n][e % 2]) run.o[j][n][e] += acc[e];
@@ -557,14 +583,14 @@ __device__ __forceinline__ float last_factor(const CacheAttnArgs& a, float m, fl
 }
 
 template <bool kBf16, int P, int NT>
-__global__ void __launch_bounds__(kAttnWarps * 32) cache_attn_kernel(const CacheAttnArgs a) {
-  constexpr int UB = 256 / P, KC = P / 32;
+__global__ void __launch_bounds__(Shape<P, NT>::kWarps * 32) cache_attn_kernel(const CacheAttnArgs a) {
+  constexpr int UB = Shape<P, NT>::kUnitBlocks, KC = P / 32, kStages = Shape<P, NT>::kStages, kWarps = Shape<P, NT>::kWarps;
   using T = Tile<P, UB>;
   constexpr int kBytes = cache_page_bytes(P);
   extern __shared__ __align__(128) uint8_t smem[];
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   uint8_t* ring = smem + (threadIdx.x >> 5) * (kStages * T::kStage);       // a warp has its own
-  const int64_t workers = static_cast<int64_t>(gridDim.x) * kAttnWarps;
+  const int64_t workers = static_cast<int64_t>(gridDim.x) * kWarps;
   const int64_t self = static_cast<int64_t>(threadIdx.x >> 5) * gridDim.x + blockIdx.x;    // neighbours on other SMs
   const int segments = a.column_tiles * a.H;       // of a sequence
   int64_t unused, all;
@@ -854,10 +880,10 @@ __global__ void __launch_bounds__(kWarps * 32, 16 / kWarps) cache_attn_short_ker
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");   // blocks stay until they have been read
 }
 
-constexpr int kJoinWarps = 8;
+constexpr int kJoinWarps = 16;
 
 // Joins the parts of the segments that several warps worked on, and clears those that no warp did: `split` warps of a block
-// share the parts of a column, 8 where there are few columns (and many parts of each), else one.
+// share the parts of a column, all 16 where there are few columns (and many parts of each), else one.
 template <bool kBf16, int P, int NT>
 __global__ void __launch_bounds__(kJoinWarps * 32) cache_join_kernel(const CacheAttnArgs a, const int64_t workers, const int split) {
   __shared__ float s_y[kJoinWarps][P], s_m[kJoinWarps], s_l[kJoinWarps];
@@ -873,24 +899,34 @@ __global__ void __launch_bounds__(kJoinWarps * 32) cache_join_kernel(const Cache
   float y[kPer] = {}, top = -INFINITY, sum = 0.f;
   bool write = b < a.B && c < a.T * a.G, some = false;
   if (write) {
-    const Units<256 / P> units(a, b);
+    const Units<Shape<P, NT>::kUnitBlocks> units(a, b);
     if (units.count > 0) {
       int64_t before, all;
-      sum_units<256 / P>(a, b, before, all);
+      sum_units<Shape<P, NT>::kUnitBlocks>(a, b, before, all);
       const Deal deal(all * segments, workers);
       const int64_t begin = before * segments + static_cast<int64_t>(seg) * units.count;
       const int64_t first = min(deal.worker(begin), workers - 1), last = min(deal.worker(begin + units.count - 1), workers - 1);
       write = first != last;
       some = write && c / a.G < units.fresh;
       if (some) {
-        for (int64_t w0 = first + share * 32; w0 <= last; w0 += 32 * split) {
-          const int n = static_cast<int>(min(last - w0 + 1, int64_t{32}));
+        // lane i of a warp has the maximum and the sum of its i-th part, four parts' outputs are under way at a time
+        for (int64_t w0 = first + share; w0 <= last; w0 += 32 * split) {
+          const int n = static_cast<int>(min((last - w0) / split + 1, int64_t{32}));
+          auto part = [&](int i) {
+            const int64_t w = w0 + static_cast<int64_t>(i) * split;
+            return part_of<P, NT>(a, 2 * w + (w == first));
+          };
           float m = -INFINITY, l = 0.f;
           if (lane < n) {
-            const float* part = part_of<P, NT>(a, 2 * (w0 + lane) + (w0 + lane == first));
-            m = part[8 * NT * P + in];
-            l = part[8 * NT * (P + 1) + in];
+            m = part(lane)[8 * NT * P + in];
+            l = part(lane)[8 * NT * (P + 1) + in];
           }
+          float z[4][kPer];
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (j < n)
+#pragma unroll
+              for (int i = 0; i < kPer; ++i) z[j][i] = part(j)[in * P + lane * kPer + i];
           float x = m;
 #pragma unroll
           for (int o = 16; o > 0; o >>= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
@@ -903,12 +939,24 @@ __global__ void __launch_bounds__(kJoinWarps * 32) cache_join_kernel(const Cache
           sum = fmaf(sum, old, l);
 #pragma unroll
           for (int i = 0; i < kPer; ++i) y[i] *= old;
-#pragma unroll 8
-          for (int j = 0; j < n; ++j) {
-            const float* part = part_of<P, NT>(a, 2 * (w0 + j) + (w0 + j == first)) + in * P + lane * kPer;
-            const float fj = __shfl_sync(0xffffffffu, f, j);
+          for (int j0 = 0; j0 < n; j0 += 4) {
+            float next[4][kPer];
 #pragma unroll
-            for (int i = 0; i < kPer; ++i) y[i] = fmaf(part[i], fj, y[i]);
+            for (int j = 0; j < 4; ++j)
+              if (j0 + 4 + j < n)
+#pragma unroll
+                for (int i = 0; i < kPer; ++i) next[j][i] = part(j0 + 4 + j)[in * P + lane * kPer + i];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const float fj = __shfl_sync(0xffffffffu, f, (j0 + j) & 31);
+              if (j0 + j < n)
+#pragma unroll
+                for (int i = 0; i < kPer; ++i) y[i] = fmaf(z[j][i], fj, y[i]);
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+#pragma unroll
+              for (int i = 0; i < kPer; ++i) z[j][i] = next[j][i];
           }
         }
       }
@@ -958,18 +1006,19 @@ __global__ void __launch_bounds__(kJoinWarps * 32) cache_join_kernel(const Cache
 
 template <bool kBf16, int P, int NT>
 cudaError_t attn_t(const CacheAttnArgs& a, int sms, cudaStream_t stream) {
-  constexpr int kSmem = kAttnWarps * kStages * Tile<P, 256 / P>::kStage;
+  using S = Shape<P, NT>;
+  constexpr int kSmem = S::kWarps * S::kStages * Tile<P, S::kUnitBlocks>::kStage;
   static PerDeviceFlags flags;
   cudaError_t e = ensure_dynamic_smem(cache_attn_kernel<kBf16, P, NT>, kSmem, flags);
   if (e != cudaSuccess) return e;
-  cache_attn_kernel<kBf16, P, NT><<<sms, kAttnWarps * 32, kSmem, stream>>>(a);
+  cache_attn_kernel<kBf16, P, NT><<<sms, S::kWarps * 32, kSmem, stream>>>(a);
   if ((e = cudaGetLastError()) != cudaSuccess) return e;
   const int64_t width = static_cast<int64_t>(a.T) * a.G < 8 * NT ? a.T * a.G : 8 * NT;
   const int64_t columns = static_cast<int64_t>(a.B) * a.column_tiles * a.H * width;
   const int split = columns <= sms * 4 ? kJoinWarps : 1;
   const int64_t blocks = (columns + kJoinWarps / split - 1) / (kJoinWarps / split);
   return launch_dependent(cache_join_kernel<kBf16, P, NT>, dim3(static_cast<unsigned>(blocks)), kJoinWarps * 32, 0, stream, a,
-                          static_cast<int64_t>(sms) * kAttnWarps, split);
+                          static_cast<int64_t>(sms) * S::kWarps, split);
 }
 
 // Blocks of a cluster that share a segment in the kernel for short sequences, 0: not that kernel. It is for one tile of columns
@@ -981,7 +1030,7 @@ int short_ranks(int64_t segments, int64_t columns, int max_pages, int sms) {
   if (columns > 8 || max_pages > kShort / kPageTokens) return 0;
   const int64_t units = static_cast<int64_t>(max_pages) * kPageBlocks / 2;
   int ranks = 1;
-  while (ranks < 8 && segments * ranks * 2 <= sms && units > kAttnWarps * ranks) ranks *= 2;
+  while (ranks < 8 && segments * ranks * 2 <= sms && units > kShortWarps * ranks) ranks *= 2;
   return ranks;
 }
 
@@ -1011,19 +1060,33 @@ template <bool kBf16, int P>
 cudaError_t attn_p(const CacheAttnArgs& a, int sms, cudaStream_t stream) {
   const int64_t segments = static_cast<int64_t>(a.B) * a.H;
   if (const int ranks = short_ranks(segments, static_cast<int64_t>(a.T) * a.G, a.max_pages, sms))
-    return segments > 2 * sms ? short_t<kBf16, P, 4>(a, ranks, stream) : short_t<kBf16, P, 8>(a, ranks, stream);
-  return cache_attn_tiles(a.T, a.G, P) == 1 ? attn_t<kBf16, P, 1>(a, sms, stream) : attn_t<kBf16, P, 256 / P>(a, sms, stream);
+    return segments > 2 * sms ? short_t<kBf16, P, 4>(a, ranks, stream) : short_t<kBf16, P, kShortWarps>(a, ranks, stream);
+  switch (cache_attn_tiles(a.T, a.G, P)) {
+    case 1: return attn_t<kBf16, P, 1>(a, sms, stream);
+    case 2: return attn_t<kBf16, P, 2>(a, sms, stream);
+    default:
+      if constexpr (P == 64) {
+        if (cache_attn_tiles(a.T, a.G, P) == 3) return attn_t<kBf16, P, 3>(a, sms, stream);
+        return attn_t<kBf16, P, 4>(a, sms, stream);
+      }
+  }
+  return cudaErrorInvalidValue;
 }
 
 }  // namespace
 
-// Operand tiles of 8 columns that a warp works on at a time: as many as its registers hold where there is more than one.
-int cache_attn_tiles(int T, int G, int P) { return static_cast<int64_t>(T) * G <= 8 ? 1 : 256 / P; }
+// Operand tiles of 8 columns that a warp works on at a time: as few rounds over the cache as its registers allow (32 columns, 16
+// at 128 dims), and as few empty columns as that many rounds allow.
+int cache_attn_tiles(int T, int G, int P) {
+  const int64_t tiles = (static_cast<int64_t>(T) * G + 7) / 8, most = 256 / P, rounds = (tiles + most - 1) / most;
+  return static_cast<int>((tiles + rounds - 1) / rounds);
+}
 
 size_t cache_attn_workspace_bytes(int B, int H, int G, int T, int D, int max_pages, int sms) {
   const int P = cache_columns(D);
   if (short_ranks(static_cast<int64_t>(B) * H, static_cast<int64_t>(T) * G, max_pages, sms)) return 0;
-  return static_cast<size_t>(sms) * kAttnWarps * 2 * 8 * cache_attn_tiles(T, G, P) * (P + 2) * sizeof(float);
+  const int tiles = cache_attn_tiles(T, G, P), warps = tiles > 1 ? Shape<64, 2>::kWarps : Shape<64, 1>::kWarps;
+  return static_cast<size_t>(sms) * warps * 2 * 8 * tiles * (P + 2) * sizeof(float);
 }
 
 cudaError_t launch_cache_attn(CacheAttnArgs a, bool bf16, int sms, cudaStream_t stream) {
