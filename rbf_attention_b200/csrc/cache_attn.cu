@@ -142,20 +142,14 @@ struct Units {
   }
 };
 
-// Sums over sequences [0, n) and over all of the units of a segment, by a whole warp
+// Sum over the sequences of the units of a segment, by a whole warp
 template <int UB>
-__device__ __forceinline__ void sum_units(const CacheAttnArgs& a, int n, int64_t& before, int64_t& all) {
-  before = all = 0;
-  for (int b = threadIdx.x & 31; b < a.B; b += 32) {
-    const int u = Units<UB>(a, b).count;
-    all += u;
-    if (b < n) before += u;
-  }
+__device__ __forceinline__ int64_t sum_units(const CacheAttnArgs& a) {
+  int64_t all = 0;
+  for (int b = threadIdx.x & 31; b < a.B; b += 32) all += Units<UB>(a, b).count;
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    before += __shfl_xor_sync(0xffffffffu, before, o);
-    all += __shfl_xor_sync(0xffffffffu, all, o);
-  }
+  for (int o = 16; o > 0; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
+  return all;
 }
 
 // Element offset of output column c of a segment (new token c / G of query head h * G + c % G)
@@ -166,10 +160,16 @@ __device__ __forceinline__ const uint16_t* q_row(const CacheAttnArgs& a, int b, 
   return static_cast<const uint16_t*>(a.q) + b * a.qs[0] + (h * a.G + c % a.G) * a.qs[1] + c / a.G * a.qs[2];
 }
 
-// One part: per column P outputs, then the maxima and the sums of all columns
+// The workspace: a note per warp, then two parts per warp. A warp that has the first units of a segment which goes on with the
+// next warp leaves a note about it; its part of that segment is its second, the parts of the others are their first ones.
+struct Note {
+  int b, seg, last, fresh;                         // sequence (-1: no such segment), segment in it, last warp, real new tokens
+};
+// One part: per column P outputs, then of all columns the maxima, the sums and what the variant without a denominator needs
+constexpr int part_floats(int P, int NT) { return 8 * NT * (P + 4); }
 template <int P, int NT>
-__device__ __forceinline__ float* part_of(const CacheAttnArgs& a, int64_t index) {
-  return a.parts + index * (8 * NT) * (P + 2);
+__device__ __forceinline__ float* part_of(const CacheAttnArgs& a, int64_t workers, int64_t index) {
+  return a.parts + workers * (sizeof(Note) / sizeof(float)) + index * part_floats(P, NT);
 }
 
 // A warp's state for one segment
@@ -593,11 +593,17 @@ __global__ void __launch_bounds__(Shape<P, NT>::kWarps * 32) cache_attn_kernel(c
   const int64_t workers = static_cast<int64_t>(gridDim.x) * kWarps;
   const int64_t self = static_cast<int64_t>(threadIdx.x >> 5) * gridDim.x + blockIdx.x;    // neighbours on other SMs
   const int segments = a.column_tiles * a.H;       // of a sequence
-  int64_t unused, all;
-  sum_units<UB>(a, 0, unused, all);
-  const Deal deal(all * segments, workers);
+  const Deal deal(sum_units<UB>(a) * segments, workers);
   int64_t at = deal.begin(self);
   const int64_t stop = deal.begin(self + 1);
+  Note* const note = reinterpret_cast<Note*>(a.parts) + self;
+  if (lane == 0) note->b = -1;
+  for (int64_t empty = self; empty < a.B; empty += workers) {              // sequences without new tokens
+    if (Units<UB>(a, static_cast<int>(empty)).count != 0) continue;
+    const int64_t words = static_cast<int64_t>(a.H) * a.G * a.T * a.D / 8;
+    uint4* out = reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out)) + empty * words;
+    for (int64_t i = lane; i < words; i += 32) out[i] = make_uint4(0, 0, 0, 0);
+  }
   if (at >= stop) return;
 
   // the sequence of the first unit
@@ -698,7 +704,9 @@ __global__ void __launch_bounds__(Shape<P, NT>::kWarps * 32) cache_attn_kernel(c
     // ---- the segment's output, or this warp's part of it
     run.sum_up();
     const bool complete = u0 == 0 && u1 == units.count;
-    float* part = part_of<P, NT>(a, 2 * self + (u0 == 0));
+    float* part = part_of<P, NT>(a, workers, 2 * self + (u0 == 0));
+    if (!complete && u0 == 0 && lane == 0)
+      *note = {b, seg, static_cast<int>(min(deal.worker(at - u0 + units.count - 1), workers - 1)), units.fresh};
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -724,6 +732,7 @@ __global__ void __launch_bounds__(Shape<P, NT>::kWarps * 32) cache_attn_kernel(c
           if (g == 0) {
             part[8 * NT * P + in] = m;
             part[8 * NT * (P + 1) + in] = l;
+            part[8 * NT * (P + 2) + in] = q.sq[n][e];
           }
         }
       }
@@ -880,128 +889,107 @@ __global__ void __launch_bounds__(kWarps * 32, 16 / kWarps) cache_attn_short_ker
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");   // blocks stay until they have been read
 }
 
-constexpr int kJoinWarps = 16;
+constexpr int kJoinWarps = 8;
 
-// Joins the parts of the segments that several warps worked on, and clears those that no warp did: `split` warps of a block
-// share the parts of a column, all 16 where there are few columns (and many parts of each), else one.
+// Joins the parts of the segments that several warps worked on, a block for each that begins with warp blockIdx.x: columns go
+// to the block's warps in turn, as many warps share the parts of a column as there are warps for them.
 template <bool kBf16, int P, int NT>
-__global__ void __launch_bounds__(kJoinWarps * 32) cache_join_kernel(const CacheAttnArgs a, const int64_t workers, const int split) {
+__global__ void __launch_bounds__(kJoinWarps * 32) cache_join_kernel(const CacheAttnArgs a, const int workers) {
   __shared__ float s_y[kJoinWarps][P], s_m[kJoinWarps], s_l[kJoinWarps];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int segments = a.column_tiles * a.H, width = min(8 * NT, a.T * a.G);
-  const int64_t column = static_cast<int64_t>(blockIdx.x) * (kJoinWarps / split) + warp / split;
-  const int64_t segment = column / width;
-  const int in = static_cast<int>(column % width), share = warp % split;
-  const int b = static_cast<int>(segment / segments), seg = static_cast<int>(segment % segments);
-  const int h = seg % a.H, c = seg / a.H * (8 * NT) + in;
   grid_dependency_wait();
+  const int first = blockIdx.x;
+  const Note note = reinterpret_cast<const Note*>(a.parts)[first];
+  if (note.b < 0) return;
+  const int h = note.seg % a.H, c0 = note.seg / a.H * (8 * NT), columns = min(8 * NT, a.T * a.G - c0);
+  const int split = columns == 1 ? 8 : columns == 2 ? 4 : columns <= 4 ? 2 : 1;
+  const int share = warp % split;
   constexpr int kPer = P / 32;
-  float y[kPer] = {}, top = -INFINITY, sum = 0.f;
-  bool write = b < a.B && c < a.T * a.G, some = false;
-  if (write) {
-    const Units<Shape<P, NT>::kUnitBlocks> units(a, b);
-    if (units.count > 0) {
-      int64_t before, all;
-      sum_units<Shape<P, NT>::kUnitBlocks>(a, b, before, all);
-      const Deal deal(all * segments, workers);
-      const int64_t begin = before * segments + static_cast<int64_t>(seg) * units.count;
-      const int64_t first = min(deal.worker(begin), workers - 1), last = min(deal.worker(begin + units.count - 1), workers - 1);
-      write = first != last;
-      some = write && c / a.G < units.fresh;
-      if (some) {
-        // lane i of a warp has the maximum and the sum of its i-th part, four parts' outputs are under way at a time
-        for (int64_t w0 = first + share; w0 <= last; w0 += 32 * split) {
-          const int n = static_cast<int>(min((last - w0) / split + 1, int64_t{32}));
-          auto part = [&](int i) {
-            const int64_t w = w0 + static_cast<int64_t>(i) * split;
-            return part_of<P, NT>(a, 2 * w + (w == first));
-          };
-          float m = -INFINITY, l = 0.f;
-          if (lane < n) {
-            m = part(lane)[8 * NT * P + in];
-            l = part(lane)[8 * NT * (P + 1) + in];
-          }
-          float z[4][kPer];
+  for (int in = warp / split; in - warp / split < columns; in += kJoinWarps / split) {     // as often for every warp
+    const bool real = in < columns;
+    const int c = c0 + in;
+    float y[kPer] = {}, top = -INFINITY, sum = 0.f, q_sq = 0.f;
+    if (real && c / a.G < note.fresh) {
+      q_sq = part_of<P, NT>(a, workers, 2 * first + 1)[8 * NT * (P + 2) + in];
+      // lane i has the maximum and the sum of the warp's i-th part, four parts' outputs are under way at a time
+      for (int w0 = first + share; w0 <= note.last; w0 += 32 * split) {
+        const int n = min((note.last - w0) / split + 1, 32);
+        auto part = [&](int i) {
+          const int w = w0 + i * split;
+          return part_of<P, NT>(a, workers, 2 * w + (w == first));
+        };
+        float m = -INFINITY, l = 0.f;
+        if (lane < n) {
+          m = part(lane)[8 * NT * P + in];
+          l = part(lane)[8 * NT * (P + 1) + in];
+        }
+        float z[4][kPer];
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+          for (int i = 0; i < kPer; ++i) z[j][i] = j < n ? part(j)[in * P + lane * kPer + i] : 0.f;
+        float x = m;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
+        x = fmaxf(x, top);
+        const float ref = x == -INFINITY ? 0.f : x, f = attn_ex2(m - ref), old = attn_ex2(top - ref);
+        top = x;
+        l *= f;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+        sum = fmaf(sum, old, l);
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) y[i] *= old;
+        for (int j0 = 0; j0 < n; j0 += 4) {
+          float next[4][kPer];
 #pragma unroll
           for (int j = 0; j < 4; ++j)
-            if (j < n)
 #pragma unroll
-              for (int i = 0; i < kPer; ++i) z[j][i] = part(j)[in * P + lane * kPer + i];
-          float x = m;
+            for (int i = 0; i < kPer; ++i) next[j][i] = j0 + 4 + j < n ? part(j0 + 4 + j)[in * P + lane * kPer + i] : 0.f;
 #pragma unroll
-          for (int o = 16; o > 0; o >>= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
-          x = fmaxf(x, top);
-          const float ref = x == -INFINITY ? 0.f : x, f = attn_ex2(m - ref), old = attn_ex2(top - ref);
-          top = x;
-          l *= f;
+          for (int j = 0; j < 4; ++j) {
+            const float fj = __shfl_sync(0xffffffffu, f, (j0 + j) & 31);
+            if (j0 + j < n)
 #pragma unroll
-          for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
-          sum = fmaf(sum, old, l);
-#pragma unroll
-          for (int i = 0; i < kPer; ++i) y[i] *= old;
-          for (int j0 = 0; j0 < n; j0 += 4) {
-            float next[4][kPer];
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-              if (j0 + 4 + j < n)
-#pragma unroll
-                for (int i = 0; i < kPer; ++i) next[j][i] = part(j0 + 4 + j)[in * P + lane * kPer + i];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              const float fj = __shfl_sync(0xffffffffu, f, (j0 + j) & 31);
-              if (j0 + j < n)
-#pragma unroll
-                for (int i = 0; i < kPer; ++i) y[i] = fmaf(z[j][i], fj, y[i]);
-            }
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-#pragma unroll
-              for (int i = 0; i < kPer; ++i) z[j][i] = next[j][i];
+              for (int i = 0; i < kPer; ++i) y[i] = fmaf(z[j][i], fj, y[i]);
           }
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int i = 0; i < kPer; ++i) z[j][i] = next[j][i];
         }
       }
     }
-  }
-  if (split > 1) {                                 // the whole block has one column
+    if (split > 1) {                               // one round: every column has its warps
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) s_y[warp][lane * kPer + i] = y[i];
-    if (lane == 0) {
-      s_m[warp] = top;
-      s_l[warp] = sum;
-    }
-    __syncthreads();
-    if (warp != 0) return;
-    for (int w = 1; w < kJoinWarps; ++w) {
-      const float x = fmaxf(top, s_m[w]), ref = x == -INFINITY ? 0.f : x;
-      const float f0 = attn_ex2(top - ref), f1 = attn_ex2(s_m[w] - ref);
-      top = x;
-      sum = sum * f0 + s_l[w] * f1;
-#pragma unroll
-      for (int i = 0; i < kPer; ++i) y[i] = y[i] * f0 + s_y[w][lane * kPer + i] * f1;
-    }
-  }
-  if (!write) return;
-  if (some) {
-    float q_sq = 0.f;
-    if (!a.softmax) {
-      const uint16_t* q = q_row(a, b, h, c);
-      float sq = 0.f;
-      for (int d = lane * 2; d < a.D; d += 64) {
-        const float2 x = unpack2<kBf16>(*reinterpret_cast<const uint32_t*>(q + d));
-        sq = fmaf(x.x, x.x, fmaf(x.y, x.y, sq));
+      for (int i = 0; i < kPer; ++i) s_y[warp][lane * kPer + i] = y[i];
+      if (lane == 0) {
+        s_m[warp] = top;
+        s_l[warp] = sum;
       }
+      __syncthreads();
+      if (share != 0) return;
+      for (int w = warp + 1; w < warp + split; ++w) {
+        const float x = fmaxf(top, s_m[w]), ref = x == -INFINITY ? 0.f : x;
+        const float f0 = attn_ex2(top - ref), f1 = attn_ex2(s_m[w] - ref);
+        top = x;
+        sum = sum * f0 + s_l[w] * f1;
 #pragma unroll
-      for (int o = 16; o > 0; o >>= 1) sq += __shfl_xor_sync(0xffffffffu, sq, o);
-      q_sq = a.scale * sq;
+        for (int i = 0; i < kPer; ++i) y[i] = y[i] * f0 + s_y[w][lane * kPer + i] * f1;
+      }
     }
-    const float f = last_factor(a, top, sum, q_sq);
+    if (!real) continue;
+    if (c / a.G < note.fresh) {
+      const float f = last_factor(a, top, sum, q_sq);
+      const bool none = top == -INFINITY && sum == 0.f;
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) y[i] *= f;
+      for (int i = 0; i < kPer; ++i) y[i] = none ? 0.f : y[i] * f;
+    }
+    if (lane * kPer >= a.D) continue;
+    uint16_t* to = static_cast<uint16_t*>(a.out) + out_offset(a, note.b, h, c) + lane * kPer;
+#pragma unroll
+    for (int i = 0; i < kPer; i += 2) *reinterpret_cast<uint32_t*>(to + i) = pack2<kBf16>(y[i], y[i + 1]);
   }
-  if (lane * kPer >= a.D) return;
-  uint16_t* to = static_cast<uint16_t*>(a.out) + out_offset(a, b, h, c) + lane * kPer;
-#pragma unroll
-  for (int i = 0; i < kPer; i += 2) *reinterpret_cast<uint32_t*>(to + i) = pack2<kBf16>(y[i], y[i + 1]);
 }
 
 template <bool kBf16, int P, int NT>
@@ -1013,12 +1001,8 @@ cudaError_t attn_t(const CacheAttnArgs& a, int sms, cudaStream_t stream) {
   if (e != cudaSuccess) return e;
   cache_attn_kernel<kBf16, P, NT><<<sms, S::kWarps * 32, kSmem, stream>>>(a);
   if ((e = cudaGetLastError()) != cudaSuccess) return e;
-  const int64_t width = static_cast<int64_t>(a.T) * a.G < 8 * NT ? a.T * a.G : 8 * NT;
-  const int64_t columns = static_cast<int64_t>(a.B) * a.column_tiles * a.H * width;
-  const int split = columns <= sms * 4 ? kJoinWarps : 1;
-  const int64_t blocks = (columns + kJoinWarps / split - 1) / (kJoinWarps / split);
-  return launch_dependent(cache_join_kernel<kBf16, P, NT>, dim3(static_cast<unsigned>(blocks)), kJoinWarps * 32, 0, stream, a,
-                          static_cast<int64_t>(sms) * S::kWarps, split);
+  const int workers = sms * S::kWarps;
+  return launch_dependent(cache_join_kernel<kBf16, P, NT>, dim3(workers), kJoinWarps * 32, 0, stream, a, workers);
 }
 
 // Blocks of a cluster that share a segment in the kernel for short sequences, 0: not that kernel. It is for one tile of columns
@@ -1086,7 +1070,7 @@ size_t cache_attn_workspace_bytes(int B, int H, int G, int T, int D, int max_pag
   const int P = cache_columns(D);
   if (short_ranks(static_cast<int64_t>(B) * H, static_cast<int64_t>(T) * G, max_pages, sms)) return 0;
   const int tiles = cache_attn_tiles(T, G, P), warps = tiles > 1 ? Shape<64, 2>::kWarps : Shape<64, 1>::kWarps;
-  return static_cast<size_t>(sms) * warps * 2 * 8 * tiles * (P + 2) * sizeof(float);
+  return static_cast<size_t>(sms) * warps * (sizeof(Note) + 2 * part_floats(P, tiles) * sizeof(float));
 }
 
 cudaError_t launch_cache_attn(CacheAttnArgs a, bool bf16, int sms, cudaStream_t stream) {
