@@ -79,20 +79,6 @@ __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], 
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
   }
 }
-// The product alone: with the zeros as an operand nothing has to be cleared, which took four moves a product.
-template <bool kBf16>
-__device__ __forceinline__ void mma16816_first(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  if constexpr (kBf16) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
-                 : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
-                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
-  } else {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
-                 : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
-                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
-  }
-}
-
 // 8 x 8 16-bit matrix, row lane / 4 and columns 2 (lane % 4), + 1 in each lane, transposed
 __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
   uint32_t y;
@@ -172,12 +158,17 @@ __device__ __forceinline__ float* part_of(const CacheAttnArgs& a, int64_t worker
   return a.parts + workers * (sizeof(Note) / sizeof(float)) + index * part_floats(P, NT);
 }
 
+// 2^x for -126 <= x <= 127
+__device__ __forceinline__ float power2(int x) { return __int_as_float((x + 127) << 23); }
+
 // A warp's state for one segment
 template <int P, int NT>
 struct Running {
   float o[P / 16][NT][4];                  // tile j: dims 32 (j / 2) + 4 g + 2 (j % 2), + 1 of columns 2t, 2t + 1
   float m[NT][2], l[NT][2];                        // of columns 8n + 2t, + 1; l: this lane's share
+  int unit;                                        // o is in units of 2^unit
   __device__ __forceinline__ void clear() {
+    unit = 0;
 #pragma unroll
     for (int j = 0; j < P / 16; ++j)
 #pragma unroll
@@ -192,8 +183,43 @@ struct Running {
         l[n][e] = 0.f;
       }
   }
-  // l of the whole warp
+  // A block's value scale goes into its weights, so that all products add up in o: weights are at most 2^8, so the unit is
+  // chosen to have the largest scale at hand in [2^6, 2^7), fp16 below its limit and its smallest normal number at 2^-20 of
+  // a weight of 1. It is changed, by a power of two, where a scale is above that or below 2^-6, up or down; not so far down
+  // that o would leave fp32's range (it is 2^100 of what is added then).
+  __device__ __forceinline__ void refer(float scale) {
+    const float now = scale * power2(-unit);
+    if (now < 128.f && (now >= 0.015625f || scale == 0.f)) return;
+    int to = static_cast<int>(__float_as_uint(scale) >> 23) - 127 - 6;
+    float top = 0.f;
+#pragma unroll
+    for (int j = 0; j < P / 16; ++j)
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) top = fmaxf(top, fabsf(o[j][n][e]));
+    const uint32_t bits = __reduce_max_sync(0xffffffffu, __float_as_uint(top));
+    if (bits != 0) {
+      to = max(to, unit - min(120, max(0, 100 - (static_cast<int>(bits >> 23) - 127))));
+      const float f = power2(max(unit - to, -126));
+#pragma unroll
+      for (int j = 0; j < P / 16; ++j)
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[j][n][e] *= f;
+    }
+    unit = to;
+  }
+  // l of the whole warp, o in units of 1
   __device__ __forceinline__ void sum_up() {
+    const float up = power2(unit);
+#pragma unroll
+    for (int j = 0; j < P / 16; ++j)
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[j][n][e] *= up;
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -381,10 +407,14 @@ __device__ __forceinline__ void codes_unit(const CacheAttnArgs& a, const Queries
 #pragma unroll
       for (int e = 0; e < 4; ++e) s[k][n][e] = -INFINITY;
     if (k >= whole) continue;
-    const float scale = scales[k].x;
+    const float key_scale = scales[k].x;
     const uint4* key = reinterpret_cast<const uint4*>(stage + k * kSlot) + lane;
     int sq0 = 0, sq1 = 0;
     float acc[NT][4];
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[n][e] = 0.f;
 #pragma unroll
     for (int d = 0; d < P / 64; ++d) {
       const uint4 w0 = key[2 * d * 32], w1 = key[(2 * d + 1) * 32];
@@ -395,10 +425,7 @@ __device__ __forceinline__ void codes_unit(const CacheAttnArgs& a, const Queries
         sq1 += dot4(r1[i]);
         const uint32_t A[4] = {codes_lo(r0[i]), codes_lo(r1[i]), codes_hi(r0[i]), codes_hi(r1[i])};
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          if (d == 0 && i == 0) mma16816_first<false>(acc[n], A, q.w[n][0][0], q.w[n][0][1]);
-          else mma16816<false>(acc[n], A, q.w[n][d * 4 + i][0], q.w[n][d * 4 + i][1]);
-        }
+        for (int n = 0; n < NT; ++n) mma16816<false>(acc[n], A, q.w[n][d * 4 + i][0], q.w[n][d * 4 + i][1]);
       }
     }
 #pragma unroll
@@ -406,13 +433,13 @@ __device__ __forceinline__ void codes_unit(const CacheAttnArgs& a, const Queries
       sq0 += __shfl_xor_sync(0xffffffffu, sq0, x);
       sq1 += __shfl_xor_sync(0xffffffffu, sq1, x);
     }
-    const float bias = a.scale * scale * scale;
+    const float bias = a.scale * key_scale * key_scale;
     const float b0 = bias * static_cast<float>(sq0), b1 = bias * static_cast<float>(sq1);
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        const float mul = q.mul[n][e] * scale;
+        const float mul = q.mul[n][e] * key_scale;
         s[k][n][e] = fmaf(acc[n][e], mul, -b0);
         s[k][n][2 + e] = fmaf(acc[n][2 + e], mul, -b1);
       }
@@ -427,19 +454,32 @@ __device__ __forceinline__ void codes_unit(const CacheAttnArgs& a, const Queries
     }
   }
   run.weigh(s);
+  float scale[UB], most = 0.f;
+#pragma unroll
+  for (int k = 0; k < UB; ++k) {
+    scale[k] = k < whole ? scales[k].y : 0.f;
+    if (scale[k] < INFINITY) most = fmaxf(most, scale[k]);
+  }
+  run.refer(most);
+  const float down = power2(-run.unit);
 #pragma unroll
   for (int k = 0; k < UB; ++k) {
     if (k >= whole) continue;
     uint32_t p[NT][2];
+    const float by = scale[k] * down;
+    const bool finite = fabsf(scale[k]) < INFINITY;
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        s[k][n][e] *= by;
+        // a block that is not finite reaches the columns that see it, whatever its weight, and no other
+        if (!finite) s[k][n][e] = begin + k * kBlockTokens <= q.limit[n][e % 2] ? __int_as_float(0x7fc00000) : 0.f;
+      }
       p[n][0] = transpose8(pack2<false>(s[k][n][0], s[k][n][1]));
       p[n][1] = transpose8(pack2<false>(s[k][n][2], s[k][n][3]));
     }
     const uint4* value = reinterpret_cast<const uint4*>(stage + k * kSlot + 16 * P) + lane;
-    const float scale = scales[k].y;
-    const bool finite = fabsf(scale) < INFINITY;
-    const int base = begin + k * kBlockTokens;
 #pragma unroll
     for (int i = 0; i < P / 32; ++i) {
       const uint4 w = value[i * 32];
@@ -448,19 +488,7 @@ __device__ __forceinline__ void codes_unit(const CacheAttnArgs& a, const Queries
         const uint32_t r0 = half ? w.z : w.x, r1 = half ? w.w : w.y;
         const uint32_t A[4] = {codes_lo(r0), codes_lo(r1), codes_hi(r0), codes_hi(r1)};
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          float acc[4];
-          mma16816_first<false>(acc, A, p[n][0], p[n][1]);
-          float(&o)[4] = run.o[2 * i + half][n];
-          if (finite) {
-            ffma2v(o[0], o[1], acc[0], acc[1], scale, scale, o[0], o[1]);
-            ffma2v(o[2], o[3], acc[2], acc[3], scale, scale, o[2], o[3]);
-          } else {                                  // a block that is not finite reaches the columns that see it
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              if (base <= q.limit[n][e % 2]) o[e] = fmaf(acc[e], scale, o[e]);
-          }
-        }
+        for (int n = 0; n < NT; ++n) mma16816<false>(run.o[2 * i + half][n], A, p[n][0], p[n][1]);
       }
     }
   }
@@ -533,22 +561,20 @@ __device__ __forceinline__ void rest_unit(const CacheAttnArgs& a, const Queries<
     p[n][1] = transpose8(pack2<kBf16>(s[0][n][2], s[0][n][3]));
   }
   uint2 x[KC][4];                                  // dims 32 i + 4 g ... + 3 of tokens 4 t + r
-  bool odd = false;                                // a value that is not finite
+  uint32_t most = 0;                               // largest magnitudes of even and odd dims, as integers
 #pragma unroll
   for (int i = 0; i < KC; ++i)
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       x[i][r] = make_uint2(0, 0);
       if (base + 4 * t + r < total) x[i][r] = *reinterpret_cast<const uint2*>(values + (4 * t + r) * P + 32 * i + 4 * g);
-      constexpr uint32_t kInf = kBf16 ? 0x7f80u : 0x7c00u;
-#pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        const uint32_t y = half ? x[i][r].y : x[i][r].x;
-        odd |= (y & kInf) == kInf || (y >> 16 & kInf) == kInf;
-      }
+      most = __vmaxu2(most, __vmaxu2(x[i][r].x & 0x7fff7fffu, x[i][r].y & 0x7fff7fffu));
     }
+  most = __reduce_max_sync(0xffffffffu, max(most & 0xffffu, most >> 16));
+  const bool finite = most < (kBf16 ? 0x7f80u : 0x7c00u);
+  if (finite) run.refer(unpack2<kBf16>(most).x * 0.0078125f);
   // A product 0 * inf of a column that does not see the token must not reach it: such blocks go token by token.
-  const bool slow = __any_sync(0xffffffffu, odd) && total - 1 > q.first_limit;
+  const bool slow = !finite && total - 1 > q.first_limit;
 #pragma unroll 1
   for (int only = slow ? 0 : kBlockTokens - 1; only < kBlockTokens; ++only) {
 #pragma unroll
@@ -566,11 +592,11 @@ __device__ __forceinline__ void rest_unit(const CacheAttnArgs& a, const Queries<
       }
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
-        float acc[4];
-        mma16816_first<kBf16>(acc, A, p[n][0], p[n][1]);
+        float acc[4] = {0.f, 0.f, 0.f, 0.f};
+        mma16816<kBf16>(acc, A, p[n][0], p[n][1]);
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-          if (!slow || base + only <= q.limit[n][e % 2]) run.o[j][n][e] += acc[e];
+          if (!slow || base + only <= q.limit[n][e % 2]) run.o[j][n][e] = fmaf(acc[e], power2(-run.unit), run.o[j][n][e]);
       }
     }
   }

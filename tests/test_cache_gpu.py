@@ -296,6 +296,28 @@ def test_extreme_queries_and_keys():
            _reference(pool, q, [299] * 4, [1] * 4, False)[1:3], BF16)
 
 
+@pytest.mark.parametrize("long", [False, True])
+@pytest.mark.parametrize("D", [64, 128])
+def test_values_of_very_different_sizes(D, long):
+    """Blocks whose scales jump by large powers of two either way, seen by queries that attend to the large or the small ones."""
+    pool = Pool(3, 2, D, 512, BF16, long=long)
+    N = 300
+    k, v = _randn(3, 2, N, D, seed=60), _randn(3, 2, N, D, seed=61)
+    size = torch.ones(3, 1, N, 1, device=DEV)
+    size[0, 0, 32:64], size[0, 0, 64:80], size[0, 0, 200:] = 2.0**40, 2.0**-60, 2.0**90
+    size[1, 0, :100], size[1, 0, 100:250], size[1, 0, 250:] = 2.0**100, 2.0**-90, 2.0**-20
+    size[2, 0, ::7] = 2.0**30
+    v = (v.float() * size).to(BF16)
+    k[1, :, :100] *= 40                     # far from every query: weight zero
+    pool.append(k, v)
+    q = _randn(3, 2, 4, D, seed=62)
+    got = ops.cache_attention(q, pool.pages, pool.table, _ints([N - 4] * 3))
+    want = _reference(pool, q, [N - 4] * 3, [4] * 3, True)
+    for b in range(3):
+        scale = want[b].abs().max()
+        _check(got[b].double() / scale, want[b] / scale, BF16)
+
+
 def test_copied_pages():
     for layers in (None, 1, 3):
         for copies in (1, 7, 600):
