@@ -86,14 +86,15 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
   return y;
 }
 
-// Bytes 0, 1 (2, 3) of a word of codes as two fp16 numbers
-__device__ __forceinline__ uint32_t codes_lo(uint32_t w) {
-  const uint32_t x = __byte_perm(w, 0x64646464u, 0x4140);
+// Bytes 0, 1 (2, 3) of a word of codes as two fp16 numbers. `exponents` is 0x64 in every byte, from the kernel's arguments: of a
+// constant that it knows the compiler makes a move before almost every permute (43 for 64).
+__device__ __forceinline__ uint32_t codes_lo(uint32_t w, uint32_t exponents) {
+  const uint32_t x = __byte_perm(w, exponents, 0x4140);
   const __half2 y = __hsub2(*reinterpret_cast<const __half2*>(&x), __half2half2(__ushort_as_half(0x6480)));
   return *reinterpret_cast<const uint32_t*>(&y);
 }
-__device__ __forceinline__ uint32_t codes_hi(uint32_t w) {
-  const uint32_t x = __byte_perm(w, 0x64646464u, 0x4342);
+__device__ __forceinline__ uint32_t codes_hi(uint32_t w, uint32_t exponents) {
+  const uint32_t x = __byte_perm(w, exponents, 0x4342);
   const __half2 y = __hsub2(*reinterpret_cast<const __half2*>(&x), __half2half2(__ushort_as_half(0x6480)));
   return *reinterpret_cast<const uint32_t*>(&y);
 }
@@ -310,9 +311,11 @@ struct Queries {
   int limit[NT][2];                                // last token that the column sees
   int first_limit, last_limit;                     // every column of the tile sees at least, none sees more
   int b, h, c0, total;
+  uint32_t exponents;
 
   __device__ __forceinline__ void load(const CacheAttnArgs& a, int b_, int h_, int c0_, int held, int total_) {
     b = b_, h = h_, c0 = c0_, total = total_;
+    exponents = a.exponents;
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
@@ -423,7 +426,8 @@ __device__ __forceinline__ void codes_unit(const CacheAttnArgs& a, const Queries
       for (int i = 0; i < 4; ++i) {
         sq0 += dot4(r0[i]);
         sq1 += dot4(r1[i]);
-        const uint32_t A[4] = {codes_lo(r0[i]), codes_lo(r1[i]), codes_hi(r0[i]), codes_hi(r1[i])};
+        const uint32_t A[4] = {codes_lo(r0[i], q.exponents), codes_lo(r1[i], q.exponents), codes_hi(r0[i], q.exponents),
+                               codes_hi(r1[i], q.exponents)};
 #pragma unroll
         for (int n = 0; n < NT; ++n) mma16816<false>(acc[n], A, q.w[n][d * 4 + i][0], q.w[n][d * 4 + i][1]);
       }
@@ -486,7 +490,7 @@ __device__ __forceinline__ void codes_unit(const CacheAttnArgs& a, const Queries
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
         const uint32_t r0 = half ? w.z : w.x, r1 = half ? w.w : w.y;
-        const uint32_t A[4] = {codes_lo(r0), codes_lo(r1), codes_hi(r0), codes_hi(r1)};
+        const uint32_t A[4] = {codes_lo(r0, q.exponents), codes_lo(r1, q.exponents), codes_hi(r0, q.exponents), codes_hi(r1, q.exponents)};
 #pragma unroll
         for (int n = 0; n < NT; ++n) mma16816<false>(run.o[2 * i + half][n], A, p[n][0], p[n][1]);
       }
@@ -1104,6 +1108,7 @@ cudaError_t launch_cache_attn(CacheAttnArgs a, bool bf16, int sms, cudaStream_t 
   const int64_t columns = 8 * cache_attn_tiles(a.T, a.G, cache_columns(a.D)), tiles = (static_cast<int64_t>(a.T) * a.G + columns - 1) / columns;
   if (tiles * columns * a.H * a.B > 0x7fffffffll) return cudaErrorInvalidConfiguration;
   a.column_tiles = static_cast<int>(tiles);
+  a.exponents = 0x64646464u;
   if (cache_columns(a.D) == 64) return bf16 ? attn_p<true, 64>(a, sms, stream) : attn_p<false, 64>(a, sms, stream);
   return bf16 ? attn_p<true, 128>(a, sms, stream) : attn_p<false, 128>(a, sms, stream);
 }

@@ -229,7 +229,8 @@ struct CacheAttnArgs {
   int B, H, G, T, D, max_pages, num_pages;
   int softmax;
   float scale;               // log2(e) / sqrt(head dim)
-  int column_tiles;          // set by the launcher
+  int column_tiles;          // set by the launcher, as what follows
+  uint32_t exponents;        // a constant that the compiler is not to know
 };
 int cache_attn_tiles(int T, int G, int P);
 size_t cache_attn_workspace_bytes(int B, int H, int G, int T, int D, int max_pages, int sms);
