@@ -147,16 +147,18 @@ __device__ __forceinline__ const uint16_t* q_row(const CacheAttnArgs& a, int b, 
   return static_cast<const uint16_t*>(a.q) + b * a.qs[0] + (h * a.G + c % a.G) * a.qs[1] + c / a.G * a.qs[2];
 }
 
-// The workspace: a note per warp, then two parts per warp. A warp that has the first units of a segment which goes on with the
-// next warp leaves a note about it; its part of that segment is its second, the parts of the others are their first ones.
-struct Note {
-  int b, seg, last, fresh;                         // sequence (-1: no such segment), segment in it, last warp, real new tokens
+// The workspace: notes, one per segment or per warp, whichever are fewer, then two parts per warp. A warp that has the first
+// units of a segment which goes on with the next warp leaves a note about it; its part of that segment is its second, the
+// parts of the others are their first ones.
+struct alignas(16) Note {
+  int b, seg, first, last, fresh, unused[3];       // sequence (-1: nothing to join), segment in it, its warps, real new tokens
 };
-// One part: per column P outputs, then of all columns the maxima, the sums and what the variant without a denominator needs
-constexpr int part_floats(int P, int NT) { return 8 * NT * (P + 4); }
+// One part: per column P outputs and three numbers, the maximum, the sum and what the variant without a denominator needs; of
+// as many columns as a tile has at most
+constexpr int part_pitch(int P) { return P + 4; }
 template <int P, int NT>
-__device__ __forceinline__ float* part_of(const CacheAttnArgs& a, int64_t workers, int64_t index) {
-  return a.parts + workers * (sizeof(Note) / sizeof(float)) + index * part_floats(P, NT);
+__device__ __forceinline__ float* part_of(const CacheAttnArgs& a, int64_t index) {
+  return a.parts + a.notes * (sizeof(Note) / sizeof(float)) + index * (min(8 * NT, a.T * a.G) * part_pitch(P));
 }
 
 // 2^x for -126 <= x <= 127
@@ -626,13 +628,16 @@ __global__ void __launch_bounds__(Shape<P, NT>::kWarps * 32) cache_attn_kernel(c
   const Deal deal(sum_units<UB>(a) * segments, workers);
   int64_t at = deal.begin(self);
   const int64_t stop = deal.begin(self + 1);
-  Note* const note = reinterpret_cast<Note*>(a.parts) + self;
-  if (lane == 0) note->b = -1;
+  Note* const notes = reinterpret_cast<Note*>(a.parts);
+  const bool by_segment = a.notes < workers;
+  if (lane == 0 && !by_segment) notes[self].b = -1;
   for (int64_t empty = self; empty < a.B; empty += workers) {              // sequences without new tokens
     if (Units<UB>(a, static_cast<int>(empty)).count != 0) continue;
     const int64_t words = static_cast<int64_t>(a.H) * a.G * a.T * a.D / 8;
     uint4* out = reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out)) + empty * words;
     for (int64_t i = lane; i < words; i += 32) out[i] = make_uint4(0, 0, 0, 0);
+    if (by_segment)
+      for (int i = lane; i < segments; i += 32) notes[empty * segments + i].b = -1;
   }
   if (at >= stop) return;
 
@@ -734,9 +739,11 @@ __global__ void __launch_bounds__(Shape<P, NT>::kWarps * 32) cache_attn_kernel(c
     // ---- the segment's output, or this warp's part of it
     run.sum_up();
     const bool complete = u0 == 0 && u1 == units.count;
-    float* part = part_of<P, NT>(a, workers, 2 * self + (u0 == 0));
-    if (!complete && u0 == 0 && lane == 0)
-      *note = {b, seg, static_cast<int>(min(deal.worker(at - u0 + units.count - 1), workers - 1)), units.fresh};
+    float* part = part_of<P, NT>(a, 2 * self + (u0 == 0));
+    if (u0 == 0 && lane == 0 && (by_segment || !complete)) {
+      const int last = static_cast<int>(min(deal.worker(at + units.count - 1), workers - 1));
+      notes[by_segment ? static_cast<int64_t>(b) * segments + seg : self] = {complete ? -1 : b, seg, static_cast<int>(self), last, units.fresh, {}};
+    }
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -758,17 +765,34 @@ __global__ void __launch_bounds__(Shape<P, NT>::kWarps * 32) cache_attn_kernel(c
             *reinterpret_cast<uint2*>(out + d) = y;
           }
         } else {
-          run.store(part + in * P, n, e);
-          if (g == 0) {
-            part[8 * NT * P + in] = m;
-            part[8 * NT * (P + 1) + in] = l;
-            part[8 * NT * (P + 2) + in] = q.sq[n][e];
-          }
+          run.store(part + in * part_pitch(P), n, e);
+          if (g == 0) *reinterpret_cast<float4*>(part + in * part_pitch(P) + P) = make_float4(m, l, q.sq[n][e], 0.f);
         }
       }
     at += u1 - u0;
   }
   grid_dependents_launch();
+}
+
+// (m, l, y) of a column from two sets of its tokens
+template <int kCount>
+__device__ __forceinline__ void join(float& m, float& l, float (&y)[kCount], float m2, float l2, const float (&y2)[kCount]) {
+  const float x = fmaxf(m, m2), ref = x == -INFINITY ? 0.f : x;
+  const float f = attn_ex2(m - ref), f2 = attn_ex2(m2 - ref);
+  m = x;
+  l = l * f + l2 * f2;
+#pragma unroll
+  for (int i = 0; i < kCount; ++i) y[i] = y[i] * f + y2[i] * f2;
+}
+template <int kCount>
+__device__ __forceinline__ void load_floats(const float* from, float (&x)[kCount]) {
+  if constexpr (kCount == 4) {
+    const float4 v = *reinterpret_cast<const float4*>(from);
+    x[0] = v.x, x[1] = v.y, x[2] = v.z, x[3] = v.w;
+  } else {
+    const float2 v = *reinterpret_cast<const float2*>(from);
+    x[0] = v.x, x[1] = v.y;
+  }
 }
 
 // A segment per block, or per cluster of blocks, whose warps take its units in turn: for short sequences, whose time is the
@@ -851,24 +875,15 @@ __global__ void __launch_bounds__(kWarps * 32, 16 / kWarps) cache_attn_short_ker
   float* parts = reinterpret_cast<float*>(smem);
   constexpr int kPerColumn = P / 4;                // threads of a column, four dims each
   const int used = columns * kPerColumn;
-  // y, m and l of column i / kPerColumn from `count` parts `pitch` floats apart
   struct Joined {
-    float m, l;
-    float4 y;
-    __device__ void add(float m2, float l2, float4 y2) {
-      const float x = fmaxf(m, m2), ref = x == -INFINITY ? 0.f : x;
-      const float f0 = attn_ex2(m - ref), f1 = attn_ex2(m2 - ref);
-      m = x;
-      l = l * f0 + l2 * f1;
-      y = make_float4(y.x * f0 + y2.x * f1, y.y * f0 + y2.y * f1, y.z * f0 + y2.z * f1, y.w * f0 + y2.w * f1);
-    }
+    float m = -INFINITY, l = 0.f, y[4] = {};
   };
   auto write = [&](int i, const Joined& j) {
     const int c = i / kPerColumn, d = i % kPerColumn * 4;
     if (d >= a.D) return;
     float f = 0.f;
     if (c / a.G < units.fresh) f = last_factor(a, j.m, j.l, parts[8 * P + 16 + c]);
-    uint2 y = make_uint2(pack2<kBf16>(j.y.x * f, j.y.y * f), pack2<kBf16>(j.y.z * f, j.y.w * f));
+    uint2 y = make_uint2(pack2<kBf16>(j.y[0] * f, j.y[1] * f), pack2<kBf16>(j.y[2] * f, j.y[3] * f));
     if (c / a.G >= units.fresh || (j.m == -INFINITY && j.l == 0.f)) y = make_uint2(0, 0);
     *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.out) + out_offset(a, b, h, c) + d) = y;
   };
@@ -877,17 +892,19 @@ __global__ void __launch_bounds__(kWarps * 32, 16 / kWarps) cache_attn_short_ker
   __syncthreads();
   for (int i = threadIdx.x; i < used; i += kWarps * 32) {
     const int c = i / kPerColumn, at = c * P + i % kPerColumn * 4;
-    Joined j{-INFINITY, 0.f, make_float4(0.f, 0.f, 0.f, 0.f)};
+    Joined j;
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) {
       const float* p = parts + w * kPart;
-      j.add(p[8 * P + c], p[8 * P + 8 + c], *reinterpret_cast<const float4*>(p + at));
+      float y2[4];
+      load_floats(p + at, y2);
+      join(j.m, j.l, j.y, p[8 * P + c], p[8 * P + 8 + c], y2);
     }
     if (ranks == 1) {
       write(i, j);
     } else {                                       // the block's part, where the second warp's was: read by this thread alone
       float* p = parts + kPart;
-      *reinterpret_cast<float4*>(p + at) = j.y;
+      *reinterpret_cast<float4*>(p + at) = make_float4(j.y[0], j.y[1], j.y[2], j.y[3]);
       if (i % kPerColumn == 0) {
         p[8 * P + 32 + c] = j.m;
         p[8 * P + 40 + c] = j.l;
@@ -900,17 +917,16 @@ __global__ void __launch_bounds__(kWarps * 32, 16 / kWarps) cache_attn_short_ker
   if (rank == 0) {
     for (int i = threadIdx.x; i < used; i += kWarps * 32) {
       const int c = i / kPerColumn, at = c * P + i % kPerColumn * 4;
-      Joined j{-INFINITY, 0.f, make_float4(0.f, 0.f, 0.f, 0.f)};
+      Joined j;
       for (uint32_t r = 0; r < ranks; ++r) {
         uint32_t there;
         asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(smem_u32(parts + kPart)), "r"(r));
-        float m2, l2;
-        float4 y2;
+        float m2, l2, y2[4];
         asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(m2) : "r"(there + (8 * P + 32 + c) * 4));
         asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(l2) : "r"(there + (8 * P + 40 + c) * 4));
         asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
-                     : "=f"(y2.x), "=f"(y2.y), "=f"(y2.z), "=f"(y2.w) : "r"(there + at * 4));
-        j.add(m2, l2, y2);
+                     : "=f"(y2[0]), "=f"(y2[1]), "=f"(y2[2]), "=f"(y2[3]) : "r"(there + at * 4));
+        join(j.m, j.l, j.y, m2, l2, y2);
       }
       write(i, j);
     }
@@ -919,120 +935,87 @@ __global__ void __launch_bounds__(kWarps * 32, 16 / kWarps) cache_attn_short_ker
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");   // blocks stay until they have been read
 }
 
-constexpr int kJoinWarps = 8;
+constexpr int kJoinWarps = 32;                     // of a block at most
 
-// Joins the parts of the segments that several warps worked on, a block for each that begins with warp blockIdx.x: columns go
-// to the block's warps in turn, as many warps share the parts of a column as there are warps for them.
+// Joins the parts of the segments that several warps worked on: blocks (i, ...) the segment of note i, a block's warps its
+// columns in groups of `split` to a column.
 template <bool kBf16, int P, int NT>
-__global__ void __launch_bounds__(kJoinWarps * 32) cache_join_kernel(const CacheAttnArgs a, const int workers) {
+__global__ void __launch_bounds__(kJoinWarps * 32) cache_join_kernel(const CacheAttnArgs a, const int workers, const int split) {
   __shared__ float s_y[kJoinWarps][P], s_m[kJoinWarps], s_l[kJoinWarps];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  grid_dependency_wait();
-  const int first = blockIdx.x;
-  const Note note = reinterpret_cast<const Note*>(a.parts)[first];
-  if (note.b < 0) return;
-  const int h = note.seg % a.H, c0 = note.seg / a.H * (8 * NT), columns = min(8 * NT, a.T * a.G - c0);
-  const int split = columns == 1 ? 8 : columns == 2 ? 4 : columns <= 4 ? 2 : 1;
-  const int share = warp % split;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, share = warp % split;
   constexpr int kPer = P / 32;
-  for (int in = warp / split; in - warp / split < columns; in += kJoinWarps / split) {     // as often for every warp
-    const bool real = in < columns;
-    const int c = c0 + in;
-    float y[kPer] = {}, top = -INFINITY, sum = 0.f, q_sq = 0.f;
-    if (real && c / a.G < note.fresh) {
-      q_sq = part_of<P, NT>(a, workers, 2 * first + 1)[8 * NT * (P + 2) + in];
-      // lane i has the maximum and the sum of the warp's i-th part, four parts' outputs are under way at a time
-      for (int w0 = first + share; w0 <= note.last; w0 += 32 * split) {
-        const int n = min((note.last - w0) / split + 1, 32);
-        auto part = [&](int i) {
-          const int w = w0 + i * split;
-          return part_of<P, NT>(a, workers, 2 * w + (w == first));
-        };
-        float m = -INFINITY, l = 0.f;
-        if (lane < n) {
-          m = part(lane)[8 * NT * P + in];
-          l = part(lane)[8 * NT * (P + 1) + in];
-        }
-        float z[4][kPer];
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-#pragma unroll
-          for (int i = 0; i < kPer; ++i) z[j][i] = j < n ? part(j)[in * P + lane * kPer + i] : 0.f;
-        float x = m;
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
-        x = fmaxf(x, top);
-        const float ref = x == -INFINITY ? 0.f : x, f = attn_ex2(m - ref), old = attn_ex2(top - ref);
-        top = x;
-        l *= f;
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
-        sum = fmaf(sum, old, l);
-#pragma unroll
-        for (int i = 0; i < kPer; ++i) y[i] *= old;
-        for (int j0 = 0; j0 < n; j0 += 4) {
-          float next[4][kPer];
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-#pragma unroll
-            for (int i = 0; i < kPer; ++i) next[j][i] = j0 + 4 + j < n ? part(j0 + 4 + j)[in * P + lane * kPer + i] : 0.f;
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const float fj = __shfl_sync(0xffffffffu, f, (j0 + j) & 31);
-            if (j0 + j < n)
-#pragma unroll
-              for (int i = 0; i < kPer; ++i) y[i] = fmaf(z[j][i], fj, y[i]);
-          }
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-#pragma unroll
-            for (int i = 0; i < kPer; ++i) z[j][i] = next[j][i];
-        }
-      }
+  grid_dependency_wait();
+  const int in = static_cast<int>(blockIdx.y) * (static_cast<int>(blockDim.x) / 32 / split) + warp / split;
+  const Note note = reinterpret_cast<const Note*>(a.parts)[blockIdx.x];
+  // nothing to join; and lengths that changed while the kernels ran must not lead outside of the tensors
+  if (note.b < 0 || note.b >= a.B || static_cast<unsigned>(note.seg) >= static_cast<unsigned>(a.column_tiles * a.H) ||
+      note.first < 0 || note.first > note.last || note.last >= workers)
+    return;
+  const int first = note.first;
+  const int h = note.seg % a.H, c = note.seg / a.H * (8 * NT) + in;
+  const bool real = in < 8 * NT && c < a.T * a.G, some = real && c / a.G < note.fresh;
+  float y[kPer] = {}, m = -INFINITY, l = 0.f, q_sq = 0.f;
+  if (some) {
+    const int64_t pitch = min(8 * NT, a.T * a.G) * part_pitch(P);
+    const float* part = part_of<P, NT>(a, 2 * (first + share) + (share == 0)) + in * part_pitch(P);
+    if (share == 0) q_sq = part[P + 2];
+#pragma unroll 4
+    for (int w = first + share; w <= note.last; w += split) {
+      float y2[kPer];
+      load_floats(part + lane * kPer, y2);
+      const float4 of_column = *reinterpret_cast<const float4*>(part + P);
+      join(m, l, y, of_column.x, of_column.y, y2);
+      part += (2 * split - (w == first)) * pitch;
     }
-    if (split > 1) {                               // one round: every column has its warps
-#pragma unroll
-      for (int i = 0; i < kPer; ++i) s_y[warp][lane * kPer + i] = y[i];
-      if (lane == 0) {
-        s_m[warp] = top;
-        s_l[warp] = sum;
-      }
-      __syncthreads();
-      if (share != 0) return;
-      for (int w = warp + 1; w < warp + split; ++w) {
-        const float x = fmaxf(top, s_m[w]), ref = x == -INFINITY ? 0.f : x;
-        const float f0 = attn_ex2(top - ref), f1 = attn_ex2(s_m[w] - ref);
-        top = x;
-        sum = sum * f0 + s_l[w] * f1;
-#pragma unroll
-        for (int i = 0; i < kPer; ++i) y[i] = y[i] * f0 + s_y[w][lane * kPer + i] * f1;
-      }
-    }
-    if (!real) continue;
-    if (c / a.G < note.fresh) {
-      const float f = last_factor(a, top, sum, q_sq);
-      const bool none = top == -INFINITY && sum == 0.f;
-#pragma unroll
-      for (int i = 0; i < kPer; ++i) y[i] = none ? 0.f : y[i] * f;
-    }
-    if (lane * kPer >= a.D) continue;
-    uint16_t* to = static_cast<uint16_t*>(a.out) + out_offset(a, note.b, h, c) + lane * kPer;
-#pragma unroll
-    for (int i = 0; i < kPer; i += 2) *reinterpret_cast<uint32_t*>(to + i) = pack2<kBf16>(y[i], y[i + 1]);
   }
+  if (split > 1) {
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) s_y[warp][lane * kPer + i] = y[i];
+    if (lane == 0) {
+      s_m[warp] = m;
+      s_l[warp] = l;
+    }
+    __syncthreads();
+    if (share != 0) return;
+    for (int w = warp + 1; w < warp + split; ++w) {
+      float y2[kPer];
+      load_floats(s_y[w] + lane * kPer, y2);
+      join(m, l, y, s_m[w], s_l[w], y2);
+    }
+  }
+  if (!real || lane * kPer >= a.D) return;
+  const float f = some ? last_factor(a, m, l, q_sq) : 0.f;
+  const bool none = !some || (m == -INFINITY && l == 0.f);
+  uint32_t packed[kPer / 2];
+#pragma unroll
+  for (int i = 0; i < kPer / 2; ++i) packed[i] = none ? 0u : pack2<kBf16>(y[2 * i] * f, y[2 * i + 1] * f);
+  uint16_t* to = static_cast<uint16_t*>(a.out) + out_offset(a, note.b, h, c) + lane * kPer;
+  if constexpr (kPer == 4) *reinterpret_cast<uint2*>(to) = make_uint2(packed[0], packed[1]);
+  else *reinterpret_cast<uint32_t*>(to) = packed[0];
 }
 
+int64_t cache_attn_notes(int64_t segments, int64_t workers) { return segments < workers ? segments : workers; }
+
 template <bool kBf16, int P, int NT>
-cudaError_t attn_t(const CacheAttnArgs& a, int sms, cudaStream_t stream) {
+cudaError_t attn_t(CacheAttnArgs a, int sms, cudaStream_t stream) {
   using S = Shape<P, NT>;
   constexpr int kSmem = S::kWarps * S::kStages * Tile<P, S::kUnitBlocks>::kStage;
+  const int workers = sms * S::kWarps;
+  const int64_t segments = static_cast<int64_t>(a.B) * a.column_tiles * a.H;
+  a.notes = static_cast<int>(cache_attn_notes(segments, workers));
   static PerDeviceFlags flags;
   cudaError_t e = ensure_dynamic_smem(cache_attn_kernel<kBf16, P, NT>, kSmem, flags);
   if (e != cudaSuccess) return e;
   cache_attn_kernel<kBf16, P, NT><<<sms, S::kWarps * 32, kSmem, stream>>>(a);
   if ((e = cudaGetLastError()) != cudaSuccess) return e;
-  const int workers = sms * S::kWarps;
-  return launch_dependent(cache_join_kernel<kBf16, P, NT>, dim3(workers), kJoinWarps * 32, 0, stream, a, workers);
+  // a warp for every eight of the parts that a segment has on average, and eight warps or more to a block
+  const int width = static_cast<int64_t>(a.T) * a.G < 8 * NT ? a.T * a.G : 8 * NT;
+  const int64_t parts = workers / segments;
+  int split = 1;
+  while (split < kJoinWarps && split * 8 < parts) split *= 2;
+  const int warps = split > 8 ? split : 8, each = warps / split;
+  return launch_dependent(cache_join_kernel<kBf16, P, NT>, dim3(a.notes, (width + each - 1) / each), warps * 32, 0, stream, a,
+                          workers, split);
 }
 
 // Blocks of a cluster that share a segment in the kernel for short sequences, 0: not that kernel. It is for one tile of columns
@@ -1100,7 +1083,9 @@ size_t cache_attn_workspace_bytes(int B, int H, int G, int T, int D, int max_pag
   const int P = cache_columns(D);
   if (short_ranks(static_cast<int64_t>(B) * H, static_cast<int64_t>(T) * G, max_pages, sms)) return 0;
   const int tiles = cache_attn_tiles(T, G, P), warps = tiles > 1 ? Shape<64, 2>::kWarps : Shape<64, 1>::kWarps;
-  return static_cast<size_t>(sms) * warps * (sizeof(Note) + 2 * part_floats(P, tiles) * sizeof(float));
+  const int width = static_cast<int64_t>(T) * G < 8 * tiles ? T * G : 8 * tiles;
+  const int64_t workers = static_cast<int64_t>(sms) * warps;
+  return static_cast<size_t>(workers) * (sizeof(Note) + 2 * width * part_pitch(P) * sizeof(float));
 }
 
 cudaError_t launch_cache_attn(CacheAttnArgs a, bool bf16, int sms, cudaStream_t stream) {

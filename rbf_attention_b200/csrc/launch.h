@@ -230,6 +230,7 @@ struct CacheAttnArgs {
   int softmax;
   float scale;               // log2(e) / sqrt(head dim)
   int column_tiles;          // set by the launcher, as what follows
+  int notes;                 // segments of which several warps may have parts
   uint32_t exponents;        // a constant that the compiler is not to know
 };
 int cache_attn_tiles(int T, int G, int P);
