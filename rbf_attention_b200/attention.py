@@ -26,6 +26,7 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
+from . import ops
 from .ops import exclusive_self_attention, linear, run_triton_non_softmax_rbf, run_triton_rbf, susie_block_attention
 
 __all__ = [
@@ -269,3 +270,55 @@ class CustomCausalAttention(nn.Module):
 
         out = out.transpose(1, 2).reshape(bsz, seq_len, emb)
         return linear(self.proj, out), attn_weights
+
+    # -- with a cache ----------------------------------------------------------------------------
+    def _susie_at(self, positions: torch.Tensor, seq_len: int, like: torch.Tensor) -> torch.Tensor:
+        """(B, H, seq_len, D) additive position term, fp32, of tokens ``positions[b]`` onwards: ``_susie_embedding`` of places
+        that only the device knows."""
+        r = self.num_registers
+        at = positions[:, None] + torch.arange(seq_len, device=positions.device, dtype=positions.dtype)
+        table = self._susie_table_f32()
+        if table.device != like.device:
+            table = table.to(like.device)
+        weight = self.pos_weight.float().repeat(1, 1, 1, 2)
+        emb = table[(at - r).clamp(0, table.shape[0] - 1)][:, None] * weight
+        if r > 0:
+            learned = self.reg_pos_emb.float().squeeze(0)[:, at.clamp(max=r - 1)].transpose(0, 1)
+            emb = torch.where((at < r)[:, None, :, None], learned, emb)
+        return emb
+
+    def forward_cached(self, x, cache, layer: int, from_empty: bool = False):
+        """``forward(x)`` for the new tokens of a step of ``cache`` (between its ``begin`` and ``end``): they are appended as
+        layer ``layer`` and attend to all that their sequences hold. ``from_empty``: the sequences have nothing yet, so the
+        tokens attend to themselves, in 16 bits, and the cache is only written. RBF attention types, without gradients."""
+        kind = self.attention_type
+        if kind not in ("rbf_triton", "rbf_flex", "rbf_non_softmax"):
+            raise ValueError(f"attention_type {kind!r} has no cached form")
+        bsz, seq_len, emb = x.shape
+        softmax = kind != "rbf_non_softmax"
+        qkv = linear(self.qkv_proj, x)
+        if from_empty and self._fused_block(qkv):
+            reg = self.reg_pos_emb.squeeze(0) if self.num_registers > 0 else None
+            out, _, qk = ops.susie_block_fwd(qkv, self.pos_weight.view(self.num_heads, -1), reg, self._susie_table_f32(),
+                                             self.num_heads, softmax)
+            v = qkv.view(bsz, seq_len, 3, self.num_heads, self.head_dim)[:, :, 2].transpose(1, 2)
+            cache.append(layer, qk[1].transpose(1, 2), v)
+            return linear(self.proj, out)
+        q, k, v = qkv.view(bsz, seq_len, 3, self.num_heads, self.head_dim).permute(2, 0, 3, 1, 4).unbind(0)
+        if self.use_qk_norm:
+            q, k = F.rms_norm(q, (self.head_dim,)), F.rms_norm(k, (self.head_dim,))
+        if self.positional_encoding_type == "susie":
+            pos = self._susie_at(cache.positions, seq_len, q)
+            q, k = (q + pos).to(qkv.dtype), (k + pos).to(qkv.dtype)
+        cache.append(layer, k, v)
+        if from_empty:
+            out = (run_triton_rbf if softmax else run_triton_non_softmax_rbf)(q, k, v, is_causal=True)
+        else:
+            out = cache.attend(layer, q, softmax=softmax)
+        if self.apply_xsa:
+            if self.head_dim in (64, 128):
+                out = exclusive_self_attention(out, v)
+            else:
+                v_hat = F.normalize(v, dim=-1)
+                out = out - (out * v_hat).sum(dim=-1, keepdim=True) * v_hat
+        return linear(self.proj, out.transpose(1, 2).reshape(bsz, seq_len, emb))

@@ -12,6 +12,7 @@ import torch.nn.functional as F
 
 from . import ops
 from .attention import CustomCausalAttention
+from .cache import PagedCache
 
 
 def vocab_projection(linear: nn.Linear, x: torch.Tensor, keep_padding: bool = False) -> torch.Tensor:
@@ -99,6 +100,12 @@ class TransformerBlock(nn.Module):
         x, normed = apply_add_layer_norm(self.ln2, x, attn_out)
         return x, self._mlp(normed), attn_weights
 
+    def forward_cached(self, x, cache, layer, from_empty=False, pending=None):
+        """``forward_deferred`` for the new tokens of a step of ``cache``, see CustomCausalAttention.forward_cached."""
+        x, normed = apply_add_layer_norm(self.ln1, x, pending)
+        x, normed = apply_add_layer_norm(self.ln2, x, self.attn.forward_cached(normed, cache, layer, from_empty))
+        return x, self._mlp(normed)
+
     def _mlp(self, x):
         """``self.ff(x)`` (Linear, GELU, Linear) with the activation, its backward and the bias gradients of both
         projections from the library."""
@@ -161,6 +168,110 @@ class CausalLM(nn.Module):
             # contiguous: F.linear takes a strided 3-D input through matmul + a separate bias pass over the logits
             normed = normed[:, self.num_registers:, :].contiguous()
         return vocab_projection(self.to_logits, normed, keep_padding=padded_logits), weights
+
+    # -- answers ---------------------------------------------------------------------------------
+    def new_cache(self, max_sequences: int, max_length: int, num_pages: int | None = None) -> PagedCache:
+        """A cache for ``max_sequences`` sequences of up to ``max_length`` tokens (the register tokens come on top)."""
+        attn = self.blocks[0].attn
+        table = getattr(attn, "susie_cache", None)
+        for limit in (None if table is None else table.shape[0],
+                      self.pos_emb.num_embeddings if self.pos_emb_type == "learned" else None):
+            if limit is not None and max_length > limit:
+                raise ValueError(f"the model's positions end at {limit} tokens, {max_length} are asked for")
+        weight = self.to_logits.weight
+        return PagedCache(len(self.blocks), attn.num_heads, attn.head_dim, max_sequences, max_length + self.num_registers,
+                          num_pages, weight.dtype, weight.device)
+
+    @torch.no_grad()
+    def forward_cached(self, idx, cache: PagedCache, new=None, sequences=None, all_logits: bool = False):
+        """Logits (batch, vocab) behind each sequence's last new token - with ``all_logits`` (batch, T, vocab) behind every one -
+        of the ``idx`` (batch, T) that follow what ``cache`` holds; ``new``: how many of the T are real, per sequence (default:
+        all), ``sequences``: which of the cache's these are (default: all). Either all or none of those that get tokens are
+        empty. A sequence without new tokens has logits of no meaning."""
+        bsz, seq = idx.shape
+        batch = range(cache.max_sequences) if sequences is None else sequences
+        new = [seq] * bsz if new is None else [int(n) for n in new]
+        if len(batch) != bsz or len(new) != bsz or any(not 0 <= n <= seq for n in new):
+            raise ValueError(f"{len(batch)} sequences, new tokens {new} and ids {tuple(idx.shape)} do not go together")
+        empty = {cache.length(s) == 0 for s, n in zip(batch, new) if n}
+        if len(empty) > 1:
+            raise ValueError("some of the sequences are empty, others are not: give them their tokens in two calls")
+        from_empty = empty == {True}
+        skip = self.num_registers if from_empty else 0
+        cache.begin([n + skip if n else 0 for n in new], sequences)
+        try:
+            x = self.token_emb(idx)
+            if self.pos_emb_type == "learned":
+                at = cache.positions[:, None] + torch.arange(seq, device=idx.device) - (0 if from_empty else self.num_registers)
+                x = x + self.pos_emb(at.clamp(0, self.pos_emb.num_embeddings - 1))
+            if skip:
+                x = torch.cat([self.register_tokens.unsqueeze(0).expand(bsz, -1, -1).to(x.dtype), x], dim=1)
+            pending = None
+            for i, block in enumerate(self.blocks):
+                x, pending = block.forward_cached(x, cache, i, from_empty, pending)
+        except BaseException:
+            cache.abort()
+            raise
+        cache.end()
+        _, normed = apply_add_layer_norm(self.ln_f, x, pending)
+        if all_logits:
+            return vocab_projection(self.to_logits, normed[:, skip:].contiguous())
+        last = torch.tensor([skip + max(n - 1, 0) for n in new]).to(idx.device)
+        return vocab_projection(self.to_logits, normed[torch.arange(bsz, device=idx.device), last])
+
+    @torch.no_grad()
+    def generate(self, idx, max_new_tokens: int, lengths=None, samples: int = 1, temperature: float = 0.0, generator=None,
+                 cache: PagedCache | None = None):
+        """(batch * samples, max_new_tokens) ids that follow the prompts ``idx`` (batch, T), of ``lengths`` tokens each where
+        they are padded: the most likely ones (the reference's generation, train_rbf_transformer.py:446-530), or drawn at
+        ``temperature``. A prompt's ``samples`` answers are rows beside one another and share its pages. ``cache``: an empty one
+        of batch * samples sequences, left with what the model has read."""
+        bsz, seq = idx.shape
+        lengths = [seq] * bsz if lengths is None else [int(n) for n in lengths]
+        if max_new_tokens < 1 or samples < 1 or len(lengths) != bsz or any(not 0 < n <= seq for n in lengths):
+            raise ValueError(f"prompts {tuple(idx.shape)} of {lengths} tokens, {max_new_tokens} new ones, {samples} samples")
+        rows = bsz * samples
+        if cache is None:
+            cache = self.new_cache(rows, max(lengths) + max_new_tokens)
+        if cache.max_sequences != rows or any(cache.length(s) for s in range(rows)):
+            raise ValueError(f"the cache must be an empty one of {rows} sequences")
+
+        def choose(logits):
+            if temperature == 0.0:
+                return logits.argmax(-1)
+            return torch.multinomial(torch.softmax(logits.float() / temperature, -1), 1, generator=generator)[:, 0]
+
+        first = [b * samples for b in range(bsz)]
+        logits = self.forward_cached(idx, cache, lengths, first).repeat_interleave(samples, 0)
+        for s in first:
+            cache.fork(s, range(s + 1, s + samples))
+        out = [choose(logits)]
+        while len(out) < max_new_tokens:
+            out.append(choose(self.forward_cached(out[-1][:, None], cache)))
+        return torch.stack(out, 1)
+
+
+def token_log_probs(logits: torch.Tensor, tokens: torch.Tensor, ignore_index: int = -100) -> torch.Tensor:
+    """Log-probabilities (the shape of ``tokens``, fp32, no gradient) of given tokens under logits (..., vocab); 0 where the token
+    is ``ignore_index``. CUDA logits go through the library's single read (``ops.token_log_probs``)."""
+    logits = logits.detach()
+    flat, t = logits.reshape(-1, logits.shape[-1]), tokens.reshape(-1)
+    if logits.is_cuda:
+        return ops.token_log_probs(flat, t, ignore_index).view(tokens.shape)
+    counted = (t != ignore_index) & (t >= 0) & (t < flat.shape[-1])
+    lp = torch.log_softmax(flat.float(), -1).gather(1, torch.where(counted, t, 0)[:, None])[:, 0]
+    return torch.where(counted, lp, 0.0).view(tokens.shape)
+
+
+def policy_loss(logits, tokens, old_log_probs, advantages, ref_log_probs=None, weights=None, clip_low: float = 0.2,
+                clip_high: float = 0.2, kl_weight: float = 0.0, ignore_index: int = -100):
+    """Clipped policy loss with a KL term (``ops.policy_loss``) of logits (..., vocab) and tokens, old_log_probs, advantages,
+    ref_log_probs and weights of the leading shape: (loss, log_probs). CUDA logits only."""
+    shape = tokens.shape
+    rows = [None if t is None else t.reshape(-1) for t in (tokens, old_log_probs, advantages, ref_log_probs, weights)]
+    loss, lp = ops.policy_loss(logits.reshape(-1, logits.shape[-1]), *rows, clip_low=clip_low, clip_high=clip_high,
+                               kl_weight=kl_weight, ignore_index=ignore_index)
+    return loss, lp.view(shape)
 
 
 def zipf_token_ids(batch, seq_len, vocab_size, exponent=1.1, seed=0):
