@@ -1123,6 +1123,14 @@ def _(logits, tokens, old_log_probs, advantages, ref_log_probs, weights, clip_lo
     return logits.new_empty((), dtype=torch.float32), logits.new_empty(rows, dtype=torch.float32), dlogits
 
 
+def _scale_rows(x: torch.Tensor, factor: torch.Tensor) -> None:
+    """x *= factor (a one-element tensor) unless factor == 1, decided on the device, for a matrix whose rows may have a pitch."""
+    _lib.host().scale_rows(x, factor)
+
+
+scale_rows_ = torch.library.custom_op("rbf_attn_b200::scale_rows_", mutates_args=("x",))(_scale_rows)
+
+
 def _policy_setup_context(ctx, inputs, output):
     ctx.save_for_backward(output[2])        # an output, so that under create_graph it is linked to the logits
     ctx.with_grad = inputs[10]
@@ -1142,34 +1150,14 @@ def _policy_backward(ctx, g_loss, _g_log_probs, _g_dlogits):
                            "has been handed out; call policy_loss again")
     ctx.taken = True
     (dlogits,) = ctx.saved_tensors
-    rows, cols = dlogits.shape
-    with torch.no_grad():                   # the memory behind it, the numbers between rows included
-        flat = dlogits.detach().as_strided(((rows - 1) * dlogits.stride(0) + cols if rows else 0,), (1,))
-        if _direct(flat, g_loss):
-            _scale_unless_one(flat, g_loss)
-            torch.autograd.graph.increment_version(dlogits)
-        else:
-            torch.ops.rbf_attn_b200.scale_unless_one_(flat, g_loss)
+    with torch.no_grad():
+        torch.ops.rbf_attn_b200.scale_rows_(dlogits, g_loss)
     if torch.is_grad_enabled():
         return (_FirstOrderOnly.apply("policy_loss", dlogits, g_loss), *nothing[1:])
     return (dlogits.detach(), *nothing[1:])
 
 
 torch.library.register_autograd("rbf_attn_b200::policy_loss_fwd", _policy_backward, setup_context=_policy_setup_context)
-
-
-class _PolicyLoss(torch.autograd.Function):
-    """``rbf_attn_b200::policy_loss_fwd`` and its autograd formula for calls that go around the operator."""
-
-    @staticmethod
-    def forward(ctx, *inputs):
-        output = _policy_loss_fwd(*inputs)
-        _policy_setup_context(ctx, inputs, output)
-        return output
-
-    @staticmethod
-    def backward(ctx, g_loss, g_log_probs, g_dlogits):
-        return _policy_backward(ctx, g_loss, g_log_probs, g_dlogits)
 
 
 def policy_loss(logits, tokens, old_log_probs, advantages, ref_log_probs=None, weights=None, clip_low: float = 0.2,
@@ -1195,7 +1183,7 @@ def policy_loss(logits, tokens, old_log_probs, advantages, ref_log_probs=None, w
     inputs = (logits, tokens, old_log_probs, advantages, ref_log_probs, weights, float(clip_low), float(clip_high),
               float(kl_weight), ignore_index, with_grad)
     if type(ignore_index) is int and _direct(*inputs[:6]):
-        return (_PolicyLoss.apply if with_grad else _policy_loss_fwd)(*inputs)[:2]
+        return _lib.host().policy_loss_node(*inputs[:10]) if with_grad else _policy_loss_fwd(*inputs)[:2]
     return torch.ops.rbf_attn_b200.policy_loss_fwd(*inputs)[:2]
 
 
