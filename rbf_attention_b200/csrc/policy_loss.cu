@@ -20,7 +20,8 @@ namespace {
 constexpr int kThreads = 512;
 constexpr int kRowsPerSm = 2;                       // blocks of the loss kernel
 constexpr int kStageBytes = 113 * 1024;             // a staged row leaves room for a second block on the SM
-constexpr float kLn2 = 0.6931471805599453f;
+constexpr double kLn2 = 0.6931471805599453;
+constexpr int kCountHere = 8192;                  // rows up to which every block counts them by itself
 
 __device__ __forceinline__ float pl_ex2(float x) {
   float y;
@@ -149,6 +150,21 @@ __device__ __forceinline__ Online row_sum(const typename Number<kDtype>::type* x
   return sum;
 }
 
+// Log-probability of a row's token in 64 bits: numbers of the size of the logits and of log2(cols) nearly cancel in it, and the
+// loss compares it with others like it. The logits' factor is the one of the sum's terms, so that a shift of all logits cancels.
+__device__ __forceinline__ double log_prob(float x, const Online& sum, float& lse2) {
+  int e;
+  const float f = frexpf(sum.s, &e);                // log2f is off by units of its result's last place: of [0.5, 1) it is small
+  const double l = static_cast<double>(sum.m) + e + static_cast<double>(log2f(f));
+  lse2 = static_cast<float>(l);
+  return (static_cast<double>(x) * static_cast<double>(kLog2e) - l) * kLn2;
+}
+
+// Brings a row's 16-byte words into L2; nothing waits for it.
+__device__ __forceinline__ void prefetch_l2(const void* p, uint32_t bytes) {
+  asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(p), "r"(bytes) : "memory");
+}
+
 __device__ __forceinline__ bool counts(const PolicyArgs& a, int64_t token) {
   return token != a.ignore_index && token >= 0 && token < a.cols;
 }
@@ -165,7 +181,8 @@ __global__ void __launch_bounds__(kThreads) token_log_probs_kernel(const PolicyA
     }
     const T* x = static_cast<const T*>(a.logits) + row * a.ld;
     const Online sum = row_sum<kDtype, false>(x, a.cols, nullptr);
-    if (threadIdx.x == 0) a.log_probs[row] = (fmaf(N::widen(x[token]), kLog2e, -sum.m) - log2f(sum.s)) * kLn2;
+    float lse2;
+    if (threadIdx.x == 0) a.log_probs[row] = static_cast<float>(log_prob(N::widen(x[token]), sum, lse2));
     __syncthreads();                                // the warps' slots are used again
   }
 }
@@ -197,39 +214,53 @@ __global__ void __launch_bounds__(kThreads, kRowsPerSm) policy_loss_kernel(const
   const int tid = threadIdx.x;
   grid_dependency_wait();
   if (a.weights == nullptr) {
-    if (tid < 32) {
-      int n = 0;
-      for (int i = tid; i < a.count_blocks; i += 32) n += a.counts[i];
-      n = __reduce_add_sync(0xffffffffu, n);
-      if (tid == 0) s_count = n;
+    if (tid == 0) s_count = 0;
+    __syncthreads();
+    int n = 0;
+    if (a.count_blocks > 0) {
+      for (int i = tid; i < a.count_blocks; i += kThreads) n += a.counts[i];
+    } else {
+      for (int64_t r = tid; r < a.rows; r += kThreads) n += counts(a, a.tokens[r]);
     }
+    n = __reduce_add_sync(0xffffffffu, n);
+    if ((tid & 31) == 0 && n != 0) atomicAdd(&s_count, n);
     __syncthreads();
   }
   double loss = 0.0;                                // of this block's rows, thread 0
+  if (a.weights == nullptr && s_count == 0) loss = __longlong_as_double(0x7ff8000000000000ll);      // the mean of nothing
+  int64_t next_token = blockIdx.x < a.rows ? a.tokens[blockIdx.x] : 0;
   for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
     const T* x = static_cast<const T*>(a.logits) + row * a.ld;
     T* dx = static_cast<T*>(a.dlogits) + row * a.ld_out;
     const Cut<T> cut(x, a.cols);
-    const int64_t token = a.tokens[row];
-    const bool counted = counts(a, token);
+    const int64_t token = next_token;
+    const bool counted = counts(a, token), more = row + gridDim.x < a.rows;
+    if (more) next_token = a.tokens[row + gridDim.x];
     if (counted) {
       const Online sum = row_sum<kDtype, kStage>(x, a.cols, s_row);
+      // a staged row has been read: the block's next one comes into L2 while this one is reduced and its gradient written
+      if (kStage && tid == kThreads - 32 && more && counts(a, next_token)) {
+        const T* next = x + static_cast<int64_t>(gridDim.x) * a.ld;
+        const Cut<T> next_cut(next, a.cols);
+        if (next_cut.words > 0) prefetch_l2(next + next_cut.head, next_cut.words * 16);
+      }
       if (tid == 0) {
-        const float lse2 = log2f(sum.s), lp = (fmaf(N::widen(x[token]), kLog2e, -sum.m) - lse2) * kLn2;
-        const float A = a.advantages[row], r = expf(lp - a.old_log_probs[row]);
+        float lse2;
+        const double lp = log_prob(N::widen(x[token]), sum, lse2);
+        const float A = a.advantages[row], r = expf(static_cast<float>(lp - a.old_log_probs[row]));
         const float plain = r * A, clipped = fminf(fmaxf(r, 1.f - a.clip_low), 1.f + a.clip_high) * A;
         const float w = a.weights != nullptr ? a.weights[row] : 1.f / static_cast<float>(s_count);
         float value = -fminf(plain, clipped), slope = plain <= clipped ? -plain : 0.f;
         if (plain != plain) value = slope = plain;  // fminf would pass over it
         if (a.ref_log_probs != nullptr) {
-          const float gap = a.ref_log_probs[row] - lp, away = expf(gap);
+          const float gap = static_cast<float>(a.ref_log_probs[row] - lp), away = expf(gap);
           value = fmaf(a.kl_weight, away - gap - 1.f, value);
           slope = fmaf(a.kl_weight, 1.f - away, slope);
         }
-        a.log_probs[row] = lp;
+        a.log_probs[row] = static_cast<float>(lp);
         loss += static_cast<double>(w) * static_cast<double>(value);
         s_slope = w * slope;
-        s_shift = -(sum.m + lse2);
+        s_shift = -lse2;
       }
     } else if (tid == 0) {
       a.log_probs[row] = 0.f;
@@ -297,11 +328,6 @@ __global__ void __launch_bounds__(32) policy_finish_kernel(const PolicyArgs a, c
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
   if (threadIdx.x != 0) return;
-  if (a.weights == nullptr) {                       // no row that counts: the mean of nothing
-    int n = 0;
-    for (int i = 0; i < a.count_blocks; ++i) n += a.counts[i];
-    if (n == 0) sum = __longlong_as_double(0x7ff8000000000000ll);
-  }
   *a.loss = static_cast<float>(sum);
 }
 
@@ -318,8 +344,8 @@ cudaError_t policy_t(PolicyArgs a, int sms, cudaStream_t stream) {
   const int64_t most = policy_blocks(sms);
   const int blocks = a.rows == 0 ? 1 : static_cast<int>(a.rows < most ? a.rows : most);
   const int64_t wanted = (a.rows + kThreads - 1) / kThreads;
-  a.count_blocks = wanted == 0 ? 1 : static_cast<int>(wanted < sms ? wanted : sms);
-  if (a.weights == nullptr) {
+  a.count_blocks = a.rows <= kCountHere ? 0 : static_cast<int>(wanted < sms ? wanted : sms);
+  if (a.weights == nullptr && a.count_blocks > 0) {
     policy_count_kernel<<<a.count_blocks, kThreads, 0, stream>>>(a);
     const cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) return e;
