@@ -11,6 +11,9 @@ namespace rbf {
 namespace {
 
 constexpr int kWriteThreads = 128;                 // four warps, a block of 16 tokens of one head each
+// Blocks on an SM: a warp waits for one load, so as many as registers allow. 8 x 16 heads x 8190 tokens written, of 128 columns
+// (spilling 80 to 100 bytes) and of 64: 162 and 90 us so, 209 and 103 with four blocks, 254 and 100 with 10 and 16.
+template <int P> constexpr int kWriteBlocks = P == 64 ? 10 : 8;
 
 // Two 16-bit numbers as fp32
 template <bool kBf16>
@@ -24,25 +27,24 @@ __device__ __forceinline__ void widen8(const uint4& raw, float (&x)[8]) {
   }
 }
 
-// code + 128 of a value: nearest integer of x * (127 / amax), ties to even, both steps in fp32 (|code| <= 127: x / amax is at
-// most 1, and the two roundings cannot lift 127 by half). Non-finite products have code 0; their block's scale is not finite.
-__device__ __forceinline__ uint32_t code_of(float x, float inverse) {
-  return static_cast<uint32_t>(__float2int_rn(__fmul_rn(x, inverse)) + 128) & 0xffu;
+// code + 128 of four values: nearest integers of x * (127 / amax), ties to even, both steps in fp32 (|code| <= 127: x / amax is
+// at most 1, and the two roundings cannot lift 127 by half). Adding 1.5 * 2^23 leaves the integer in the low bits: a conversion
+// runs at an eighth of the rate.
+__device__ __forceinline__ uint32_t codes_of(float x0, float x1, float x2, float x3, float inverse) {
+  auto code = [&](float x) { return __float_as_uint(__fadd_rn(__fmul_rn(x, inverse), 12582912.f + 128.f)); };
+  return __byte_perm(__byte_perm(code(x0), code(x1), 0x0040), __byte_perm(code(x2), code(x3), 0x0040), 0x5410);
 }
 
 // One warp per block of 16 tokens that the new tokens touch, of one head's keys or values. The warp of the first block also
 // stores what is left behind the last complete one: both use the rows of the incomplete block, which are read first.
 template <bool kBf16, int P>
-__global__ void __launch_bounds__(kWriteThreads) cache_append_kernel(const CacheAppendArgs a) {
+__global__ void __launch_bounds__(kWriteThreads, kWriteBlocks<P>) cache_append_kernel(const CacheAppendArgs a) {
   const int lane = threadIdx.x & 31;
-  const int64_t unit = static_cast<int64_t>(blockIdx.x) * (kWriteThreads / 32) + (threadIdx.x >> 5);
-  const int j = static_cast<int>(unit % a.blocks);
-  const int64_t head = unit / a.blocks;
-  const int kv = static_cast<int>(head & 1);
-  const int h = static_cast<int>((head >> 1) % a.H);
-  const int64_t b64 = (head >> 1) / a.H;
-  if (b64 >= a.B) return;
-  const int b = static_cast<int>(b64);
+  const unsigned unit = blockIdx.x * (kWriteThreads / 32) + (threadIdx.x >> 5);          // below 2^31: 32-bit divisions
+  const unsigned head = unit / a.blocks, heads = (head >> 1) / a.H;
+  const int j = static_cast<int>(unit - head * a.blocks), kv = static_cast<int>(head & 1);
+  const int h = static_cast<int>((head >> 1) - heads * a.H), b = static_cast<int>(heads);
+  if (b >= a.B) return;
   const CacheSpan span = cache_span(a.lengths, a.fresh, b, a.T, a.max_pages);
   if (span.fresh == 0) return;
   const int end = span.held + span.fresh;
@@ -87,34 +89,29 @@ __global__ void __launch_bounds__(kWriteThreads) cache_append_kernel(const Cache
       const float scale = !finite ? __uint_as_float(0x7fc00000u) : held ? __fdiv_rn(amax, 127.f) : 0.f;
       const float inverse = finite && held ? __fdiv_rn(127.f, amax) : 0.f;
       uint8_t* slot = page + kPageHeader + (block % kPageBlocks) * kSlot + kv * 16 * P;
-      uint2 code[kPer];
 #pragma unroll
-      for (int i = 0; i < kPer; ++i) {
-        float x[8];
-        widen8<kBf16>(raw[i], x);
-        uint32_t w[2];
+      for (int i = 0; i < kPer; i += 4) {           // four tokens at a time
+        uint2 code[4];
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          w[e] = 0;
-#pragma unroll
-          for (int f = 0; f < 4; ++f) w[e] |= code_of(x[4 * e + f], inverse) << (8 * f);
+        for (int k = 0; k < 4; ++k) {
+          float x[8];
+          widen8<kBf16>(raw[i + k], x);
+          // a block with a number that is not finite has codes of zero, and its scale makes them NaN
+          code[k] = finite ? make_uint2(codes_of(x[0], x[1], x[2], x[3], inverse), codes_of(x[4], x[5], x[6], x[7], inverse))
+                           : make_uint2(0x80808080u, 0x80808080u);
         }
-        code[i] = make_uint2(w[0], w[1]);
-      }
-      if (kv == 0) {
+        if (kv == 0) {
 #pragma unroll
-        for (int i = 0; i < kPer; ++i) {
-          const int tok = token(i), half = (tok >> 1) & 1, g = (tok >> 2) * 2 + (tok & 1);
-          *reinterpret_cast<uint2*>(slot + ((c / 8) * 2 + half) * 512 + g * 64 + (c % 8) * 8) = code[i];
-        }
-      } else {
-#pragma unroll
-        for (int i = 0; i < kPer; i += 4) {
+          for (int k = 0; k < 4; ++k) {
+            const int tok = token(i + k), half = (tok >> 1) & 1, g = (tok >> 2) * 2 + (tok & 1);
+            *reinterpret_cast<uint2*>(slot + ((c / 8) * 2 + half) * 512 + g * 64 + (c % 8) * 8) = code[k];
+          }
+        } else {
           const int t = token(i) / 4;
 #pragma unroll
           for (int e = 0; e < 2; ++e) {             // four tokens x four dims, transposed
-            const uint32_t r0 = e ? code[i].y : code[i].x, r1 = e ? code[i + 1].y : code[i + 1].x;
-            const uint32_t r2 = e ? code[i + 2].y : code[i + 2].x, r3 = e ? code[i + 3].y : code[i + 3].x;
+            const uint32_t r0 = e ? code[0].y : code[0].x, r1 = e ? code[1].y : code[1].x;
+            const uint32_t r2 = e ? code[2].y : code[2].x, r3 = e ? code[3].y : code[3].x;
             const uint32_t lo01 = __byte_perm(r0, r1, 0x5140), hi01 = __byte_perm(r0, r1, 0x7362);
             const uint32_t lo23 = __byte_perm(r2, r3, 0x5140), hi23 = __byte_perm(r2, r3, 0x7362);
             const uint4 out = make_uint4(__byte_perm(lo01, lo23, 0x5410), __byte_perm(lo01, lo23, 0x7632),
@@ -140,24 +137,21 @@ __global__ void __launch_bounds__(kWriteThreads) cache_append_kernel(const Cache
   }
 }
 
-// Four tokens (a quad of a block) x four columns of one head's keys and values per thread
+// Four tokens (a quad of a block) x eight columns of one head's keys and values per thread
 template <bool kBf16, int P>
 __global__ void __launch_bounds__(256) cache_read_kernel(const CacheReadArgs a) {
   constexpr int kBytes = cache_page_bytes(P), kSlot = cache_slot_bytes(P);
-  const int64_t at = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-  const int groups = a.D / 4;
-  const int d = static_cast<int>(at % groups) * 4;
-  const int quad = static_cast<int>(at / groups % a.quads);
-  const int64_t head = at / groups / a.quads;
-  if (head >= static_cast<int64_t>(a.B) * a.H) return;
-  const int b = static_cast<int>(head / a.H), h = static_cast<int>(head % a.H);
+  const unsigned head = blockIdx.x / a.chunks;      // 32-bit divisions, these the same for the block
+  const unsigned at = (blockIdx.x - head * a.chunks) * 256 + threadIdx.x, groups = a.D / 8, quad = at / groups;
+  const int b = static_cast<int>(head / a.H), h = static_cast<int>(head - b * a.H), d = static_cast<int>(at - quad * groups) * 8;
+  if (quad >= static_cast<unsigned>(a.quads)) return;
   const int n = cache_span(a.lengths, nullptr, b, 0, a.max_pages).held;
-  int first = a.first != nullptr ? a.first[b] : 0;
+  const int first = a.first != nullptr ? a.first[b] : 0;
   const int64_t begin = first < 0 ? 0 : first;      // (a negative start reads from the first token on)
   const int64_t pos64 = (begin / 4 + quad) * 4;
-  uint2 k[4], v[4];                                 // four columns of four tokens
+  uint4 k[4], v[4];                                 // eight columns of four tokens
 #pragma unroll
-  for (int r = 0; r < 4; ++r) k[r] = v[r] = make_uint2(0, 0);
+  for (int r = 0; r < 4; ++r) k[r] = v[r] = make_uint4(0, 0, 0, 0);
   const int pos = static_cast<int>(pos64 < n ? pos64 : 0);
   const uint8_t* page = pos64 < n ? cache_page(a.pages, a.table, b, a.max_pages, a.num_pages, a.H, h, kBytes, pos) : nullptr;
   if (page != nullptr) {
@@ -165,28 +159,38 @@ __global__ void __launch_bounds__(256) cache_read_kernel(const CacheReadArgs a) 
     if (block < n / kBlockTokens) {
       const uint8_t* slot = page + kPageHeader + (block % kPageBlocks) * kSlot;
       const float2 scale = reinterpret_cast<const float2*>(page)[block % kPageBlocks];
-      const uint4 w4 = *reinterpret_cast<const uint4*>(slot + 16 * P + d / 32 * 512 + (d % 32 / 4 * 4 + in_block / 4) * 16);
-      const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
+      uint4 w[2];                                   // word i: dim i of four tokens
+      uint2 kw[4];                                  // of each token eight dims
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+        w[e] = *reinterpret_cast<const uint4*>(slot + 16 * P + d / 32 * 512 + ((d % 32 / 4 + e) * 4 + in_block / 4) * 16);
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         const int tok = in_block + r, half = (tok >> 1) & 1, g = (tok >> 2) * 2 + (tok & 1);
-        const uint32_t kw = *reinterpret_cast<const uint32_t*>(slot + ((d / 64) * 2 + half) * 512 + g * 64 + d % 64);
-        float kx[4], vx[4];
+        kw[r] = *reinterpret_cast<const uint2*>(slot + ((d / 64) * 2 + half) * 512 + g * 64 + d % 64);
+      }
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          kx[i] = static_cast<float>(static_cast<int>(kw >> (8 * i) & 0xffu) - 128) * scale.x;
-          vx[i] = static_cast<float>(static_cast<int>(w[i] >> (8 * r) & 0xffu) - 128) * scale.y;
+      for (int r = 0; r < 4; ++r) {
+        float kx[8], vx[8];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const uint32_t words[4] = {w[e].x, w[e].y, w[e].z, w[e].w}, key = e ? kw[r].y : kw[r].x;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            kx[4 * e + i] = static_cast<float>(static_cast<int>(key >> (8 * i) & 0xffu) - 128) * scale.x;
+            vx[4 * e + i] = static_cast<float>(static_cast<int>(words[i] >> (8 * r) & 0xffu) - 128) * scale.y;
+          }
         }
-        k[r] = make_uint2(pack2<kBf16>(kx[0], kx[1]), pack2<kBf16>(kx[2], kx[3]));
-        v[r] = make_uint2(pack2<kBf16>(vx[0], vx[1]), pack2<kBf16>(vx[2], vx[3]));
+        k[r] = make_uint4(pack2<kBf16>(kx[0], kx[1]), pack2<kBf16>(kx[2], kx[3]), pack2<kBf16>(kx[4], kx[5]), pack2<kBf16>(kx[6], kx[7]));
+        v[r] = make_uint4(pack2<kBf16>(vx[0], vx[1]), pack2<kBf16>(vx[2], vx[3]), pack2<kBf16>(vx[4], vx[5]), pack2<kBf16>(vx[6], vx[7]));
       }
     } else {
       const uint8_t* tail = page + kPageHeader + kPageBlocks * kSlot;
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         if (pos + r >= n) break;
-        k[r] = *reinterpret_cast<const uint2*>(tail + ((in_block + r) * P + d) * 2);
-        v[r] = *reinterpret_cast<const uint2*>(tail + kSlot + ((in_block + r) * P + d) * 2);
+        k[r] = *reinterpret_cast<const uint4*>(tail + ((in_block + r) * P + d) * 2);
+        v[r] = *reinterpret_cast<const uint4*>(tail + kSlot + ((in_block + r) * P + d) * 2);
       }
     }
   }
@@ -194,9 +198,9 @@ __global__ void __launch_bounds__(256) cache_read_kernel(const CacheReadArgs a) 
   for (int r = 0; r < 4; ++r) {
     const int64_t i = pos64 + r - begin;
     if (i < 0 || i >= a.count) continue;
-    const int64_t to = (head * a.count + i) * a.D + d;
-    *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.k) + to) = k[r];
-    *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.v) + to) = v[r];
+    const int64_t to = (static_cast<int64_t>(head) * a.count + i) * a.D + d;
+    *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.k) + to) = k[r];
+    *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.v) + to) = v[r];
   }
 }
 
@@ -220,13 +224,16 @@ __global__ void __launch_bounds__(kCopyThreads) cache_copy_kernel(const __grid_c
 template <bool kBf16, int P>
 cudaError_t append_t(const CacheAppendArgs& a, cudaStream_t stream) {
   const int64_t units = static_cast<int64_t>(a.B) * a.H * 2 * a.blocks, per = kWriteThreads / 32;
+  if (units > 0x7fffffffll) return cudaErrorInvalidConfiguration;
   cache_append_kernel<kBf16, P><<<static_cast<unsigned>((units + per - 1) / per), kWriteThreads, 0, stream>>>(a);
   return cudaGetLastError();
 }
 template <bool kBf16, int P>
-cudaError_t read_t(const CacheReadArgs& a, cudaStream_t stream) {
-  const int64_t threads = static_cast<int64_t>(a.B) * a.H * a.quads * (a.D / 4);
-  cache_read_kernel<kBf16, P><<<static_cast<unsigned>((threads + 255) / 256), 256, 0, stream>>>(a);
+cudaError_t read_t(CacheReadArgs a, cudaStream_t stream) {
+  const int64_t chunks = (static_cast<int64_t>(a.quads) * (a.D / 8) + 255) / 256, blocks = chunks * a.B * a.H;
+  if (blocks > 0x7fffffffll) return cudaErrorInvalidConfiguration;
+  a.chunks = static_cast<unsigned>(chunks);
+  cache_read_kernel<kBf16, P><<<static_cast<unsigned>(blocks), 256, 0, stream>>>(a);
   return cudaGetLastError();
 }
 

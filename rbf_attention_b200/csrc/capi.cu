@@ -863,7 +863,7 @@ int rbf_b200_cache_append(void* pages, const int* page_table, const int* lengths
   set_strides(a.ks, k_strides); set_strides(a.vs, v_strides);
   a.B = B; a.H = H; a.T = T; a.D = D; a.max_pages = max_pages; a.num_pages = num_pages;
   a.blocks = static_cast<int>((static_cast<int64_t>(T) + rbf::kBlockTokens - 2) / rbf::kBlockTokens + 1);
-  if (static_cast<int64_t>(B) * H > 0x7fffffffll / 2 || static_cast<int64_t>(B) * H * 2 * a.blocks / 4 >= 0x7fffffffll)
+  if (static_cast<double>(B) * H * 2 * a.blocks >= 2147483647.0)
     return fail(RBF_B200_ERR_BAD_ARGUMENT, "B * H * T is too large for one call");
   const cudaError_t e = rbf::launch_cache_append(a, dtype == 0, static_cast<cudaStream_t>(stream_v));
   if (e != cudaSuccess) return fail(RBF_B200_ERR_LAUNCH, "cache append launch failed: %s", cudaGetErrorString(e));
@@ -884,7 +884,7 @@ int rbf_b200_cache_read(const void* pages, const int* page_table, const int* len
   a.pages = static_cast<const uint8_t*>(pages); a.table = page_table; a.lengths = lengths; a.first = first; a.k = k; a.v = v;
   a.B = B; a.H = H; a.D = D; a.count = count; a.max_pages = max_pages; a.num_pages = num_pages;
   a.quads = static_cast<int>((static_cast<int64_t>(count) + 6) / 4);
-  if (static_cast<double>(B) * H * a.quads * (D / 4) / 256 >= 2147483646.0)
+  if (static_cast<double>(B) * H * (static_cast<double>(a.quads) * (D / 8) / 256 + 1) >= 2147483646.0)
     return fail(RBF_B200_ERR_BAD_ARGUMENT, "B * H * count is too large for one call");
   const cudaError_t e = rbf::launch_cache_read(a, dtype == 0, static_cast<cudaStream_t>(stream_v));
   if (e != cudaSuccess) return fail(RBF_B200_ERR_LAUNCH, "cache read launch failed: %s", cudaGetErrorString(e));
