@@ -34,7 +34,7 @@ template <int P, int NT>
 struct Shape {
   static constexpr int kUnitBlocks = NT == 1 ? 256 / P : 2;
   static constexpr int kWarps = NT == 1 ? 12 : 8;
-  static constexpr int kStages = NT == 1 ? 2 : 3;
+  static constexpr int kStages = NT == 1 || P == 128 ? 2 : 3;
 };
 constexpr int kShortWarps = 8;                     // of the kernel for short sequences, 4 where there are many
 constexpr float kSlack = 8.f;                      // growth of a score, in powers of two, that does not move the maximum
