@@ -20,6 +20,8 @@
 #include <cstdint>
 #include <cuda_runtime.h>
 
+#include <type_traits>
+
 #include "cache.cuh"
 #include "launch.h"
 
@@ -70,11 +72,11 @@ __device__ __forceinline__ float attn_ex2(float x) {
 template <bool kBf16>
 __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   if constexpr (kBf16) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
   } else {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
   }
@@ -82,7 +84,7 @@ __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], 
 // 8 x 8 16-bit matrix, row lane / 4 and columns 2 (lane % 4), + 1 in each lane, transposed
 __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
   uint32_t y;
-  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
   return y;
 }
 
@@ -129,14 +131,49 @@ struct Units {
   }
 };
 
-// Sum over the sequences of the units of a segment, by a whole warp
+// Groups of blocks, the incomplete one among them
 template <int UB>
+struct AllUnits {
+  int held, fresh, count;
+  __device__ AllUnits(const CacheAttnArgs& a, int b) {
+    const CacheSpan s = cache_span(a.lengths, a.fresh, b, a.T, a.max_pages);
+    held = s.held;
+    fresh = s.fresh;
+    count = fresh == 0 ? 0 : (held + fresh + UB * kBlockTokens - 1) / (UB * kBlockTokens);
+  }
+};
+
+// Sum over the sequences of the units of a segment, by a whole warp
+template <class U>
 __device__ __forceinline__ int64_t sum_units(const CacheAttnArgs& a) {
   int64_t all = 0;
-  for (int b = threadIdx.x & 31; b < a.B; b += 32) all += Units<UB>(a, b).count;
+  for (int b = threadIdx.x & 31; b < a.B; b += 32) all += U(a, b).count;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
   return all;
+}
+// The sequence that unit `at` belongs to and its first unit, by a whole warp
+template <class U>
+__device__ __forceinline__ int find_sequence(const CacheAttnArgs& a, int segments, int64_t at, int64_t& begin) {
+  const int lane = threadIdx.x & 31;
+  begin = 0;
+  for (int b = 0; b < a.B; b += 32) {
+    const int64_t mine = b + lane < a.B ? static_cast<int64_t>(U(a, b + lane).count) * segments : 0;
+    int64_t upto = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t x = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += x;
+    }
+    const unsigned past = __ballot_sync(0xffffffffu, begin + upto > at);
+    if (past != 0) {
+      const int l = __ffs(past) - 1;
+      begin += __shfl_sync(0xffffffffu, upto - mine, l);
+      return b + l;
+    }
+    begin += __shfl_sync(0xffffffffu, upto, 31);
+  }
+  return a.B;
 }
 
 // Element offset of output column c of a segment (new token c / G of query head h * G + c % G)
@@ -625,7 +662,7 @@ __global__ void __launch_bounds__(Shape<P, NT>::kWarps * 32) cache_attn_kernel(c
   const int64_t workers = static_cast<int64_t>(gridDim.x) * kWarps;
   const int64_t self = static_cast<int64_t>(threadIdx.x >> 5) * gridDim.x + blockIdx.x;    // neighbours on other SMs
   const int segments = a.column_tiles * a.H;       // of a sequence
-  const Deal deal(sum_units<UB>(a) * segments, workers);
+  const Deal deal(sum_units<Units<UB>>(a) * segments, workers);
   int64_t at = deal.begin(self);
   const int64_t stop = deal.begin(self + 1);
   Note* const notes = reinterpret_cast<Note*>(a.parts);
@@ -641,26 +678,8 @@ __global__ void __launch_bounds__(Shape<P, NT>::kWarps * 32) cache_attn_kernel(c
   }
   if (at >= stop) return;
 
-  // the sequence of the first unit
-  int b = 0;
-  int64_t seq_begin = 0;
-  for (; b < a.B; b += 32) {
-    const int64_t mine = b + lane < a.B ? static_cast<int64_t>(Units<UB>(a, b + lane).count) * segments : 0;
-    int64_t upto = mine;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int64_t x = __shfl_up_sync(0xffffffffu, upto, o);
-      if (lane >= o) upto += x;
-    }
-    const unsigned past = __ballot_sync(0xffffffffu, seq_begin + upto > at);
-    if (past != 0) {
-      const int l = __ffs(past) - 1;
-      seq_begin += __shfl_sync(0xffffffffu, upto - mine, l);
-      b += l;
-      break;
-    }
-    seq_begin += __shfl_sync(0xffffffffu, upto, 31);
-  }
+  int64_t seq_begin;
+  int b = find_sequence<Units<UB>>(a, segments, at, seq_begin);
 
   // ---- loads: lane i looks up the i-th of the next 32 units, so that page numbers are waited for once in 32 units
   struct Lookup {
@@ -935,6 +954,573 @@ __global__ void __launch_bounds__(kWarps * 32, 16 / kWarps) cache_attn_short_ker
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");   // blocks stay until they have been read
 }
 
+// ---------------------------------------------------------------------------------------------------------------------
+// Many columns: the queries are the 16-row operand
+// ---------------------------------------------------------------------------------------------------------------------
+// With more than 8 columns of queries (chunks of a prompt, many query heads to a key head) a byte's widening is shared by a
+// block: its four warps widen a unit of four blocks of tokens, one each, into operand order in shared memory (the cache's order
+// with two bytes for one: lane (g, t)'s 16 codes are the second operand of four products, of the keys' dims and of the values'
+// tokens alike), and every warp multiplies 16 query rows with it: S (16 rows x 8 tokens) = Q K^T, O += P V, where the
+// accumulators of S are in place as the operand P. RW warps have different rows; where fewer than four are needed the others
+// have other blocks of the unit, and the warps with the same rows join at the end of the segment.
+// The block that is not complete is brought to fp16 by powers of two, its largest key and value to [1, 2): exact but for
+// elements below 2^-14 of it (off by 2^-25 of it), and is then a block like the others.
+constexpr int kRowWarps = 4;
+template <int P>
+struct RowTile {
+  static constexpr int kRaw = kRowWarps * cache_slot_bytes(P);             // codes as they come, two units
+  static constexpr int kStage = kRaw + 64;                                 // and their scales
+  static constexpr int kWide = 2 * kRaw;                                   // a unit's operands: keys, then values
+  static constexpr int kSmem = 2 * kStage + kWide;
+  static constexpr int kBlocks = P == 64 ? 3 : 2;                          // on an SM
+};
+
+// A warp's state for its 16 rows: rows g and g + 8 of a lane
+template <int P>
+struct RowState {
+  float o[P / 32][4][4];                           // [c][i]: dims 32 c + 8 t + i and + 4 + i of row g, then of row g + 8
+  float m[2], l[2];
+  int unit;                                        // o is in units of 2^unit
+  __device__ __forceinline__ void clear() {
+    unit = 0;
+#pragma unroll
+    for (int c = 0; c < P / 32; ++c)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[c][i][e] = 0.f;
+    m[0] = m[1] = -INFINITY;
+    l[0] = l[1] = 0.f;
+  }
+  __device__ __forceinline__ void times(float f0, float f1) {
+#pragma unroll
+    for (int c = 0; c < P / 32; ++c)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        o[c][i][0] *= f0;
+        o[c][i][1] *= f0;
+        o[c][i][2] *= f1;
+        o[c][i][3] *= f1;
+      }
+  }
+  // See Running::refer
+  __device__ __forceinline__ void refer(float scale) {
+    const float now = scale * power2(-unit);
+    if (now < 128.f && (now >= 0.015625f || scale == 0.f)) return;
+    int to = static_cast<int>(__float_as_uint(scale) >> 23) - 127 - 6;
+    float top = 0.f;
+#pragma unroll
+    for (int c = 0; c < P / 32; ++c)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) top = fmaxf(top, fabsf(o[c][i][e]));
+    const uint32_t bits = __reduce_max_sync(0xffffffffu, __float_as_uint(top));
+    if (bits != 0) {
+      to = max(to, unit - min(120, max(0, 100 - (static_cast<int>(bits >> 23) - 127))));
+      const float f = power2(max(unit - to, -126));
+      times(f, f);
+    }
+    unit = to;
+  }
+};
+
+// 16 codes of a lane as the second operands of four products
+__device__ __forceinline__ void widen_codes(uint4 w, uint32_t exponents, uint4* to) {
+  to[0] = make_uint4(codes_lo(w.x, exponents), codes_hi(w.x, exponents), codes_lo(w.y, exponents), codes_hi(w.y, exponents));
+  to[32] = make_uint4(codes_lo(w.z, exponents), codes_hi(w.z, exponents), codes_lo(w.w, exponents), codes_hi(w.w, exponents));
+}
+
+template <bool kBf16>
+__device__ __forceinline__ uint32_t rescale2(uint32_t w, float f) {
+  const float2 x = unpack2<kBf16>(w);
+  return pack2<false>(x.x * f, x.y * f);
+}
+// The power of two that brings a number of these bits (of a float's magnitude) to [1, 2), and its inverse
+__device__ __forceinline__ float to_one(uint32_t bits, float& back) {
+  uint32_t exponent = bits >> 23;
+  exponent = exponent == 0 ? 127u : min(exponent, 253u);
+  back = __uint_as_float(exponent << 23);
+  return __uint_as_float((254u - exponent) << 23);
+}
+
+template <bool kBf16, int P, int RW>
+__global__ void __launch_bounds__(kRowWarps * 32, RowTile<P>::kBlocks) cache_attn_rows_kernel(const CacheAttnArgs a) {
+  using T = RowTile<P>;
+  constexpr int KC = P / 32, UB = kRowWarps, kSlot = cache_slot_bytes(P), kBytes = cache_page_bytes(P);
+  constexpr int kRows = 16 * RW, kUnitTokens = UB * kBlockTokens;
+  constexpr int NT = kRows / 8;                    // for the parts: columns in tiles of 8
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ float s_bias[UB][kBlockTokens], s_key[UB], s_value[UB];
+  __shared__ int s_there;                          // blocks of the unit that are there
+  __shared__ bool s_odd[UB];                       // the incomplete block has a value that is not finite
+  uint8_t* const wide = smem + 2 * T::kStage;
+  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, warp = threadIdx.x >> 5;
+  const int row0 = warp % RW * 16, group = warp / RW;                      // its rows, its RW blocks of a unit
+  const int workers = gridDim.x, self = blockIdx.x, segments = a.column_tiles * a.H;
+  const Deal deal(sum_units<AllUnits<UB>>(a) * segments, workers);
+  int64_t at = deal.begin(self);
+  const int64_t stop = deal.begin(self + 1);
+  Note* const notes = reinterpret_cast<Note*>(a.parts);
+  const bool by_segment = a.notes < workers;
+  if (threadIdx.x == 0 && !by_segment) notes[self].b = -1;
+  for (int empty = self; empty < a.B; empty += workers) {                  // sequences without new tokens
+    if (AllUnits<UB>(a, empty).count != 0) continue;
+    const int64_t words = static_cast<int64_t>(a.H) * a.G * a.T * a.D / 8;
+    uint4* out = reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out)) + empty * words;
+    for (int64_t i = threadIdx.x; i < words; i += kRowWarps * 32) out[i] = make_uint4(0, 0, 0, 0);
+    if (by_segment)
+      for (int i = threadIdx.x; i < segments; i += kRowWarps * 32) notes[static_cast<int64_t>(empty) * segments + i].b = -1;
+  }
+  if (at >= stop) return;
+
+  int64_t seq_begin;
+  int b = find_sequence<AllUnits<UB>>(a, segments, at, seq_begin);
+
+  // ---- loads: two units ahead of their use, their page numbers one more, so that nothing waits for these
+  int64_t look_left = stop - at;                   // units of the block whose page has not been looked up
+  int look_b = b, look_seg = static_cast<int>((at - seq_begin) / AllUnits<UB>(a, b).count);
+  int look_u = static_cast<int>((at - seq_begin) % AllUnits<UB>(a, b).count), look_count = 0, look_blocks = 0;
+  auto look_at = [&](int sequence) {
+    const AllUnits<UB> units(a, sequence);
+    look_count = units.count;
+    look_blocks = (units.held + units.fresh) / kBlockTokens;
+  };
+  look_at(b);
+  int next_id = -1, next_h = 0, next_what = 0;     // page number, head, first block in the page | complete blocks << 8
+  auto look_up = [&]() {
+    next_id = -1;
+    if (look_left == 0) return;
+    --look_left;
+    const int column = look_u * kUnitTokens / kPageTokens;
+    if (column < a.max_pages) next_id = a.table[static_cast<int64_t>(look_b) * a.max_pages + column];
+    next_h = look_seg % a.H;
+    next_what = look_u * UB % kPageBlocks | max(0, min(UB, look_blocks - look_u * UB)) << 8;
+    if (++look_u < look_count) return;
+    look_u = 0;
+    if (++look_seg < segments) return;
+    look_seg = 0;
+    do {
+      if (++look_b == a.B) break;
+      look_at(look_b);
+    } while (look_count == 0);
+    if (look_b == a.B) look_left = 0;
+  };
+  const uint8_t *page = nullptr, *next_page = nullptr;                     // of the unit at hand and of the next
+  auto fetch = [&](int slot) {
+    page = next_page;
+    next_page = next_id < 0 || next_id >= a.num_pages ? nullptr : a.pages + (static_cast<int64_t>(next_id) * a.H + next_h) * kBytes;
+    if (next_page != nullptr) {
+      const uint8_t* src = next_page + kPageHeader + (next_what & 0xff) * kSlot + threadIdx.x * 16;
+      const uint32_t to = smem_u32(smem + slot * T::kStage);
+      const int bytes = (next_what >> 8) * kSlot;
+#pragma unroll
+      for (int i = 0; i < T::kRaw / (kRowWarps * 512); ++i)
+        if (i * (kRowWarps * 512) + static_cast<int>(threadIdx.x) * 16 < bytes)
+          copy16(to + i * (kRowWarps * 512) + threadIdx.x * 16, src + i * (kRowWarps * 512));
+      if (threadIdx.x < 2 && bytes > 0) copy16(to + T::kRaw + threadIdx.x * 16, next_page + (next_what & 0xff) * 8 + threadIdx.x * 16);
+    }
+    copies_close();
+    look_up();
+  };
+  look_up();
+  fetch(0);
+  fetch(1);
+
+  int slot = 0;
+  while (at < stop && b < a.B) {
+    const AllUnits<UB> units(a, b);
+    if (at >= seq_begin + static_cast<int64_t>(units.count) * segments) {
+      seq_begin += static_cast<int64_t>(units.count) * segments;
+      ++b;
+      continue;
+    }
+    const int total = units.held + units.fresh;
+    const int seg = static_cast<int>((at - seq_begin) / units.count);
+    const int u0 = static_cast<int>((at - seq_begin) % units.count);
+    const int64_t left = stop - at;
+    const int u1 = left < units.count - u0 ? u0 + static_cast<int>(left) : units.count;
+    const int h = seg % a.H, c0 = seg / a.H * kRows;
+    const int columns = min(kRows, a.T * a.G - c0);
+
+    // ---- queries, as in Queries::load; rows g and g + 8
+    uint32_t q[P / 16][4];
+    float mul[2], q_sq[2];
+    int limit[2];
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int c = c0 + row0 + g + 8 * e;
+      uint32_t raw[P / 16][2];
+      load_q<P>(a, b, h, c, t, raw);
+      uint32_t top = 0;
+      float square = 0.f;
+#pragma unroll
+      for (int i = 0; i < P / 16; ++i)
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const float2 f = unpack2<kBf16>(raw[i][k]);
+          top = max(top, max(__float_as_uint(f.x) & 0x7fffffffu, __float_as_uint(f.y) & 0x7fffffffu));
+          square = fmaf(f.x, f.x, fmaf(f.y, f.y, square));
+        }
+#pragma unroll
+      for (int o = 1; o < 4; o <<= 1) {
+        top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+        square += __shfl_xor_sync(0xffffffffu, square, o);
+      }
+      float up;
+      const float down = to_one(top, up);
+#pragma unroll
+      for (int i = 0; i < P / 16; ++i)
+#pragma unroll
+        for (int k = 0; k < 2; ++k) q[i][2 * k + e] = rescale2<kBf16>(raw[i][k], down);
+      mul[e] = 2.f * a.scale * up;
+      q_sq[e] = a.scale * square;
+      limit[e] = c < a.T * a.G ? units.held + c / a.G : total - 1;
+    }
+    const int first_limit = units.held + (c0 + row0) / a.G, last_limit = units.held + (c0 + columns - 1) / a.G;
+    const bool active = row0 < columns;            // some of the warp's rows are real
+
+    RowState<P> run;
+    run.clear();
+    for (int u = u0; u < u1; ++u) {
+      const int begin = u * kUnitTokens;
+      const bool seen = begin <= last_limit;       // by some column of the tile
+      copies_wait<1>();
+      __syncthreads();                             // the unit is there, and the last one's operands have been read
+      const uint8_t* raw = smem + slot * T::kStage;
+      if (threadIdx.x == 0)
+        s_there = page == nullptr || !seen ? 0 : min(UB, (total - begin + kBlockTokens - 1) / kBlockTokens);
+      if (page != nullptr && seen) {
+        const int base = begin + warp * kBlockTokens;
+        uint4* keys = reinterpret_cast<uint4*>(wide) + warp * (2 * P / 64) * 64 + lane;
+        uint4* values = reinterpret_cast<uint4*>(wide + T::kRaw) + warp * KC * 64 + lane;
+        if (base + kBlockTokens <= total) {
+          const uint4* from = reinterpret_cast<const uint4*>(raw + warp * kSlot) + lane;
+          const float2 scale = reinterpret_cast<const float2*>(raw + T::kRaw)[warp];
+          int sq[2] = {0, 0};
+#pragma unroll
+          for (int d = 0; d < P / 64; ++d)
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+              const uint4 w = from[(2 * d + half) * 32];
+              sq[half] += dot4(w.x) + dot4(w.y) + dot4(w.z) + dot4(w.w);
+              widen_codes(w, a.exponents, keys + (half * (P / 64) + d) * 64);
+            }
+#pragma unroll
+          for (int i = 0; i < KC; ++i) widen_codes(from[(KC + i) * 32], a.exponents, values + i * 64);
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            sq[half] += __shfl_xor_sync(0xffffffffu, sq[half], 1);
+            sq[half] += __shfl_xor_sync(0xffffffffu, sq[half], 2);
+            if (t == 0) s_bias[warp][4 * (g >> 1) + 2 * half + (g & 1)] = a.scale * scale.x * scale.x * static_cast<float>(sq[half]);
+          }
+          if (lane == 0) {
+            s_key[warp] = scale.x;
+            s_value[warp] = scale.y;
+            s_odd[warp] = false;
+          }
+        } else if (base < total) {
+          const uint16_t* rest = reinterpret_cast<const uint16_t*>(page + kPageHeader + kPageBlocks * kSlot);
+          uint32_t k[2][P / 64][8], top = 0;
+          float sq[2] = {0.f, 0.f};
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            const int tok = 4 * (g >> 1) + 2 * half + (g & 1);
+#pragma unroll
+            for (int d = 0; d < P / 64; ++d) {
+              const uint4* row = reinterpret_cast<const uint4*>(rest + tok * P + d * 64 + t * 16);
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                const uint4 x = base + tok < total ? row[e] : make_uint4(0, 0, 0, 0);
+                k[half][d][4 * e] = x.x, k[half][d][4 * e + 1] = x.y, k[half][d][4 * e + 2] = x.z, k[half][d][4 * e + 3] = x.w;
+              }
+#pragma unroll
+              for (int i = 0; i < 8; ++i) {
+                const float2 f = unpack2<kBf16>(k[half][d][i]);
+                sq[half] = fmaf(f.x, f.x, fmaf(f.y, f.y, sq[half]));
+                top = max(top, max(__float_as_uint(f.x) & 0x7fffffffu, __float_as_uint(f.y) & 0x7fffffffu));
+              }
+            }
+            sq[half] += __shfl_xor_sync(0xffffffffu, sq[half], 1);
+            sq[half] += __shfl_xor_sync(0xffffffffu, sq[half], 2);
+            if (t == 0) s_bias[warp][tok] = a.scale * sq[half];
+          }
+          float up;
+          float down = to_one(__reduce_max_sync(0xffffffffu, top), up);
+#pragma unroll
+          for (int half = 0; half < 2; ++half)
+#pragma unroll
+            for (int d = 0; d < P / 64; ++d)
+#pragma unroll
+              for (int e = 0; e < 2; ++e)
+                keys[(half * (P / 64) + d) * 64 + e * 32] =
+                    make_uint4(rescale2<kBf16>(k[half][d][4 * e], down), rescale2<kBf16>(k[half][d][4 * e + 1], down),
+                               rescale2<kBf16>(k[half][d][4 * e + 2], down), rescale2<kBf16>(k[half][d][4 * e + 3], down));
+          if (lane == 0) s_key[warp] = up;
+          uint2 x[KC][4];                          // dims 32 i + 4 g ... + 3 of tokens 4 t + r
+          bool odd = false;
+          top = 0;                                 // of the finite ones
+#pragma unroll
+          for (int i = 0; i < KC; ++i)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              x[i][r] = make_uint2(0, 0);
+              if (base + 4 * t + r < total) x[i][r] = *reinterpret_cast<const uint2*>(rest + kSlot / 2 + (4 * t + r) * P + 32 * i + 4 * g);
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                const float2 f = unpack2<kBf16>(e ? x[i][r].y : x[i][r].x);
+                const uint32_t b0 = __float_as_uint(f.x) & 0x7fffffffu, b1 = __float_as_uint(f.y) & 0x7fffffffu;
+                odd |= b0 >= 0x7f800000u || b1 >= 0x7f800000u;
+                top = max(top, max(b0 < 0x7f800000u ? b0 : 0u, b1 < 0x7f800000u ? b1 : 0u));
+              }
+            }
+          down = to_one(__reduce_max_sync(0xffffffffu, top), up);
+          odd = __any_sync(0xffffffffu, odd);
+          if (lane == 0) {
+            s_value[warp] = up;
+            s_odd[warp] = odd;
+          }
+#pragma unroll
+          for (int i = 0; i < KC; ++i)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {          // dims 4 g + 2 e, + 1: tokens 0, 1 and 2, 3 of each
+              const uint32_t x0 = e ? x[i][0].y : x[i][0].x, x1 = e ? x[i][1].y : x[i][1].x;
+              const uint32_t x2 = e ? x[i][2].y : x[i][2].x, x3 = e ? x[i][3].y : x[i][3].x;
+              values[i * 64 + e * 32] =
+                  make_uint4(rescale2<kBf16>(__byte_perm(x0, x1, 0x5410), down), rescale2<kBf16>(__byte_perm(x2, x3, 0x5410), down),
+                             rescale2<kBf16>(__byte_perm(x0, x1, 0x7632), down), rescale2<kBf16>(__byte_perm(x2, x3, 0x7632), down));
+            }
+        }
+      }
+      __syncthreads();                             // the operands are there, the codes have been read
+      fetch(slot);
+      slot ^= 1;
+      const int there = s_there;
+      if (!active || there <= group * RW) continue;
+
+      // Whole units whose tokens all rows see, with finite scales, are most: without a branch in them.
+      auto work = [&](auto plain) {
+      constexpr bool kPlain = decltype(plain)::value;
+      // ---- scores of this warp's blocks
+      float s[RW][2][4];
+#pragma unroll
+      for (int j = 0; j < RW; ++j) {
+        const int k = group * RW + j;
+        if (!kPlain && k >= there) {
+#pragma unroll
+          for (int half = 0; half < 2; ++half)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[j][half][e] = -INFINITY;
+          continue;
+        }
+        const uint4* keys = reinterpret_cast<const uint4*>(wide) + k * (2 * P / 64) * 64 + lane;
+        const float key = s_key[k], mul0 = mul[0] * key, mul1 = mul[1] * key;
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          float(&acc)[4] = s[j][half];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[e] = 0.f;
+#pragma unroll
+          for (int d = 0; d < P / 64; ++d) {
+            const uint4 x = keys[(half * (P / 64) + d) * 64], y = keys[(half * (P / 64) + d) * 64 + 32];
+            mma16816<false>(acc, q[d * 4], x.x, x.y);
+            mma16816<false>(acc, q[d * 4 + 1], x.z, x.w);
+            mma16816<false>(acc, q[d * 4 + 2], y.x, y.y);
+            mma16816<false>(acc, q[d * 4 + 3], y.z, y.w);
+          }
+          const float2 bias = *reinterpret_cast<const float2*>(&s_bias[k][4 * t + 2 * half]);
+          acc[0] = fmaf(acc[0], mul0, -bias.x);
+          acc[1] = fmaf(acc[1], mul0, -bias.y);
+          acc[2] = fmaf(acc[2], mul1, -bias.x);
+          acc[3] = fmaf(acc[3], mul1, -bias.y);
+          if (!kPlain) {
+            const int tok = begin + k * kBlockTokens + 4 * t + 2 * half;
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (tok + e % 2 > limit[e / 2] || tok + e % 2 >= total) acc[e] = -INFINITY;
+          }
+        }
+      }
+      // ---- weights, as Running::weigh
+      float top[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+      for (int j = 0; j < RW; ++j)
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          top[0] = fmaxf(top[0], fmaxf(s[j][half][0], s[j][half][1]));
+          top[1] = fmaxf(top[1], fmaxf(s[j][half][2], s[j][half][3]));
+        }
+      if (__any_sync(0xffffffffu, top[0] > run.m[0] + kSlack || top[1] > run.m[1] + kSlack)) {
+        float f[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          float x = fmaxf(top[e], run.m[e]);
+          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
+          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
+          f[e] = run.m[e] == x ? 1.f : attn_ex2(run.m[e] - x);
+          run.m[e] = x;
+          run.l[e] *= f[e];
+        }
+        run.times(f[0], f[1]);
+      }
+      const float ref[2] = {run.m[0] == -INFINITY ? 0.f : run.m[0], run.m[1] == -INFINITY ? 0.f : run.m[1]};
+      float most = 0.f;
+#pragma unroll
+      for (int j = 0; j < RW; ++j)
+        if (kPlain || (group * RW + j < there && s_value[group * RW + j] < INFINITY)) most = fmaxf(most, s_value[group * RW + j]);
+      run.refer(most);
+      const float down = power2(-run.unit);
+#pragma unroll
+      for (int j = 0; j < RW; ++j) {
+        const int k = group * RW + j;
+        if (!kPlain && k >= there) continue;
+        const float value = s_value[k], by = value * down;
+        const bool finite = fabsf(value) < INFINITY;
+        uint32_t p[4];
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[j][half][e] = attn_ex2(s[j][half][e] - ref[e / 2]);
+          run.l[0] += s[j][half][0] + s[j][half][1];
+          run.l[1] += s[j][half][2] + s[j][half][3];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            s[j][half][e] *= by;
+            if (!kPlain && !finite) s[j][half][e] = begin + k * kBlockTokens <= limit[e / 2] ? __int_as_float(0x7fc00000) : 0.f;
+          }
+          p[2 * half] = pack2<false>(s[j][half][0], s[j][half][1]);
+          p[2 * half + 1] = pack2<false>(s[j][half][2], s[j][half][3]);
+        }
+        const uint4* values = reinterpret_cast<const uint4*>(wide + T::kRaw) + k * KC * 64 + lane;
+        if (kPlain || !s_odd[k]) {
+#pragma unroll
+          for (int c = 0; c < KC; ++c) {
+            const uint4 x = values[c * 64], y = values[c * 64 + 32];
+            mma16816<false>(run.o[c][0], p, x.x, x.y);
+            mma16816<false>(run.o[c][1], p, x.z, x.w);
+            mma16816<false>(run.o[c][2], p, y.x, y.y);
+            mma16816<false>(run.o[c][3], p, y.z, y.w);
+          }
+        } else {                                   // token by token: 0 * inf must not reach rows that do not see it
+#pragma unroll 1
+          for (int only = 0; only < kBlockTokens; ++only) {
+            const uint32_t mask = only % 2 ? 0xffff0000u : 0x0000ffffu;
+            const uint32_t lo = t == only / 4 && only % 4 < 2 ? mask : 0u, hi = t == only / 4 && only % 4 >= 2 ? mask : 0u;
+            const int token = begin + k * kBlockTokens + only;
+#pragma unroll
+            for (int c = 0; c < KC; ++c) {
+              const uint4 x = values[c * 64], y = values[c * 64 + 32];
+              const uint32_t w[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                float acc[4] = {0.f, 0.f, 0.f, 0.f};
+                mma16816<false>(acc, p, w[2 * i] & lo, w[2 * i + 1] & hi);
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                  if (token <= limit[e / 2]) run.o[c][i][e] += acc[e];
+              }
+            }
+          }
+        }
+      }
+      };
+      const bool whole = begin + kUnitTokens - 1 <= first_limit && begin + kUnitTokens <= total;
+      bool finite_values = true;
+#pragma unroll
+      for (int j = 0; j < RW; ++j) finite_values &= s_value[group * RW + j] < INFINITY;
+      if (whole && finite_values) work(std::true_type{});
+      else work(std::false_type{});
+    }
+
+    // ---- the rows' warps with other blocks join the first, in the operands' place; then the output, or a part of it
+    const float up = power2(run.unit);
+    run.times(up, up);
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      run.l[e] += __shfl_xor_sync(0xffffffffu, run.l[e], 1);
+      run.l[e] += __shfl_xor_sync(0xffffffffu, run.l[e], 2);
+    }
+    if constexpr (RW < kRowWarps) {
+      constexpr int kState = KC * 4 + 1;           // 16-byte words of a lane
+      static_assert((kRowWarps - RW) * kState * 512 <= T::kWide, "states in the operands' place");
+      __syncthreads();
+      float4* state = reinterpret_cast<float4*>(wide) + lane;
+      if (group > 0) {
+        float4* to = state + (warp - RW) * kState * 32;
+#pragma unroll
+        for (int c = 0; c < KC; ++c)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) to[(c * 4 + i) * 32] = make_float4(run.o[c][i][0], run.o[c][i][1], run.o[c][i][2], run.o[c][i][3]);
+        to[KC * 4 * 32] = make_float4(run.m[0], run.m[1], run.l[0], run.l[1]);
+      }
+      __syncthreads();
+      if (group == 0) {
+#pragma unroll 1
+        for (int other = warp; other < kRowWarps - RW; other += RW) {
+          const float4* from = state + other * kState * 32;
+          const float4 z = from[KC * 4 * 32];
+          const float m2[2] = {z.x, z.y}, l2[2] = {z.z, z.w};
+          float f[2], f2[2];
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const float x = fmaxf(run.m[e], m2[e]), r = x == -INFINITY ? 0.f : x;
+            f[e] = attn_ex2(run.m[e] - r);
+            f2[e] = attn_ex2(m2[e] - r);
+            run.m[e] = x;
+            run.l[e] = run.l[e] * f[e] + l2[e] * f2[e];
+          }
+#pragma unroll
+          for (int c = 0; c < KC; ++c)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const float4 y = from[(c * 4 + i) * 32];
+              run.o[c][i][0] = run.o[c][i][0] * f[0] + y.x * f2[0];
+              run.o[c][i][1] = run.o[c][i][1] * f[0] + y.y * f2[0];
+              run.o[c][i][2] = run.o[c][i][2] * f[1] + y.z * f2[1];
+              run.o[c][i][3] = run.o[c][i][3] * f[1] + y.w * f2[1];
+            }
+        }
+      }
+    }
+    const bool complete = u0 == 0 && u1 == units.count;
+    if (u0 == 0 && threadIdx.x == 0 && (by_segment || !complete)) {
+      const int last = static_cast<int>(min(deal.worker(at + units.count - 1), static_cast<int64_t>(workers - 1)));
+      notes[by_segment ? static_cast<int64_t>(b) * segments + seg : self] = {complete ? -1 : b, seg, self, last, units.fresh, {}};
+    }
+    if (group == 0) {
+      float* part = part_of<P, NT>(a, 2 * self + (u0 == 0));
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int in = row0 + g + 8 * e, c = c0 + in;
+        if (c >= a.T * a.G) continue;
+        const float m = run.m[e], l = run.l[e];
+        const float f = complete ? last_factor(a, m, l, q_sq[e]) : 1.f;
+        const bool none = c / a.G >= units.fresh || (m == -INFINITY && l == 0.f);
+        uint16_t* out = static_cast<uint16_t*>(a.out) + out_offset(a, b, h, c);
+#pragma unroll
+        for (int i = 0; i < KC; ++i) {
+          const float(&o)[4][4] = run.o[i];
+          const int d = 32 * i + 8 * t;
+          if (complete) {
+            if (d >= a.D) continue;
+            uint4 y = make_uint4(pack2<kBf16>(o[0][2 * e] * f, o[1][2 * e] * f), pack2<kBf16>(o[2][2 * e] * f, o[3][2 * e] * f),
+                                 pack2<kBf16>(o[0][2 * e + 1] * f, o[1][2 * e + 1] * f), pack2<kBf16>(o[2][2 * e + 1] * f, o[3][2 * e + 1] * f));
+            if (none) y = make_uint4(0, 0, 0, 0);
+            *reinterpret_cast<uint4*>(out + d) = y;
+          } else {
+            float4* to = reinterpret_cast<float4*>(part + in * part_pitch(P) + d);
+            to[0] = make_float4(o[0][2 * e], o[1][2 * e], o[2][2 * e], o[3][2 * e]);
+            to[1] = make_float4(o[0][2 * e + 1], o[1][2 * e + 1], o[2][2 * e + 1], o[3][2 * e + 1]);
+          }
+        }
+        if (!complete && t == 0) *reinterpret_cast<float4*>(part + in * part_pitch(P) + P) = make_float4(m, l, q_sq[e], 0.f);
+      }
+    }
+    at += u1 - u0;
+  }
+  grid_dependents_launch();
+}
+
 constexpr int kJoinWarps = 32;                     // of a block at most
 
 // Joins the parts of the segments that several warps worked on: blocks (i, ...) the segment of note i, a block's warps its
@@ -994,6 +1580,19 @@ __global__ void __launch_bounds__(kJoinWarps * 32) cache_join_kernel(const Cache
   else *reinterpret_cast<uint32_t*>(to) = packed[0];
 }
 
+template <bool kBf16, int P, int NT>
+cudaError_t join_t(const CacheAttnArgs& a, int workers, cudaStream_t stream) {
+  const int64_t segments = static_cast<int64_t>(a.B) * a.column_tiles * a.H;
+  // a warp for every eight of the parts that a segment has on average, and eight warps or more to a block
+  const int width = static_cast<int64_t>(a.T) * a.G < 8 * NT ? a.T * a.G : 8 * NT;
+  const int64_t parts = workers / segments;
+  int split = 1;
+  while (split < kJoinWarps && split * 8 < parts) split *= 2;
+  const int warps = split > 8 ? split : 8, each = warps / split;
+  return launch_dependent(cache_join_kernel<kBf16, P, NT>, dim3(a.notes, (width + each - 1) / each), warps * 32, 0, stream, a,
+                          workers, split);
+}
+
 int64_t cache_attn_notes(int64_t segments, int64_t workers) { return segments < workers ? segments : workers; }
 
 template <bool kBf16, int P, int NT>
@@ -1008,14 +1607,7 @@ cudaError_t attn_t(CacheAttnArgs a, int sms, cudaStream_t stream) {
   if (e != cudaSuccess) return e;
   cache_attn_kernel<kBf16, P, NT><<<sms, S::kWarps * 32, kSmem, stream>>>(a);
   if ((e = cudaGetLastError()) != cudaSuccess) return e;
-  // a warp for every eight of the parts that a segment has on average, and eight warps or more to a block
-  const int width = static_cast<int64_t>(a.T) * a.G < 8 * NT ? a.T * a.G : 8 * NT;
-  const int64_t parts = workers / segments;
-  int split = 1;
-  while (split < kJoinWarps && split * 8 < parts) split *= 2;
-  const int warps = split > 8 ? split : 8, each = warps / split;
-  return launch_dependent(cache_join_kernel<kBf16, P, NT>, dim3(a.notes, (width + each - 1) / each), warps * 32, 0, stream, a,
-                          workers, split);
+  return join_t<kBf16, P, NT>(a, workers, stream);
 }
 
 // Blocks of a cluster that share a segment in the kernel for short sequences, 0: not that kernel. It is for one tile of columns
@@ -1053,44 +1645,51 @@ cudaError_t short_t(const CacheAttnArgs& a, int ranks, cudaStream_t stream) {
   return launched;
 }
 
+template <bool kBf16, int P, int RW>
+cudaError_t rows_t(CacheAttnArgs a, int sms, cudaStream_t stream) {
+  using T = RowTile<P>;
+  const int workers = sms * T::kBlocks;
+  a.notes = static_cast<int>(cache_attn_notes(static_cast<int64_t>(a.B) * a.column_tiles * a.H, workers));
+  static PerDeviceFlags flags;
+  cudaError_t e = ensure_dynamic_smem(cache_attn_rows_kernel<kBf16, P, RW>, T::kSmem, flags);
+  if (e != cudaSuccess) return e;
+  cache_attn_rows_kernel<kBf16, P, RW><<<workers, kRowWarps * 32, T::kSmem, stream>>>(a);
+  if ((e = cudaGetLastError()) != cudaSuccess) return e;
+  return join_t<kBf16, P, 2 * RW>(a, workers, stream);
+}
+
 template <bool kBf16, int P>
 cudaError_t attn_p(const CacheAttnArgs& a, int sms, cudaStream_t stream) {
   const int64_t segments = static_cast<int64_t>(a.B) * a.H;
   if (const int ranks = short_ranks(segments, static_cast<int64_t>(a.T) * a.G, a.max_pages, sms))
     return segments > 2 * sms ? short_t<kBf16, P, 4>(a, ranks, stream) : short_t<kBf16, P, kShortWarps>(a, ranks, stream);
-  switch (cache_attn_tiles(a.T, a.G, P)) {
-    case 1: return attn_t<kBf16, P, 1>(a, sms, stream);
-    case 2: return attn_t<kBf16, P, 2>(a, sms, stream);
-    default:
-      if constexpr (P == 64) {
-        if (cache_attn_tiles(a.T, a.G, P) == 3) return attn_t<kBf16, P, 3>(a, sms, stream);
-        return attn_t<kBf16, P, 4>(a, sms, stream);
-      }
+  switch (cache_attn_columns(a.T, a.G)) {
+    case 8: return attn_t<kBf16, P, 1>(a, sms, stream);
+    case 16: return rows_t<kBf16, P, 1>(a, sms, stream);
+    case 32: return rows_t<kBf16, P, 2>(a, sms, stream);
+    default: return rows_t<kBf16, P, 4>(a, sms, stream);
   }
-  return cudaErrorInvalidValue;
 }
 
 }  // namespace
 
-// Operand tiles of 8 columns that a warp works on at a time: as few rounds over the cache as its registers allow (32 columns, 16
-// at 128 dims), and as few empty columns as that many rounds allow.
-int cache_attn_tiles(int T, int G, int P) {
-  const int64_t tiles = (static_cast<int64_t>(T) * G + 7) / 8, most = 256 / P, rounds = (tiles + most - 1) / most;
-  return static_cast<int>((tiles + rounds - 1) / rounds);
+// Columns of a tile: new tokens of the query heads that share a key/value head
+int cache_attn_columns(int T, int G) {
+  const int64_t columns = static_cast<int64_t>(T) * G;
+  return columns <= 8 ? 8 : columns <= 16 ? 16 : columns <= 32 ? 32 : 64;
 }
 
 size_t cache_attn_workspace_bytes(int B, int H, int G, int T, int D, int max_pages, int sms) {
   const int P = cache_columns(D);
   if (short_ranks(static_cast<int64_t>(B) * H, static_cast<int64_t>(T) * G, max_pages, sms)) return 0;
-  const int tiles = cache_attn_tiles(T, G, P), warps = tiles > 1 ? Shape<64, 2>::kWarps : Shape<64, 1>::kWarps;
-  const int width = static_cast<int64_t>(T) * G < 8 * tiles ? T * G : 8 * tiles;
-  const int64_t workers = static_cast<int64_t>(sms) * warps;
+  const int tile = cache_attn_columns(T, G), width = static_cast<int64_t>(T) * G < tile ? T * G : tile;
+  const int64_t workers = static_cast<int64_t>(sms) * (tile == 8 ? Shape<64, 1>::kWarps : P == 64 ? RowTile<64>::kBlocks : RowTile<128>::kBlocks);
   return static_cast<size_t>(workers) * (sizeof(Note) + 2 * width * part_pitch(P) * sizeof(float));
 }
 
 cudaError_t launch_cache_attn(CacheAttnArgs a, bool bf16, int sms, cudaStream_t stream) {
   if (a.B == 0 || a.T == 0) return cudaSuccess;
-  const int64_t columns = 8 * cache_attn_tiles(a.T, a.G, cache_columns(a.D)), tiles = (static_cast<int64_t>(a.T) * a.G + columns - 1) / columns;
+  const int64_t columns = cache_attn_columns(a.T, a.G), tiles = (static_cast<int64_t>(a.T) * a.G + columns - 1) / columns;
   if (tiles * columns * a.H * a.B > 0x7fffffffll) return cudaErrorInvalidConfiguration;
   a.column_tiles = static_cast<int>(tiles);
   a.exponents = 0x64646464u;

@@ -234,7 +234,7 @@ struct CacheAttnArgs {
   int notes;                 // segments of which several warps may have parts
   uint32_t exponents;        // a constant that the compiler is not to know
 };
-int cache_attn_tiles(int T, int G, int P);
+int cache_attn_columns(int T, int G);
 size_t cache_attn_workspace_bytes(int B, int H, int G, int T, int D, int max_pages, int sms);
 cudaError_t launch_cache_attn(CacheAttnArgs a, bool bf16, int sms, cudaStream_t stream);
 
