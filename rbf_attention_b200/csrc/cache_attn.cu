@@ -28,16 +28,11 @@
 namespace rbf {
 namespace {
 
-// Warps of a block (one per SM), blocks of a unit, and units of a warp that are loaded ahead, the current one among them: what
-// registers (65536) and shared memory (227 KB) hold. One tile of columns: 8 KB units, 12 warps with two each; 16 x 32768 tokens
-// of 128 columns took 115 us with 8 warps and three units, 104 so; 8 x 16384 of 64 columns 36 and 33.5 us, with 16 warps and
-// three units of 4 KB 35.5. Several tiles: 216 to 255 registers, 8 warps; units of two blocks, whose code is half as long.
-template <int P, int NT>
-struct Shape {
-  static constexpr int kUnitBlocks = NT == 1 ? 256 / P : 2;
-  static constexpr int kWarps = NT == 1 ? 12 : 8;
-  static constexpr int kStages = NT == 1 || P == 128 ? 2 : 3;
-};
+// Up to 8 columns: warps of a block (one per SM), blocks of a unit, and units of a warp that are loaded ahead, the current one among
+// them: what registers (65536) and shared memory (227 KB) hold with 8 KB units. 16 x 32768 tokens of 128 columns took 115 us with
+// 8 warps and three units, 104 so; 8 x 16384 of 64 columns 36 and 33.5 us, with 16 warps and three units of 4 KB 35.5.
+constexpr int kWarpsOf8 = 12, kStagesOf8 = 2;
+template <int P> constexpr int kUnitBlocks = 256 / P;
 constexpr int kShortWarps = 8;                     // of the kernel for short sequences, 4 where there are many
 constexpr float kSlack = 8.f;                      // growth of a score, in powers of two, that does not move the maximum
 
@@ -193,35 +188,28 @@ struct alignas(16) Note {
 // One part: per column P outputs and three numbers, the maximum, the sum and what the variant without a denominator needs; of
 // as many columns as a tile has at most
 constexpr int part_pitch(int P) { return P + 4; }
-template <int P, int NT>
-__device__ __forceinline__ float* part_of(const CacheAttnArgs& a, int64_t index) {
-  return a.parts + a.notes * (sizeof(Note) / sizeof(float)) + index * (min(8 * NT, a.T * a.G) * part_pitch(P));
+template <int P>
+__device__ __forceinline__ float* part_of(const CacheAttnArgs& a, int columns, int64_t index) {
+  return a.parts + a.notes * (sizeof(Note) / sizeof(float)) + index * (min(columns, a.T * a.G) * part_pitch(P));
 }
 
 // 2^x for -126 <= x <= 127
 __device__ __forceinline__ float power2(int x) { return __int_as_float((x + 127) << 23); }
 
 // A warp's state for one segment
-template <int P, int NT>
+template <int P>
 struct Running {
-  float o[P / 16][NT][4];                  // tile j: dims 32 (j / 2) + 4 g + 2 (j % 2), + 1 of columns 2t, 2t + 1
-  float m[NT][2], l[NT][2];                        // of columns 8n + 2t, + 1; l: this lane's share
+  float o[P / 16][4];                              // tile j: dims 32 (j / 2) + 4 g + 2 (j % 2), + 1 of columns 2t, 2t + 1
+  float m[2], l[2];                                // of columns 2t, 2t + 1; l: this lane's share
   int unit;                                        // o is in units of 2^unit
   __device__ __forceinline__ void clear() {
     unit = 0;
 #pragma unroll
     for (int j = 0; j < P / 16; ++j)
 #pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) o[j][n][e] = 0.f;
-#pragma unroll
-    for (int n = 0; n < NT; ++n)
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        m[n][e] = -INFINITY;
-        l[n][e] = 0.f;
-      }
+      for (int e = 0; e < 4; ++e) o[j][e] = 0.f;
+    m[0] = m[1] = -INFINITY;
+    l[0] = l[1] = 0.f;
   }
   // A block's value scale goes into its weights, so that all products add up in o: weights are at most 2^8, so the unit is
   // chosen to have the largest scale at hand in [2^6, 2^7), fp16 below its limit and its smallest normal number at 2^-20 of
@@ -235,9 +223,7 @@ struct Running {
 #pragma unroll
     for (int j = 0; j < P / 16; ++j)
 #pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) top = fmaxf(top, fabsf(o[j][n][e]));
+      for (int e = 0; e < 4; ++e) top = fmaxf(top, fabsf(o[j][e]));
     const uint32_t bits = __reduce_max_sync(0xffffffffu, __float_as_uint(top));
     if (bits != 0) {
       to = max(to, unit - min(120, max(0, 100 - (static_cast<int>(bits >> 23) - 127))));
@@ -245,9 +231,7 @@ struct Running {
 #pragma unroll
       for (int j = 0; j < P / 16; ++j)
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) o[j][n][e] *= f;
+        for (int e = 0; e < 4; ++e) o[j][e] *= f;
     }
     unit = to;
   }
@@ -257,67 +241,56 @@ struct Running {
 #pragma unroll
     for (int j = 0; j < P / 16; ++j)
 #pragma unroll
-      for (int n = 0; n < NT; ++n)
+      for (int e = 0; e < 4; ++e) o[j][e] *= up;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) o[j][n][e] *= up;
+    for (int e = 0; e < 2; ++e)
 #pragma unroll
-    for (int n = 0; n < NT; ++n)
-#pragma unroll
-      for (int e = 0; e < 2; ++e)
-#pragma unroll
-        for (int w = 4; w < 32; w <<= 1) l[n][e] += __shfl_xor_sync(0xffffffffu, l[n][e], w);
+      for (int w = 4; w < 32; w <<= 1) l[e] += __shfl_xor_sync(0xffffffffu, l[e], w);
   }
-  // this lane's outputs of column 8n + 2t + e, in the order of the dims
-  __device__ __forceinline__ void store(float* row, int n, int e) const {
+  // this lane's outputs of column 2t + e, in the order of the dims
+  __device__ __forceinline__ void store(float* row, int e) const {
 #pragma unroll
     for (int i = 0; i < P / 32; ++i)
       *reinterpret_cast<float4*>(row + 32 * i + (threadIdx.x & 31) / 4 * 4) =
-          make_float4(o[2 * i][n][e], o[2 * i][n][2 + e], o[2 * i + 1][n][e], o[2 * i + 1][n][2 + e]);
+          make_float4(o[2 * i][e], o[2 * i][2 + e], o[2 * i + 1][e], o[2 * i + 1][2 + e]);
   }
   // The maximum moves only if a score exceeds it by more than the slack; s becomes the weights, l their sum.
   template <int kBlocks>
-  __device__ __forceinline__ void weigh(float (&s)[kBlocks][NT][4]) {
-    float top[NT][2];
+  __device__ __forceinline__ void weigh(float (&s)[kBlocks][4]) {
+    float top[2];
     bool over = false;
 #pragma unroll
-    for (int n = 0; n < NT; ++n)
+    for (int e = 0; e < 2; ++e) {
+      top[e] = fmaxf(s[0][e], s[0][2 + e]);
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        top[n][e] = fmaxf(s[0][n][e], s[0][n][2 + e]);
-#pragma unroll
-        for (int k = 1; k < kBlocks; ++k) top[n][e] = fmaxf(top[n][e], fmaxf(s[k][n][e], s[k][n][2 + e]));
-        over |= top[n][e] > m[n][e] + kSlack;
-      }
+      for (int k = 1; k < kBlocks; ++k) top[e] = fmaxf(top[e], fmaxf(s[k][e], s[k][2 + e]));
+      over |= top[e] > m[e] + kSlack;
+    }
     if (__any_sync(0xffffffffu, over)) {
 #pragma unroll
-      for (int n = 0; n < NT; ++n)
+      for (int e = 0; e < 2; ++e) {
+        float x = fmaxf(top[e], m[e]);
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          float x = fmaxf(top[n][e], m[n][e]);
+        for (int w = 4; w < 32; w <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, w));
+        const float f = m[e] == x ? 1.f : attn_ex2(m[e] - x);
+        m[e] = x;
+        l[e] *= f;
 #pragma unroll
-          for (int w = 4; w < 32; w <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, w));
-          const float f = m[n][e] == x ? 1.f : attn_ex2(m[n][e] - x);
-          m[n][e] = x;
-          l[n][e] *= f;
-#pragma unroll
-          for (int j = 0; j < P / 16; ++j) {
-            o[j][n][e] *= f;
-            o[j][n][2 + e] *= f;
-          }
+        for (int j = 0; j < P / 16; ++j) {
+          o[j][e] *= f;
+          o[j][2 + e] *= f;
         }
-    }
-#pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      float ref[2];
-#pragma unroll
-      for (int e = 0; e < 2; ++e) ref[e] = m[n][e] == -INFINITY ? 0.f : m[n][e];      // no token seen yet
-#pragma unroll
-      for (int k = 0; k < kBlocks; ++k) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) s[k][n][e] = attn_ex2(s[k][n][e] - ref[e % 2]);
-        l[n][0] += s[k][n][0] + s[k][n][2];
-        l[n][1] += s[k][n][1] + s[k][n][3];
       }
+    }
+    float ref[2];
+#pragma unroll
+    for (int e = 0; e < 2; ++e) ref[e] = m[e] == -INFINITY ? 0.f : m[e];      // no token seen yet
+#pragma unroll
+    for (int k = 0; k < kBlocks; ++k) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s[k][e] = attn_ex2(s[k][e] - ref[e % 2]);
+      l[0] += s[k][0] + s[k][2];
+      l[1] += s[k][1] + s[k][3];
     }
   }
 };
@@ -343,61 +316,58 @@ __device__ __forceinline__ void load_q(const CacheAttnArgs& a, int b, int h, int
 }
 
 // The query columns of a segment: operands, their scales, and how far each column sees
-template <bool kBf16, int P, int NT>
+template <bool kBf16, int P>
 struct Queries {
-  uint32_t w[NT][P / 16][2];                       // fp16, scaled
-  float mul[NT][2], sq[NT][2];                     // of columns 2t, 2t + 1: what the scores are multiplied by, g log2(e) |q|^2
-  int limit[NT][2];                                // last token that the column sees
+  uint32_t w[P / 16][2];                       // fp16, scaled
+  float mul[2], sq[2];                     // of columns 2t, 2t + 1: what the scores are multiplied by, g log2(e) |q|^2
+  int limit[2];                                // last token that the column sees
   int first_limit, last_limit;                     // every column of the tile sees at least, none sees more
-  int b, h, c0, total;
+  int b, h, total;
   uint32_t exponents;
 
-  __device__ __forceinline__ void load(const CacheAttnArgs& a, int b_, int h_, int c0_, int held, int total_) {
-    b = b_, h = h_, c0 = c0_, total = total_;
+  __device__ __forceinline__ void load(const CacheAttnArgs& a, int b_, int h_, int held, int total_) {
+    b = b_, h = h_, total = total_;
     exponents = a.exponents;
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    uint32_t raw[P / 16][2];
+    load_q<P>(a, b, h, g, t, raw);
+    uint32_t top = 0;
+    float square = 0.f;
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      uint32_t raw[P / 16][2];
-      load_q<P>(a, b, h, c0 + n * 8 + g, t, raw);
-      uint32_t top = 0;
-      float square = 0.f;
-#pragma unroll
-      for (int i = 0; i < P / 16; ++i) {
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const float2 f = unpack2<kBf16>(raw[i][e]);
-          top = max(top, max(__float_as_uint(f.x) & 0x7fffffffu, __float_as_uint(f.y) & 0x7fffffffu));
-          square = fmaf(f.x, f.x, fmaf(f.y, f.y, square));
-        }
-      }
-#pragma unroll
-      for (int o = 1; o < 4; o <<= 1) {
-        top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-        square += __shfl_xor_sync(0xffffffffu, square, o);
-      }
-      uint32_t exponent = top >> 23;                 // of the largest element; zero and infinity keep their meaning
-      exponent = exponent == 0 ? 127u : min(exponent, 253u);
-      const float down = __uint_as_float((254u - exponent) << 23), up = __uint_as_float(exponent << 23);
-#pragma unroll
-      for (int i = 0; i < P / 16; ++i) {
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const float2 f = unpack2<kBf16>(raw[i][e]);
-          w[n][i][e] = pack2<false>(f.x * down, f.y * down);
-        }
-      }
+    for (int i = 0; i < P / 16; ++i) {
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        const int from = (2 * t + e) * 4;
-        mul[n][e] = 2.f * a.scale * __shfl_sync(0xffffffffu, up, from);
-        sq[n][e] = a.scale * __shfl_sync(0xffffffffu, square, from);
-        const int c = c0 + n * 8 + 2 * t + e;
-        limit[n][e] = c < a.T * a.G ? held + c / a.G : total - 1;
+        const float2 f = unpack2<kBf16>(raw[i][e]);
+        top = max(top, max(__float_as_uint(f.x) & 0x7fffffffu, __float_as_uint(f.y) & 0x7fffffffu));
+        square = fmaf(f.x, f.x, fmaf(f.y, f.y, square));
       }
     }
-    first_limit = held + c0 / a.G;
-    last_limit = held + (c0 + 8 * NT - 1) / a.G;
+#pragma unroll
+    for (int o = 1; o < 4; o <<= 1) {
+      top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+      square += __shfl_xor_sync(0xffffffffu, square, o);
+    }
+    uint32_t exponent = top >> 23;                 // of the largest element; zero and infinity keep their meaning
+    exponent = exponent == 0 ? 127u : min(exponent, 253u);
+    const float down = __uint_as_float((254u - exponent) << 23), up = __uint_as_float(exponent << 23);
+#pragma unroll
+    for (int i = 0; i < P / 16; ++i) {
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const float2 f = unpack2<kBf16>(raw[i][e]);
+        w[i][e] = pack2<false>(f.x * down, f.y * down);
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int from = (2 * t + e) * 4;
+      mul[e] = 2.f * a.scale * __shfl_sync(0xffffffffu, up, from);
+      sq[e] = a.scale * __shfl_sync(0xffffffffu, square, from);
+      const int c = 2 * t + e;
+      limit[e] = c < a.T * a.G ? held + c / a.G : total - 1;
+    }
+    first_limit = held;
+    last_limit = held + 7 / a.G;
   }
 };
 
@@ -430,33 +400,27 @@ __device__ __forceinline__ void fetch_unit(uint8_t* stage, const uint8_t* page, 
   if (lane < UB / 2) copy16(to + T::kScales + lane * 16, page + (what & 0xff) * 8 + lane * 16);
 }
 
-// A group of complete blocks, the first of them at token `begin`
-template <bool kBf16, int P, int NT, int UB>
-__device__ __forceinline__ void codes_unit(const CacheAttnArgs& a, const Queries<kBf16, P, NT>& q, Running<P, NT>& run,
-                                           const uint8_t* stage, int begin) {
+// A group of complete blocks, the first of them at token `begin`. kPlain: all of the unit's blocks are there, their scales are
+// finite and every column sees them: the code has no branches, so that the blocks' chains of products overlap.
+template <bool kPlain, bool kBf16, int P, int UB>
+__device__ __forceinline__ void codes_blocks(const CacheAttnArgs& a, const Queries<kBf16, P>& q, Running<P>& run,
+                                             const uint8_t* stage, int begin, int whole) {
   using T = Tile<P, UB>;
   constexpr int kSlot = cache_slot_bytes(P);
   const int lane = threadIdx.x & 31, g = lane >> 2;
-  if (begin > q.last_limit) return;
-  const int whole = min(UB, q.total / kBlockTokens - begin / kBlockTokens);
-  const bool hidden = begin + T::kUnit - 1 > q.first_limit;
   const float2* scales = reinterpret_cast<const float2*>(stage + T::kScales);
-  float s[UB][NT][4];
+  float s[UB][4];
 #pragma unroll
   for (int k = 0; k < UB; ++k) {
 #pragma unroll
-    for (int n = 0; n < NT; ++n)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) s[k][n][e] = -INFINITY;
-    if (k >= whole) continue;
+    for (int e = 0; e < 4; ++e) s[k][e] = -INFINITY;
+    if (!kPlain && k >= whole) continue;
     const float key_scale = scales[k].x;
     const uint4* key = reinterpret_cast<const uint4*>(stage + k * kSlot) + lane;
     int sq0 = 0, sq1 = 0;
-    float acc[NT][4];
+    float acc[4];
 #pragma unroll
-    for (int n = 0; n < NT; ++n)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) acc[n][e] = 0.f;
+    for (int e = 0; e < 4; ++e) acc[e] = 0.f;
 #pragma unroll
     for (int d = 0; d < P / 64; ++d) {
       const uint4 w0 = key[2 * d * 32], w1 = key[(2 * d + 1) * 32];
@@ -467,8 +431,7 @@ __device__ __forceinline__ void codes_unit(const CacheAttnArgs& a, const Queries
         sq1 += dot4(r1[i]);
         const uint32_t A[4] = {codes_lo(r0[i], q.exponents), codes_lo(r1[i], q.exponents), codes_hi(r0[i], q.exponents),
                                codes_hi(r1[i], q.exponents)};
-#pragma unroll
-        for (int n = 0; n < NT; ++n) mma16816<false>(acc[n], A, q.w[n][d * 4 + i][0], q.w[n][d * 4 + i][1]);
+        mma16816<false>(acc, A, q.w[d * 4 + i][0], q.w[d * 4 + i][1]);
       }
     }
 #pragma unroll
@@ -479,49 +442,41 @@ __device__ __forceinline__ void codes_unit(const CacheAttnArgs& a, const Queries
     const float bias = a.scale * key_scale * key_scale;
     const float b0 = bias * static_cast<float>(sq0), b1 = bias * static_cast<float>(sq1);
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const float mul = q.mul[n][e] * key_scale;
-        s[k][n][e] = fmaf(acc[n][e], mul, -b0);
-        s[k][n][2 + e] = fmaf(acc[n][2 + e], mul, -b1);
-      }
+    for (int e = 0; e < 2; ++e) {
+      const float mul = q.mul[e] * key_scale;
+      s[k][e] = fmaf(acc[e], mul, -b0);
+      s[k][2 + e] = fmaf(acc[2 + e], mul, -b1);
     }
-    if (hidden) {
+    if (!kPlain) {
       const int tok = begin + k * kBlockTokens + 4 * (g >> 1) + (g & 1);
 #pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (tok + 2 * (e / 2) > q.limit[n][e % 2]) s[k][n][e] = -INFINITY;
+      for (int e = 0; e < 4; ++e)
+        if (tok + 2 * (e / 2) > q.limit[e % 2]) s[k][e] = -INFINITY;
     }
   }
   run.weigh(s);
   float scale[UB], most = 0.f;
 #pragma unroll
   for (int k = 0; k < UB; ++k) {
-    scale[k] = k < whole ? scales[k].y : 0.f;
-    if (scale[k] < INFINITY) most = fmaxf(most, scale[k]);
+    scale[k] = kPlain || k < whole ? scales[k].y : 0.f;
+    if (kPlain || scale[k] < INFINITY) most = fmaxf(most, scale[k]);
   }
   run.refer(most);
   const float down = power2(-run.unit);
 #pragma unroll
   for (int k = 0; k < UB; ++k) {
-    if (k >= whole) continue;
-    uint32_t p[NT][2];
+    if (!kPlain && k >= whole) continue;
+    uint32_t p[2];
     const float by = scale[k] * down;
     const bool finite = fabsf(scale[k]) < INFINITY;
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        s[k][n][e] *= by;
-        // a block that is not finite reaches the columns that see it, whatever its weight, and no other
-        if (!finite) s[k][n][e] = begin + k * kBlockTokens <= q.limit[n][e % 2] ? __int_as_float(0x7fc00000) : 0.f;
-      }
-      p[n][0] = transpose8(pack2<false>(s[k][n][0], s[k][n][1]));
-      p[n][1] = transpose8(pack2<false>(s[k][n][2], s[k][n][3]));
+    for (int e = 0; e < 4; ++e) {
+      s[k][e] *= by;
+      // a block that is not finite reaches the columns that see it, whatever its weight, and no other
+      if (!kPlain && !finite) s[k][e] = begin + k * kBlockTokens <= q.limit[e % 2] ? __int_as_float(0x7fc00000) : 0.f;
     }
+    p[0] = transpose8(pack2<false>(s[k][0], s[k][1]));
+    p[1] = transpose8(pack2<false>(s[k][2], s[k][3]));
     const uint4* value = reinterpret_cast<const uint4*>(stage + k * kSlot + 16 * P) + lane;
 #pragma unroll
     for (int i = 0; i < P / 32; ++i) {
@@ -530,16 +485,29 @@ __device__ __forceinline__ void codes_unit(const CacheAttnArgs& a, const Queries
       for (int half = 0; half < 2; ++half) {
         const uint32_t r0 = half ? w.z : w.x, r1 = half ? w.w : w.y;
         const uint32_t A[4] = {codes_lo(r0, q.exponents), codes_lo(r1, q.exponents), codes_hi(r0, q.exponents), codes_hi(r1, q.exponents)};
-#pragma unroll
-        for (int n = 0; n < NT; ++n) mma16816<false>(run.o[2 * i + half][n], A, p[n][0], p[n][1]);
+        mma16816<false>(run.o[2 * i + half], A, p[0], p[1]);
       }
     }
   }
 }
 
+template <bool kBf16, int P, int UB>
+__device__ __forceinline__ void codes_unit(const CacheAttnArgs& a, const Queries<kBf16, P>& q, Running<P>& run,
+                                           const uint8_t* stage, int begin) {
+  using T = Tile<P, UB>;
+  if (begin > q.last_limit) return;
+  const int whole = min(UB, q.total / kBlockTokens - begin / kBlockTokens);
+  bool plain = whole == UB && begin + T::kUnit - 1 <= q.first_limit;
+  const float2* scales = reinterpret_cast<const float2*>(stage + T::kScales);
+#pragma unroll
+  for (int k = 0; k < UB; ++k) plain &= scales[k].y < INFINITY;
+  if (plain) codes_blocks<true, kBf16, P, UB>(a, q, run, stage, begin, whole);
+  else codes_blocks<false, kBf16, P, UB>(a, q, run, stage, begin, whole);
+}
+
 // The block that is not complete, in 16 bits
-template <bool kBf16, int P, int NT>
-__device__ __forceinline__ void rest_unit(const CacheAttnArgs& a, const Queries<kBf16, P, NT>& q, Running<P, NT>& run,
+template <bool kBf16, int P>
+__device__ __forceinline__ void rest_unit(const CacheAttnArgs& a, const Queries<kBf16, P>& q, Running<P>& run,
                                           const uint8_t* stage) {
   constexpr int J = P / 16, KC = P / 32;
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
@@ -547,15 +515,12 @@ __device__ __forceinline__ void rest_unit(const CacheAttnArgs& a, const Queries<
   if (base > q.last_limit) return;
   const uint16_t* keys = reinterpret_cast<const uint16_t*>(stage);
   const uint16_t* values = keys + cache_slot_bytes(P) / 2;
-  float s[1][NT][4];
+  float s[1][4];
 #pragma unroll
-  for (int n = 0; n < NT; ++n)
-#pragma unroll
-    for (int e = 0; e < 4; ++e) s[0][n][e] = 0.f;
+  for (int e = 0; e < 4; ++e) s[0][e] = 0.f;
   float sq[2] = {0.f, 0.f};
-  uint32_t qt[NT][P / 16][2];
-#pragma unroll
-  for (int n = 0; n < NT; ++n) load_q<P>(a, q.b, q.h, q.c0 + n * 8 + g, t, qt[n]);
+  uint32_t qt[P / 16][2];
+  load_q<P>(a, q.b, q.h, g, t, qt);
 #pragma unroll
   for (int d = 0; d < P / 64; ++d) {
     uint32_t r[2][8];
@@ -580,8 +545,7 @@ __device__ __forceinline__ void rest_unit(const CacheAttnArgs& a, const Queries<
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const uint32_t A[4] = {r[0][2 * i], r[1][2 * i], r[0][2 * i + 1], r[1][2 * i + 1]};
-#pragma unroll
-      for (int n = 0; n < NT; ++n) mma16816<kBf16>(s[0][n], A, qt[n][d * 4 + i][0], qt[n][d * 4 + i][1]);
+        mma16816<kBf16>(s[0], A, qt[d * 4 + i][0], qt[d * 4 + i][1]);
     }
   }
 #pragma unroll
@@ -590,19 +554,14 @@ __device__ __forceinline__ void rest_unit(const CacheAttnArgs& a, const Queries<
     sq[1] += __shfl_xor_sync(0xffffffffu, sq[1], x);
   }
 #pragma unroll
-  for (int n = 0; n < NT; ++n)
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int token = base + tok + 2 * (e / 2);
-      s[0][n][e] = token <= q.limit[n][e % 2] && token < total ? fmaf(s[0][n][e], 2.f * a.scale, -a.scale * sq[e / 2]) : -INFINITY;
-    }
-  run.weigh(s);
-  uint32_t p[NT][2];
-#pragma unroll
-  for (int n = 0; n < NT; ++n) {
-    p[n][0] = transpose8(pack2<kBf16>(s[0][n][0], s[0][n][1]));
-    p[n][1] = transpose8(pack2<kBf16>(s[0][n][2], s[0][n][3]));
+  for (int e = 0; e < 4; ++e) {
+    const int token = base + tok + 2 * (e / 2);
+    s[0][e] = token <= q.limit[e % 2] && token < total ? fmaf(s[0][e], 2.f * a.scale, -a.scale * sq[e / 2]) : -INFINITY;
   }
+  run.weigh(s);
+  uint32_t p[2];
+  p[0] = transpose8(pack2<kBf16>(s[0][0], s[0][1]));
+  p[1] = transpose8(pack2<kBf16>(s[0][2], s[0][3]));
   uint2 x[KC][4];                                  // dims 32 i + 4 g ... + 3 of tokens 4 t + r
   uint32_t most = 0;                               // largest magnitudes of even and odd dims, as integers
 #pragma unroll
@@ -633,14 +592,11 @@ __device__ __forceinline__ void rest_unit(const CacheAttnArgs& a, const Queries<
         }
         A[e] = __byte_perm(lo, hi, e % 2 ? 0x7632 : 0x5410);
       }
+      float acc[4] = {0.f, 0.f, 0.f, 0.f};
+      mma16816<kBf16>(acc, A, p[0], p[1]);
 #pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        float acc[4] = {0.f, 0.f, 0.f, 0.f};
-        mma16816<kBf16>(acc, A, p[n][0], p[n][1]);
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (!slow || base + only <= q.limit[n][e % 2]) run.o[j][n][e] = fmaf(acc[e], power2(-run.unit), run.o[j][n][e]);
-      }
+      for (int e = 0; e < 4; ++e)
+        if (!slow || base + only <= q.limit[e % 2]) run.o[j][e] = fmaf(acc[e], power2(-run.unit), run.o[j][e]);
     }
   }
 }
@@ -651,9 +607,9 @@ __device__ __forceinline__ float last_factor(const CacheAttnArgs& a, float m, fl
   return a.softmax ? 1.f / l : attn_ex2((m == -INFINITY ? 0.f : m) - q_sq);
 }
 
-template <bool kBf16, int P, int NT>
-__global__ void __launch_bounds__(Shape<P, NT>::kWarps * 32) cache_attn_kernel(const CacheAttnArgs a) {
-  constexpr int UB = Shape<P, NT>::kUnitBlocks, KC = P / 32, kStages = Shape<P, NT>::kStages, kWarps = Shape<P, NT>::kWarps;
+template <bool kBf16, int P>
+__global__ void __launch_bounds__(kWarpsOf8 * 32) cache_attn_kernel(const CacheAttnArgs a) {
+  constexpr int UB = kUnitBlocks<P>, KC = P / 32, kStages = kStagesOf8, kWarps = kWarpsOf8;
   using T = Tile<P, UB>;
   constexpr int kBytes = cache_page_bytes(P);
   extern __shared__ __align__(128) uint8_t smem[];
@@ -736,14 +692,13 @@ __global__ void __launch_bounds__(Shape<P, NT>::kWarps * 32) cache_attn_kernel(c
       ++b;
       continue;
     }
-    const int seg = static_cast<int>((at - seq_begin) / units.count);
+    const int h = static_cast<int>((at - seq_begin) / units.count);
     const int u0 = static_cast<int>((at - seq_begin) % units.count);
     const int64_t left = stop - at;
     const int u1 = left < units.count - u0 ? u0 + static_cast<int>(left) : units.count;
-    const int h = seg % a.H, c0 = seg / a.H * (8 * NT);
-    Queries<kBf16, P, NT> q;
-    q.load(a, b, h, c0, units.held, units.held + units.fresh);
-    Running<P, NT> run;
+    Queries<kBf16, P> q;
+    q.load(a, b, h, units.held, units.held + units.fresh);
+    Running<P> run;
     run.clear();
     for (int u = u0; u < u1; ++u) {
       const uint8_t* stage = ring + static_cast<int>(taken % kStages) * T::kStage;
@@ -751,43 +706,41 @@ __global__ void __launch_bounds__(Shape<P, NT>::kWarps * 32) cache_attn_kernel(c
       fetch();
       ++taken;
       if (*reinterpret_cast<const int*>(stage + T::kFlag) == 0) continue;  // a page outside the pool: its tokens are absent
-      if (u < units.groups) codes_unit<kBf16, P, NT, UB>(a, q, run, stage, u * T::kUnit);
-      else rest_unit<kBf16, P, NT>(a, q, run, stage);
+      if (u < units.groups) codes_unit<kBf16, P, UB>(a, q, run, stage, u * T::kUnit);
+      else rest_unit<kBf16, P>(a, q, run, stage);
     }
 
     // ---- the segment's output, or this warp's part of it
     run.sum_up();
     const bool complete = u0 == 0 && u1 == units.count;
-    float* part = part_of<P, NT>(a, 2 * self + (u0 == 0));
+    float* part = part_of<P>(a, 8, 2 * self + (u0 == 0));
     if (u0 == 0 && lane == 0 && (by_segment || !complete)) {
       const int last = static_cast<int>(min(deal.worker(at + units.count - 1), workers - 1));
-      notes[by_segment ? static_cast<int64_t>(b) * segments + seg : self] = {complete ? -1 : b, seg, static_cast<int>(self), last, units.fresh, {}};
+      notes[by_segment ? static_cast<int64_t>(b) * segments + h : self] = {complete ? -1 : b, h, static_cast<int>(self), last, units.fresh, {}};
     }
 #pragma unroll
-    for (int n = 0; n < NT; ++n)
+    for (int e = 0; e < 2; ++e) {
+      const int c = 2 * t + e;
+      if (c >= a.T * a.G) continue;
+      const float m = run.m[e], l = run.l[e];
+      if (complete) {
+        const float f = last_factor(a, m, l, q.sq[e]);
+        const bool none = c / a.G >= units.fresh || (m == -INFINITY && l == 0.f);
+        uint16_t* out = static_cast<uint16_t*>(a.out) + out_offset(a, b, h, c);
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int in = n * 8 + 2 * t + e, c = c0 + in;
-        if (c >= a.T * a.G) continue;
-        const float m = run.m[n][e], l = run.l[n][e];
-        if (complete) {
-          const float f = last_factor(a, m, l, q.sq[n][e]);
-          const bool none = c / a.G >= units.fresh || (m == -INFINITY && l == 0.f);
-          uint16_t* out = static_cast<uint16_t*>(a.out) + out_offset(a, b, h, c);
-#pragma unroll
-          for (int i = 0; i < KC; ++i) {
-            const int d = 32 * i + 4 * g;
-            if (d >= a.D) continue;
-            uint2 y = make_uint2(pack2<kBf16>(run.o[2 * i][n][e] * f, run.o[2 * i][n][2 + e] * f),
-                                 pack2<kBf16>(run.o[2 * i + 1][n][e] * f, run.o[2 * i + 1][n][2 + e] * f));
-            if (none) y = make_uint2(0, 0);
-            *reinterpret_cast<uint2*>(out + d) = y;
-          }
-        } else {
-          run.store(part + in * part_pitch(P), n, e);
-          if (g == 0) *reinterpret_cast<float4*>(part + in * part_pitch(P) + P) = make_float4(m, l, q.sq[n][e], 0.f);
+        for (int i = 0; i < KC; ++i) {
+          const int d = 32 * i + 4 * g;
+          if (d >= a.D) continue;
+          uint2 y = make_uint2(pack2<kBf16>(run.o[2 * i][e] * f, run.o[2 * i][2 + e] * f),
+                               pack2<kBf16>(run.o[2 * i + 1][e] * f, run.o[2 * i + 1][2 + e] * f));
+          if (none) y = make_uint2(0, 0);
+          *reinterpret_cast<uint2*>(out + d) = y;
         }
+      } else {
+        run.store(part + c * part_pitch(P), e);
+        if (g == 0) *reinterpret_cast<float4*>(part + c * part_pitch(P) + P) = make_float4(m, l, q.sq[e], 0.f);
       }
+    }
     at += u1 - u0;
   }
   grid_dependents_launch();
@@ -819,7 +772,7 @@ __device__ __forceinline__ void load_floats(const float* from, float (&x)[kCount
 // shared memory, the blocks' through the cluster's, in a fixed order.
 template <bool kBf16, int P, int kWarps>
 __global__ void __launch_bounds__(kWarps * 32, 16 / kWarps) cache_attn_short_kernel(const CacheAttnArgs a) {
-  constexpr int UB = 2, NT = 1, kRing = 2;
+  constexpr int UB = 2, kRing = 2;
   using T = Tile<P, UB>;
   constexpr int kBytes = cache_page_bytes(P);
   static_assert(kRing * T::kStage >= (8 * P + 16) * 4, "a warp's part takes the place of its ring");
@@ -860,17 +813,17 @@ __global__ void __launch_bounds__(kWarps * 32, 16 / kWarps) cache_attn_short_ker
   };
 #pragma unroll
   for (int i = 0; i < kRing; ++i) fetch();
-  Queries<kBf16, P, NT> q;
-  Running<P, NT> run;
+  Queries<kBf16, P> q;
+  Running<P> run;
   run.clear();
-  if (units.count > 0) q.load(a, b, h, 0, units.held, total);
+  if (units.count > 0) q.load(a, b, h, units.held, total);
   for (int i = 0; i < mine; ++i) {
     const uint8_t* stage = ring + i % kRing * T::kStage;
     copies_wait<kRing - 1>();
     if (*reinterpret_cast<const int*>(stage + T::kFlag) != 0) {
       const int u = first + i * each;
-      if (u < units.groups) codes_unit<kBf16, P, NT, UB>(a, q, run, stage, u * T::kUnit);
-      else rest_unit<kBf16, P, NT>(a, q, run, stage);
+      if (u < units.groups) codes_unit<kBf16, P, UB>(a, q, run, stage, u * T::kUnit);
+      else rest_unit<kBf16, P>(a, q, run, stage);
     }
     __syncwarp();                                  // every lane has read the stage
     fetch();
@@ -883,10 +836,10 @@ __global__ void __launch_bounds__(kWarps * 32, 16 / kWarps) cache_attn_short_ker
   __syncwarp();
 #pragma unroll
   for (int e = 0; e < 2; ++e) {
-    run.store(part + (2 * t + e) * P, 0, e);
+    run.store(part + (2 * t + e) * P, e);
     if (g == 0) {
-      part[8 * P + 2 * t + e] = run.m[0][e];
-      part[8 * P + 8 + 2 * t + e] = run.l[0][e];
+      part[8 * P + 2 * t + e] = run.m[e];
+      part[8 * P + 8 + 2 * t + e] = run.l[e];
     }
   }
   __syncthreads();
@@ -907,7 +860,7 @@ __global__ void __launch_bounds__(kWarps * 32, 16 / kWarps) cache_attn_short_ker
     *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.out) + out_offset(a, b, h, c) + d) = y;
   };
   if (warp == 0 && g == 0)                         // |q|^2, which every warp has
-    for (int e = 0; e < 2; ++e) parts[8 * P + 16 + 2 * t + e] = units.count > 0 ? q.sq[0][e] : 0.f;
+    for (int e = 0; e < 2; ++e) parts[8 * P + 16 + 2 * t + e] = units.count > 0 ? q.sq[e] : 0.f;
   __syncthreads();
   for (int i = threadIdx.x; i < used; i += kWarps * 32) {
     const int c = i / kPerColumn, at = c * P + i % kPerColumn * 4;
@@ -1049,7 +1002,6 @@ __global__ void __launch_bounds__(kRowWarps * 32, RowTile<P>::kBlocks) cache_att
   using T = RowTile<P>;
   constexpr int KC = P / 32, UB = kRowWarps, kSlot = cache_slot_bytes(P), kBytes = cache_page_bytes(P);
   constexpr int kRows = 16 * RW, kUnitTokens = UB * kBlockTokens;
-  constexpr int NT = kRows / 8;                    // for the parts: columns in tiles of 8
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ float s_bias[UB][kBlockTokens], s_key[UB], s_value[UB];
   __shared__ int s_there;                          // blocks of the unit that are there
@@ -1488,7 +1440,7 @@ __global__ void __launch_bounds__(kRowWarps * 32, RowTile<P>::kBlocks) cache_att
       notes[by_segment ? static_cast<int64_t>(b) * segments + seg : self] = {complete ? -1 : b, seg, self, last, units.fresh, {}};
     }
     if (group == 0) {
-      float* part = part_of<P, NT>(a, 2 * self + (u0 == 0));
+      float* part = part_of<P>(a, kRows, 2 * self + (u0 == 0));
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const int in = row0 + g + 8 * e, c = c0 + in;
@@ -1525,7 +1477,7 @@ constexpr int kJoinWarps = 32;                     // of a block at most
 
 // Joins the parts of the segments that several warps worked on: blocks (i, ...) the segment of note i, a block's warps its
 // columns in groups of `split` to a column.
-template <bool kBf16, int P, int NT>
+template <bool kBf16, int P, int kColumns>
 __global__ void __launch_bounds__(kJoinWarps * 32) cache_join_kernel(const CacheAttnArgs a, const int workers, const int split) {
   __shared__ float s_y[kJoinWarps][P], s_m[kJoinWarps], s_l[kJoinWarps];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, share = warp % split;
@@ -1538,12 +1490,12 @@ __global__ void __launch_bounds__(kJoinWarps * 32) cache_join_kernel(const Cache
       note.first < 0 || note.first > note.last || note.last >= workers)
     return;
   const int first = note.first;
-  const int h = note.seg % a.H, c = note.seg / a.H * (8 * NT) + in;
-  const bool real = in < 8 * NT && c < a.T * a.G, some = real && c / a.G < note.fresh;
+  const int h = note.seg % a.H, c = note.seg / a.H * kColumns + in;
+  const bool real = in < kColumns && c < a.T * a.G, some = real && c / a.G < note.fresh;
   float y[kPer] = {}, m = -INFINITY, l = 0.f, q_sq = 0.f;
   if (some) {
-    const int64_t pitch = min(8 * NT, a.T * a.G) * part_pitch(P);
-    const float* part = part_of<P, NT>(a, 2 * (first + share) + (share == 0)) + in * part_pitch(P);
+    const int64_t pitch = min(kColumns, a.T * a.G) * part_pitch(P);
+    const float* part = part_of<P>(a, kColumns, 2 * (first + share) + (share == 0)) + in * part_pitch(P);
     if (share == 0) q_sq = part[P + 2];
 #pragma unroll 4
     for (int w = first + share; w <= note.last; w += split) {
@@ -1580,34 +1532,33 @@ __global__ void __launch_bounds__(kJoinWarps * 32) cache_join_kernel(const Cache
   else *reinterpret_cast<uint32_t*>(to) = packed[0];
 }
 
-template <bool kBf16, int P, int NT>
+template <bool kBf16, int P, int kColumns>
 cudaError_t join_t(const CacheAttnArgs& a, int workers, cudaStream_t stream) {
   const int64_t segments = static_cast<int64_t>(a.B) * a.column_tiles * a.H;
   // a warp for every eight of the parts that a segment has on average, and eight warps or more to a block
-  const int width = static_cast<int64_t>(a.T) * a.G < 8 * NT ? a.T * a.G : 8 * NT;
+  const int width = static_cast<int64_t>(a.T) * a.G < kColumns ? a.T * a.G : kColumns;
   const int64_t parts = workers / segments;
   int split = 1;
   while (split < kJoinWarps && split * 8 < parts) split *= 2;
   const int warps = split > 8 ? split : 8, each = warps / split;
-  return launch_dependent(cache_join_kernel<kBf16, P, NT>, dim3(a.notes, (width + each - 1) / each), warps * 32, 0, stream, a,
+  return launch_dependent(cache_join_kernel<kBf16, P, kColumns>, dim3(a.notes, (width + each - 1) / each), warps * 32, 0, stream, a,
                           workers, split);
 }
 
 int64_t cache_attn_notes(int64_t segments, int64_t workers) { return segments < workers ? segments : workers; }
 
-template <bool kBf16, int P, int NT>
+template <bool kBf16, int P>
 cudaError_t attn_t(CacheAttnArgs a, int sms, cudaStream_t stream) {
-  using S = Shape<P, NT>;
-  constexpr int kSmem = S::kWarps * S::kStages * Tile<P, S::kUnitBlocks>::kStage;
-  const int workers = sms * S::kWarps;
+  constexpr int kSmem = kWarpsOf8 * kStagesOf8 * Tile<P, kUnitBlocks<P>>::kStage;
+  const int workers = sms * kWarpsOf8;
   const int64_t segments = static_cast<int64_t>(a.B) * a.column_tiles * a.H;
   a.notes = static_cast<int>(cache_attn_notes(segments, workers));
   static PerDeviceFlags flags;
-  cudaError_t e = ensure_dynamic_smem(cache_attn_kernel<kBf16, P, NT>, kSmem, flags);
+  cudaError_t e = ensure_dynamic_smem(cache_attn_kernel<kBf16, P>, kSmem, flags);
   if (e != cudaSuccess) return e;
-  cache_attn_kernel<kBf16, P, NT><<<sms, S::kWarps * 32, kSmem, stream>>>(a);
+  cache_attn_kernel<kBf16, P><<<sms, kWarpsOf8 * 32, kSmem, stream>>>(a);
   if ((e = cudaGetLastError()) != cudaSuccess) return e;
-  return join_t<kBf16, P, NT>(a, workers, stream);
+  return join_t<kBf16, P, 8>(a, workers, stream);
 }
 
 // Blocks of a cluster that share a segment in the kernel for short sequences, 0: not that kernel. It is for one tile of columns
@@ -1639,7 +1590,7 @@ cudaError_t short_t(const CacheAttnArgs& a, int ranks, cudaStream_t stream) {
   config.dynamicSmemBytes = kSmem;
   config.stream = stream;
   config.attrs = &attr;
-  config.numAttrs = 1;
+  config.numAttrs = ranks > 1 ? 1 : 0;             // a cluster of one block takes longer to launch than a block
   const cudaError_t launched = cudaLaunchKernelEx(&config, cache_attn_short_kernel<kBf16, P, kWarps>, a);
   if (launched != cudaSuccess) cudaGetLastError();
   return launched;
@@ -1655,7 +1606,7 @@ cudaError_t rows_t(CacheAttnArgs a, int sms, cudaStream_t stream) {
   if (e != cudaSuccess) return e;
   cache_attn_rows_kernel<kBf16, P, RW><<<workers, kRowWarps * 32, T::kSmem, stream>>>(a);
   if ((e = cudaGetLastError()) != cudaSuccess) return e;
-  return join_t<kBf16, P, 2 * RW>(a, workers, stream);
+  return join_t<kBf16, P, 16 * RW>(a, workers, stream);
 }
 
 template <bool kBf16, int P>
@@ -1664,7 +1615,7 @@ cudaError_t attn_p(const CacheAttnArgs& a, int sms, cudaStream_t stream) {
   if (const int ranks = short_ranks(segments, static_cast<int64_t>(a.T) * a.G, a.max_pages, sms))
     return segments > 2 * sms ? short_t<kBf16, P, 4>(a, ranks, stream) : short_t<kBf16, P, kShortWarps>(a, ranks, stream);
   switch (cache_attn_columns(a.T, a.G)) {
-    case 8: return attn_t<kBf16, P, 1>(a, sms, stream);
+    case 8: return attn_t<kBf16, P>(a, sms, stream);
     case 16: return rows_t<kBf16, P, 1>(a, sms, stream);
     case 32: return rows_t<kBf16, P, 2>(a, sms, stream);
     default: return rows_t<kBf16, P, 4>(a, sms, stream);
@@ -1683,7 +1634,7 @@ size_t cache_attn_workspace_bytes(int B, int H, int G, int T, int D, int max_pag
   const int P = cache_columns(D);
   if (short_ranks(static_cast<int64_t>(B) * H, static_cast<int64_t>(T) * G, max_pages, sms)) return 0;
   const int tile = cache_attn_columns(T, G), width = static_cast<int64_t>(T) * G < tile ? T * G : tile;
-  const int64_t workers = static_cast<int64_t>(sms) * (tile == 8 ? Shape<64, 1>::kWarps : P == 64 ? RowTile<64>::kBlocks : RowTile<128>::kBlocks);
+  const int64_t workers = static_cast<int64_t>(sms) * (tile == 8 ? kWarpsOf8 : P == 64 ? RowTile<64>::kBlocks : RowTile<128>::kBlocks);
   return static_cast<size_t>(workers) * (sizeof(Note) + 2 * width * part_pitch(P) * sizeof(float));
 }
 
