@@ -209,11 +209,18 @@ class PagedCache:
 
     def abort(self) -> None:
         """Leaves the step without its tokens. If any layer has been written, the step's sequences are freed: tokens that fill a
-        block up take the place of the ones that were held in 16 bits until then."""
+        block up take the place of the ones that were held in 16 bits until then. Otherwise the pages for them are free again."""
         batch, counts, *_ = self._current("abort()")
         written, self._step = self._written, None
         if written:
             self.free([s for s, n in zip(batch, counts) if n])
+            return
+        for s in batch:
+            kept = -(-self._tokens[s] // PAGE_TOKENS)
+            for page in self._held[s][kept:]:
+                self._drop(page)
+            self._held[s] = self._held[s][:kept]
+        self._write_rows(batch)
 
     def read(self, layer: int, sequences=None, count: int | None = None, first=None):
         """(k, v) (batch, heads, count, head_dim) as the cache holds them, from token ``first`` (one for each, default 0) on,

@@ -237,3 +237,18 @@ def test_fake_kernels():
     loss, lp, grad = torch.ops.rbf_attn_b200.policy_loss_fwd(logits, t, row, row, None, None, 0.2, 0.2, 0.0, -100, True)
     assert loss.shape == () and lp.shape == (4,) and grad.shape == logits.shape and grad.dtype == logits.dtype
     assert torch.ops.rbf_attn_b200.token_log_probs(logits, t, -100).dtype == torch.float32
+
+
+def test_pages_of_a_step_that_was_left_are_not_shared(copies):
+    """A step that was begun and left before anything was written has its pages back: a fork afterwards shares only held tokens,
+    and the page that the sequence writes into next is its own."""
+    c = _cache(3)
+    _step(c, [100, 0, 0])
+    c.begin([300, 0, 0])
+    c.abort()
+    assert len(c._held[0]) == 1 and c.free_pages == c.num_pages - 1
+    _check(c)
+    c.fork(0, [1])
+    _step(c, [200, 200, 0])
+    assert not set(c._held[0]) & set(c._held[1])
+    _check(c)
