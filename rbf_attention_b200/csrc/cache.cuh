@@ -10,7 +10,7 @@
 // Inside a slot the bytes stand in the order in which a warp's lanes take them as operands of mma.m16n8k16, 16 bytes per lane
 // and 512 per warp-wide load, so that loads are dense and nothing is transposed:
 //   keys:   chunk (dims / 64) * 2 + half, lane (g, t): row g of the half, dims 64 * (chunk / 2) + 16 t ... + 15.
-//           Row g of half h is token 4 (g / 2) + 2 h + g % 2, which makes the scores' accumulator rows the k index of ...
+//           Row g of half h is token 4 (g / 2) + 2 h + g % 2, so that the scores' rows are the values' k index as they are;
 //   values: chunk dims / 32, lane (g, t): four words, word i = dim 32 * chunk + 4 g + i of tokens 4 t ... 4 t + 3.
 #pragma once
 

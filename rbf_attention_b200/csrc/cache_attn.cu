@@ -3,20 +3,27 @@
 //
 // A step of generation reads the whole cache once and does two products per byte: the roofline is HBM, and what has to be cheap
 // is making 16-bit operands of the bytes. So the products are mma.m16n8k16 with the *cache* as the 16-row operand (tokens of a
-// block, then dims) and the queries - the new tokens of the query heads that share a key/value head - as the 8 columns: a byte
-// is widened once for 8 columns (32 where there are that many), and a lane's bytes lie in the cache in the order in which the
-// instruction wants them. A code becomes an exact fp16 number in one permute (the byte under 0x64 is 1024 + byte) and one
-// subtraction, for two values. Scales stay outside: a block's scores are multiplied by its key scale in fp32, its products with
-// the values by its value scale as they are added to the output. |k|^2 is the integer sum of the codes' squares.
+// block, then dims) and the queries - the new tokens of the query heads that share a key/value head - as the 8 columns, and a
+// lane's bytes lie in the cache in the order in which the instruction wants them. A code becomes an exact fp16 number in one
+// permute (the byte under 0x64 is 1024 + byte) and one subtraction, for two values. Scales stay outside: a block's scores are
+// multiplied by its key scale in fp32, its weights by its value scale (see Running::refer). |k|^2 is the integer sum of the
+// codes' squares.
 //   S^T (16 tokens x 8 columns) = K Q^T,  P^T by exponentials in fp32,  O^T (16 dims x 8 columns) += V^T P^T
 // Queries are multiplied by the power of two that brings their largest element to [1, 2) and rounded to fp16: exact for every
 // element within 2^-14 of the largest in 16-bit types, off by 2^-25 of it below. P is rounded to fp16 (2^-11 of it).
 // The block that is not complete yet is held in 16 bits and multiplied in its own type.
 //
-// Work is split evenly whatever the lengths: all (sequence, head, column tile) segments in a row, cut into units of one load,
-// are dealt to the warps of one wave in contiguous ranges. A warp works by itself - no barrier - with a running maximum (moved
-// only when a score exceeds it by 2^8, which keeps P below 2^8) and writes its segment's output, or its part (unnormalised
-// output, maximum, sum) where the segment is shared with other warps; a second kernel joins the parts in the order of the tokens.
+// Three kernels share this. Long sequences: work is split evenly whatever the lengths, all (sequence, head) segments in a row,
+// cut into units of one load, are dealt to the warps of one wave in contiguous ranges. A warp works by itself - no barrier - with
+// a running maximum (moved only when a score exceeds it by 2^8, which keeps P below 2^8) and writes its segment's output, or its
+// part (unnormalised output, maximum, sum) where the segment is shared with other warps; a second kernel joins the parts in the
+// order of the tokens. Joining a block's warps at the end of each segment instead, so that a segment has fewer parts, took 5 to 8
+// us longer: the warps wait for the slowest. Short sequences: a segment per block or cluster, one launch. More than 8 columns:
+// see cache_attn_rows_kernel.
+//
+// Bounds, one B200: 16 sequences of up to 32768 tokens, 8 key heads of 128, 32 query heads (549 MB): 100 us a call, the first
+// kernel 93 us at 5.9 TB/s = 90 % of the copy bandwidth. 64 sequences of up to 1028 tokens, 8 heads of 64 (35.5 MB, 5.4 us at
+// that bandwidth): 16.9 us, of which the chain of launch, lengths, pages, codes and join is the larger part.
 #include <cstdint>
 #include <cuda_runtime.h>
 
@@ -918,6 +925,11 @@ __global__ void __launch_bounds__(kWarps * 32, 16 / kWarps) cache_attn_short_ker
 // have other blocks of the unit, and the warps with the same rows join at the end of the segment.
 // The block that is not complete is brought to fp16 by powers of two, its largest key and value to [1, 2): exact but for
 // elements below 2^-14 of it (off by 2^-25 of it), and is then a block like the others.
+// What bounds it is the chain inside a unit - barrier, widening, barrier, products, exponentials, products - with 12 (8 at 128
+// dims) warps on an SM: the tensor pipe is busy for 19 to 28 % of the time, the issue slots for 33 to 44 %. 37 new tokens on 6
+// histories of up to 5003, 16 heads of 64: 39 us a call; 200 on 32 of up to 500: 76 (112 with the cache as the row operand and 32
+// columns a warp). Three blocks of 168 registers on an SM, or two of 255; four and three of them spill (50 and 93 us).
+// Three units under way instead of two, the incomplete block's rows among them: 41 and 81 us.
 constexpr int kRowWarps = 4;
 template <int P>
 struct RowTile {
@@ -1561,13 +1573,15 @@ cudaError_t attn_t(CacheAttnArgs a, int sms, cudaStream_t stream) {
   return join_t<kBf16, P, 8>(a, workers, stream);
 }
 
-// Blocks of a cluster that share a segment in the kernel for short sequences, 0: not that kernel. It is for one tile of columns
-// and page tables of up to kShort tokens - what the lengths are is known on the device alone. A block's warps have the units
-// of 256 tokens (128 at 128 columns) in flight at a time; more blocks where the segments leave SMs free and have units for them.
-constexpr int kShort = 4096;
+// Blocks of a cluster that share a segment in the kernel for short sequences, 0: not that kernel. What the lengths are is known on
+// the device alone, so the rule goes by the page table's width: up to 4096 tokens, up to 8192 where the segments are no more than
+// the SMs (columns: 8 at most). Calls with 8 heads of 64, this kernel and the dealing one: 1 x 1000 tokens 7.8 and 11.4 us,
+// 64 x 1028 16.8 and 24.3, 200 x 400 21.0 and 28.4, 4 x 4000 10.8 and 14.7, 16 x 4000 20.7 and 23.1, but 64 x 4000 43.6 and 41.7
+// (128 columns: 67.9 and 61.8). A segment has more blocks where that leaves none of the SMs without one and its units suffice.
+constexpr int kShort = 4096, kShortOfFew = 8192;
 int short_ranks(int64_t segments, int64_t columns, int max_pages, int sms) {
-  static_assert(kShort / kPageTokens <= 32, "a lane holds a page number");
-  if (columns > 8 || max_pages > kShort / kPageTokens) return 0;
+  static_assert(kShortOfFew / kPageTokens <= 32, "a lane holds a page number");
+  if (columns > 8 || max_pages > (segments <= sms ? kShortOfFew : kShort) / kPageTokens) return 0;
   const int64_t units = static_cast<int64_t>(max_pages) * kPageBlocks / 2;
   int ranks = 1;
   while (ranks < 8 && segments * ranks * 2 <= sms && units > kShortWarps * ranks) ranks *= 2;
@@ -1614,6 +1628,7 @@ cudaError_t attn_p(const CacheAttnArgs& a, int sms, cudaStream_t stream) {
   const int64_t segments = static_cast<int64_t>(a.B) * a.H;
   if (const int ranks = short_ranks(segments, static_cast<int64_t>(a.T) * a.G, a.max_pages, sms))
     return segments > 2 * sms ? short_t<kBf16, P, 4>(a, ranks, stream) : short_t<kBf16, P, kShortWarps>(a, ranks, stream);
+  // more than 8 columns: tiles of 64, or the one tile that holds them
   switch (cache_attn_columns(a.T, a.G)) {
     case 8: return attn_t<kBf16, P>(a, sms, stream);
     case 16: return rows_t<kBf16, P, 1>(a, sms, stream);

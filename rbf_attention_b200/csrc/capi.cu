@@ -946,6 +946,8 @@ int rbf_b200_cache_attention(const void* q, const int64_t* q_strides, const void
   if (B == 0 || T == 0) return RBF_B200_OK;
   if (static_cast<int64_t>(H) * G > 0x7fffffffll || static_cast<int64_t>(T) * G > 0x7fffff00ll)
     return fail(RBF_B200_ERR_BAD_ARGUMENT, "too many query heads or tokens");
+  if ((static_cast<double>(T) * G + 63) / 64 * H * (static_cast<double>(max_pages) * 4 + 1) >= 2147483647.0)
+    return fail(RBF_B200_ERR_BAD_ARGUMENT, "too many new tokens for one call on so many pages");
   if ((rc = check_rows("q", q, q_strides, B, H * G, T))) return rc;
   if (out == nullptr || reinterpret_cast<uintptr_t>(out) % 16 != 0)
     return fail(RBF_B200_ERR_BAD_LAYOUT, "out is NULL or not 16-byte aligned");

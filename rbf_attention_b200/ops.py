@@ -1293,7 +1293,8 @@ def cache_attention(q, pages, page_table, lengths, new_lengths=None, softmax: bo
     """RBF attention of the T newest tokens of every sequence, q (B, Hq, T, D), over a cache that holds them too (``cache_append``
     with the same arguments goes first): token i of sequence b sees tokens 0 to ``lengths[b] + i``, its own among them. Query head
     h reads key/value head ``h // (Hq // H)``. Returns (B, Hq, T, D); rows from ``new_lengths[b]`` on are zero. ``softmax=False``:
-    ``exp(-g |q - k|^2) V``. No backward: a q that requires a gradient is refused in grad mode."""
+    ``exp(-g |q - k|^2) V``. These are the newest tokens that the cache holds: of a shorter prefix it has whole blocks of 16 only,
+    the 16-bit rows are those of the last block. No backward: a q that requires a gradient is refused in grad mode."""
     if _needs_grad(q):
         raise RuntimeError("cache_attention has no backward: call it under torch.no_grad() or on detached tensors")
     if type(softmax) is bool and _direct(q, pages, page_table, lengths, new_lengths):

@@ -274,6 +274,23 @@ def test_blocks_that_are_not_finite(D):
     _check(got[1, 1, :2], want[1, 1, :2], FP16)
 
 
+@pytest.mark.parametrize("long", [False, True])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("T", [1, 6])
+def test_blocks_that_are_not_finite_and_few_rows(T, D, long):
+    pool = Pool(2, 2, D, 256, FP16, long=long)
+    k, v = _randn(2, 2, 60, D, dtype=FP16, seed=23), _randn(2, 2, 60, D, dtype=FP16, seed=24)
+    v[0, 0, 59 - T // 2, 3] = math.inf     # incomplete block, seen by the last rows only
+    v[1, 1, 37, 5] = math.nan              # a whole one, seen by all
+    pool.append(k, v)
+    q = _randn(2, 2, T, D, dtype=FP16, seed=25)
+    got = ops.cache_attention(q, pool.pages, pool.table, _ints([60 - T, 60 - T]))
+    first = T - 1 - T // 2
+    assert got[0, 1].isfinite().all() and got[1, 0].isfinite().all() and got[1, 1].isnan().all()
+    assert got[0, 0, :first].isfinite().all() and not got[0, 0, first:, 3].isfinite().any()
+    assert got[0, 0, first:, 4:].isfinite().all() and got[0, 0, first:, :3].isfinite().all()
+
+
 def test_extreme_queries_and_keys():
     """Large and tiny queries, keys far from every query, blocks of zeros."""
     pool = Pool(4, 1, 64, 512, BF16)
@@ -424,3 +441,105 @@ def test_offsets_beyond_32_bits():
     ops.cache_copy_pages(pages, [n - 1, n - 2], [n - 3, 0])
     assert torch.equal(ops.cache_attention(q, pages, _ints([[n - 3, 0]]), _ints([399])),
                        ops.cache_attention(q, small.pages, small.table, _ints([399])))
+
+
+def test_refusals():
+    pool = Pool(2, 4, 64, 256, BF16)
+    x = _randn(2, 4, 3, 64)
+    P, t, n = pool.pages, pool.table, pool.lengths
+    append = dict(pages=P, page_table=t, lengths=n, k=x, v=x, new_lengths=_ints([1, 2]))
+    attend = dict(q=x, pages=P, page_table=t, lengths=n, new_lengths=_ints([1, 2]), softmax=True)
+    read = dict(pages=P, page_table=t, lengths=n, head_dim=64, dtype=BF16, count=4, first=_ints([0, 0]))
+    shared = [{"pages": P[0]}, {"pages": P.float()}, {"pages": P[..., :-16]}, {"pages": P[:, :, ::2]}, {"pages": P.cpu()},
+              {"page_table": t.long()}, {"page_table": t[0]}, {"page_table": t.cpu()}, {"page_table": t[:1]}, {"lengths": n.long()},
+              {"lengths": n[:1]}, {"lengths": n.cpu()}, {"lengths": n[:, None]}]
+    bad = {ops.cache_append: (append, [{"k": x[:, :2]}, {"v": x[:, :, :2]}, {"k": x.half()}, {"k": x.float(), "v": x.float()}, {"k": x[0]},
+                                       {"k": x[..., :60], "v": x[..., :60]}, {"k": x.cpu()}, {"v": x.cpu()}, {"k": x[:1], "v": x[:1]},
+                                       {"new_lengths": _ints([1])}, {"new_lengths": torch.ones(2, device=DEV)},
+                                       {"new_lengths": _ints([1, 2]).cpu()}, {"k": _randn(2, 4, 3, 128), "v": _randn(2, 4, 3, 128)}]),
+           ops.cache_attention: (attend, [{"q": x[:, :3]}, {"q": x.float()}, {"q": x[0]}, {"q": x[..., :60]}, {"q": x.cpu()}, {"q": x[:1]},
+                                          {"new_lengths": _ints([1])}, {"q": _randn(2, 4, 3, 128)}]),
+           ops.cache_read: (read, [{"head_dim": 128}, {"head_dim": 0}, {"dtype": torch.float32}, {"count": -1}, {"first": _ints([0])},
+                                   {"first": torch.zeros(2, device=DEV)}])}
+    for call, (good, changes) in bad.items():
+        call(**good)
+        for change in changes + shared:
+            with pytest.raises((ValueError, RuntimeError)):
+                call(**{**good, **change})
+    grown = x.clone().requires_grad_(True)
+    with pytest.raises(RuntimeError, match="no backward"):
+        ops.cache_attention(**{**attend, "q": grown})
+    with torch.no_grad():
+        ops.cache_attention(**{**attend, "q": grown})
+    number = P.shape[0]
+    for src, dst in (([0], [number]), ([number], [0]), ([-1], [0]), ([0, 1], [2]), ([0, 1], [2, 2]), ([0, 1], [1, 2]), ([0], [0]),
+                     ([2**40], [0]), ([0.5], [1])):
+        with pytest.raises((ValueError, RuntimeError, TypeError)):
+            ops.cache_copy_pages(P, src, dst)
+    for pages in (P[0, 0], P.float(), P[:, :, ::2], P.cpu()):
+        with pytest.raises((ValueError, RuntimeError)):
+            ops.cache_copy_pages(pages, [0], [1])
+
+
+def test_through_the_registered_operators():
+    """Under a dispatch mode the operators run as registered: the same bytes and numbers."""
+    from torch.utils._python_dispatch import TorchDispatchMode
+
+    seen = []
+
+    class Mode(TorchDispatchMode):
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            seen.append(str(func))
+            return func(*args, **(kwargs or {}))
+
+    pools = [Pool(2, 2, 64, 256, FP16) for _ in range(2)]
+    k, v, q = (_randn(2, 2, 21, 64, dtype=FP16, seed=s) for s in (70, 71, 72))
+    outs = []
+    for i, p in enumerate(pools):
+        start = p.lengths.clone()
+
+        def run():
+            ops.cache_append(p.pages, p.table, start, k, v)
+            ops.cache_copy_pages(p.pages, [int(p.table[0, 0])], [max(set(range(5)) - set(p.table.flatten().tolist()))])
+            return ops.cache_attention(q, p.pages, p.table, start), *ops.cache_read(p.pages, p.table, start + 21, 64, FP16, 21)
+
+        if i:
+            with Mode():
+                outs.append(run())
+        else:
+            outs.append(run())
+    assert torch.equal(pools[0].pages, pools[1].pages) and all(torch.equal(a, b) for a, b in zip(*outs))
+    for name in ("cache_append", "cache_copy_pages", "cache_attention", "cache_read"):
+        assert any(name in s for s in seen)
+
+
+def test_inference_mode_and_versions():
+    p = Pool(1, 1, 64, 256, BF16)
+    x = _randn(1, 1, 4, 64)
+    version = p.pages._version
+    ops.cache_append(p.pages, p.table, p.lengths, x, x)
+    ops.cache_copy_pages(p.pages, [0], [1])
+    assert p.pages._version > version
+    with torch.inference_mode():
+        pages = torch.zeros_like(p.pages)
+        ops.cache_append(pages, p.table, p.lengths, x, x)
+        ops.cache_copy_pages(pages, [0], [1])
+        assert ops.cache_attention(x, pages, p.table, p.lengths).isfinite().all()
+
+
+def test_another_stream_than_the_default_and_reused_memory():
+    """Results of a side stream whose workspaces the allocator hands on at once."""
+    p = Pool(3, 4, 64, 8192, BF16)
+    k, v = _randn(3, 4, 5000, 64, seed=73), _randn(3, 4, 5000, 64, seed=74)
+    p.append(k, v)
+    q = _randn(3, 8, 2, 64, seed=75)
+    want = ops.cache_attention(q, p.pages, p.table, p.lengths - 2)
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        outs = []
+        for _ in range(30):
+            outs.append(ops.cache_attention(q, p.pages, p.table, p.lengths - 2))
+            torch.full((1 << 20,), float("nan"), device=DEV)
+    stream.synchronize()
+    assert all(torch.equal(x, want) for x in outs)

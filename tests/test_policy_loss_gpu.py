@@ -227,3 +227,60 @@ def test_captured_and_replayed():
                 to.copy_(value)
         graph.replay()
         assert all(torch.equal(a, b) for a, b in zip(outs, run()))
+
+
+def test_refusals():
+    x, t, old, ref, adv = _case(8, 20, torch.float32, seed=15)
+    good = dict(logits=x, tokens=t, old_log_probs=old, advantages=adv, ref_log_probs=ref, weights=old, clip_low=0.1, clip_high=0.1,
+                kl_weight=0.1)
+    ops.policy_loss(**good)
+    for change in ({"logits": x[0]}, {"logits": x.double()}, {"logits": x.cpu()}, {"logits": x[:4]}, {"logits": x[:, :0]},
+                   {"tokens": t.int()}, {"tokens": t[:, None]}, {"tokens": t.cpu()}, {"old_log_probs": old.half()},
+                   {"old_log_probs": old[:4]}, {"advantages": adv.double()}, {"advantages": adv.cpu()}, {"ref_log_probs": ref[:, None]},
+                   {"weights": old.bfloat16()}, {"clip_low": -0.1}, {"clip_high": float("nan")}, {"ref_log_probs": None}):
+        for leaf in (False, True):
+            call = {**good, **change}
+            if leaf:
+                call["logits"] = call["logits"].detach().requires_grad_(True)
+            with pytest.raises((ValueError, RuntimeError)):
+                ops.policy_loss(**call)
+    for change in ({"logits": x[0]}, {"tokens": t.int()}, {"tokens": t[:3]}, {"logits": x.double()}):
+        with pytest.raises((ValueError, RuntimeError)):
+            ops.token_log_probs(**{"logits": x, "tokens": t, **change})
+    leaf = x.clone().requires_grad_(True)
+    for name in ("old_log_probs", "advantages", "ref_log_probs", "weights"):
+        with pytest.raises(RuntimeError, match=f"{name}.*detach"):
+            ops.policy_loss(**{**good, "logits": leaf, name: good[name].clone().requires_grad_(True)})
+
+
+def test_two_losses_of_one_leaf_and_accumulated_gradients():
+    x, t, old, ref, adv = _case(40, 300, torch.bfloat16, seed=16)
+    leaf = x.clone().requires_grad_(True)
+    one, _ = ops.policy_loss(leaf, t, old, adv)
+    two, _ = ops.policy_loss(leaf, t, old, adv, ref_log_probs=ref, kl_weight=1.0)
+    (one * 0.5 + two * 0.25).backward()
+    want = 0.5 * _reference(x, t, old, None, adv, 0.2, 0.2, 0.0)[1] + 0.25 * _reference(x, t, old, ref, adv, 0.2, 0.2, 1.0)[1]
+    # two gradients rounded, scaled and rounded, added and rounded: five half steps at most, of numbers that may cancel by half
+    half = torch.finfo(x.dtype).eps / 2
+    assert (leaf.grad.double() - want).norm() <= 10 * half * want.norm()
+    again, _ = ops.policy_loss(leaf, t, old, adv)
+    before = leaf.grad.clone()
+    again.backward()
+    single = _reference(x, t, old, None, adv, 0.2, 0.2, 0.0)[1]
+    assert ((leaf.grad.double() - before.double()) - single).norm() <= 4 * half * (before.double().norm() + single.norm())
+
+
+def test_strided_rows_of_the_statistics():
+    x, t, old, ref, adv = _case(30, 100, torch.float16, seed=17)
+    wide = torch.stack([old, ref, adv], 1)
+    tokens = torch.stack([t, t + 1], 1)[:, 0]
+    a = ops.policy_loss(x, t, old, adv, ref_log_probs=ref, kl_weight=0.2)
+    b = ops.policy_loss(x, tokens, wide[:, 0], wide[:, 2], ref_log_probs=wide[:, 1], kl_weight=0.2)
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+
+
+@pytest.mark.parametrize("rows", [8192, 8193, 20000])
+def test_many_rows_are_counted_alike(rows):
+    """Few rows are counted by every block, many by a kernel of their own."""
+    x, t, old, ref, adv = _case(rows, 33, torch.float32, seed=18)
+    _check(x, t, old, ref, adv)
