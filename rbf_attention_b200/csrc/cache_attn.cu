@@ -1185,7 +1185,7 @@ __global__ void __launch_bounds__(kRowWarps * 32, RowTile<P>::kBlocks) cache_att
           }
         } else if (base < total) {
           const uint16_t* rest = reinterpret_cast<const uint16_t*>(page + kPageHeader + kPageBlocks * kSlot);
-          uint32_t k[2][P / 64][8], top = 0;
+          uint32_t k[2][P / 64][8], top = 0;       // largest magnitude of the finite ones: rows may see these alone
           float sq[2] = {0.f, 0.f};
 #pragma unroll
           for (int half = 0; half < 2; ++half) {
@@ -1202,7 +1202,8 @@ __global__ void __launch_bounds__(kRowWarps * 32, RowTile<P>::kBlocks) cache_att
               for (int i = 0; i < 8; ++i) {
                 const float2 f = unpack2<kBf16>(k[half][d][i]);
                 sq[half] = fmaf(f.x, f.x, fmaf(f.y, f.y, sq[half]));
-                top = max(top, max(__float_as_uint(f.x) & 0x7fffffffu, __float_as_uint(f.y) & 0x7fffffffu));
+                const uint32_t b0 = __float_as_uint(f.x) & 0x7fffffffu, b1 = __float_as_uint(f.y) & 0x7fffffffu;
+                top = max(top, max(b0 < 0x7f800000u ? b0 : 0u, b1 < 0x7f800000u ? b1 : 0u));
               }
             }
             sq[half] += __shfl_xor_sync(0xffffffffu, sq[half], 1);

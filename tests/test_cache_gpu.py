@@ -291,6 +291,28 @@ def test_blocks_that_are_not_finite_and_few_rows(T, D, long):
     assert got[0, 0, first:, 4:].isfinite().all() and got[0, 0, first:, :3].isfinite().all()
 
 
+@pytest.mark.parametrize("bad", [math.inf, math.nan])
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("T", [6, 12, 30, 50])
+def test_a_key_that_is_not_finite_in_the_incomplete_block(T, D, dtype, bad):
+    """Rows that do not see it have what they had without it."""
+    pool = Pool(1, 2, D, 256, dtype)
+    k, v = _randn(1, 2, 60, D, dtype=dtype, seed=27), _randn(1, 2, 60, D, dtype=dtype, seed=28)
+    k[0, 1, 57, 5] = bad
+    pool.append(k, v)
+    q = _randn(1, 2, T, D, dtype=dtype, seed=29)
+    got = ops.cache_attention(q, pool.pages, pool.table, _ints([60 - T]))
+    clean = Pool(1, 2, D, 256, dtype)
+    k[0, 1, 57, 5] = 0
+    clean.append(k, v)
+    want = _reference(clean, q, [60 - T], [T], True)
+    _check(got[0, 0], want[0, 0], dtype)
+    _check(got[0, 1, :-3], want[0, 1, :-3], dtype)
+    if math.isnan(bad):
+        assert got[0, 1, -3:].isnan().all()
+
+
 def test_extreme_queries_and_keys():
     """Large and tiny queries, keys far from every query, blocks of zeros."""
     pool = Pool(4, 1, 64, 512, BF16)
