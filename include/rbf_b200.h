@@ -283,7 +283,8 @@ int rbf_b200_cache_read(const void* pages, const int* page_table, const int* len
                         int B, int H, int D, int count, int max_pages, int num_pages, int dtype, void* stream);
 
 /* pages[l][dst[i]] = pages[l][src[i]] for all i and all `layers` pools of num_pages x page_bytes bytes behind one another;
- * page_bytes (all heads) is a multiple of 16. src and dst are host arrays. No page may be a destination twice, nor a source and a destination. */
+ * page_bytes (all heads) is a multiple of 16. src and dst are host arrays. No page may be a destination twice, nor a source
+ * and a destination. */
 int rbf_b200_cache_copy_pages(void* pages, int layers, int num_pages, size_t page_bytes, const int* src, const int* dst,
                               int count, void* stream);
 
@@ -308,8 +309,8 @@ int rbf_b200_token_log_probs(const void* logits, const int64_t* tokens, float* l
  *   loss = sum over rows of w * (kl_weight * (exp(ref - lp) - (ref - lp) - 1) - min(r A, clip(r, 1 - clip_low, 1 + clip_high) A))
  * with w = weights[r], or 1 / number of counting rows where weights is NULL (no such row: NaN); ref_log_probs NULL: no KL term.
  * Writes lp (as above), the loss, and - unless dlogits is NULL - the gradient with respect to the logits (row pitch ld_out,
- * in their dtype, zero for rows that do not count). dlogits needs the alignment of logits modulo 16 bytes in every row. Everything is
- * summed in a fixed order. The workspace is 8-byte aligned. */
+ * in their dtype, zero for rows that do not count). dlogits needs the alignment of logits modulo 16 bytes in every row.
+ * Everything is summed in a fixed order. The workspace is 8-byte aligned. */
 size_t rbf_b200_policy_loss_workspace_bytes(void);
 int rbf_b200_policy_loss(const void* logits, const int64_t* tokens, const float* old_log_probs, const float* advantages,
                          const float* ref_log_probs, const float* weights, float* loss, float* log_probs, void* dlogits,

@@ -35,9 +35,9 @@
 namespace rbf {
 namespace {
 
-// Up to 8 columns: warps of a block (one per SM), blocks of a unit, and units of a warp that are loaded ahead, the current one among
-// them: what registers (65536) and shared memory (227 KB) hold with 8 KB units. 16 x 32768 tokens of 128 columns took 115 us with
-// 8 warps and three units, 104 so; 8 x 16384 of 64 columns 36 and 33.5 us, with 16 warps and three units of 4 KB 35.5.
+// Up to 8 columns: warps of a block (one per SM), blocks of a unit, and units of a warp that are loaded ahead, the current one
+// among them: what registers (65536) and shared memory (227 KB) hold with 8 KB units. 16 x 32768 tokens of 128 columns took 115
+// us with 8 warps and three units, 104 so; 8 x 16384 of 64 columns 36 and 33.5 us, with 16 warps and three units of 4 KB 35.5.
 constexpr int kWarpsOf8 = 12, kStagesOf8 = 2;
 template <int P> constexpr int kUnitBlocks = 256 / P;
 constexpr int kShortWarps = 8;                     // of the kernel for short sequences, 4 where there are many
@@ -225,7 +225,7 @@ struct Running {
   __device__ __forceinline__ void refer(float scale) {
     const float now = scale * power2(-unit);
     if (now < 128.f && (now >= 0.015625f || scale == 0.f)) return;
-    int to = static_cast<int>(__float_as_uint(scale) >> 23) - 127 - 6;
+    int to = max(static_cast<int>(__float_as_uint(scale) >> 23) - 127 - 6, -126);
     float top = 0.f;
 #pragma unroll
     for (int j = 0; j < P / 16; ++j)
@@ -302,7 +302,8 @@ struct Running {
   }
 };
 
-// Operand words of query column c (lane g's of a tile) as they are in memory: k step i has dims 64 (i / 4) + 16 t + 4 (i % 4) ... + 3
+// Operand words of query column c (lane g's of a tile) as they are in memory: k step i has dims 64 (i / 4) + 16 t + 4 (i % 4)
+// to + 3
 template <int P>
 __device__ __forceinline__ void load_q(const CacheAttnArgs& a, int b, int h, int c, int t, uint32_t (&w)[P / 16][2]) {
   const bool real = c < a.T * a.G;
@@ -325,8 +326,8 @@ __device__ __forceinline__ void load_q(const CacheAttnArgs& a, int b, int h, int
 // The query columns of a segment: operands, their scales, and how far each column sees
 template <bool kBf16, int P>
 struct Queries {
-  uint32_t w[P / 16][2];                       // fp16, scaled
-  float mul[2], sq[2];                     // of columns 2t, 2t + 1: what the scores are multiplied by, g log2(e) |q|^2
+  uint32_t w[P / 16][2];                           // fp16, scaled
+  float mul[2], sq[2];                             // of columns 2t, 2t + 1: what the scores are multiplied by, g log2(e) |q|^2
   int limit[2];                                // last token that the column sees
   int first_limit, last_limit;                     // every column of the tile sees at least, none sees more
   int b, h, total;
@@ -491,7 +492,8 @@ __device__ __forceinline__ void codes_blocks(const CacheAttnArgs& a, const Queri
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
         const uint32_t r0 = half ? w.z : w.x, r1 = half ? w.w : w.y;
-        const uint32_t A[4] = {codes_lo(r0, q.exponents), codes_lo(r1, q.exponents), codes_hi(r0, q.exponents), codes_hi(r1, q.exponents)};
+        const uint32_t A[4] = {codes_lo(r0, q.exponents), codes_lo(r1, q.exponents), codes_hi(r0, q.exponents),
+                               codes_hi(r1, q.exponents)};
         mma16816<false>(run.o[2 * i + half], A, p[0], p[1]);
       }
     }
@@ -552,7 +554,7 @@ __device__ __forceinline__ void rest_unit(const CacheAttnArgs& a, const Queries<
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const uint32_t A[4] = {r[0][2 * i], r[1][2 * i], r[0][2 * i + 1], r[1][2 * i + 1]};
-        mma16816<kBf16>(s[0], A, qt[d * 4 + i][0], qt[d * 4 + i][1]);
+      mma16816<kBf16>(s[0], A, qt[d * 4 + i][0], qt[d * 4 + i][1]);
     }
   }
 #pragma unroll
@@ -590,7 +592,7 @@ __device__ __forceinline__ void rest_unit(const CacheAttnArgs& a, const Queries<
     for (int j = 0; j < J; ++j) {
       uint32_t A[4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {                // row g: dim 4 g + 2 (j % 2), row g + 8: the next; k 2t.. : tokens 0, 1 then 2, 3
+      for (int e = 0; e < 4; ++e) {                // row g: dim 4 g + 2 (j % 2), row g + 8: the next; k: tokens 0, 1 then 2, 3
         uint32_t lo = j % 2 ? x[j / 2][e / 2 * 2].y : x[j / 2][e / 2 * 2].x;
         uint32_t hi = j % 2 ? x[j / 2][e / 2 * 2 + 1].y : x[j / 2][e / 2 * 2 + 1].x;
         if (slow) {
@@ -723,7 +725,8 @@ __global__ void __launch_bounds__(kWarpsOf8 * 32) cache_attn_kernel(const CacheA
     float* part = part_of<P>(a, 8, 2 * self + (u0 == 0));
     if (u0 == 0 && lane == 0 && (by_segment || !complete)) {
       const int last = static_cast<int>(min(deal.worker(at + units.count - 1), workers - 1));
-      notes[by_segment ? static_cast<int64_t>(b) * segments + h : self] = {complete ? -1 : b, h, static_cast<int>(self), last, units.fresh, {}};
+      Note& note = notes[by_segment ? static_cast<int64_t>(b) * segments + h : self];
+      note = {complete ? -1 : b, h, static_cast<int>(self), last, units.fresh, {}};
     }
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
@@ -782,7 +785,7 @@ __global__ void __launch_bounds__(kWarps * 32, 16 / kWarps) cache_attn_short_ker
   constexpr int UB = 2, kRing = 2;
   using T = Tile<P, UB>;
   constexpr int kBytes = cache_page_bytes(P);
-  static_assert(kRing * T::kStage >= (8 * P + 16) * 4, "a warp's part takes the place of its ring");
+  static_assert(kRing * T::kStage >= (8 * P + 48) * 4, "a warp's part, and the block's, take the place of a ring");
   extern __shared__ __align__(128) uint8_t smem[];
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, warp = threadIdx.x >> 5;
   uint8_t* ring = smem + warp * (kRing * T::kStage);
@@ -911,7 +914,8 @@ __global__ void __launch_bounds__(kWarps * 32, 16 / kWarps) cache_attn_short_ker
     }
   }
   __syncwarp();
-  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");   // blocks stay until they have been read
+  // blocks stay until they have been read
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
@@ -972,7 +976,7 @@ struct RowState {
   __device__ __forceinline__ void refer(float scale) {
     const float now = scale * power2(-unit);
     if (now < 128.f && (now >= 0.015625f || scale == 0.f)) return;
-    int to = static_cast<int>(__float_as_uint(scale) >> 23) - 127 - 6;
+    int to = max(static_cast<int>(__float_as_uint(scale) >> 23) - 127 - 6, -126);
     float top = 0.f;
 #pragma unroll
     for (int c = 0; c < P / 32; ++c)
@@ -1015,7 +1019,8 @@ __global__ void __launch_bounds__(kRowWarps * 32, RowTile<P>::kBlocks) cache_att
   constexpr int KC = P / 32, UB = kRowWarps, kSlot = cache_slot_bytes(P), kBytes = cache_page_bytes(P);
   constexpr int kRows = 16 * RW, kUnitTokens = UB * kBlockTokens;
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ float s_bias[UB][kBlockTokens], s_key[UB], s_value[UB];
+  __shared__ alignas(16) float s_bias[UB][kBlockTokens];
+  __shared__ float s_key[UB], s_value[UB];
   __shared__ int s_there;                          // blocks of the unit that are there
   __shared__ bool s_odd[UB];                       // the incomplete block has a value that is not finite
   uint8_t* const wide = smem + 2 * T::kStage;
@@ -1073,8 +1078,9 @@ __global__ void __launch_bounds__(kRowWarps * 32, RowTile<P>::kBlocks) cache_att
   const uint8_t *page = nullptr, *next_page = nullptr;                     // of the unit at hand and of the next
   auto fetch = [&](int slot) {
     page = next_page;
-    next_page = next_id < 0 || next_id >= a.num_pages ? nullptr : a.pages + (static_cast<int64_t>(next_id) * a.H + next_h) * kBytes;
-    if (next_page != nullptr) {
+    next_page = nullptr;
+    if (next_id >= 0 && next_id < a.num_pages) {
+      next_page = a.pages + (static_cast<int64_t>(next_id) * a.H + next_h) * kBytes;
       const uint8_t* src = next_page + kPageHeader + (next_what & 0xff) * kSlot + threadIdx.x * 16;
       const uint32_t to = smem_u32(smem + slot * T::kStage);
       const int bytes = (next_what >> 8) * kSlot;
@@ -1082,7 +1088,8 @@ __global__ void __launch_bounds__(kRowWarps * 32, RowTile<P>::kBlocks) cache_att
       for (int i = 0; i < T::kRaw / (kRowWarps * 512); ++i)
         if (i * (kRowWarps * 512) + static_cast<int>(threadIdx.x) * 16 < bytes)
           copy16(to + i * (kRowWarps * 512) + threadIdx.x * 16, src + i * (kRowWarps * 512));
-      if (threadIdx.x < 2 && bytes > 0) copy16(to + T::kRaw + threadIdx.x * 16, next_page + (next_what & 0xff) * 8 + threadIdx.x * 16);
+      if (threadIdx.x < 2 && bytes > 0)
+        copy16(to + T::kRaw + threadIdx.x * 16, next_page + (next_what & 0xff) * 8 + threadIdx.x * 16);
     }
     copies_close();
     look_up();
@@ -1176,7 +1183,8 @@ __global__ void __launch_bounds__(kRowWarps * 32, RowTile<P>::kBlocks) cache_att
           for (int half = 0; half < 2; ++half) {
             sq[half] += __shfl_xor_sync(0xffffffffu, sq[half], 1);
             sq[half] += __shfl_xor_sync(0xffffffffu, sq[half], 2);
-            if (t == 0) s_bias[warp][4 * (g >> 1) + 2 * half + (g & 1)] = a.scale * scale.x * scale.x * static_cast<float>(sq[half]);
+            if (t == 0)
+              s_bias[warp][4 * (g >> 1) + 2 * half + (g & 1)] = a.scale * scale.x * scale.x * static_cast<float>(sq[half]);
           }
           if (lane == 0) {
             s_key[warp] = scale.x;
@@ -1230,7 +1238,8 @@ __global__ void __launch_bounds__(kRowWarps * 32, RowTile<P>::kBlocks) cache_att
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
               x[i][r] = make_uint2(0, 0);
-              if (base + 4 * t + r < total) x[i][r] = *reinterpret_cast<const uint2*>(rest + kSlot / 2 + (4 * t + r) * P + 32 * i + 4 * g);
+              if (base + 4 * t + r < total)
+                x[i][r] = *reinterpret_cast<const uint2*>(rest + kSlot / 2 + (4 * t + r) * P + 32 * i + 4 * g);
 #pragma unroll
               for (int e = 0; e < 2; ++e) {
                 const float2 f = unpack2<kBf16>(e ? x[i][r].y : x[i][r].x);
@@ -1252,8 +1261,10 @@ __global__ void __launch_bounds__(kRowWarps * 32, RowTile<P>::kBlocks) cache_att
               const uint32_t x0 = e ? x[i][0].y : x[i][0].x, x1 = e ? x[i][1].y : x[i][1].x;
               const uint32_t x2 = e ? x[i][2].y : x[i][2].x, x3 = e ? x[i][3].y : x[i][3].x;
               values[i * 64 + e * 32] =
-                  make_uint4(rescale2<kBf16>(__byte_perm(x0, x1, 0x5410), down), rescale2<kBf16>(__byte_perm(x2, x3, 0x5410), down),
-                             rescale2<kBf16>(__byte_perm(x0, x1, 0x7632), down), rescale2<kBf16>(__byte_perm(x2, x3, 0x7632), down));
+                  make_uint4(rescale2<kBf16>(__byte_perm(x0, x1, 0x5410), down),
+                             rescale2<kBf16>(__byte_perm(x2, x3, 0x5410), down),
+                             rescale2<kBf16>(__byte_perm(x0, x1, 0x7632), down),
+                             rescale2<kBf16>(__byte_perm(x2, x3, 0x7632), down));
             }
         }
       }
@@ -1265,129 +1276,131 @@ __global__ void __launch_bounds__(kRowWarps * 32, RowTile<P>::kBlocks) cache_att
 
       // Whole units whose tokens all rows see, with finite scales, are most: without a branch in them.
       auto work = [&](auto plain) {
-      constexpr bool kPlain = decltype(plain)::value;
-      // ---- scores of this warp's blocks
-      float s[RW][2][4];
+        constexpr bool kPlain = decltype(plain)::value;
+        // ---- scores of this warp's blocks
+        float s[RW][2][4];
 #pragma unroll
-      for (int j = 0; j < RW; ++j) {
-        const int k = group * RW + j;
-        if (!kPlain && k >= there) {
+        for (int j = 0; j < RW; ++j) {
+          const int k = group * RW + j;
+          if (!kPlain && k >= there) {
 #pragma unroll
-          for (int half = 0; half < 2; ++half)
+            for (int half = 0; half < 2; ++half)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) s[j][half][e] = -INFINITY;
-          continue;
-        }
-        const uint4* keys = reinterpret_cast<const uint4*>(wide) + k * (2 * P / 64) * 64 + lane;
-        const float key = s_key[k], mul0 = mul[0] * key, mul1 = mul[1] * key;
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          float(&acc)[4] = s[j][half];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) acc[e] = 0.f;
-#pragma unroll
-          for (int d = 0; d < P / 64; ++d) {
-            const uint4 x = keys[(half * (P / 64) + d) * 64], y = keys[(half * (P / 64) + d) * 64 + 32];
-            mma16816<false>(acc, q[d * 4], x.x, x.y);
-            mma16816<false>(acc, q[d * 4 + 1], x.z, x.w);
-            mma16816<false>(acc, q[d * 4 + 2], y.x, y.y);
-            mma16816<false>(acc, q[d * 4 + 3], y.z, y.w);
+              for (int e = 0; e < 4; ++e) s[j][half][e] = -INFINITY;
+            continue;
           }
-          const float2 bias = *reinterpret_cast<const float2*>(&s_bias[k][4 * t + 2 * half]);
-          acc[0] = fmaf(acc[0], mul0, -bias.x);
-          acc[1] = fmaf(acc[1], mul0, -bias.y);
-          acc[2] = fmaf(acc[2], mul1, -bias.x);
-          acc[3] = fmaf(acc[3], mul1, -bias.y);
-          if (!kPlain) {
-            const int tok = begin + k * kBlockTokens + 4 * t + 2 * half;
+          const uint4* keys = reinterpret_cast<const uint4*>(wide) + k * (2 * P / 64) * 64 + lane;
+          const float key = s_key[k], mul0 = mul[0] * key, mul1 = mul[1] * key;
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-              if (tok + e % 2 > limit[e / 2] || tok + e % 2 >= total) acc[e] = -INFINITY;
+          for (int half = 0; half < 2; ++half) {
+            float(&acc)[4] = s[j][half];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[e] = 0.f;
+#pragma unroll
+            for (int d = 0; d < P / 64; ++d) {
+              const uint4 x = keys[(half * (P / 64) + d) * 64], y = keys[(half * (P / 64) + d) * 64 + 32];
+              mma16816<false>(acc, q[d * 4], x.x, x.y);
+              mma16816<false>(acc, q[d * 4 + 1], x.z, x.w);
+              mma16816<false>(acc, q[d * 4 + 2], y.x, y.y);
+              mma16816<false>(acc, q[d * 4 + 3], y.z, y.w);
+            }
+            const float2 bias = *reinterpret_cast<const float2*>(&s_bias[k][4 * t + 2 * half]);
+            acc[0] = fmaf(acc[0], mul0, -bias.x);
+            acc[1] = fmaf(acc[1], mul0, -bias.y);
+            acc[2] = fmaf(acc[2], mul1, -bias.x);
+            acc[3] = fmaf(acc[3], mul1, -bias.y);
+            if (!kPlain) {
+              const int tok = begin + k * kBlockTokens + 4 * t + 2 * half;
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                if (tok + e % 2 > limit[e / 2] || tok + e % 2 >= total) acc[e] = -INFINITY;
+            }
           }
         }
-      }
-      // ---- weights, as Running::weigh
-      float top[2] = {-INFINITY, -INFINITY};
+        // ---- weights, as Running::weigh
+        float top[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-      for (int j = 0; j < RW; ++j)
+        for (int j = 0; j < RW; ++j)
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          top[0] = fmaxf(top[0], fmaxf(s[j][half][0], s[j][half][1]));
-          top[1] = fmaxf(top[1], fmaxf(s[j][half][2], s[j][half][3]));
-        }
-      if (__any_sync(0xffffffffu, top[0] > run.m[0] + kSlack || top[1] > run.m[1] + kSlack)) {
-        float f[2];
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          float x = fmaxf(top[e], run.m[e]);
-          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
-          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
-          f[e] = run.m[e] == x ? 1.f : attn_ex2(run.m[e] - x);
-          run.m[e] = x;
-          run.l[e] *= f[e];
-        }
-        run.times(f[0], f[1]);
-      }
-      const float ref[2] = {run.m[0] == -INFINITY ? 0.f : run.m[0], run.m[1] == -INFINITY ? 0.f : run.m[1]};
-      float most = 0.f;
-#pragma unroll
-      for (int j = 0; j < RW; ++j)
-        if (kPlain || (group * RW + j < there && s_value[group * RW + j] < INFINITY)) most = fmaxf(most, s_value[group * RW + j]);
-      run.refer(most);
-      const float down = power2(-run.unit);
-#pragma unroll
-      for (int j = 0; j < RW; ++j) {
-        const int k = group * RW + j;
-        if (!kPlain && k >= there) continue;
-        const float value = s_value[k], by = value * down;
-        const bool finite = fabsf(value) < INFINITY;
-        uint32_t p[4];
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) s[j][half][e] = attn_ex2(s[j][half][e] - ref[e / 2]);
-          run.l[0] += s[j][half][0] + s[j][half][1];
-          run.l[1] += s[j][half][2] + s[j][half][3];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            s[j][half][e] *= by;
-            if (!kPlain && !finite) s[j][half][e] = begin + k * kBlockTokens <= limit[e / 2] ? __int_as_float(0x7fc00000) : 0.f;
+          for (int half = 0; half < 2; ++half) {
+            top[0] = fmaxf(top[0], fmaxf(s[j][half][0], s[j][half][1]));
+            top[1] = fmaxf(top[1], fmaxf(s[j][half][2], s[j][half][3]));
           }
-          p[2 * half] = pack2<false>(s[j][half][0], s[j][half][1]);
-          p[2 * half + 1] = pack2<false>(s[j][half][2], s[j][half][3]);
-        }
-        const uint4* values = reinterpret_cast<const uint4*>(wide + T::kRaw) + k * KC * 64 + lane;
-        if (kPlain || !s_odd[k]) {
+        if (__any_sync(0xffffffffu, top[0] > run.m[0] + kSlack || top[1] > run.m[1] + kSlack)) {
+          float f[2];
 #pragma unroll
-          for (int c = 0; c < KC; ++c) {
-            const uint4 x = values[c * 64], y = values[c * 64 + 32];
-            mma16816<false>(run.o[c][0], p, x.x, x.y);
-            mma16816<false>(run.o[c][1], p, x.z, x.w);
-            mma16816<false>(run.o[c][2], p, y.x, y.y);
-            mma16816<false>(run.o[c][3], p, y.z, y.w);
+          for (int e = 0; e < 2; ++e) {
+            float x = fmaxf(top[e], run.m[e]);
+            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
+            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
+            f[e] = run.m[e] == x ? 1.f : attn_ex2(run.m[e] - x);
+            run.m[e] = x;
+            run.l[e] *= f[e];
           }
-        } else {                                   // token by token: 0 * inf must not reach rows that do not see it
-#pragma unroll 1
-          for (int only = 0; only < kBlockTokens; ++only) {
-            const uint32_t mask = only % 2 ? 0xffff0000u : 0x0000ffffu;
-            const uint32_t lo = t == only / 4 && only % 4 < 2 ? mask : 0u, hi = t == only / 4 && only % 4 >= 2 ? mask : 0u;
-            const int token = begin + k * kBlockTokens + only;
+          run.times(f[0], f[1]);
+        }
+        const float ref[2] = {run.m[0] == -INFINITY ? 0.f : run.m[0], run.m[1] == -INFINITY ? 0.f : run.m[1]};
+        float most = 0.f;
+#pragma unroll
+        for (int j = 0; j < RW; ++j)
+          if (kPlain || (group * RW + j < there && s_value[group * RW + j] < INFINITY))
+            most = fmaxf(most, s_value[group * RW + j]);
+        run.refer(most);
+        const float down = power2(-run.unit);
+#pragma unroll
+        for (int j = 0; j < RW; ++j) {
+          const int k = group * RW + j;
+          if (!kPlain && k >= there) continue;
+          const float value = s_value[k], by = value * down;
+          const bool finite = fabsf(value) < INFINITY;
+          uint32_t p[4];
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[j][half][e] = attn_ex2(s[j][half][e] - ref[e / 2]);
+            run.l[0] += s[j][half][0] + s[j][half][1];
+            run.l[1] += s[j][half][2] + s[j][half][3];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              s[j][half][e] *= by;
+              if (!kPlain && !finite)
+                s[j][half][e] = begin + k * kBlockTokens <= limit[e / 2] ? __int_as_float(0x7fc00000) : 0.f;
+            }
+            p[2 * half] = pack2<false>(s[j][half][0], s[j][half][1]);
+            p[2 * half + 1] = pack2<false>(s[j][half][2], s[j][half][3]);
+          }
+          const uint4* values = reinterpret_cast<const uint4*>(wide + T::kRaw) + k * KC * 64 + lane;
+          if (kPlain || !s_odd[k]) {
 #pragma unroll
             for (int c = 0; c < KC; ++c) {
               const uint4 x = values[c * 64], y = values[c * 64 + 32];
-              const uint32_t w[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+              mma16816<false>(run.o[c][0], p, x.x, x.y);
+              mma16816<false>(run.o[c][1], p, x.z, x.w);
+              mma16816<false>(run.o[c][2], p, y.x, y.y);
+              mma16816<false>(run.o[c][3], p, y.z, y.w);
+            }
+          } else {                                   // token by token: 0 * inf must not reach rows that do not see it
+#pragma unroll 1
+            for (int only = 0; only < kBlockTokens; ++only) {
+              const uint32_t mask = only % 2 ? 0xffff0000u : 0x0000ffffu;
+              const uint32_t lo = t == only / 4 && only % 4 < 2 ? mask : 0u, hi = t == only / 4 && only % 4 >= 2 ? mask : 0u;
+              const int token = begin + k * kBlockTokens + only;
 #pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                float acc[4] = {0.f, 0.f, 0.f, 0.f};
-                mma16816<false>(acc, p, w[2 * i] & lo, w[2 * i + 1] & hi);
+              for (int c = 0; c < KC; ++c) {
+                const uint4 x = values[c * 64], y = values[c * 64 + 32];
+                const uint32_t w[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
 #pragma unroll
-                for (int e = 0; e < 4; ++e)
-                  if (token <= limit[e / 2]) run.o[c][i][e] += acc[e];
+                for (int i = 0; i < 4; ++i) {
+                  float acc[4] = {0.f, 0.f, 0.f, 0.f};
+                  mma16816<false>(acc, p, w[2 * i] & lo, w[2 * i + 1] & hi);
+#pragma unroll
+                  for (int e = 0; e < 4; ++e)
+                    if (token <= limit[e / 2]) run.o[c][i][e] += acc[e];
+                }
               }
             }
           }
         }
-      }
       };
       const bool whole = begin + kUnitTokens - 1 <= first_limit && begin + kUnitTokens <= total;
       bool finite_values = true;
@@ -1415,7 +1428,8 @@ __global__ void __launch_bounds__(kRowWarps * 32, RowTile<P>::kBlocks) cache_att
 #pragma unroll
         for (int c = 0; c < KC; ++c)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) to[(c * 4 + i) * 32] = make_float4(run.o[c][i][0], run.o[c][i][1], run.o[c][i][2], run.o[c][i][3]);
+          for (int i = 0; i < 4; ++i)
+            to[(c * 4 + i) * 32] = make_float4(run.o[c][i][0], run.o[c][i][1], run.o[c][i][2], run.o[c][i][3]);
         to[KC * 4 * 32] = make_float4(run.m[0], run.m[1], run.l[0], run.l[1]);
       }
       __syncthreads();
@@ -1469,7 +1483,8 @@ __global__ void __launch_bounds__(kRowWarps * 32, RowTile<P>::kBlocks) cache_att
           if (complete) {
             if (d >= a.D) continue;
             uint4 y = make_uint4(pack2<kBf16>(o[0][2 * e] * f, o[1][2 * e] * f), pack2<kBf16>(o[2][2 * e] * f, o[3][2 * e] * f),
-                                 pack2<kBf16>(o[0][2 * e + 1] * f, o[1][2 * e + 1] * f), pack2<kBf16>(o[2][2 * e + 1] * f, o[3][2 * e + 1] * f));
+                                 pack2<kBf16>(o[0][2 * e + 1] * f, o[1][2 * e + 1] * f),
+                             pack2<kBf16>(o[2][2 * e + 1] * f, o[3][2 * e + 1] * f));
             if (none) y = make_uint4(0, 0, 0, 0);
             *reinterpret_cast<uint4*>(out + d) = y;
           } else {
@@ -1650,7 +1665,8 @@ size_t cache_attn_workspace_bytes(int B, int H, int G, int T, int D, int max_pag
   const int P = cache_columns(D);
   if (short_ranks(static_cast<int64_t>(B) * H, static_cast<int64_t>(T) * G, max_pages, sms)) return 0;
   const int tile = cache_attn_columns(T, G), width = static_cast<int64_t>(T) * G < tile ? T * G : tile;
-  const int64_t workers = static_cast<int64_t>(sms) * (tile == 8 ? kWarpsOf8 : P == 64 ? RowTile<64>::kBlocks : RowTile<128>::kBlocks);
+  const int each = tile == 8 ? kWarpsOf8 : P == 64 ? RowTile<64>::kBlocks : RowTile<128>::kBlocks;
+  const int64_t workers = static_cast<int64_t>(sms) * each;
   return static_cast<size_t>(workers) * (sizeof(Note) + 2 * width * part_pitch(P) * sizeof(float));
 }
 

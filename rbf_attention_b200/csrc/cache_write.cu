@@ -15,7 +15,7 @@ constexpr int kWriteThreads = 128;                 // four warps, a block of 16 
 // (spilling 80 to 100 bytes) and of 64: 162 and 90 us so, 209 and 103 with four blocks, 254 and 100 with 10 and 16.
 template <int P> constexpr int kWriteBlocks = P == 64 ? 10 : 8;
 
-// Two 16-bit numbers as fp32
+// Eight 16-bit numbers as fp32, and back
 template <bool kBf16>
 __device__ __forceinline__ void widen8(const uint4& raw, float (&x)[8]) {
   const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
@@ -25,6 +25,11 @@ __device__ __forceinline__ void widen8(const uint4& raw, float (&x)[8]) {
     x[2 * i] = f.x;
     x[2 * i + 1] = f.y;
   }
+}
+
+template <bool kBf16>
+__device__ __forceinline__ uint4 narrow8(const float (&x)[8]) {
+  return make_uint4(pack2<kBf16>(x[0], x[1]), pack2<kBf16>(x[2], x[3]), pack2<kBf16>(x[4], x[5]), pack2<kBf16>(x[6], x[7]));
 }
 
 // code + 128 of four values: nearest integers of x * (127 / amax), ties to even, both steps in fp32 (|code| <= 127: x / amax is
@@ -64,7 +69,8 @@ __global__ void __launch_bounds__(kWriteThreads, kWriteBlocks<P>) cache_append_k
 
   const int block = first + j;
   if ((block + 1) * static_cast<int64_t>(kBlockTokens) <= end) {
-    uint8_t* page = const_cast<uint8_t*>(cache_page(a.pages, a.table, b, a.max_pages, a.num_pages, a.H, h, kBytes, block * kBlockTokens));
+    uint8_t* page = const_cast<uint8_t*>(
+        cache_page(a.pages, a.table, b, a.max_pages, a.num_pages, a.H, h, kBytes, block * kBlockTokens));
     if (page != nullptr) {
       const uint8_t* tail = page + kPageHeader + (kPageBlocks + kv) * kSlot;
       // lane (r, c): tokens r, r + kRows, ... of 8-column group c
@@ -181,8 +187,8 @@ __global__ void __launch_bounds__(256) cache_read_kernel(const CacheReadArgs a) 
             vx[4 * e + i] = static_cast<float>(static_cast<int>(words[i] >> (8 * r) & 0xffu) - 128) * scale.y;
           }
         }
-        k[r] = make_uint4(pack2<kBf16>(kx[0], kx[1]), pack2<kBf16>(kx[2], kx[3]), pack2<kBf16>(kx[4], kx[5]), pack2<kBf16>(kx[6], kx[7]));
-        v[r] = make_uint4(pack2<kBf16>(vx[0], vx[1]), pack2<kBf16>(vx[2], vx[3]), pack2<kBf16>(vx[4], vx[5]), pack2<kBf16>(vx[6], vx[7]));
+        k[r] = narrow8<kBf16>(kx);
+        v[r] = narrow8<kBf16>(vx);
       }
     } else {
       const uint8_t* tail = page + kPageHeader + kPageBlocks * kSlot;

@@ -848,8 +848,8 @@ PyObject* cache_attention(const Args& a) {
   const float gamma = static_cast<float>(1.0 / std::sqrt(static_cast<double>(D)));
   const int rc = rbf_b200_cache_attention(qc.const_data_ptr(), strides3(qc), c.pages.const_data_ptr(), c.table_ptr(),
                                           c.lengths_ptr(), int_ptr(fresh), out.data_ptr(),
-                                          bytes > 0 ? ws.data_ptr() : nullptr, bytes, c.B, c.H, G, T, D, c.max_pages, c.num_pages, dtype_code(q.scalar_type()), softmax, gamma,
-                                          stream_of(q));
+                                          bytes > 0 ? ws.data_ptr() : nullptr, bytes, c.B, c.H, G, T, D, c.max_pages,
+                                          c.num_pages, dtype_code(q.scalar_type()), softmax, gamma, stream_of(q));
   check(rc, "rbf_b200_cache_attention");
   unlocked.lock();
   return wrap(out);
@@ -877,7 +877,7 @@ struct Logits {
   }
   void contiguous() {
     tokens = tokens.contiguous();
-    if (x.stride(1) != 1 && cols > 1 || rows > 1 && x.stride(0) < cols) x = x.contiguous();
+    if ((x.stride(1) != 1 && cols > 1) || (rows > 1 && x.stride(0) < cols)) x = x.contiguous();
   }
   int64_t pitch() const { return rows > 1 ? x.stride(0) : cols; }
   // fp32 per row, on the device

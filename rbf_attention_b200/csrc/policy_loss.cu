@@ -24,7 +24,7 @@ constexpr int kShortBytes = 24 * 1024;              // of a row
 template <int kThreads> constexpr int kBlocks = kThreads == kLong ? 2 : 8;
 constexpr int kStageBytes = 113 * 1024;             // a staged row leaves room for a second block on the SM
 constexpr double kLn2 = 0.6931471805599453;
-constexpr int kCountHere = 8192;                  // rows up to which every block counts them by itself
+constexpr int kCountHere = 8192;                    // rows up to which every block counts them by itself
 
 __device__ __forceinline__ float pl_ex2(float x) {
   float y;
@@ -196,7 +196,8 @@ __global__ void __launch_bounds__(kLong) policy_count_kernel(const PolicyArgs a)
   grid_dependents_launch();
   __shared__ int s_n[kThreads / 32];
   int n = 0;
-  for (int64_t r = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x; r < a.rows; r += static_cast<int64_t>(gridDim.x) * kThreads)
+  const int64_t step = static_cast<int64_t>(gridDim.x) * kThreads;
+  for (int64_t r = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x; r < a.rows; r += step)
     n += counts(a, a.tokens[r]);
   n = __reduce_add_sync(0xffffffffu, n);
   if ((threadIdx.x & 31) == 0) s_n[threadIdx.x >> 5] = n;
@@ -375,7 +376,8 @@ cudaError_t policy_of(const PolicyArgs& a, int sms, cudaStream_t stream) {
   const bool stage = a.dlogits != nullptr;
   if (bytes <= kShortBytes)
     return stage ? policy_t<kDtype, true, kShort>(a, sms, stream) : policy_t<kDtype, false, kShort>(a, sms, stream);
-  return stage && bytes <= kStageBytes ? policy_t<kDtype, true, kLong>(a, sms, stream) : policy_t<kDtype, false, kLong>(a, sms, stream);
+  return stage && bytes <= kStageBytes ? policy_t<kDtype, true, kLong>(a, sms, stream)
+                                       : policy_t<kDtype, false, kLong>(a, sms, stream);
 }
 
 }  // namespace

@@ -187,7 +187,8 @@ class CausalLM(nn.Module):
         """Logits (batch, vocab) behind each sequence's last new token - with ``all_logits`` (batch, T, vocab) behind every one -
         of the ``idx`` (batch, T) that follow what ``cache`` holds; ``new``: how many of the T are real, per sequence (default:
         all), ``sequences``: which of the cache's these are (default: all). Either all or none of those that get tokens are
-        empty. A sequence without new tokens has logits of no meaning."""
+        empty. A sequence without new tokens has logits of no meaning. If it raises, no sequence has got tokens; where a layer had
+        been written, those that would have got some are empty (``PagedCache.abort``)."""
         bsz, seq = idx.shape
         batch = range(cache.max_sequences) if sequences is None else sequences
         new = [seq] * bsz if new is None else [int(n) for n in new]
@@ -209,15 +210,18 @@ class CausalLM(nn.Module):
             pending = None
             for i, block in enumerate(self.blocks):
                 x, pending = block.forward_cached(x, cache, i, from_empty, pending)
+            _, normed = apply_add_layer_norm(self.ln_f, x, pending)
+            if all_logits:
+                normed = normed[:, skip:].contiguous()
+            else:
+                last = torch.tensor([skip + max(n - 1, 0) for n in new]).to(idx.device)
+                normed = normed[torch.arange(bsz, device=idx.device), last]
+            logits = vocab_projection(self.to_logits, normed)
         except BaseException:
             cache.abort()
             raise
         cache.end()
-        _, normed = apply_add_layer_norm(self.ln_f, x, pending)
-        if all_logits:
-            return vocab_projection(self.to_logits, normed[:, skip:].contiguous())
-        last = torch.tensor([skip + max(n - 1, 0) for n in new]).to(idx.device)
-        return vocab_projection(self.to_logits, normed[torch.arange(bsz, device=idx.device), last])
+        return logits
 
     @torch.no_grad()
     def generate(self, idx, max_new_tokens: int, lengths=None, samples: int = 1, temperature: float = 0.0, generator=None,
