@@ -15,29 +15,84 @@ constexpr int kWriteThreads = 128;                 // four warps, a block of 16 
 // (spilling 80 to 100 bytes) and of 64: 162 and 90 us so, 209 and 103 with four blocks, 254 and 100 with 10 and 16.
 template <int P> constexpr int kWriteBlocks = P == 64 ? 10 : 8;
 
-// Eight 16-bit numbers as fp32, and back
-template <bool kBf16>
-__device__ __forceinline__ void widen8(const uint4& raw, float (&x)[8]) {
-  const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float2 f = unpack2<kBf16>(w[i]);
-    x[2 * i] = f.x;
-    x[2 * i + 1] = f.y;
-  }
-}
-
 template <bool kBf16>
 __device__ __forceinline__ uint4 narrow8(const float (&x)[8]) {
   return make_uint4(pack2<kBf16>(x[0], x[1]), pack2<kBf16>(x[2], x[3]), pack2<kBf16>(x[4], x[5]), pack2<kBf16>(x[6], x[7]));
 }
 
-// code + 128 of four values: nearest integers of x * (127 / amax), ties to even, both steps in fp32 (|code| <= 127: x / amax is
-// at most 1, and the two roundings cannot lift 127 by half). Adding 1.5 * 2^23 leaves the integer in the low bits: a conversion
+// code + 128 of four 16-bit numbers: nearest integers of x * (127 / amax), ties to even, both steps in fp32 (|code| <= 127: x / amax
+// is at most 1, and the two roundings cannot lift 127 by half). Adding 1.5 * 2^23 leaves the integer in the low bits: a conversion
 // runs at an eighth of the rate.
-__device__ __forceinline__ uint32_t codes_of(float x0, float x1, float x2, float x3, float inverse) {
-  auto code = [&](float x) { return __float_as_uint(__fadd_rn(__fmul_rn(x, inverse), 12582912.f + 128.f)); };
-  return __byte_perm(__byte_perm(code(x0), code(x1), 0x0040), __byte_perm(code(x2), code(x3), 0x0040), 0x5410);
+template <bool kBf16>
+__device__ __forceinline__ uint32_t codes_of(uint32_t lo, uint32_t hi, float inverse) {
+  constexpr float kLift = 12582912.f + 128.f;
+  float2 x = unpack2<kBf16>(lo), y = unpack2<kBf16>(hi);
+  fmul2(x.x, x.y, x.x, x.y, inverse, inverse);
+  fmul2(y.x, y.y, y.x, y.y, inverse, inverse);
+  // single additions: the compiler makes one rounding of a product and an addition of pairs
+  auto lift = [&](float f) { return __float_as_uint(__fadd_rn(f, kLift)); };
+  return __byte_perm(__byte_perm(lift(x.x), lift(x.y), 0x0040), __byte_perm(lift(y.x), lift(y.y), 0x0040), 0x5410);
+}
+
+// A warp writes the codes and the scale of a block's keys or values: its first `old` tokens are rows of `tail`, the others rows of
+// `src`, `ld` apart (`src` is where the block's first token would be).
+template <bool kBf16, int P, bool kValues>
+__device__ __forceinline__ void write_block(const uint16_t* src, int64_t ld, const uint16_t* tail, int old, int D, uint8_t* slot,
+                                            float* scale_out) {
+  // lane (r, c): tokens r, r + kRows, ... of 8-column group c; of values, four tokens of a quad, which the lane transposes
+  constexpr int kGroups = P / 8, kRows = 32 / kGroups, kPer = kBlockTokens / kRows;
+  const int lane = threadIdx.x & 31, r = lane / kGroups, c = lane % kGroups;
+  auto token = [&](int i) { return kValues ? (i / 4) * 4 * kRows + r * 4 + i % 4 : i * kRows + r; };
+  uint4 raw[kPer];
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    const int t = token(i);
+    const uint16_t* from = t < old ? tail + t * P : src + t * ld;
+    raw[i] = c * 8 < D ? *reinterpret_cast<const uint4*>(from + c * 8) : make_uint4(0, 0, 0, 0);
+  }
+  uint32_t top = 0;                                 // magnitudes as integers: NaN is above infinity is above every number
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) top = __vmaxu2(top, w[e] & 0x7fff7fffu);
+  }
+  top = __reduce_max_sync(0xffffffffu, max(top & 0xffffu, top >> 16));
+  const float amax = unpack2<kBf16>(top).x;
+  const bool finite = top < (kBf16 ? 0x7f80u : 0x7c00u), held = amax >= kSmallestHeld;
+  const float inverse = finite && held ? __fdiv_rn(127.f, amax) : 0.f;
+#pragma unroll
+  for (int i = 0; i < kPer; i += 4) {               // four tokens at a time
+    uint2 code[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const uint4 w = raw[i + k];
+      // a block with a number that is not finite has codes of zero, and its scale makes them NaN
+      code[k] = finite ? make_uint2(codes_of<kBf16>(w.x, w.y, inverse), codes_of<kBf16>(w.z, w.w, inverse))
+                       : make_uint2(0x80808080u, 0x80808080u);
+    }
+    if constexpr (!kValues) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int tok = token(i + k), half = (tok >> 1) & 1, g = (tok >> 2) * 2 + (tok & 1);
+        *reinterpret_cast<uint2*>(slot + ((c / 8) * 2 + half) * 512 + g * 64 + (c % 8) * 8) = code[k];
+      }
+    } else {
+      const int t = token(i) / 4;
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {                 // four tokens x four dims, transposed
+        const uint32_t r0 = e ? code[0].y : code[0].x, r1 = e ? code[1].y : code[1].x;
+        const uint32_t r2 = e ? code[2].y : code[2].x, r3 = e ? code[3].y : code[3].x;
+        const uint32_t lo01 = __byte_perm(r0, r1, 0x5140), hi01 = __byte_perm(r0, r1, 0x7362);
+        const uint32_t lo23 = __byte_perm(r2, r3, 0x5140), hi23 = __byte_perm(r2, r3, 0x7362);
+        const uint4 out = make_uint4(__byte_perm(lo01, lo23, 0x5410), __byte_perm(lo01, lo23, 0x7632),
+                                     __byte_perm(hi01, hi23, 0x5410), __byte_perm(hi01, hi23, 0x7632));
+        const int d4 = c * 2 + e;                   // group of four dims
+        *reinterpret_cast<uint4*>(slot + 16 * P + (d4 / 8) * 512 + ((d4 % 8) * 4 + t) * 16) = out;
+      }
+    }
+  }
+  if (lane == 0) scale_out[kValues] = !finite ? __uint_as_float(0x7fc00000u) : held ? __fdiv_rn(amax, 127.f) : 0.f;
 }
 
 // One warp per block of 16 tokens that the new tokens touch, of one head's keys or values. The warp of the first block also
@@ -60,74 +115,18 @@ __global__ void __launch_bounds__(kWriteThreads, kWriteBlocks<P>) cache_append_k
   constexpr int kBytes = cache_page_bytes(P), kSlot = cache_slot_bytes(P);
   const int D = a.D;
 
-  // columns 8 x ... of token `pos`: from the incomplete block or from the call's tokens
-  auto load8 = [&](const uint8_t* tail, int pos, int col) -> uint4 {
-    if (col >= D) return make_uint4(0, 0, 0, 0);
-    if (pos < span.held) return *reinterpret_cast<const uint4*>(tail + ((pos % kBlockTokens) * P + col) * 2);
-    return *reinterpret_cast<const uint4*>(src + static_cast<int64_t>(pos - span.held) * st[2] + col);
-  };
-
   const int block = first + j;
   if ((block + 1) * static_cast<int64_t>(kBlockTokens) <= end) {
     uint8_t* page = const_cast<uint8_t*>(
         cache_page(a.pages, a.table, b, a.max_pages, a.num_pages, a.H, h, kBytes, block * kBlockTokens));
     if (page != nullptr) {
       const uint8_t* tail = page + kPageHeader + (kPageBlocks + kv) * kSlot;
-      // lane (r, c): tokens r, r + kRows, ... of 8-column group c
-      constexpr int kGroups = P / 8, kRows = 32 / kGroups, kPer = kBlockTokens / kRows;
-      const int r = lane / kGroups, c = lane % kGroups;
-      // keys: tokens r + i * kRows; values: four tokens of a quad belong to one lane, which transposes them in registers
-      auto token = [&](int i) { return kv ? (i / 4) * 4 * kRows + r * 4 + i % 4 : i * kRows + r; };
-      uint4 raw[kPer];
-#pragma unroll
-      for (int i = 0; i < kPer; ++i) raw[i] = load8(tail, block * kBlockTokens + token(i), c * 8);
-      uint32_t top = 0;                             // magnitudes as integers: NaN is above infinity is above every number
-#pragma unroll
-      for (int i = 0; i < kPer; ++i) {
-        float x[8];
-        widen8<kBf16>(raw[i], x);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(x[e]) & 0x7fffffffu);
-      }
-      top = __reduce_max_sync(0xffffffffu, top);
-      const float amax = __uint_as_float(top);
-      const bool finite = top < 0x7f800000u, held = amax >= kSmallestHeld;
-      const float scale = !finite ? __uint_as_float(0x7fc00000u) : held ? __fdiv_rn(amax, 127.f) : 0.f;
-      const float inverse = finite && held ? __fdiv_rn(127.f, amax) : 0.f;
-      uint8_t* slot = page + kPageHeader + (block % kPageBlocks) * kSlot + kv * 16 * P;
-#pragma unroll
-      for (int i = 0; i < kPer; i += 4) {           // four tokens at a time
-        uint2 code[4];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          float x[8];
-          widen8<kBf16>(raw[i + k], x);
-          // a block with a number that is not finite has codes of zero, and its scale makes them NaN
-          code[k] = finite ? make_uint2(codes_of(x[0], x[1], x[2], x[3], inverse), codes_of(x[4], x[5], x[6], x[7], inverse))
-                           : make_uint2(0x80808080u, 0x80808080u);
-        }
-        if (kv == 0) {
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const int tok = token(i + k), half = (tok >> 1) & 1, g = (tok >> 2) * 2 + (tok & 1);
-            *reinterpret_cast<uint2*>(slot + ((c / 8) * 2 + half) * 512 + g * 64 + (c % 8) * 8) = code[k];
-          }
-        } else {
-          const int t = token(i) / 4;
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {             // four tokens x four dims, transposed
-            const uint32_t r0 = e ? code[0].y : code[0].x, r1 = e ? code[1].y : code[1].x;
-            const uint32_t r2 = e ? code[2].y : code[2].x, r3 = e ? code[3].y : code[3].x;
-            const uint32_t lo01 = __byte_perm(r0, r1, 0x5140), hi01 = __byte_perm(r0, r1, 0x7362);
-            const uint32_t lo23 = __byte_perm(r2, r3, 0x5140), hi23 = __byte_perm(r2, r3, 0x7362);
-            const uint4 out = make_uint4(__byte_perm(lo01, lo23, 0x5410), __byte_perm(lo01, lo23, 0x7632),
-                                         __byte_perm(hi01, hi23, 0x5410), __byte_perm(hi01, hi23, 0x7632));
-            const int d4 = c * 2 + e;               // group of four dims
-            *reinterpret_cast<uint4*>(slot + (d4 / 8) * 512 + ((d4 % 8) * 4 + t) * 16) = out;
-          }
-        }
-      }
-      if (lane == 0) reinterpret_cast<float*>(page)[(block % kPageBlocks) * 2 + kv] = scale;
+      uint8_t* slot = page + kPageHeader + (block % kPageBlocks) * kSlot;
+      float* scales = reinterpret_cast<float*>(page) + (block % kPageBlocks) * 2;
+      const int64_t at = static_cast<int64_t>(block) * kBlockTokens - span.held;
+      const uint16_t* rows = reinterpret_cast<const uint16_t*>(tail);
+      if (kv) write_block<kBf16, P, true>(src + at * st[2], st[2], rows, static_cast<int>(at < 0 ? -at : 0), D, slot, scales);
+      else write_block<kBf16, P, false>(src + at * st[2], st[2], rows, static_cast<int>(at < 0 ? -at : 0), D, slot, scales);
     }
   }
   if (j != 0 || end % kBlockTokens == 0) return;
@@ -139,8 +138,16 @@ __global__ void __launch_bounds__(kWriteThreads, kWriteBlocks<P>) cache_append_k
   const int from = last > span.held ? last : span.held;
   for (int i = lane; i < (end - from) * (P / 8); i += 32) {
     const int pos = from + i / (P / 8), col = i % (P / 8) * 8;
-    *reinterpret_cast<uint4*>(tail + ((pos % kBlockTokens) * P + col) * 2) = load8(tail, pos, col);
+    uint4 x = make_uint4(0, 0, 0, 0);
+    if (col < D) x = *reinterpret_cast<const uint4*>(src + static_cast<int64_t>(pos - span.held) * st[2] + col);
+    *reinterpret_cast<uint4*>(tail + ((pos % kBlockTokens) * P + col) * 2) = x;
   }
+}
+
+// (x0, x1) of two codes that are held as 2^23 + 128 + code, times the scale
+__device__ __forceinline__ void scaled2(float& x0, float& x1, float a0, float a1, float scale) {
+  fadd2(a0, a1, a0, a1, -8388736.f, -8388736.f);
+  fmul2(x0, x1, a0, a1, scale, scale);
 }
 
 // Four tokens (a quad of a block) x eight columns of one head's keys and values per thread
@@ -155,6 +162,8 @@ __global__ void __launch_bounds__(256) cache_read_kernel(const CacheReadArgs a) 
   const int first = a.first != nullptr ? a.first[b] : 0;
   const int64_t begin = first < 0 ? 0 : first;      // (a negative start reads from the first token on)
   const int64_t pos64 = (begin / 4 + quad) * 4;
+  // byte i of a word under the exponent of 2^23: the float 2^23 + byte (a conversion runs at a quarter of the rate)
+  auto lifted = [&](uint32_t word, int i) { return __uint_as_float(__byte_perm(word, a.exponent, 0x7440 + i)); };
   uint4 k[4], v[4];                                 // eight columns of four tokens
 #pragma unroll
   for (int r = 0; r < 4; ++r) k[r] = v[r] = make_uint4(0, 0, 0, 0);
@@ -182,9 +191,9 @@ __global__ void __launch_bounds__(256) cache_read_kernel(const CacheReadArgs a) 
         for (int e = 0; e < 2; ++e) {
           const uint32_t words[4] = {w[e].x, w[e].y, w[e].z, w[e].w}, key = e ? kw[r].y : kw[r].x;
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            kx[4 * e + i] = static_cast<float>(static_cast<int>(key >> (8 * i) & 0xffu) - 128) * scale.x;
-            vx[4 * e + i] = static_cast<float>(static_cast<int>(words[i] >> (8 * r) & 0xffu) - 128) * scale.y;
+          for (int i = 0; i < 4; i += 2) {
+            scaled2(kx[4 * e + i], kx[4 * e + i + 1], lifted(key, i), lifted(key, i + 1), scale.x);
+            scaled2(vx[4 * e + i], vx[4 * e + i + 1], lifted(words[i], r), lifted(words[i + 1], r), scale.y);
           }
         }
         k[r] = narrow8<kBf16>(kx);
@@ -239,6 +248,7 @@ cudaError_t read_t(CacheReadArgs a, cudaStream_t stream) {
   const int64_t chunks = (static_cast<int64_t>(a.quads) * (a.D / 8) + 255) / 256, blocks = chunks * a.B * a.H;
   if (blocks > 0x7fffffffll) return cudaErrorInvalidConfiguration;
   a.chunks = static_cast<unsigned>(chunks);
+  a.exponent = 0x4b000000u;
   cache_read_kernel<kBf16, P><<<static_cast<unsigned>(blocks), 256, 0, stream>>>(a);
   return cudaGetLastError();
 }

@@ -205,7 +205,7 @@ struct CacheReadArgs {
   void* v;
   int B, H, D, count, max_pages, num_pages;
   int quads;                 // groups of four tokens that the range can touch
-  unsigned chunks;           // set by the launcher
+  unsigned chunks, exponent; // set by the launcher
 };
 cudaError_t launch_cache_read(const CacheReadArgs& a, bool bf16, cudaStream_t stream);
 // pages[layer][dst] = pages[layer][src] for a list of pairs, in all layers; the pairs travel as kernel parameters.
