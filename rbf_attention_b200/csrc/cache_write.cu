@@ -13,7 +13,7 @@ namespace {
 constexpr int kWriteThreads = 128;                 // four warps, a block of 16 tokens of one head each
 // Blocks on an SM: a warp waits for one load, so as many as registers allow. 8 x 16 heads x 8190 tokens written, of 128 columns
 // (spilling 80 to 100 bytes) and of 64: 162 and 90 us so, 209 and 103 with four blocks, 254 and 100 with 10 and 16.
-template <int P> constexpr int kWriteBlocks = P == 64 ? 10 : 8;
+template <int P> constexpr int kWriteBlocks = 8;
 
 template <bool kBf16>
 __device__ __forceinline__ uint4 narrow8(const float (&x)[8]) {
@@ -34,22 +34,36 @@ __device__ __forceinline__ uint32_t codes_of(uint32_t lo, uint32_t hi, float inv
   return __byte_perm(__byte_perm(lift(x.x), lift(x.y), 0x0040), __byte_perm(lift(y.x), lift(y.y), 0x0040), 0x5410);
 }
 
-// A warp writes the codes and the scale of a block's keys or values: its first `old` tokens are rows of `tail`, the others rows of
-// `src`, `ld` apart (`src` is where the block's first token would be).
-template <bool kBf16, int P, bool kValues>
-__device__ __forceinline__ void write_block(const uint16_t* src, int64_t ld, const uint16_t* tail, int old, int D, uint8_t* slot,
-                                            float* scale_out) {
-  // lane (r, c): tokens r, r + kRows, ... of 8-column group c; of values, four tokens of a quad, which the lane transposes
-  constexpr int kGroups = P / 8, kRows = 32 / kGroups, kPer = kBlockTokens / kRows;
-  const int lane = threadIdx.x & 31, r = lane / kGroups, c = lane % kGroups;
-  auto token = [&](int i) { return kValues ? (i / 4) * 4 * kRows + r * 4 + i % 4 : i * kRows + r; };
+// A warp's share of a block's keys or values: lane (r, c) has tokens r, r + kRows, ... of 8-column group c; of values, four tokens
+// of a quad, which it transposes
+template <int P, bool kValues>
+struct Share {
+  static constexpr int kGroups = P / 8, kRows = 32 / kGroups, kPer = kBlockTokens / kRows;
   uint4 raw[kPer];
-#pragma unroll
-  for (int i = 0; i < kPer; ++i) {
-    const int t = token(i);
-    const uint16_t* from = t < old ? tail + t * P : src + t * ld;
-    raw[i] = c * 8 < D ? *reinterpret_cast<const uint4*>(from + c * 8) : make_uint4(0, 0, 0, 0);
+  static __device__ __forceinline__ int column() { return (threadIdx.x & 31) % kGroups; }
+  static __device__ __forceinline__ int token(int i) {
+    const int r = static_cast<int>(threadIdx.x & 31) / kGroups;
+    return kValues ? (i / 4) * 4 * kRows + r * 4 + i % 4 : i * kRows + r;
   }
+  // The first `old` tokens are rows of `tail`, the others rows of `src`, `ld` apart (`src` is where the block's first token would be).
+  __device__ __forceinline__ void load(const uint16_t* src, int64_t ld, const uint16_t* tail, int old, int D) {
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      const int t = token(i), col = column() * 8;
+      const uint16_t* from = t < old ? tail + t * P : src + t * ld;
+      raw[i] = col < D ? *reinterpret_cast<const uint4*>(from + col) : make_uint4(0, 0, 0, 0);
+    }
+  }
+};
+
+// Its codes and the block's scale into the cache
+template <bool kBf16, int P, bool kValues>
+__device__ __forceinline__ void write_block(const Share<P, kValues>& in, uint8_t* slot, float* scale_out) {
+  using S = Share<P, kValues>;
+  constexpr int kPer = S::kPer;
+  const uint4(&raw)[kPer] = in.raw;
+  const int lane = threadIdx.x & 31, c = S::column();
+  auto token = [](int i) { return S::token(i); };
   uint32_t top = 0;                                 // magnitudes as integers: NaN is above infinity is above every number
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
@@ -95,38 +109,42 @@ __device__ __forceinline__ void write_block(const uint16_t* src, int64_t ld, con
   if (lane == 0) scale_out[kValues] = !finite ? __uint_as_float(0x7fc00000u) : held ? __fdiv_rn(amax, 127.f) : 0.f;
 }
 
-// One warp per block of 16 tokens that the new tokens touch, of one head's keys or values. The warp of the first block also
-// stores what is left behind the last complete one: both use the rows of the incomplete block, which are read first.
+// One warp per block of 16 tokens that the new tokens touch, of one head's keys or values - of 64 columns both, so that a warp
+// has eight loads under way. Neighbours have the heads of a block, which are beside one another in what a projection writes (with
+// the blocks of a head as neighbours 138 and 86 us). The warp of the first block also stores what is left behind the last
+// complete one: both use the rows of the incomplete block, which are read first.
+template <int P> constexpr bool kBothOf = P == 64;
 template <bool kBf16, int P>
 __global__ void __launch_bounds__(kWriteThreads, kWriteBlocks<P>) cache_append_kernel(const CacheAppendArgs a) {
+  constexpr bool kBoth = kBothOf<P>;
+  constexpr int kBytes = cache_page_bytes(P), kSlot = cache_slot_bytes(P);
   const int lane = threadIdx.x & 31;
   const unsigned unit = blockIdx.x * (kWriteThreads / 32) + (threadIdx.x >> 5);          // below 2^31: 32-bit divisions
-  const unsigned head = unit / a.blocks, heads = (head >> 1) / a.H;
-  const int j = static_cast<int>(unit - head * a.blocks), kv = static_cast<int>(head & 1);
-  const int h = static_cast<int>((head >> 1) - heads * a.H), b = static_cast<int>(heads);
+  const unsigned columns = kBoth ? a.H : 2 * a.H, slow = unit / columns, fast = unit - slow * columns;
+  const bool values = !kBoth && fast >= static_cast<unsigned>(a.H);
+  const int h = static_cast<int>(values ? fast - a.H : fast), b = static_cast<int>(slow / a.blocks);
+  const int j = static_cast<int>(slow - static_cast<unsigned>(b) * a.blocks);
   if (b >= a.B) return;
   const CacheSpan span = cache_span(a.lengths, a.fresh, b, a.T, a.max_pages);
   if (span.fresh == 0) return;
-  const int end = span.held + span.fresh;
-  const int first = span.held / kBlockTokens;
-  const uint16_t* src = static_cast<const uint16_t*>(kv ? a.v : a.k);
-  const int64_t* st = kv ? a.vs : a.ks;
-  src += b * st[0] + h * st[1];
-  constexpr int kBytes = cache_page_bytes(P), kSlot = cache_slot_bytes(P);
-  const int D = a.D;
-
-  const int block = first + j;
+  const int end = span.held + span.fresh, block = span.held / kBlockTokens + j;
+  const uint16_t* k = static_cast<const uint16_t*>(a.k) + b * a.ks[0] + h * a.ks[1];
+  const uint16_t* v = static_cast<const uint16_t*>(a.v) + b * a.vs[0] + h * a.vs[1];
   if ((block + 1) * static_cast<int64_t>(kBlockTokens) <= end) {
     uint8_t* page = const_cast<uint8_t*>(
         cache_page(a.pages, a.table, b, a.max_pages, a.num_pages, a.H, h, kBytes, block * kBlockTokens));
     if (page != nullptr) {
-      const uint8_t* tail = page + kPageHeader + (kPageBlocks + kv) * kSlot;
+      const uint16_t* tail = reinterpret_cast<const uint16_t*>(page + kPageHeader + kPageBlocks * kSlot);
       uint8_t* slot = page + kPageHeader + (block % kPageBlocks) * kSlot;
       float* scales = reinterpret_cast<float*>(page) + (block % kPageBlocks) * 2;
       const int64_t at = static_cast<int64_t>(block) * kBlockTokens - span.held;
-      const uint16_t* rows = reinterpret_cast<const uint16_t*>(tail);
-      if (kv) write_block<kBf16, P, true>(src + at * st[2], st[2], rows, static_cast<int>(at < 0 ? -at : 0), D, slot, scales);
-      else write_block<kBf16, P, false>(src + at * st[2], st[2], rows, static_cast<int>(at < 0 ? -at : 0), D, slot, scales);
+      const int old = static_cast<int>(at < 0 ? -at : 0);
+      Share<P, false> keys;
+      Share<P, true> vals;
+      if (!values) keys.load(k + at * a.ks[2], a.ks[2], tail, old, a.D);
+      if (kBoth || values) vals.load(v + at * a.vs[2], a.vs[2], tail + kSlot / 2, old, a.D);
+      if (!values) write_block<kBf16>(keys, slot, scales);
+      if (kBoth || values) write_block<kBf16>(vals, slot, scales);
     }
   }
   if (j != 0 || end % kBlockTokens == 0) return;
@@ -134,13 +152,19 @@ __global__ void __launch_bounds__(kWriteThreads, kWriteBlocks<P>) cache_append_k
   const int last = end / kBlockTokens * kBlockTokens;
   uint8_t* page = const_cast<uint8_t*>(cache_page(a.pages, a.table, b, a.max_pages, a.num_pages, a.H, h, kBytes, last));
   if (page == nullptr) return;
-  uint8_t* tail = page + kPageHeader + (kPageBlocks + kv) * kSlot;
   const int from = last > span.held ? last : span.held;
-  for (int i = lane; i < (end - from) * (P / 8); i += 32) {
-    const int pos = from + i / (P / 8), col = i % (P / 8) * 8;
-    uint4 x = make_uint4(0, 0, 0, 0);
-    if (col < D) x = *reinterpret_cast<const uint4*>(src + static_cast<int64_t>(pos - span.held) * st[2] + col);
-    *reinterpret_cast<uint4*>(tail + ((pos % kBlockTokens) * P + col) * 2) = x;
+#pragma unroll
+  for (int kv = 0; kv < 2; ++kv) {
+    if (!kBoth && kv != values) continue;
+    uint8_t* tail = page + kPageHeader + (kPageBlocks + kv) * kSlot;
+    const uint16_t* src = kv ? v : k;
+    const int64_t ld = kv ? a.vs[2] : a.ks[2];
+    for (int i = lane; i < (end - from) * (P / 8); i += 32) {
+      const int pos = from + i / (P / 8), col = i % (P / 8) * 8;
+      uint4 x = make_uint4(0, 0, 0, 0);
+      if (col < a.D) x = *reinterpret_cast<const uint4*>(src + static_cast<int64_t>(pos - span.held) * ld + col);
+      *reinterpret_cast<uint4*>(tail + ((pos % kBlockTokens) * P + col) * 2) = x;
+    }
   }
 }
 
@@ -238,7 +262,7 @@ __global__ void __launch_bounds__(kCopyThreads) cache_copy_kernel(const __grid_c
 
 template <bool kBf16, int P>
 cudaError_t append_t(const CacheAppendArgs& a, cudaStream_t stream) {
-  const int64_t units = static_cast<int64_t>(a.B) * a.H * 2 * a.blocks, per = kWriteThreads / 32;
+  const int64_t units = static_cast<int64_t>(a.B) * a.H * (kBothOf<P> ? 1 : 2) * a.blocks, per = kWriteThreads / 32;
   if (units > 0x7fffffffll) return cudaErrorInvalidConfiguration;
   cache_append_kernel<kBf16, P><<<static_cast<unsigned>((units + per - 1) / per), kWriteThreads, 0, stream>>>(a);
   return cudaGetLastError();
