@@ -11,9 +11,10 @@ namespace rbf {
 namespace {
 
 constexpr int kWriteThreads = 128;                 // four warps, a block of 16 tokens of one head each
-// Blocks on an SM: a warp waits for one load, so as many as registers allow. 8 x 16 heads x 8190 tokens written, of 128 columns
-// (spilling 80 to 100 bytes) and of 64: 162 and 90 us so, 209 and 103 with four blocks, 254 and 100 with 10 and 16.
-template <int P> constexpr int kWriteBlocks = 8;
+// Blocks on an SM: a warp waits for one round of loads, eight of 16 bytes a lane, so as many as registers allow without much
+// spilling. 8 x 16 heads x 8190 tokens written, of 128 columns and of 64: 124 us (6.5 TB/s) and 75 so, 134 and 84 with six blocks,
+// 144 and 83 with ten.
+constexpr int kWriteBlocks = 8;
 
 template <bool kBf16>
 __device__ __forceinline__ uint4 narrow8(const float (&x)[8]) {
@@ -115,7 +116,7 @@ __device__ __forceinline__ void write_block(const Share<P, kValues>& in, uint8_t
 // complete one: both use the rows of the incomplete block, which are read first.
 template <int P> constexpr bool kBothOf = P == 64;
 template <bool kBf16, int P>
-__global__ void __launch_bounds__(kWriteThreads, kWriteBlocks<P>) cache_append_kernel(const CacheAppendArgs a) {
+__global__ void __launch_bounds__(kWriteThreads, kWriteBlocks) cache_append_kernel(const CacheAppendArgs a) {
   constexpr bool kBoth = kBothOf<P>;
   constexpr int kBytes = cache_page_bytes(P), kSlot = cache_slot_bytes(P);
   const int lane = threadIdx.x & 31;
