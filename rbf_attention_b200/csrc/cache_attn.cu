@@ -933,7 +933,8 @@ __global__ void __launch_bounds__(kWarps * 32, 16 / kWarps) cache_attn_short_ker
 // dims) warps on an SM: the tensor pipe is busy for 19 to 28 % of the time, the issue slots for 33 to 44 %. 37 new tokens on 6
 // histories of up to 5003, 16 heads of 64: 39 us a call; 200 on 32 of up to 500: 76 (112 with the cache as the row operand and 32
 // columns a warp). Three blocks of 168 registers on an SM, or two of 255; four and three of them spill (50 and 93 us).
-// Three units under way instead of two, the incomplete block's rows among them: 41 and 81 us.
+// Three units under way instead of two, the incomplete block's rows among them: 41 and 81 us; the next unit widened beside the
+// products, with one barrier a unit instead of two: 40 and 79.
 constexpr int kRowWarps = 4;
 template <int P>
 struct RowTile {

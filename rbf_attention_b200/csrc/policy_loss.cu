@@ -6,9 +6,10 @@
 // one kernel reads the logits and writes the gradient of the loss, as the cross entropy does. Roofline: HBM. A block owns a
 // row, reads it with an online maximum and sum and keeps it in shared memory where two blocks' rows fit an SM; longer rows come
 // a second time out of L2. The rows' bases may have any alignment: a row is a head of single elements up to the first 16-byte
-// boundary, 16-byte words, and a tail. 16384 x 50304 bfloat16: 581 us, 5.7 TB/s = 87 % of a copy. Its special-function unit is
-// busy for 60 % of that and its issue slots for 47; a quarter of the exponentials by polynomials took 599 us, fetching the next row into shared
-// memory word by word behind the gradient 616. Sums over rows are in 64 bits and in the order of the rows of a block, then of the blocks.
+// boundary, 16-byte words, and a tail. Sums over rows are in 64 bits and in the order of the rows of a block, then of the blocks.
+// 16384 x 50304 bfloat16: 581 us, 5.7 TB/s = 87 % of a copy. The special-function unit is busy for 60 % of that, the issue slots
+// for 47; a quarter of the exponentials by polynomials took 599 us, fetching the next row into shared memory word by word behind
+// the gradient 616.
 #include <cstdint>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
