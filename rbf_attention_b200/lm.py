@@ -173,14 +173,18 @@ class CausalLM(nn.Module):
     def new_cache(self, max_sequences: int, max_length: int, num_pages: int | None = None) -> PagedCache:
         """A cache for ``max_sequences`` sequences of up to ``max_length`` tokens (the register tokens come on top)."""
         attn = self.blocks[0].attn
-        table = getattr(attn, "susie_cache", None)
-        for limit in (None if table is None else table.shape[0],
-                      self.pos_emb.num_embeddings if self.pos_emb_type == "learned" else None):
-            if limit is not None and max_length > limit:
-                raise ValueError(f"the model's positions end at {limit} tokens, {max_length} are asked for")
+        self._check_positions(max_length)
         weight = self.to_logits.weight
         return PagedCache(len(self.blocks), attn.num_heads, attn.head_dim, max_sequences, max_length + self.num_registers,
                           num_pages, weight.dtype, weight.device)
+
+    def _check_positions(self, length: int) -> None:
+        """Refuses sequences that the model has no positions for."""
+        table = getattr(self.blocks[0].attn, "susie_cache", None)
+        for limit in (None if table is None else table.shape[0],
+                      self.pos_emb.num_embeddings if self.pos_emb_type == "learned" else None):
+            if limit is not None and length > limit:
+                raise ValueError(f"the model's positions end at {limit} tokens, {length} are asked for")
 
     @torch.no_grad()
     def forward_cached(self, idx, cache: PagedCache, new=None, sequences=None, all_logits: bool = False):
@@ -198,6 +202,8 @@ class CausalLM(nn.Module):
         if len(empty) > 1:
             raise ValueError("some of the sequences are empty, others are not: give them their tokens in two calls")
         from_empty = empty == {True}
+        self._check_positions(max((cache.length(s) + n - (0 if from_empty else self.num_registers) for s, n in zip(batch, new) if n),
+                                  default=0))
         skip = self.num_registers if from_empty else 0
         cache.begin([n + skip if n else 0 for n in new], sequences)
         try:

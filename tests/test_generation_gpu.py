@@ -302,3 +302,21 @@ def test_refusals():
     with pytest.raises(ValueError, match="float32"):
         lm.CausalLM(VOCAB, 128, 1, 2, 64, attention_type="rbf_triton").to(DEV).new_cache(1, 10)
     ops.check_device_status()
+
+
+@pytest.mark.parametrize("pos", ["rope", "learned"])
+def test_positions_end_with_the_model(pos):
+    """A cache of the caller's own may be longer than the model's positions: the token behind the last one is refused, before
+    anything is written."""
+    model = _model(pos=pos)
+    limit = 700
+    cache = PagedCache(len(model.blocks), 2, 64, 1, 2000, device=DEV)
+    with pytest.raises(ValueError, match="positions end"):
+        model.forward_cached(_ids(1, limit + 1), cache)
+    model.forward_cached(_ids(1, limit - 1), cache)
+    assert model.forward_cached(_ids(1, 1), cache).isfinite().all()
+    held = cache.length(0)
+    assert held == limit + model.num_registers
+    with pytest.raises(ValueError, match="positions end"):
+        model.forward_cached(_ids(1, 1), cache)
+    assert cache.length(0) == held
