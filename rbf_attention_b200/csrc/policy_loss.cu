@@ -4,8 +4,8 @@
 //   d loss / d lp = w (kl_weight (1 - e^(ref - lp)) - [r A <= clipped] r A) = c,   d loss / d z = c (onehot(t) - softmax(z))
 // Everything but the row's lse is a handful of scalars per row, so the gradient is known as soon as the row has been read once:
 // one kernel reads the logits and writes the gradient of the loss, as the cross entropy does. Roofline: HBM. A block owns a
-// row, reads it with an online maximum and sum and keeps it in shared memory where two blocks' rows fit an SM; longer rows come
-// a second time out of L2. The rows' bases may have any alignment: a row is a head of single elements up to the first 16-byte
+// row, reads it with an online maximum and sum and keeps it in shared memory where it fits; longer rows come a second time out
+// of L2. The rows' bases may have any alignment: a row is a head of single elements up to the first 16-byte
 // boundary, 16-byte words, and a tail. Sums over rows are in 64 bits and in the order of the rows of a block, then of the blocks.
 // 16384 x 50304 bfloat16: 581 us, 5.7 TB/s = 87 % of a copy. The special-function unit is busy for 60 % of that, the issue slots
 // for 47; a quarter of the exponentials by polynomials took 599 us, fetching the next row into shared memory word by word behind
@@ -21,11 +21,16 @@ namespace rbf {
 namespace {
 
 // A block's threads, and blocks of the loss kernel on an SM: a short row is little work between two barriers, so many small
-// blocks share an SM (8000 rows of 8192 bfloat16: 100 us with 512 threads, 59 with 128).
+// blocks share an SM (8000 rows of 8192 bfloat16: 100 us with 512 threads, 59 with 128). The threads go by the row's length alone:
+// they decide the order of its sum, and a row has the same log-probability from both operators, with or without a gradient,
+// among any number of rows.
 constexpr int kLong = 512, kShort = 128;
 constexpr int kShortBytes = 24 * 1024;              // of a row
-template <int kThreads> constexpr int kBlocks = kThreads == kLong ? 2 : 8;
+constexpr int kBlocksOfShort = 8, kBlocksOfLong = 2;
 constexpr int kStageBytes = 113 * 1024;             // a staged row leaves room for a second block on the SM
+// Longer ones have the SM alone, unless all rows run at once two to an SM and unstaged (float32 x 50257: 5000 rows 396 us, read a
+// second time by two blocks on an SM 453; 200 rows 26 and 23; 3000 x 100000 bfloat16 242 and 295).
+constexpr int kAloneBytes = 226 * 1024;
 constexpr double kLn2 = 0.6931471805599453;
 constexpr int kCountHere = 8192;                    // rows up to which every block counts them by itself
 
@@ -211,8 +216,8 @@ __global__ void __launch_bounds__(kLong) policy_count_kernel(const PolicyArgs a)
   }
 }
 
-template <int kDtype, bool kStage, int kThreads>
-__global__ void __launch_bounds__(kThreads, kBlocks<kThreads>) policy_loss_kernel(const PolicyArgs a) {
+template <int kDtype, bool kStage, int kThreads, int kBlocks>
+__global__ void __launch_bounds__(kThreads, kBlocks) policy_loss_kernel(const PolicyArgs a) {
   using N = Number<kDtype>;
   using T = typename N::type;
   constexpr int V = Cut<T>::kPer;
@@ -353,9 +358,9 @@ cudaError_t log_probs_t(const PolicyArgs& a, int sms, cudaStream_t stream) {
   return cudaGetLastError();
 }
 
-template <int kDtype, bool kStage, int kThreads>
+template <int kDtype, bool kStage, int kThreads, int kBlocks>
 cudaError_t policy_t(PolicyArgs a, int sms, cudaStream_t stream) {
-  const int64_t most = static_cast<int64_t>(sms) * kBlocks<kThreads>;
+  const int64_t most = static_cast<int64_t>(sms) * kBlocks;
   const int blocks = a.rows == 0 ? 1 : static_cast<int>(a.rows < most ? a.rows : most);
   const int64_t wanted = (a.rows + kLong - 1) / kLong;
   a.count_blocks = a.rows <= kCountHere ? 0 : static_cast<int>(wanted < sms ? wanted : sms);
@@ -366,11 +371,12 @@ cudaError_t policy_t(PolicyArgs a, int sms, cudaStream_t stream) {
   }
   size_t smem = 0;
   if constexpr (kStage) {
+    constexpr int kMost = kBlocks == 1 ? kAloneBytes : kStageBytes;
     static PerDeviceFlags flags;
-    if ((e = ensure_dynamic_smem(policy_loss_kernel<kDtype, kStage, kThreads>, kStageBytes, flags)) != cudaSuccess) return e;
+    if ((e = ensure_dynamic_smem(policy_loss_kernel<kDtype, kStage, kThreads, kBlocks>, kMost, flags)) != cudaSuccess) return e;
     smem = (static_cast<size_t>(a.cols) * sizeof(typename Number<kDtype>::type) + 15) / 16 * 16;
   }
-  e = launch_dependent(policy_loss_kernel<kDtype, kStage, kThreads>, dim3(blocks), kThreads, smem, stream, a);
+  e = launch_dependent(policy_loss_kernel<kDtype, kStage, kThreads, kBlocks>, dim3(blocks), kThreads, smem, stream, a);
   if (e != cudaSuccess) return e;
   return launch_dependent(policy_finish_kernel, dim3(1), 32, 0, stream, a, blocks);
 }
@@ -385,14 +391,16 @@ cudaError_t policy_of(const PolicyArgs& a, int sms, cudaStream_t stream) {
   const int64_t bytes = static_cast<int64_t>(a.cols) * sizeof(typename Number<kDtype>::type);
   const bool stage = a.dlogits != nullptr;
   if (bytes <= kShortBytes)
-    return stage ? policy_t<kDtype, true, kShort>(a, sms, stream) : policy_t<kDtype, false, kShort>(a, sms, stream);
-  return stage && bytes <= kStageBytes ? policy_t<kDtype, true, kLong>(a, sms, stream)
-                                       : policy_t<kDtype, false, kLong>(a, sms, stream);
+    return stage ? policy_t<kDtype, true, kShort, kBlocksOfShort>(a, sms, stream)
+                 : policy_t<kDtype, false, kShort, kBlocksOfShort>(a, sms, stream);
+  if (stage && bytes <= kStageBytes) return policy_t<kDtype, true, kLong, kBlocksOfLong>(a, sms, stream);
+  if (stage && bytes <= kAloneBytes && a.rows > kBlocksOfLong * sms) return policy_t<kDtype, true, kLong, 1>(a, sms, stream);
+  return policy_t<kDtype, false, kLong, kBlocksOfLong>(a, sms, stream);
 }
 
 }  // namespace
 
-int policy_blocks(int sms) { return sms * kBlocks<kShort>; }
+int policy_blocks(int sms) { return sms * kBlocksOfShort; }
 
 cudaError_t launch_token_log_probs(const PolicyArgs& a, int dtype, int sms, cudaStream_t stream) {
   if (a.rows == 0) return cudaSuccess;

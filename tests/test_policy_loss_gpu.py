@@ -74,7 +74,10 @@ def _check(x, t, old, ref, adv, low=0.2, high=0.3, kl=0.05, weights=None):
     # a row's gradient: w slope (onehot - p): relative errors of the slope and of p (both off by lp's error), then the rounding
     half = torch.finfo(x.dtype).eps / 2
     rel = ((leaf.grad.double() - grad).norm() / grad.norm().clamp(min=1e-300)).item()
-    assert rel <= half + 16 * off, rel
+    # below 2^-14 the numbers of float16 are 2^-24 apart, so each element is off by up to 2^-25 whatever its size: 2^-25 sqrt(elements)
+    # in the norm. (Many long rows are there: 1 / 300 rows / 50000 columns.)
+    small = 2.0**-25 * math.sqrt(keep.sum().item() * x.shape[1]) / grad.norm().clamp(min=1e-300).item() if x.dtype == torch.float16 else 0.0
+    assert rel <= half + 16 * off + small, rel
     assert not leaf.grad[~keep].any()
     with torch.no_grad():
         again, lp2 = ops.policy_loss(leaf, t, old, adv, ref_log_probs=ref, weights=weights, clip_low=low, clip_high=high, kl_weight=kl)
@@ -284,3 +287,10 @@ def test_many_rows_are_counted_alike(rows):
     """Few rows are counted by every block, many by a kernel of their own."""
     x, t, old, ref, adv = _case(rows, 33, torch.float32, seed=18)
     _check(x, t, old, ref, adv)
+
+
+@pytest.mark.parametrize("rows", [297, 460])
+@pytest.mark.parametrize("cols,dtype", [(29001, torch.float32), (57857, torch.float16), (115711, torch.bfloat16), (57857, torch.float32)])
+def test_long_rows_at_every_way_of_holding_them(rows, cols, dtype):
+    """Rows just above what two blocks on an SM hold, just below and above what one does, more of them than run at once."""
+    _check(*_case(rows, cols, dtype, seed=rows + cols))
