@@ -310,12 +310,26 @@ int rbf_b200_token_log_probs(const void* logits, const int64_t* tokens, float* l
  * with w = weights[r], or 1 / number of counting rows where weights is NULL (no such row: NaN); ref_log_probs NULL: no KL term.
  * Writes lp (as above), the loss, and - unless dlogits is NULL - the gradient with respect to the logits (row pitch ld_out,
  * in their dtype, zero for rows that do not count). dlogits needs the alignment of logits modulo 16 bytes in every row.
- * Everything is summed in a fixed order. The workspace is 8-byte aligned. */
+ * Everything is summed in a fixed order. The workspace is 8-byte aligned. float16 gradients that are to be scaled should come from
+ * rbf_b200_loss_gradient: below 2^-25 they are zero here, and no factor brings them back. */
 size_t rbf_b200_policy_loss_workspace_bytes(void);
 int rbf_b200_policy_loss(const void* logits, const int64_t* tokens, const float* old_log_probs, const float* advantages,
                          const float* ref_log_probs, const float* weights, float* loss, float* log_probs, void* dlogits,
                          void* workspace, size_t workspace_bytes, int64_t rows, int cols, int64_t ld, int64_t ld_out,
                          int64_t ignore_index, float clip_low, float clip_high, float kl_weight, int dtype, void* stream);
+
+/* The same without the gradient, but with what it needs: row_stats[2 r] = -log2(sum of e^logits[r]), row_stats[2 r + 1] =
+ * d(loss)/d(lp), zeros for rows that do not count; 8-byte aligned. */
+int rbf_b200_policy_loss_rows(const void* logits, const int64_t* tokens, const float* old_log_probs, const float* advantages,
+                              const float* ref_log_probs, const float* weights, float* loss, float* log_probs, float* row_stats,
+                              void* workspace, size_t workspace_bytes, int64_t rows, int cols, int64_t ld, int64_t ignore_index,
+                              float clip_low, float clip_high, float kl_weight, int dtype, void* stream);
+
+/* dlogits[r] = *factor * row_stats[2 r + 1] * (onehot(tokens[r]) - softmax(logits[r])) of float16 logits, rounded once; zeros for rows
+ * whose token is `ignore_index` or outside [0, cols). `factor` (device memory) is what the loss is scaled by: it comes before the
+ * rounding. dlogits needs the alignment of logits modulo 16 bytes in every row. */
+int rbf_b200_loss_gradient(const void* logits, const int64_t* tokens, const float* row_stats, const float* factor, void* dlogits,
+                           int64_t rows, int cols, int64_t ld, int64_t ld_out, int64_t ignore_index, void* stream);
 
 /* Synchronises `stream` and reads the device status word that the last call using `workspace` left:
  * 0 = ok, otherwise (site << 24 | work unit) of the bounded wait that ran out; the work unit is the linear block

@@ -148,6 +148,15 @@ SIGNATURES = {
         [ctypes.c_void_p] * 10 + [ctypes.c_size_t, ctypes.c_int64, ctypes.c_int] + [ctypes.c_int64] * 3
         + [ctypes.c_float] * 3 + [ctypes.c_int, ctypes.c_void_p],
     ),
+    "rbf_b200_policy_loss_rows": (
+        ctypes.c_int,
+        [ctypes.c_void_p] * 10 + [ctypes.c_size_t, ctypes.c_int64, ctypes.c_int] + [ctypes.c_int64] * 2
+        + [ctypes.c_float] * 3 + [ctypes.c_int, ctypes.c_void_p],
+    ),
+    "rbf_b200_loss_gradient": (
+        ctypes.c_int,
+        [ctypes.c_void_p] * 5 + [ctypes.c_int64, ctypes.c_int] + [ctypes.c_int64] * 3 + [ctypes.c_void_p],
+    ),
     "rbf_b200_post_device_status": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p]),
     "rbf_b200_qkv_prep": (
         ctypes.c_int,

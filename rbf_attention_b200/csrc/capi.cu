@@ -1002,23 +1002,28 @@ size_t rbf_b200_policy_loss_workspace_bytes(void) {
   return sms <= 0 ? 0 : static_cast<size_t>(rbf::policy_blocks(sms)) * (sizeof(double) + sizeof(int));
 }
 
-int rbf_b200_policy_loss(const void* logits, const int64_t* tokens, const float* old_log_probs, const float* advantages,
-                         const float* ref_log_probs, const float* weights, float* loss, float* log_probs, void* dlogits,
-                         void* workspace, size_t workspace_bytes, int64_t rows, int cols, int64_t ld, int64_t ld_out,
-                         int64_t ignore_index, float clip_low, float clip_high, float kl_weight, int dtype, void* stream_v) {
+// dlogits of the alignment of logits modulo 16 bytes in every row
+static int check_dlogits(const void* logits, const void* dlogits, int64_t rows, int cols, int64_t ld, int64_t ld_out, int item) {
+  if (ld_out < cols) return fail(RBF_B200_ERR_BAD_ARGUMENT, "the row pitches must be at least cols");
+  if ((reinterpret_cast<uintptr_t>(logits) - reinterpret_cast<uintptr_t>(dlogits)) % 16 != 0 ||
+      (rows > 1 && (ld - ld_out) * item % 16 != 0))
+    return fail(RBF_B200_ERR_BAD_LAYOUT, "the rows of dlogits must have the alignment of the logits' modulo 16 bytes");
+  return RBF_B200_OK;
+}
+
+static int policy_loss(const void* logits, const int64_t* tokens, const float* old_log_probs, const float* advantages,
+                       const float* ref_log_probs, const float* weights, float* loss, float* log_probs, void* dlogits,
+                       float* row_stats, void* workspace, size_t workspace_bytes, int64_t rows, int cols, int64_t ld,
+                       int64_t ld_out, int64_t ignore_index, float clip_low, float clip_high, float kl_weight, int dtype,
+                       void* stream_v) {
   g_last_error[0] = 0;
   int rc;
   if ((rc = check_logits(logits, tokens, log_probs, rows, cols, ld, dtype))) return rc;
   if (loss == nullptr || (rows > 0 && (!old_log_probs || !advantages)))
     return fail(RBF_B200_ERR_BAD_ARGUMENT, "NULL tensor pointer");
   if (!(clip_low >= 0.f) || !(clip_high >= 0.f)) return fail(RBF_B200_ERR_BAD_ARGUMENT, "clip_low and clip_high must be at least 0");
-  const int item = dtype == 2 ? 4 : 2;
-  if (dlogits != nullptr) {
-    if (ld_out < cols) return fail(RBF_B200_ERR_BAD_ARGUMENT, "the row pitches must be at least cols");
-    if ((reinterpret_cast<uintptr_t>(logits) - reinterpret_cast<uintptr_t>(dlogits)) % 16 != 0 ||
-        (rows > 1 && (ld - ld_out) * item % 16 != 0))
-      return fail(RBF_B200_ERR_BAD_LAYOUT, "the rows of dlogits must have the alignment of the logits' modulo 16 bytes");
-  }
+  if (dlogits != nullptr && (rc = check_dlogits(logits, dlogits, rows, cols, ld, ld_out, dtype == 2 ? 4 : 2))) return rc;
+  if (reinterpret_cast<uintptr_t>(row_stats) % 8 != 0) return fail(RBF_B200_ERR_BAD_LAYOUT, "row_stats must be 8-byte aligned");
   const int sms = sm_count();
   if (sms <= 0) return fail(RBF_B200_ERR_LAUNCH, "cannot read the SM count of the current device");
   if (workspace == nullptr || reinterpret_cast<uintptr_t>(workspace) % 8 != 0 ||
@@ -1026,12 +1031,48 @@ int rbf_b200_policy_loss(const void* logits, const int64_t* tokens, const float*
     return fail(RBF_B200_ERR_WORKSPACE, "workspace is NULL, not 8-byte aligned or too small");
   rbf::PolicyArgs a{};
   a.logits = logits; a.ld = ld; a.tokens = tokens; a.ignore_index = ignore_index; a.log_probs = log_probs;
-  a.rows = rows; a.cols = cols; a.dlogits = dlogits; a.ld_out = ld_out; a.old_log_probs = old_log_probs;
+  a.rows = rows; a.cols = cols; a.dlogits = dlogits; a.ld_out = ld_out; a.row_stats = reinterpret_cast<float2*>(row_stats);
+  a.old_log_probs = old_log_probs;
   a.ref_log_probs = ref_log_probs; a.advantages = advantages; a.weights = weights; a.clip_low = clip_low;
   a.clip_high = clip_high; a.kl_weight = kl_weight; a.loss = loss;
   a.sums = static_cast<double*>(workspace); a.counts = reinterpret_cast<int*>(a.sums + rbf::policy_blocks(sms));
   const cudaError_t e = rbf::launch_policy_loss(a, dtype, sms, static_cast<cudaStream_t>(stream_v));
   if (e != cudaSuccess) return fail(RBF_B200_ERR_LAUNCH, "policy loss launch failed: %s", cudaGetErrorString(e));
+  return RBF_B200_OK;
+}
+
+int rbf_b200_policy_loss(const void* logits, const int64_t* tokens, const float* old_log_probs, const float* advantages,
+                         const float* ref_log_probs, const float* weights, float* loss, float* log_probs, void* dlogits,
+                         void* workspace, size_t workspace_bytes, int64_t rows, int cols, int64_t ld, int64_t ld_out,
+                         int64_t ignore_index, float clip_low, float clip_high, float kl_weight, int dtype, void* stream_v) {
+  return policy_loss(logits, tokens, old_log_probs, advantages, ref_log_probs, weights, loss, log_probs, dlogits, nullptr, workspace,
+                     workspace_bytes, rows, cols, ld, ld_out, ignore_index, clip_low, clip_high, kl_weight, dtype, stream_v);
+}
+
+int rbf_b200_policy_loss_rows(const void* logits, const int64_t* tokens, const float* old_log_probs, const float* advantages,
+                              const float* ref_log_probs, const float* weights, float* loss, float* log_probs, float* row_stats,
+                              void* workspace, size_t workspace_bytes, int64_t rows, int cols, int64_t ld, int64_t ignore_index,
+                              float clip_low, float clip_high, float kl_weight, int dtype, void* stream_v) {
+  if (rows > 0 && row_stats == nullptr) return fail(RBF_B200_ERR_BAD_ARGUMENT, "NULL tensor pointer");
+  return policy_loss(logits, tokens, old_log_probs, advantages, ref_log_probs, weights, loss, log_probs, nullptr, row_stats, workspace,
+                     workspace_bytes, rows, cols, ld, cols, ignore_index, clip_low, clip_high, kl_weight, dtype, stream_v);
+}
+
+int rbf_b200_loss_gradient(const void* logits, const int64_t* tokens, const float* row_stats, const float* factor, void* dlogits,
+                           int64_t rows, int cols, int64_t ld, int64_t ld_out, int64_t ignore_index, void* stream_v) {
+  g_last_error[0] = 0;
+  int rc;
+  if ((rc = check_logits(logits, tokens, row_stats, rows, cols, ld, 1))) return rc;
+  if ((rc = check_dlogits(logits, dlogits, rows, cols, ld, ld_out, 2))) return rc;
+  if (rows == 0) return RBF_B200_OK;
+  if (factor == nullptr || dlogits == nullptr) return fail(RBF_B200_ERR_BAD_ARGUMENT, "NULL tensor pointer");
+  if (reinterpret_cast<uintptr_t>(row_stats) % 8 != 0) return fail(RBF_B200_ERR_BAD_LAYOUT, "row_stats must be 8-byte aligned");
+  rbf::LossGradientArgs a{};
+  a.logits = logits; a.ld = ld; a.tokens = tokens; a.ignore_index = ignore_index;
+  a.row_stats = reinterpret_cast<const float2*>(row_stats); a.factor = factor; a.dlogits = dlogits; a.ld_out = ld_out;
+  a.rows = rows; a.cols = cols;
+  const cudaError_t e = rbf::launch_loss_gradient(a, static_cast<cudaStream_t>(stream_v));
+  if (e != cudaSuccess) return fail(RBF_B200_ERR_LAUNCH, "loss gradient launch failed: %s", cudaGetErrorString(e));
   return RBF_B200_OK;
 }
 

@@ -862,7 +862,8 @@ struct Logits {
   int64_t rows, cols;
   int code;
 
-  Logits(const Args& a, Py_ssize_t i) : x(a.tensor(i, "logits")), tokens(a.tensor(i + 1, "tokens")) {
+  Logits(const Args& a, Py_ssize_t i) : Logits(a.tensor(i, "logits"), a.tensor(i + 1, "tokens")) {}
+  Logits(Tensor logits, Tensor tokens_of_rows) : x(std::move(logits)), tokens(std::move(tokens_of_rows)) {
     TORCH_CHECK(x.is_cuda(), "logits must be a CUDA tensor: rbf_attention_b200 has no CPU path");
     TORCH_CHECK_VALUE(x.dim() == 2 && tokens.dim() == 1 && tokens.size(0) == x.size(0),
                       "logits must be (rows, cols) and tokens (rows,), got ", x.sizes(), " and ", tokens.sizes());
@@ -880,6 +881,13 @@ struct Logits {
     if ((x.stride(1) != 1 && cols > 1) || (rows > 1 && x.stride(0) < cols)) x = x.contiguous();
   }
   int64_t pitch() const { return rows > 1 ? x.stride(0) : cols; }
+  // Its shape, with the same place within 16 bytes for every row of the two; its memory may be longer than it is
+  Tensor gradient() const {
+    const int64_t per16 = 16 / static_cast<int64_t>(x.element_size()), to = cols + (pitch() - cols) % per16;
+    const int64_t shift = reinterpret_cast<uintptr_t>(x.const_data_ptr()) % 16 / x.element_size();
+    if (to == cols && shift == 0) return empty({rows, cols}, x.scalar_type(), x.device());
+    return empty({shift + rows * to}, x.scalar_type(), x.device()).as_strided({rows, cols}, {to, 1}, shift);
+  }
   // fp32 per row, on the device
   Optional per_row(const char* name, Optional t) const {
     if (!t) return t;
@@ -925,9 +933,12 @@ struct PolicyCall {
         kl(static_cast<float>(a.number(8))),
         ignore(a.integer(9)) {}
 
+  // What the backward takes: the gradient, or of float16, whose small numbers a factor has to lift before they are rounded, the
+  // rows' statistics for loss_gradient
+  bool by_rows() const { return in.x.scalar_type() == at::kHalf; }
   struct Result {
     Tensor loss, log_probs;
-    Optional grad;                 // the shape of the logits, their alignment; its memory may be longer than they are
+    Optional saved;
   };
   Result run(bool want_grad) {     // without the lock
     const at::Device dev = in.x.device();
@@ -936,22 +947,23 @@ struct PolicyCall {
     for (Optional* t : {&old, &advantages, &ref, &weights})
       if (*t) *t = (*t)->contiguous();
     Result r{empty({}, at::kFloat, dev), empty({in.rows}, at::kFloat, dev), std::nullopt};
-    int64_t pitch = in.cols;
-    if (want_grad) {
-      // the same place within 16 bytes for every row of the two
-      const int64_t per16 = 16 / static_cast<int64_t>(in.x.element_size());
-      pitch = in.cols + (in.pitch() - in.cols) % per16;
-      const int64_t shift = reinterpret_cast<uintptr_t>(in.x.const_data_ptr()) % 16 / in.x.element_size();
-      if (pitch == in.cols && shift == 0)
-        r.grad = empty({in.rows, in.cols}, in.x.scalar_type(), dev);
-      else
-        r.grad = empty({shift + in.rows * pitch}, in.x.scalar_type(), dev).as_strided({in.rows, in.cols}, {pitch, 1}, shift);
-    }
     const Tensor ws = workspace(rbf_b200_policy_loss_workspace_bytes(), dev);
+    if (want_grad && by_rows()) {
+      r.saved = empty({in.rows, 2}, at::kFloat, dev);
+      const int rc = rbf_b200_policy_loss_rows(in.x.const_data_ptr(), in.tokens.const_data_ptr<int64_t>(), float_ptr(old),
+                                               float_ptr(advantages), float_ptr(ref), float_ptr(weights),
+                                               r.loss.data_ptr<float>(), r.log_probs.data_ptr<float>(),
+                                               r.saved->data_ptr<float>(), ws.data_ptr(), ws.nbytes(), in.rows, in.cols,
+                                               in.pitch(), ignore, low, high, kl, in.code, stream_of(in.x));
+      check(rc, "rbf_b200_policy_loss_rows");
+      return r;
+    }
+    if (want_grad) r.saved = in.gradient();
     const int rc = rbf_b200_policy_loss(in.x.const_data_ptr(), in.tokens.const_data_ptr<int64_t>(), float_ptr(old),
                                         float_ptr(advantages), float_ptr(ref), float_ptr(weights), r.loss.data_ptr<float>(),
-                                        r.log_probs.data_ptr<float>(), r.grad ? r.grad->data_ptr() : nullptr, ws.data_ptr(),
-                                        ws.nbytes(), in.rows, in.cols, in.pitch(), pitch, ignore, low, high, kl, in.code,
+                                        r.log_probs.data_ptr<float>(), want_grad ? r.saved->data_ptr() : nullptr, ws.data_ptr(),
+                                        ws.nbytes(), in.rows, in.cols, in.pitch(),
+                                        want_grad && in.rows > 1 ? r.saved->stride(0) : in.cols, ignore, low, high, kl, in.code,
                                         stream_of(in.x));
     check(rc, "rbf_b200_policy_loss");
     return r;
@@ -959,7 +971,7 @@ struct PolicyCall {
 };
 
 // (logits, tokens, old_log_probs, advantages, ref_log_probs or None, weights or None, clip_low, clip_high, kl_weight,
-// ignore_index, whether the gradient is wanted) -> (loss, log_probs, dlogits or None)
+// ignore_index, whether the gradient is wanted) -> (loss, log_probs, dlogits or - float16 - the rows' statistics or None)
 PyObject* policy_loss(const Args& a) {
   a.expect(11);
   PolicyCall call(a);
@@ -967,7 +979,38 @@ PyObject* policy_loss(const Args& a) {
   Unlocked unlocked;
   const PolicyCall::Result r = call.run(want_grad);
   unlocked.lock();
-  return tuple(wrap(r.loss), wrap(r.log_probs), wrap(r.grad));
+  return tuple(wrap(r.loss), wrap(r.log_probs), wrap(r.saved));
+}
+
+// factor * slope (onehot - softmax) of float16 logits, from the rows' statistics; without the lock
+Tensor loss_gradient(Logits in, const Tensor& stats, const Tensor& factor, int64_t ignore) {
+  const at::Device dev = in.x.device();
+  TORCH_CHECK_VALUE(in.x.scalar_type() == at::kHalf, "loss_gradient: float16 logits, got ", in.x.scalar_type());
+  TORCH_CHECK_VALUE(stats.dim() == 2 && stats.size(0) == in.rows && stats.size(1) == 2 && stats.scalar_type() == at::kFloat &&
+                        stats.is_contiguous() && stats.device() == dev && factor.numel() == 1,
+                    "loss_gradient: contiguous float32 statistics (", in.rows, ", 2) on the device of logits and one factor, got ",
+                    stats.scalar_type(), " ", stats.sizes(), " and ", factor.sizes());
+  const c10::cuda::CUDAGuard guard(dev);
+  const at::NoGradGuard no_grad;
+  in.contiguous();
+  const Tensor f = factor.reshape({1}).to(dev, at::kFloat), grad = in.gradient();
+  const int rc = rbf_b200_loss_gradient(in.x.const_data_ptr(), in.tokens.const_data_ptr<int64_t>(), stats.const_data_ptr<float>(),
+                                        f.const_data_ptr<float>(), grad.data_ptr(), in.rows, in.cols, in.pitch(),
+                                        in.rows > 1 ? grad.stride(0) : in.cols, ignore, stream_of(in.x));
+  check(rc, "rbf_b200_loss_gradient");
+  return grad;
+}
+
+// (logits, tokens, statistics, factor, ignore_index) -> dlogits
+PyObject* loss_gradient_entry(const Args& a) {
+  a.expect(5);
+  Logits in(a, 0);
+  const Tensor stats = a.tensor(2, "row_stats"), factor = a.tensor(3, "factor");
+  const int64_t ignore = a.integer(4);
+  Unlocked unlocked;
+  const Tensor grad = loss_gradient(std::move(in), stats, factor, ignore);
+  unlocked.lock();
+  return wrap(grad);
 }
 
 // A matrix of rows with a pitch, times a factor on the device, in place: the numbers between its rows are its memory too
@@ -982,7 +1025,9 @@ void scale_rows(const Tensor& x, const Tensor& factor) {
 
 // A gradient formed under create_graph from what carries no graph of its own, linked to its origin and not differentiable
 struct FirstOrderOnly : torch::autograd::Function<FirstOrderOnly> {
-  static Tensor forward(torch::autograd::AutogradContext*, const Tensor& grad, const Tensor&) { return grad.view_as(grad); }
+  static Tensor forward(torch::autograd::AutogradContext*, const Tensor& grad, const Tensor&, const Tensor&) {
+    return grad.view_as(grad);
+  }
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext*, const torch::autograd::variable_list&) {
     TORCH_CHECK(false, "Trying to backward through the gradient of policy_loss, which has no second-order formula");
   }
@@ -992,15 +1037,26 @@ struct FirstOrderOnly : torch::autograd::Function<FirstOrderOnly> {
 // registered operator does, without the interpreter (a forward and backward of 33 x 1000 took 100 us with a Python node).
 struct PolicyLoss : torch::autograd::Function<PolicyLoss> {
   static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const Tensor& logits, PolicyCall* call) {
-    (void)logits;                  // the call's, as the graph sees it
+    const Tensor tokens = call->in.tokens;         // as they came
     PolicyCall::Result r = call->run(true);
-    ctx->saved_data["dlogits"] = *r.grad;
+    if (call->by_rows()) {
+      ctx->save_for_backward({logits, tokens, *r.saved});
+      ctx->saved_data["ignore_index"] = call->ignore;
+    } else {
+      ctx->saved_data["dlogits"] = *r.saved;
+    }
     ctx->mark_non_differentiable({r.log_probs});
     ctx->set_materialize_grads(false);
     return {r.loss, r.log_probs};
   }
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
     if (!grads[0].defined()) return {Tensor(), Tensor()};
+    if (const auto ignore = ctx->saved_data.find("ignore_index"); ignore != ctx->saved_data.end()) {
+      const torch::autograd::variable_list held = ctx->get_saved_variables();
+      Tensor dlogits = loss_gradient(Logits(held[0].detach(), held[1]), held[2], grads[0].detach(), ignore->second.toInt());
+      if (at::GradMode::is_enabled()) dlogits = FirstOrderOnly::apply(dlogits, grads[0], held[0]);
+      return {dlogits, Tensor()};
+    }
     const auto saved = ctx->saved_data.find("dlogits");
     // its memory belongs to the first caller, who may have added to it
     TORCH_CHECK(saved != ctx->saved_data.end(), "Trying to backward through policy_loss a second time: the gradient was formed ",
@@ -1008,7 +1064,7 @@ struct PolicyLoss : torch::autograd::Function<PolicyLoss> {
     Tensor dlogits = saved->second.toTensor();
     ctx->saved_data.erase(saved);
     scale_rows(dlogits, grads[0].detach());
-    if (at::GradMode::is_enabled()) dlogits = FirstOrderOnly::apply(dlogits, grads[0]);
+    if (at::GradMode::is_enabled()) dlogits = FirstOrderOnly::apply(dlogits, grads[0], grads[0]);
     return {dlogits, Tensor()};
   }
 };
@@ -1073,6 +1129,7 @@ PyMethodDef methods[] = {
     method<cache_copy_pages>("cache_copy_pages"), method<cache_attention>("cache_attention"),
     method<token_log_probs>("token_log_probs"), method<policy_loss>("policy_loss"),
     method<policy_loss_node>("policy_loss_node"), method<scale_rows_entry>("scale_rows"),
+    method<loss_gradient_entry>("loss_gradient"),
     {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

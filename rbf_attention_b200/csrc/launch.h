@@ -250,6 +250,7 @@ struct PolicyArgs {
   // the loss only
   void* dlogits;             // (rows, cols), row pitch ld_out, or NULL
   int64_t ld_out;
+  float2* row_stats;         // (rows) pairs for launch_loss_gradient, or NULL
   const float* old_log_probs;
   const float* ref_log_probs;  // or NULL: no KL term
   const float* advantages;
@@ -263,6 +264,22 @@ struct PolicyArgs {
 int policy_blocks(int sms);
 cudaError_t launch_token_log_probs(const PolicyArgs& a, int dtype, int sms, cudaStream_t stream);
 cudaError_t launch_policy_loss(const PolicyArgs& a, int dtype, int sms, cudaStream_t stream);
+
+// The gradient of such a loss of float16 logits, times a factor that comes before the rounding. The rows of dlogits have the
+// logits' alignment modulo 16 bytes.
+struct LossGradientArgs {
+  const void* logits;        // (rows, cols), row pitch ld
+  int64_t ld;
+  const int64_t* tokens;
+  int64_t ignore_index;
+  const float2* row_stats;   // (rows): -log2(sum of e^z), d(loss)/d(log-probability)
+  const float* factor;       // one number
+  void* dlogits;             // (rows, cols), row pitch ld_out
+  int64_t ld_out;
+  int64_t rows;
+  int cols;
+};
+cudaError_t launch_loss_gradient(const LossGradientArgs& a, cudaStream_t stream);
 
 cudaError_t launch_wait_selftest(DeviceStatus* status, long long limit, cudaStream_t stream);
 // One thread stores the status word into mapped page-locked host memory (device-side address of the slot).

@@ -3,7 +3,8 @@
 //   kl = e^(ref - lp) - (ref - lp) - 1,     loss = sum over rows of w (kl_weight kl - gain)
 //   d loss / d lp = w (kl_weight (1 - e^(ref - lp)) - [r A <= clipped] r A) = c,   d loss / d z = c (onehot(t) - softmax(z))
 // Everything but the row's lse is a handful of scalars per row, so the gradient is known as soon as the row has been read once:
-// one kernel reads the logits and writes the gradient of the loss, as the cross entropy does. Roofline: HBM. A block owns a
+// one kernel reads the logits and writes the gradient of the loss, as the cross entropy does. (Not of float16 logits, whose numbers
+// end at 2^-24: there the factor that the loss is scaled by comes before the rounding, see loss_gradient_kernel.) Roofline: HBM. A block owns a
 // row, reads it with an online maximum and sum and keeps it in shared memory where it fits; longer rows come a second time out
 // of L2. The rows' bases may have any alignment: a row is a head of single elements up to the first 16-byte
 // boundary, 16-byte words, and a tail. Sums over rows are in 64 bits and in the order of the rows of a block, then of the blocks.
@@ -281,9 +282,11 @@ __global__ void __launch_bounds__(kThreads, kBlocks) policy_loss_kernel(const Po
         loss += static_cast<double>(w) * static_cast<double>(value);
         s_slope = w * slope;
         s_shift = -lse2;
+        if (a.row_stats != nullptr) a.row_stats[row] = make_float2(-lse2, w * slope);
       }
     } else if (tid == 0) {
       a.log_probs[row] = 0.f;
+      if (a.row_stats != nullptr) a.row_stats[row] = make_float2(0.f, 0.f);
     }
     if (a.dlogits == nullptr) {
       __syncthreads();                              // the warps' slots are used again
@@ -351,6 +354,68 @@ __global__ void __launch_bounds__(32) policy_finish_kernel(const PolicyArgs a, c
   *a.loss = static_cast<float>(sum);
 }
 
+// The gradient of a loss whose rows are c (onehot(t) - softmax(z)), from a number pair per row (-log2 of the row's sum of e^z, c) and
+// the factor that reaches the loss, which is multiplied in before the rounding: float16's numbers end at 2^-24, and the elements
+// of a mean over many rows are smaller than that (16384 rows of 50257: 99.5 % of them) until a loss scale lifts them. Roofline: HBM,
+// a read and a write. A block has 16 KB of a row; rows that do not count are zeros and are not read.
+constexpr int kGradThreads = 256, kGradPer = 4, kGradWords = kGradPer * kGradThreads;
+__global__ void __launch_bounds__(kGradThreads) loss_gradient_kernel(const LossGradientArgs a) {
+  using N = Number<1>;
+  using T = N::type;
+  constexpr int V = Cut<T>::kPer;
+  const int tid = threadIdx.x;
+  const float factor = *a.factor;
+  for (int64_t row = blockIdx.y; row < a.rows; row += gridDim.y) {
+    const T* x = static_cast<const T*>(a.logits) + row * a.ld;
+    T* dx = static_cast<T*>(a.dlogits) + row * a.ld_out;
+    const int64_t token = a.tokens[row];
+    const float2 stats = a.row_stats[row];
+    const bool counted = token != a.ignore_index && token >= 0 && token < a.cols;
+    const float shift = stats.x, slope = stats.y * factor;
+    const Cut<T> cut(x, a.cols);
+    const uint4* words = reinterpret_cast<const uint4*>(x + cut.head);
+    uint4* out = reinterpret_cast<uint4*>(dx + cut.head);
+    const int at = static_cast<int>(token) - cut.head, word = counted && at >= 0 ? at / V : -1, in_word = at % V;
+    const int first = static_cast<int>(blockIdx.x) * kGradWords + tid;
+    uint4 raw[kGradPer];
+#pragma unroll
+    for (int k = 0; k < kGradPer; ++k)
+      if (counted && first + k * kGradThreads < cut.words) raw[k] = __ldcs(words + first + k * kGradThreads);
+#pragma unroll
+    for (int k = 0; k < kGradPer; ++k) {
+      const int c = first + k * kGradThreads;
+      uint4 y = make_uint4(0, 0, 0, 0);
+      if (c >= cut.words) break;
+      if (counted) {
+        float v[V];
+        widen16<1>(raw[k], v);
+#pragma unroll
+        for (int i = 0; i < V; i += 2) {
+          float y0, y1;
+          ffma2_bcast(y0, y1, v[i], v[i + 1], kLog2e, shift);
+          fmul2(v[i], v[i + 1], pl_ex2(y0), pl_ex2(y1), -slope, -slope);
+        }
+        if (c == word) {
+#pragma unroll
+          for (int i = 0; i < V; ++i)
+            if (i == in_word) v[i] += slope;
+        }
+        y = make_uint4(pack2<false>(v[0], v[1]), pack2<false>(v[2], v[3]), pack2<false>(v[4], v[5]), pack2<false>(v[6], v[7]));
+      }
+      __stcs(out + c, y);
+    }
+    if (blockIdx.x == 0 && tid < cut.head + a.cols - cut.body) {
+      const int single = tid < cut.head ? tid : cut.body + tid - cut.head;
+      float v = 0.f;
+      if (counted) {
+        v = -slope * pl_ex2(fmaf(N::widen(x[single]), kLog2e, shift));
+        if (single == token) v += slope;
+      }
+      dx[single] = N::narrow(v);
+    }
+  }
+}
+
 template <int kDtype, int kThreads>
 cudaError_t log_probs_t(const PolicyArgs& a, int sms, cudaStream_t stream) {
   const int64_t most = static_cast<int64_t>(sms) * (2048 / kThreads);
@@ -410,6 +475,14 @@ cudaError_t launch_token_log_probs(const PolicyArgs& a, int dtype, int sms, cuda
     case 2: return log_probs_of<2>(a, sms, stream);
     default: return cudaErrorInvalidValue;
   }
+}
+
+cudaError_t launch_loss_gradient(const LossGradientArgs& a, cudaStream_t stream) {
+  if (a.rows == 0) return cudaSuccess;
+  const int words = a.cols / 8, chunks = words / kGradWords + 1;
+  const dim3 grid(chunks, static_cast<unsigned>(a.rows < 65535 ? a.rows : 65535));
+  loss_gradient_kernel<<<grid, kGradThreads, 0, stream>>>(a);
+  return cudaGetLastError();
 }
 
 cudaError_t launch_policy_loss(const PolicyArgs& a, int dtype, int sms, cudaStream_t stream) {

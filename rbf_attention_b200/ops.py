@@ -1102,25 +1102,48 @@ def _policy_loss_fwd(logits: torch.Tensor, tokens: torch.Tensor, old_log_probs: 
                      ref_log_probs: torch.Tensor | None, weights: torch.Tensor | None, clip_low: float, clip_high: float,
                      kl_weight: float, ignore_index: int,
                      with_grad: bool) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
-    """(loss, log_probs, d(loss)/d(logits)) from one pass over the logits; without the gradient an empty tensor for it."""
-    loss, log_probs, dlogits = _lib.host().policy_loss(logits, tokens, old_log_probs, advantages, ref_log_probs, weights,
-                                                       clip_low, clip_high, kl_weight, ignore_index, with_grad)
-    return loss, log_probs, logits.new_empty(0) if dlogits is None else dlogits
+    """(loss, log_probs, what the backward takes) from one pass over the logits: d(loss)/d(logits), or of float16 logits the rows'
+    statistics for ``loss_gradient`` - a factor on the loss has to come before the rounding to a type whose numbers end at 2^-24 -,
+    or without ``with_grad`` an empty tensor."""
+    loss, log_probs, saved = _lib.host().policy_loss(logits, tokens, old_log_probs, advantages, ref_log_probs, weights,
+                                                     clip_low, clip_high, kl_weight, ignore_index, with_grad)
+    return loss, log_probs, logits.new_empty(0) if saved is None else saved
 
 
 policy_loss_fwd = torch.library.custom_op("rbf_attn_b200::policy_loss_fwd", mutates_args=())(_policy_loss_fwd)
 
 
+def _fake_dlogits(logits):
+    rows, cols = logits.shape
+    pitch = logits.stride(0) if rows > 1 and logits.stride(1) == 1 and logits.stride(0) >= cols else cols
+    pitch = cols + (pitch - cols) % (16 // logits.element_size())       # each row's place within 16 bytes is the logits'
+    return torch.empty_strided((rows, cols), (pitch, 1), dtype=logits.dtype, device=logits.device)
+
+
 @policy_loss_fwd.register_fake
 def _(logits, tokens, old_log_probs, advantages, ref_log_probs, weights, clip_low, clip_high, kl_weight, ignore_index, with_grad):
-    rows, cols = logits.shape
-    if with_grad:
-        pitch = logits.stride(0) if rows > 1 and logits.stride(1) == 1 and logits.stride(0) >= cols else cols
-        pitch = cols + (pitch - cols) % (16 // logits.element_size())       # each row's place within 16 bytes is the logits'
-        dlogits = torch.empty_strided((rows, cols), (pitch, 1), dtype=logits.dtype, device=logits.device)
+    rows = logits.shape[0]
+    if not with_grad:
+        saved = logits.new_empty(0)
+    elif logits.dtype == torch.float16:
+        saved = logits.new_empty((rows, 2), dtype=torch.float32)
     else:
-        dlogits = logits.new_empty(0)
-    return logits.new_empty((), dtype=torch.float32), logits.new_empty(rows, dtype=torch.float32), dlogits
+        saved = _fake_dlogits(logits)
+    return logits.new_empty((), dtype=torch.float32), logits.new_empty(rows, dtype=torch.float32), saved
+
+
+def _loss_gradient(logits: torch.Tensor, tokens: torch.Tensor, row_stats: torch.Tensor, factor: torch.Tensor,
+                   ignore_index: int) -> torch.Tensor:
+    """factor * slope * (onehot(tokens) - softmax(logits)) of float16 logits, rounded once, from a forward's statistics."""
+    return _lib.host().loss_gradient(logits, tokens, row_stats, factor, ignore_index)
+
+
+loss_gradient = torch.library.custom_op("rbf_attn_b200::loss_gradient", mutates_args=())(_loss_gradient)
+
+
+@loss_gradient.register_fake
+def _(logits, tokens, row_stats, factor, ignore_index):
+    return _fake_dlogits(logits)
 
 
 def _scale_rows(x: torch.Tensor, factor: torch.Tensor) -> None:
@@ -1132,8 +1155,10 @@ scale_rows_ = torch.library.custom_op("rbf_attn_b200::scale_rows_", mutates_args
 
 
 def _policy_setup_context(ctx, inputs, output):
-    ctx.save_for_backward(output[2])        # an output, so that under create_graph it is linked to the logits
-    ctx.with_grad = inputs[10]
+    ctx.by_rows = inputs[0].dtype == torch.float16 and inputs[10]
+    # without the logits an output, so that under create_graph it is linked to them
+    ctx.save_for_backward(*((inputs[0], inputs[1], output[2]) if ctx.by_rows else (output[2],)))
+    ctx.with_grad, ctx.ignore_index = inputs[10], inputs[9]
     ctx.taken = False
     ctx.mark_non_differentiable(output[1])
     ctx.set_materialize_grads(False)        # no zero tensor of the logits' size for the unused third output
@@ -1145,6 +1170,10 @@ def _policy_backward(ctx, g_loss, _g_log_probs, _g_dlogits):
         return nothing
     if not ctx.with_grad:
         raise RuntimeError("policy_loss was called without the gradient")
+    if ctx.by_rows:
+        logits, tokens, stats = ctx.saved_tensors
+        gradient = _loss_gradient if _direct_backward(logits, tokens, stats, g_loss) else torch.ops.rbf_attn_b200.loss_gradient
+        return (gradient(logits, tokens, stats, g_loss, ctx.ignore_index), *nothing[1:])
     if ctx.taken:           # its memory belongs to the first caller, who may have added to it
         raise RuntimeError("Trying to backward through policy_loss a second time: the gradient was formed by the forward and "
                            "has been handed out; call policy_loss again")
@@ -1163,14 +1192,15 @@ torch.library.register_autograd("rbf_attn_b200::policy_loss_fwd", _policy_backwa
 def policy_loss(logits, tokens, old_log_probs, advantages, ref_log_probs=None, weights=None, clip_low: float = 0.2,
                 clip_high: float = 0.2, kl_weight: float = 0.0, ignore_index: int = -100):
     """Clipped policy loss of 2-D CUDA logits: returns (loss, log_probs), the loss an fp32 scalar whose gradient with respect to
-    the logits is formed by the same kernel that reads them, log_probs (rows,) without a gradient. Per row, with
+    the logits is formed by the same kernel that reads them (but see float16), log_probs (rows,) without a gradient. Per row, with
     ``lp = log_softmax(logits)[tokens]`` and ``r = exp(lp - old_log_probs)``,
 
         w * (kl_weight * (exp(ref - lp) - (ref - lp) - 1) - min(r * A, clip(r, 1 - clip_low, 1 + clip_high) * A))
 
     summed over the rows whose token counts (not ``ignore_index``, a column); ``w`` is ``weights`` or, without them, 1 / number of
     those rows (none: the loss is NaN, the gradient zero). The KL term needs ``ref_log_probs``. old_log_probs, advantages,
-    ref_log_probs and weights are float32 (rows,) constants. The gradient can be taken once."""
+    ref_log_probs and weights are float32 (rows,) constants. The gradient can be taken once. Of float16 logits it is formed by the
+    backward, which reads them again: a loss scale is multiplied in before the rounding, not after it."""
     for name, t in (("old_log_probs", old_log_probs), ("advantages", advantages), ("ref_log_probs", ref_log_probs),
                     ("weights", weights)):
         if _needs_grad(t):
