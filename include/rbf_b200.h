@@ -254,6 +254,12 @@ int rbf_b200_cross_entropy(const void* logits, const int64_t* targets, const flo
                            void* dlogits, int rows, int cols, int64_t ld, int64_t ld_out, int64_t ignore_index,
                            int dtype, void* stream);
 
+/* The losses of float16 logits, with what rbf_b200_loss_gradient takes in place of the gradient: row_stats[2 r] = -log2(sum of
+ * e^logits[r]), row_stats[2 r + 1] = -*grad_scale, zeros for rows that do not count; 8-byte aligned. Rounded before a factor on the
+ * loss is multiplied in, as by rbf_b200_cross_entropy, what is below 2^-25 of the gradient is lost. */
+int rbf_b200_cross_entropy_rows(const void* logits, const int64_t* targets, const float* grad_scale, float* loss_rows,
+                                float* row_stats, int rows, int cols, int64_t ld, int64_t ignore_index, void* stream);
+
 /* x[0..n) *= *factor, decided on the device: when *factor == 1 (the gradient of a loss that is the graph's output)
  * the kernel returns without touching x. Used by the backward of the cross entropy above. */
 int rbf_b200_scale_unless_one(void* x, const float* factor, int64_t n, int dtype, void* stream);

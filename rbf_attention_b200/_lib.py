@@ -119,6 +119,10 @@ SIGNATURES = {
         [ctypes.c_void_p] * 5 + [ctypes.c_int, ctypes.c_int, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, ctypes.c_int,
                                  ctypes.c_void_p],
     ),
+    "rbf_b200_cross_entropy_rows": (
+        ctypes.c_int,
+        [ctypes.c_void_p] * 5 + [ctypes.c_int, ctypes.c_int, ctypes.c_int64, ctypes.c_int64, ctypes.c_void_p],
+    ),
     "rbf_b200_scale_unless_one": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int64, ctypes.c_int,
                                                  ctypes.c_void_p]),
     "rbf_b200_cache_page_bytes": (ctypes.c_size_t, [ctypes.c_int]),

@@ -805,6 +805,25 @@ int rbf_b200_cross_entropy(const void* logits, const int64_t* targets, const flo
   return RBF_B200_OK;
 }
 
+int rbf_b200_cross_entropy_rows(const void* logits, const int64_t* targets, const float* grad_scale, float* loss_rows,
+                                float* row_stats, int rows, int cols, int64_t ld, int64_t ignore_index, void* stream_v) {
+  g_last_error[0] = 0;
+  if (rows < 0 || cols <= 0) return fail(RBF_B200_ERR_BAD_ARGUMENT, "rows must be >= 0 and cols > 0");
+  if (ld < cols) return fail(RBF_B200_ERR_BAD_ARGUMENT, "the row pitch must be at least cols");
+  if (rows == 0) return RBF_B200_OK;
+  if (!logits || !targets || !grad_scale || !loss_rows || !row_stats)
+    return fail(RBF_B200_ERR_BAD_ARGUMENT, "NULL tensor pointer");
+  if (reinterpret_cast<uintptr_t>(row_stats) % 8 != 0) return fail(RBF_B200_ERR_BAD_LAYOUT, "row_stats must be 8-byte aligned");
+  const int sms = sm_count();
+  if (sms <= 0) return fail(RBF_B200_ERR_LAUNCH, "cannot read the SM count of the current device");
+  rbf::CrossEntropyArgs a{};
+  a.logits = logits; a.ld = ld; a.targets = targets; a.row_stats = reinterpret_cast<float2*>(row_stats);
+  a.loss_rows = loss_rows; a.grad_scale = grad_scale; a.rows = rows; a.cols = cols; a.ignore_index = ignore_index;
+  const cudaError_t e = rbf::launch_cross_entropy_rows(a, sms, static_cast<cudaStream_t>(stream_v));
+  if (e != cudaSuccess) return fail(RBF_B200_ERR_LAUNCH, "cross entropy launch failed: %s", cudaGetErrorString(e));
+  return RBF_B200_OK;
+}
+
 int rbf_b200_scale_unless_one(void* x, const float* factor, int64_t n, int dtype, void* stream_v) {
   g_last_error[0] = 0;
   if (n < 0) return fail(RBF_B200_ERR_BAD_ARGUMENT, "n must be >= 0");

@@ -86,9 +86,11 @@ __device__ __forceinline__ float chunk_max(const uint4& raw) {
 
 constexpr int kCeStageBytes = 113 * 1024;          // a staged row leaves room for a second block on the SM
 
-template <int kDtype, bool kVec, bool kStage>
+// kRows: two numbers per row for launch_loss_gradient in place of the gradient. Of float16 logits the factor on the loss has to come
+// before the rounding: in a mean over many rows most elements are below the type's 2^-24.
+template <int kDtype, bool kVec, bool kStage, bool kRows = false>
 __global__ void __launch_bounds__(kCeThreads, 2) cross_entropy_kernel(const CrossEntropyArgs a) {
-  static_assert(kVec || !kStage, "staging uses the vector path");
+  static_assert((kVec && !kRows) || !kStage, "staging uses the vector path, for a second pass");
   extern __shared__ uint4 s_row[];                // kStage: the row, every 16-byte chunk kept by the thread that read it
   using E = Elem<kDtype>;
   using T = typename E::type;
@@ -108,7 +110,9 @@ __global__ void __launch_bounds__(kCeThreads, 2) cross_entropy_kernel(const Cros
     if (more) t_next = a.targets[row + gridDim.x];
     const bool next_counts = more && counted(t_next);
     if (!counted(t)) {                                // no loss, zero gradient: the row is not read
-      if constexpr (kVec) {
+      if constexpr (kRows) {
+        if (threadIdx.x == 0) a.row_stats[row] = make_float2(0.f, 0.f);
+      } else if constexpr (kVec) {
         for (int c = threadIdx.x; c < a.cols / V; c += kCeThreads) reinterpret_cast<uint4*>(dx)[c] = make_uint4(0, 0, 0, 0);
       } else {
         for (int c = threadIdx.x; c < a.cols; c += kCeThreads) dx[c] = E::from_float(0.f);
@@ -181,9 +185,11 @@ __global__ void __launch_bounds__(kCeThreads, 2) cross_entropy_kernel(const Cros
         const float lse2 = m + log2f(s);          // log2 of the sum of 2^y; +inf / nan rows propagate as they are
         s_lse2 = lse2;
         a.loss_rows[row] = (lse2 - E::to_float(x[t]) * kLog2e) * kLn2;
+        if constexpr (kRows) a.row_stats[row] = make_float2(-lse2, -scale);
       }
     }
     __syncthreads();
+    if constexpr (kRows) continue;
     const float lse2 = s_lse2;
     const float shift = log2f(scale) - lse2;       // scale > 0 whenever a row counts
     // ---- pass 2: gradient of the mean loss ------------------------------------------------------------------------
@@ -289,6 +295,15 @@ cudaError_t launch_cross_entropy(const CrossEntropyArgs& a, int dtype, int sms, 
     case 2: return launch_ce_t<2>(a, sms, stream);
     default: return cudaErrorInvalidValue;
   }
+}
+
+cudaError_t launch_cross_entropy_rows(const CrossEntropyArgs& a, int sms, cudaStream_t stream) {
+  if (a.rows == 0) return cudaSuccess;
+  const bool vec = a.cols % 8 == 0 && a.ld % 8 == 0 && reinterpret_cast<uintptr_t>(a.logits) % 16 == 0;
+  const int grid = a.rows < sms * 2 ? a.rows : sms * 2;
+  if (vec) cross_entropy_kernel<1, true, false, true><<<grid, kCeThreads, 0, stream>>>(a);
+  else cross_entropy_kernel<1, false, false, true><<<grid, kCeThreads, 0, stream>>>(a);
+  return cudaGetLastError();
 }
 
 cudaError_t launch_scale_unless_one(void* x, const float* factor, int64_t n, int dtype, int sms, cudaStream_t stream) {

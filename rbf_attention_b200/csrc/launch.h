@@ -176,8 +176,11 @@ struct CrossEntropyArgs {
   const float* grad_scale;   // device scalar multiplied into every gradient (1 / number of rows that count)
   int rows, cols;
   int64_t ignore_index;
+  float2* row_stats;         // of launch_cross_entropy_rows: (rows) pairs for launch_loss_gradient
 };
 cudaError_t launch_cross_entropy(const CrossEntropyArgs& a, int dtype, int sms, cudaStream_t stream);
+// The losses of float16 logits and, in place of dlogits, row_stats.
+cudaError_t launch_cross_entropy_rows(const CrossEntropyArgs& a, int sms, cudaStream_t stream);
 // x *= *factor unless *factor == 1 (decided on the device: nothing synchronises).
 cudaError_t launch_scale_unless_one(void* x, const float* factor, int64_t n, int dtype, int sms, cudaStream_t stream);
 

@@ -973,10 +973,8 @@ def add_layer_norm(x, residual, weight, bias, eps: float = 1e-5):
 _CE_DTYPE = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 
 
-def _cross_entropy_fwd(logits: torch.Tensor, targets: torch.Tensor, ignore_index: int) -> tuple[torch.Tensor, torch.Tensor]:
-    """Mean cross entropy over the rows whose target is not ``ignore_index`` (fp32 scalar) and its gradient with
-    respect to ``logits`` (same shape and dtype), from one pass: logits (rows, cols) with unit column stride,
-    targets (rows,) int64."""
+def _ce_inputs(logits, targets, ignore_index):
+    """Checked: (logits with dense rows, targets, 1 / number of rows that count)."""
     if logits.dim() != 2 or targets.dim() != 1 or targets.shape[0] != logits.shape[0]:
         raise ValueError(f"logits must be (rows, cols) and targets (rows,), got {tuple(logits.shape)}, {tuple(targets.shape)}")
     if not logits.is_cuda or targets.device != logits.device:
@@ -989,7 +987,15 @@ def _cross_entropy_fwd(logits: torch.Tensor, targets: torch.Tensor, ignore_index
     x = logits if logits.stride(1) == 1 and (rows <= 1 or logits.stride(0) >= cols) else logits.contiguous()
     t = targets.contiguous()
     counted = ((t != ignore_index) & (t >= 0) & (t < cols)).sum()
-    grad_scale = 1.0 / counted.to(torch.float32)          # no counted row: inf * 0 = nan, as torch's mean of nothing
+    return x, t, 1.0 / counted.to(torch.float32)          # no counted row: inf * 0 = nan, as torch's mean of nothing
+
+
+def _cross_entropy_fwd(logits: torch.Tensor, targets: torch.Tensor, ignore_index: int) -> tuple[torch.Tensor, torch.Tensor]:
+    """Mean cross entropy over the rows whose target is not ``ignore_index`` (fp32 scalar) and its gradient with
+    respect to ``logits`` (same shape and dtype), from one pass: logits (rows, cols) with unit column stride,
+    targets (rows,) int64."""
+    x, t, grad_scale = _ce_inputs(logits, targets, ignore_index)
+    rows, cols = x.shape
     loss_rows = torch.empty(rows, dtype=torch.float32, device=x.device)
     dlogits = torch.empty((rows, cols), dtype=x.dtype, device=x.device)
     with _OnDevice(x.device):
@@ -1061,9 +1067,72 @@ class _CrossEntropy(torch.autograd.Function):
         return _ce_backward(ctx, g_loss, g_dlogits)
 
 
+def _cross_entropy_rows(logits: torch.Tensor, targets: torch.Tensor, ignore_index: int) -> tuple[torch.Tensor, torch.Tensor]:
+    """``_cross_entropy_fwd`` of float16 logits with the rows' statistics for ``loss_gradient`` in place of the gradient."""
+    x, t, grad_scale = _ce_inputs(logits, targets, ignore_index)
+    if x.dtype != torch.float16:
+        raise ValueError(f"unsupported dtype {x.dtype} (float16)")
+    rows, cols = x.shape
+    loss_rows = torch.empty(rows, dtype=torch.float32, device=x.device)
+    stats = torch.empty((rows, 2), dtype=torch.float32, device=x.device)
+    with _OnDevice(x.device):
+        rc = _lib.load().rbf_b200_cross_entropy_rows(
+            x.data_ptr(), t.data_ptr(), grad_scale.data_ptr(), loss_rows.data_ptr(), stats.data_ptr(), rows, cols,
+            x.stride(0) if rows > 1 else cols, int(ignore_index), _stream_ptr(x.device))
+    _lib.check(rc, "rbf_b200_cross_entropy_rows")
+    return loss_rows.sum() * grad_scale, stats
+
+
+cross_entropy_rows = torch.library.custom_op("rbf_attn_b200::cross_entropy_rows", mutates_args=())(_cross_entropy_rows)
+
+
+@cross_entropy_rows.register_fake
+def _(logits, targets, ignore_index):
+    return logits.new_empty((), dtype=torch.float32), logits.new_empty((logits.shape[0], 2), dtype=torch.float32)
+
+
+def _ce_rows_setup_context(ctx, inputs, output):
+    ctx.save_for_backward(inputs[0], inputs[1], output[1])
+    ctx.ignore_index = inputs[2]
+    ctx.mark_non_differentiable(output[1])
+    ctx.set_materialize_grads(False)
+
+
+def _ce_rows_backward(ctx, g_loss, _g_stats):
+    if g_loss is None:
+        return None, None, None
+    logits, targets, stats = ctx.saved_tensors
+    gradient = _loss_gradient if _direct_backward(logits, targets, stats, g_loss) else torch.ops.rbf_attn_b200.loss_gradient
+    return gradient(logits, targets, stats, g_loss, ctx.ignore_index), None, None
+
+
+torch.library.register_autograd("rbf_attn_b200::cross_entropy_rows", _ce_rows_backward, setup_context=_ce_rows_setup_context)
+
+
+class _CrossEntropyRows(torch.autograd.Function):
+    """``rbf_attn_b200::cross_entropy_rows`` and its autograd formula for calls that go around the operator."""
+
+    @staticmethod
+    def forward(ctx, logits, targets, ignore_index):
+        output = _cross_entropy_rows(logits, targets, ignore_index)
+        _ce_rows_setup_context(ctx, (logits, targets, ignore_index), output)
+        return output
+
+    @staticmethod
+    def backward(ctx, g_loss, g_stats):
+        return _ce_rows_backward(ctx, g_loss, g_stats)
+
+
 def cross_entropy(logits, targets, ignore_index: int = -100):
     """``F.cross_entropy(logits, targets, ignore_index=ignore_index)`` (mean reduction) for 2-D CUDA logits, with the
-    gradient produced by the forward kernel."""
+    gradient produced by the forward kernel; of float16 logits by the backward, which reads them again, so that a loss scale
+    is multiplied in before the rounding and not after it."""
+    if logits.dtype == torch.float16:
+        if type(ignore_index) is int and _direct(logits, targets):
+            if _needs_grad(logits):
+                return _CrossEntropyRows.apply(logits, targets, ignore_index)[0]
+            return _cross_entropy_rows(logits, targets, ignore_index)[0]
+        return torch.ops.rbf_attn_b200.cross_entropy_rows(logits, targets, ignore_index)[0]
     if type(ignore_index) is int and _direct(logits, targets):
         if _needs_grad(logits):
             return _CrossEntropy.apply(logits, targets, ignore_index)[0]
