@@ -1023,7 +1023,8 @@ void scale_rows(const Tensor& x, const Tensor& factor) {
   check(rc, "rbf_b200_scale_unless_one");
 }
 
-// A gradient formed under create_graph from what carries no graph of its own, linked to its origin and not differentiable
+// A gradient formed under create_graph from what carries no graph of its own, linked to its origins - the factor, and a tensor that
+// leads to the logits: with the factor alone, which mostly is a constant, it would be one too - and not differentiable
 struct FirstOrderOnly : torch::autograd::Function<FirstOrderOnly> {
   static Tensor forward(torch::autograd::AutogradContext*, const Tensor& grad, const Tensor&, const Tensor&) {
     return grad.view_as(grad);
@@ -1042,12 +1043,16 @@ struct PolicyLoss : torch::autograd::Function<PolicyLoss> {
     if (call->by_rows()) {
       ctx->save_for_backward({logits, tokens, *r.saved});
       ctx->saved_data["ignore_index"] = call->ignore;
-    } else {
-      ctx->saved_data["dlogits"] = *r.saved;
+      ctx->mark_non_differentiable({r.log_probs});
+      ctx->set_materialize_grads(false);
+      return {r.loss, r.log_probs};
     }
+    // an output, though nobody gets it: the graph leads from it to the logits, which are not kept
+    ctx->save_for_backward({*r.saved});
+    ctx->saved_data["taken"] = false;
     ctx->mark_non_differentiable({r.log_probs});
     ctx->set_materialize_grads(false);
-    return {r.loss, r.log_probs};
+    return {r.loss, r.log_probs, *r.saved};
   }
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
     if (!grads[0].defined()) return {Tensor(), Tensor()};
@@ -1057,14 +1062,14 @@ struct PolicyLoss : torch::autograd::Function<PolicyLoss> {
       if (at::GradMode::is_enabled()) dlogits = FirstOrderOnly::apply(dlogits, grads[0], held[0]);
       return {dlogits, Tensor()};
     }
-    const auto saved = ctx->saved_data.find("dlogits");
     // its memory belongs to the first caller, who may have added to it
-    TORCH_CHECK(saved != ctx->saved_data.end(), "Trying to backward through policy_loss a second time: the gradient was formed ",
+    TORCH_CHECK(!ctx->saved_data["taken"].toBool(), "Trying to backward through policy_loss a second time: the gradient was formed ",
                 "by the forward and has been handed out; call policy_loss again");
-    Tensor dlogits = saved->second.toTensor();
-    ctx->saved_data.erase(saved);
+    const Tensor held = ctx->get_saved_variables()[0];
+    ctx->saved_data["taken"] = true;
+    Tensor dlogits = held.detach();
     scale_rows(dlogits, grads[0].detach());
-    if (at::GradMode::is_enabled()) dlogits = FirstOrderOnly::apply(dlogits, grads[0], grads[0]);
+    if (at::GradMode::is_enabled()) dlogits = FirstOrderOnly::apply(dlogits, grads[0], held);
     return {dlogits, Tensor()};
   }
 };
