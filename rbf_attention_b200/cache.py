@@ -22,7 +22,8 @@ class PagedCache:
     scale per block and head, the last few tokens of a sequence in ``dtype``.
 
     ``pages`` (layers, pages, heads, bytes), ``page_table`` (max_sequences, pages of a sequence) and ``lengths`` (max_sequences,)
-    stay where they are: a CUDA graph of a step on all sequences can be replayed between ``begin`` and ``end``."""
+    stay where they are: a CUDA graph of a step on all sequences can be replayed between ``begin`` and ``end`` (or ``abort``, which
+    takes a cache whose ``append`` has been captured to have been written)."""
 
     def __init__(self, num_layers: int, num_heads: int, head_dim: int, max_sequences: int, max_length: int,
                  num_pages: int | None = None, dtype: torch.dtype = torch.bfloat16, device="cuda"):
@@ -41,6 +42,7 @@ class PagedCache:
         self._users = [0] * num_pages                           # sequences that have the page
         self._free = list(range(num_pages))                     # a heap: low pages first
         self._step = None
+        self._captured = False                                  # a graph may append: nothing is seen of its replays
 
     # -- what there is ---------------------------------------------------------------------------
     @property
@@ -184,6 +186,7 @@ class PagedCache:
         self._check_rows("k", k, counts)
         self._check_rows("v", v, counts)
         self._written = True
+        self._captured = self._captured or ops.capturing(self.pages.device)
         ops.cache_append(self._layer(layer), table, lengths, k, v, self._fresh(k, counts, fresh))
 
     def attend(self, layer: int, q: torch.Tensor, softmax: bool = True) -> torch.Tensor:
@@ -207,12 +210,14 @@ class PagedCache:
             self.lengths.index_add_(0, at, torch.full_like(at, more, dtype=torch.int32))
         self._step = None
 
-    def abort(self) -> None:
+    def abort(self, written: bool | None = None) -> None:
         """Leaves the step without its tokens. If any layer has been written, the step's sequences are freed: tokens that fill a
-        block up take the place of the ones that were held in 16 bits until then. Otherwise the pages for them are free again."""
+        block up take the place of the ones that were held in 16 bits until then. Otherwise the pages for them are free again.
+        ``written``: whether one has been. Without it, if ``append`` was called in the step, or ever while a graph was captured, which
+        may have been replayed in it; operators that were called on ``pages`` directly are the caller's to tell."""
         batch, counts, *_ = self._current("abort()")
-        written, self._step = self._written, None
-        if written:
+        self._step = None
+        if self._written or self._captured if written is None else written:
             self.free([s for s, n in zip(batch, counts) if n])
             return
         for s in batch:

@@ -81,6 +81,11 @@ def _tma_ready(t: torch.Tensor) -> torch.Tensor:
     return _lib.host().tma_ready(t)
 
 
+def capturing(device: torch.device) -> bool:
+    """Whether what is enqueued on the device's current stream goes into a graph."""
+    return device.type == "cuda" and _lib.host().capturing(_device_index(device))
+
+
 def _device_index(device: torch.device) -> int:
     return device.index if device.index is not None else torch._C._cuda_getDevice()
 
