@@ -242,7 +242,7 @@ class CausalLM(nn.Module):
             raise ValueError(f"prompts {tuple(idx.shape)} of {lengths} tokens, {max_new_tokens} new ones, {samples} samples")
         rows = bsz * samples
         if cache is None:
-            cache = self.new_cache(rows, max(lengths) + max_new_tokens)
+            cache = self.new_cache(rows, max(lengths) + max_new_tokens - 1)        # the last ids are not read again
         if cache.max_sequences != rows or any(cache.length(s) for s in range(rows)):
             raise ValueError(f"the cache must be an empty one of {rows} sequences")
 
