@@ -190,7 +190,8 @@ class CausalLM(nn.Module):
     def forward_cached(self, idx, cache: PagedCache, new=None, sequences=None, all_logits: bool = False):
         """Logits (batch, vocab) behind each sequence's last new token - with ``all_logits`` (batch, T, vocab) behind every one -
         of the ``idx`` (batch, T) that follow what ``cache`` holds; ``new``: how many of the T are real, per sequence (default:
-        all), ``sequences``: which of the cache's these are (default: all). Either all or none of those that get tokens are
+        all; what is behind them is padding, which may be longer than the model's positions and has logits of zero or no meaning),
+        ``sequences``: which of the cache's these are (default: all). Either all or none of those that get tokens are
         empty. A sequence without new tokens has logits of no meaning. If it raises, no sequence has got tokens; where a layer had
         been written, those that would have got some are empty (``PagedCache.abort``)."""
         bsz, seq = idx.shape
@@ -204,6 +205,8 @@ class CausalLM(nn.Module):
         from_empty = empty == {True}
         self._check_positions(max((cache.length(s) + n - (0 if from_empty else self.num_registers) for s, n in zip(batch, new) if n),
                                   default=0))
+        idx = idx[:, :max([1, *new])]          # no sequence has a place for what is behind
+        cut, seq = seq - idx.shape[1], idx.shape[1]
         skip = self.num_registers if from_empty else 0
         cache.begin([n + skip if n else 0 for n in new], sequences)
         try:
@@ -223,6 +226,8 @@ class CausalLM(nn.Module):
                 last = torch.tensor([skip + max(n - 1, 0) for n in new]).to(idx.device)
                 normed = normed[torch.arange(bsz, device=idx.device), last]
             logits = vocab_projection(self.to_logits, normed)
+            if all_logits and cut:
+                logits = F.pad(logits, (0, 0, 0, cut))
         except BaseException:
             cache.abort()
             raise
