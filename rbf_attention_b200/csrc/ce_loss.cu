@@ -84,7 +84,8 @@ __device__ __forceinline__ float chunk_max(const uint4& raw) {
   }
 }
 
-constexpr int kCeStageBytes = 113 * 1024;          // a staged row leaves room for a second block on the SM
+// A staged row leaves room for a second block on the SM: of its 228 KB every block has 1 KB that is the system's, and its static arrays.
+constexpr int kCeStageBytes = 228 * 1024 / 2 - 1024 - 512;
 
 // kRows: two numbers per row for launch_loss_gradient in place of the gradient. Of float16 logits the factor on the loss has to come
 // before the rounding: in a mean over many rows most elements are below the type's 2^-24.

@@ -28,7 +28,8 @@ namespace {
 constexpr int kLong = 512, kShort = 128;
 constexpr int kShortBytes = 24 * 1024;              // of a row
 constexpr int kBlocksOfShort = 8, kBlocksOfLong = 2;
-constexpr int kStageBytes = 113 * 1024;             // a staged row leaves room for a second block on the SM
+// A staged row leaves room for a second block on the SM: of its 228 KB every block has 1 KB that is the system's, and its static arrays.
+constexpr int kStageBytes = 228 * 1024 / 2 - 1024 - 512;
 // Longer ones have the SM alone, unless all rows run at once two to an SM and unstaged (float32 x 50257: 5000 rows 396 us, read a
 // second time by two blocks on an SM 453; 200 rows 26 and 23; 3000 x 100000 bfloat16 242 and 295).
 constexpr int kAloneBytes = 226 * 1024;
