@@ -89,8 +89,11 @@ constexpr int kCeStageBytes = 228 * 1024 / 2 - 1024 - 512;
 
 // kRows: two numbers per row for launch_loss_gradient in place of the gradient. Of float16 logits the factor on the loss has to come
 // before the rounding: in a mean over many rows most elements are below the type's 2^-24.
+// A row is read once: four blocks on an SM. 16384 x 50304: 367 us, with two 398; 16384 x 50257, element by element, 600 and 732. The
+// exponentials bound it (824 million: 183 us of the special-function units alone), the gradient is at a copy's rate: 520 us.
+constexpr int kCeBlocksOfRows = 4;
 template <int kDtype, bool kVec, bool kStage, bool kRows = false>
-__global__ void __launch_bounds__(kCeThreads, 2) cross_entropy_kernel(const CrossEntropyArgs a) {
+__global__ void __launch_bounds__(kCeThreads, kRows ? kCeBlocksOfRows : 2) cross_entropy_kernel(const CrossEntropyArgs a) {
   static_assert((kVec && !kRows) || !kStage, "staging uses the vector path, for a second pass");
   extern __shared__ uint4 s_row[];                // kStage: the row, every 16-byte chunk kept by the thread that read it
   using E = Elem<kDtype>;
@@ -301,7 +304,7 @@ cudaError_t launch_cross_entropy(const CrossEntropyArgs& a, int dtype, int sms, 
 cudaError_t launch_cross_entropy_rows(const CrossEntropyArgs& a, int sms, cudaStream_t stream) {
   if (a.rows == 0) return cudaSuccess;
   const bool vec = a.cols % 8 == 0 && a.ld % 8 == 0 && reinterpret_cast<uintptr_t>(a.logits) % 16 == 0;
-  const int grid = a.rows < sms * 2 ? a.rows : sms * 2;
+  const int grid = a.rows < sms * kCeBlocksOfRows ? a.rows : sms * kCeBlocksOfRows;
   if (vec) cross_entropy_kernel<1, true, false, true><<<grid, kCeThreads, 0, stream>>>(a);
   else cross_entropy_kernel<1, false, false, true><<<grid, kCeThreads, 0, stream>>>(a);
   return cudaGetLastError();
