@@ -297,7 +297,9 @@ int rbf_b200_cache_copy_pages(void* pages, int layers, int num_pages, size_t pag
 /* out (B, H * G, T, D), dense: RBF attention (softmax = 0: without the denominator) of T new tokens, which have been appended
  * already and are the newest that the cache holds (of a shorter prefix it has the whole blocks of 16 only); token i of
  * sequence b sees tokens 0 .. lengths[b] + i. Query head h reads key/value head h / G. q (B, H * G, T, D)
- * like k above. Rows from new_lengths[b] on are zero, as are rows that see nothing. gamma: usually 1 / sqrt(head dim). The
+ * like k above. Rows from new_lengths[b] on are zero, as are rows that see nothing. Rows that see a number that is not finite are
+ * NaN - of the incomplete block only where their own sums are, and an infinite distance is a weight of zero -, others are not
+ * touched by it. gamma: usually 1 / sqrt(head dim). The
  * workspace is 256-byte aligned; where none is needed it may be NULL. */
 size_t rbf_b200_cache_attention_workspace_bytes(int B, int H, int G, int T, int D, int max_pages);
 int rbf_b200_cache_attention(const void* q, const int64_t* q_strides, const void* pages, const int* page_table,

@@ -10,8 +10,12 @@
 // codes' squares.
 //   S^T (16 tokens x 8 columns) = K Q^T,  P^T by exponentials in fp32,  O^T (16 dims x 8 columns) += V^T P^T
 // Queries are multiplied by the power of two that brings their largest element to [1, 2) and rounded to fp16: exact for every
-// element within 2^-14 of the largest in 16-bit types, off by 2^-25 of it below. P is rounded to fp16 (2^-11 of it).
-// The block that is not complete yet is held in 16 bits and multiplied in its own type.
+// element within 2^-14 of the largest in 16-bit types, off by 2^-25 of it below. P is rounded to fp16 (2^-11 of it), as the operand
+// that the codes' products take; the sum that the outputs are divided by is of the weights in fp32, so that a row's roundings
+// average out instead of moving its denominator with them. The exponentials are ex2.approx, two units of fp32 off. The block that is not
+// complete yet is held in 16 bits and multiplied in its own type, P with it: of bfloat16 2^-8 of the weights of at most 15
+// tokens, which is the output's own rounding, where fp16 operands would need the values scaled (the kernel for many
+// columns, whose operands all are fp16, does that).
 //
 // Three kernels share this. Long sequences: work is split evenly whatever the lengths, all (sequence, head) segments in a row,
 // cut into units of one load, are dealt to the warps of one wave in contiguous ranges. A warp works by itself - no barrier - with
@@ -23,7 +27,7 @@
 //
 // Bounds, one B200: 16 sequences of up to 32768 tokens, 8 key heads of 128, 32 query heads (549 MB): 100 us a call, the first
 // kernel 93 us at 5.9 TB/s = 90 % of the copy bandwidth. 64 sequences of up to 1028 tokens, 8 heads of 64 (35.5 MB, 5.4 us at
-// that bandwidth): 16.9 us, of which the chain of launch, lengths, pages, codes and join is the larger part.
+// that bandwidth): 16.4 us, of which the chain of launch, lengths, pages, codes and join is the larger part.
 #include <cstdint>
 #include <cuda_runtime.h>
 
@@ -931,8 +935,10 @@ __global__ void __launch_bounds__(kWarps * 32, 16 / kWarps) cache_attn_short_ker
 // elements below 2^-14 of it (off by 2^-25 of it), and is then a block like the others.
 // What bounds it is the chain inside a unit - barrier, widening, barrier, products, exponentials, products - with 12 (8 at 128
 // dims) warps on an SM: the tensor pipe is busy for 19 to 28 % of the time, the issue slots for 33 to 44 %. 37 new tokens on 6
-// histories of up to 5003, 16 heads of 64: 39 us a call; 200 on 32 of up to 500: 76 (112 with the cache as the row operand and 32
-// columns a warp). Three blocks of 168 registers on an SM, or two of 255; four and three of them spill (50 and 93 us).
+// histories of up to 5003, 16 heads of 64: 39 to 41 us a call; 200 on 32 of up to 500, 8 heads: 76 (112 with the cache as the row operand and 32
+// columns a warp). Three blocks of 168 registers on an SM, or two of 255, with spills of up to 92 bytes a thread (bfloat16,
+// 64 rows of 64 columns; 72 in float16, 20 to 32 with fewer rows, at 128 columns 8 to 24 in float16 and none in bfloat16); four and
+// three blocks spill more (50 and 93 us).
 // Three units under way instead of two, the incomplete block's rows among them: 41 and 81 us; the next unit widened beside the
 // products, with one barrier a unit instead of two: 40 and 79.
 constexpr int kRowWarps = 4;

@@ -8,7 +8,7 @@
 // row, reads it with an online maximum and sum and keeps it in shared memory where it fits; longer rows come a second time out
 // of L2. The rows' bases may have any alignment: a row is a head of single elements up to the first 16-byte
 // boundary, 16-byte words, and a tail. Sums over rows are in 64 bits and in the order of the rows of a block, then of the blocks.
-// 16384 x 50304 bfloat16: 581 us, 5.7 TB/s = 87 % of a copy. The special-function unit is busy for 60 % of that, the issue slots
+// 16384 x 50304 bfloat16: 581 to 588 us, 5.6 TB/s = 86 % of a copy. The special-function unit is busy for 60 % of that, the issue slots
 // for 47; a quarter of the exponentials by polynomials took 599 us, fetching the next row into shared memory word by word behind
 // the gradient 616.
 #include <cstdint>

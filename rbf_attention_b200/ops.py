@@ -1398,7 +1398,9 @@ def cache_attention(q, pages, page_table, lengths, new_lengths=None, softmax: bo
     with the same arguments goes first): token i of sequence b sees tokens 0 to ``lengths[b] + i``, its own among them. Query head
     h reads key/value head ``h // (Hq // H)``. Returns (B, Hq, T, D); rows from ``new_lengths[b]`` on are zero. ``softmax=False``:
     ``exp(-g |q - k|^2) V``. These are the newest tokens that the cache holds: of a shorter prefix it has whole blocks of 16 only,
-    the 16-bit rows are those of the last block. No backward: a q that requires a gradient is refused in grad mode."""
+    the 16-bit rows are those of the last block. A row that sees a key or value that is not finite is NaN, in a block that is not
+    complete only where its own sums are: a value's column, a key whose distance comes out as NaN (one that comes out as infinite
+    has weight zero). No backward: a q that requires a gradient is refused in grad mode."""
     if _needs_grad(q):
         raise RuntimeError("cache_attention has no backward: call it under torch.no_grad() or on detached tensors")
     if type(softmax) is bool and _direct(q, pages, page_table, lengths, new_lengths):
